@@ -1,0 +1,97 @@
+/*
+ * mamba4_retention.h -- C ABI of the MI355X (gfx950) retention layer's
+ * operators: decayed linear attention over prompts and training batches, its
+ * gradient, and its step for single tokens (the library that also holds
+ * mamba4_memread.h).
+ *
+ * Plain pointers and sizes only; every buffer is on the device and owned by
+ * the caller.  `stream` is a hipStream_t passed as void* (NULL = the null
+ * stream).  No function allocates, frees or synchronises.  Return values are
+ * those of mamba4_memread.h (M4MR_OK, M4MR_EINVAL with nothing launched,
+ * M4MR_EHIP); m4mr_last_error() gives the message.
+ */
+#ifndef MAMBA4_RETENTION_H
+#define MAMBA4_RETENTION_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Largest key and value width of the linear attention. */
+#define M4RT_MAX_WIDTH 128
+
+/*
+ * Rows [B,T,heads,width] with unit stride along the width and strides in
+ * elements along the others (the token stride is not read by
+ * m4rt_attention_step).  `heads` divides the attention's H: head h reads row
+ * h / (H / heads).  The token stride is at least `width` and 64 of it less
+ * than 2^31 bytes.
+ */
+typedef struct {
+  const void* data;
+  long batch_stride, token_stride, head_stride;
+  int heads, width;
+} m4rt_rows;
+
+/*
+ * Linear attention with a decay for each head.
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t
+ *
+ * q, k [B,T,.,N], v [B,T,.,P] in float32, or bfloat16 if `bf16` is not zero;
+ * N, P in 1..M4RT_MAX_WIDTH.  log_decay: float32, [B,T,H] if `per_token` is not
+ * zero, else [H].  lengths [B] int32, or NULL: tokens at lengths[b] and after
+ * are absent (their rows are not read into any result, their output is zero; lengths
+ * outside 0..T are clamped).  initial [B,H,N,P] float32, or NULL for zeros.
+ * output [B,T,H,P] in v's type; state [B,H,N,P] float32, after the last
+ * token, or NULL.
+ *
+ * Sums, states and decays are held in float32 or more (bfloat16 operands that are
+ * computed on the way, the scores, the state and the weighted keys, enter the
+ * products as two bfloat16 parts, those of float32 calls as three).  A row's result
+ * does not depend on the batch size.  A log decay of -infinity (or any that
+ * underflows) drops what came before exactly.  An infinity or NaN in a row
+ * that is present spreads to the outputs of its chunk of 64 tokens and after it.
+ */
+size_t m4rt_attention_workspace_bytes(int B, int T, int H, int N, int P, int bf16);
+int m4rt_attention_forward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
+                           const float* log_decay, int per_token, const int* lengths,
+                           const float* initial, float scale, int B, int T, int H, void* output,
+                           float* state, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Its gradient, from the cotangents d_output [B,T,H,P] in the inputs' type and
+ * d_state [B,H,N,P] (NULL: zero).  state: the forward's final state, required
+ * where both d_state and d_log_decay are given.  d_q, d_k, d_v:
+ * [B,T,heads,width] in the inputs' type, contiguous; d_log_decay float32,
+ * [B,T,H] if per_token else [H], or NULL; d_initial [B,H,N,P], or NULL.
+ * Gradients of shared heads are summed in float32 and rounded once.
+ */
+size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads, int k_heads,
+                                               int v_heads, int N, int P, int bf16);
+int m4rt_attention_backward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
+                            const float* log_decay, int per_token, const int* lengths,
+                            const float* initial, float scale, int B, int T, int H,
+                            const void* d_output, const float* d_state, const float* state,
+                            void* d_q, void* d_k, void* d_v, float* d_log_decay,
+                            float* d_initial, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/*
+ * One token: state [B,H,N,P] float32 to new_state (which may be state itself:
+ * in place) and output [B,H,P] in v's type.  log_decay [B,H] if per_token,
+ * else [H].  active [B] bytes, or NULL: a row whose byte is zero keeps its
+ * state and its output is zero.
+ */
+int m4rt_attention_step(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
+                        const float* log_decay, int per_token, const uint8_t* active, float scale,
+                        int B, int H, const float* state, float* new_state, void* output,
+                        void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif

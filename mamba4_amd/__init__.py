@@ -8,9 +8,16 @@ implemented by hand-written HIP kernels behind the C ABI in
 ``include/mamba4_memread.h``, plus the caller's preprocessing and read gating
 (``memory_inputs``, ``gated_read``; lm/models/mamba4.py:183-237, 266-273)
 and the order head's gated scan (``order_memory_chunked``, ``order_memory``;
-lm/models/mamba4.py:46-95).
+lm/models/mamba4.py:46-95).  Beside them, the retention layer's operators
+(``linear_attention``, ``linear_attention_step``).
 """
 
+from mamba4_amd.attention import (  # noqa: F401
+    LinearAttentionResult,
+    linear_attention,
+    linear_attention_step,
+    linear_attention_step_,
+)
 from mamba4_amd.memory import (  # noqa: F401
     MEMORY_SOLVE,
     SOLVERS,
@@ -34,12 +41,16 @@ from mamba4_amd.flashmamba import mamba3_fused  # noqa: F401
 from mamba4_amd.order import order_memory, order_memory_chunked  # noqa: F401
 
 __all__ = [
+    "LinearAttentionResult",
     "MEMORY_SOLVE",
     "MemoryInputs",
     "MixerRead",
     "SOLVERS",
     "SelectiveResult",
     "SelectiveState",
+    "linear_attention",
+    "linear_attention_step",
+    "linear_attention_step_",
     "mamba3_fused",
     "gated_read",
     "memory_inputs",

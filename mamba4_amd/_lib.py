@@ -11,7 +11,8 @@ import re
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = os.path.join(HERE, "libmamba4_memread.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "mamba4_memread.h")
-HEADERS = [HEADER, os.path.join(os.path.dirname(HERE), "include", "mamba3_scan.h")]
+HEADERS = [HEADER] + [os.path.join(os.path.dirname(HERE), "include", name)
+                      for name in ("mamba3_scan.h", "mamba4_retention.h")]
 
 EINVAL = 1
 EHIP = 2
@@ -60,6 +61,22 @@ class ResizeArray(ctypes.Structure):
         ("fill", ctypes.c_uint),
     ]
 
+
+class Rows(ctypes.Structure):
+    """m4rt_rows (include/mamba4_retention.h)."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_long),
+        ("token_stride", ctypes.c_long),
+        ("head_stride", ctypes.c_long),
+        ("heads", ctypes.c_int),
+        ("width", ctypes.c_int),
+    ]
+
+
+_R = ctypes.POINTER(Rows)
+_F = ctypes.c_float
 
 SIGNATURES = {
     "m4mr_version": (ctypes.c_char_p, []),
@@ -122,6 +139,14 @@ SIGNATURES = {
     "m3s_backward": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P] * 9 + [_P, _S, _P]),
     "m3s_forward_bf16": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P]),
     "m3s_backward_bf16": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P] * 9 + [_P, _S, _P]),
+    "m4rt_attention_workspace_bytes": (_S, [_I] * 6),
+    "m4rt_attention_forward": (
+        _I, [_R] * 3 + [_I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 3 + [_S, _P]),
+    "m4rt_attention_backward_workspace_bytes": (_S, [_I] * 9),
+    "m4rt_attention_backward": (
+        _I, [_R] * 3 + [_I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 9 + [_S, _P]),
+    "m4rt_attention_step": (
+        _I, [_R] * 3 + [_I, _P, _I, _P, _F] + [_I] * 2 + [_P] * 3 + [_P]),
     "m4mr_profile_enable": (None, [_I]),
     "m4mr_profile_select": (None, [ctypes.c_char_p]),
     "m4mr_profile_reset": (None, []),
@@ -140,10 +165,10 @@ class MemreadError(RuntimeError):
 
 
 def header_functions():
-    """Names of the functions declared in include/mamba4_memread.h and
-    include/mamba3_scan.h."""
+    """Names of the functions declared in include/mamba4_memread.h,
+    include/mamba3_scan.h and include/mamba4_retention.h."""
     text = "".join(open(h).read() for h in HEADERS)
-    pattern = r"^\s*(?:const\s+)?\w+\**\s+\**((?:m4mr|m3s)_\w+)\s*\("
+    pattern = r"^\s*(?:const\s+)?\w+\**\s+\**((?:m4mr|m3s|m4rt)_\w+)\s*\("
     return sorted(set(re.findall(pattern, text, re.M)))
 
 

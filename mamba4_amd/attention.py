@@ -1,0 +1,267 @@
+"""Linear attention with a decay for each head on MI355X.
+
+Per batch row and head, with a matrix state S [N, P]:
+
+    S_t = exp(g_t) S_{t-1} + k_t v_t^T,    o_t = scale * S_t^T q_t
+
+``linear_attention`` runs whole sequences (chunked on the matrix cores, prompts
+and training), ``linear_attention_step`` and ``linear_attention_step_`` one
+token from a cached state.  The decays are data (a gate of every token and head)
+or a constant of each head; queries, keys and values may have fewer heads than
+the attention, each shared by as many consecutive heads.
+
+Runs on the gfx950 HIP library (``m4rt_attention_*``,
+include/mamba4_retention.h) on the current stream; there is no other
+implementation.  With queries, keys and values all bfloat16 the kernels read
+them as they are and return bfloat16; any other mix is computed in float32 and
+returned in the values' dtype.  States, decays and sums are float32 or wider.
+"""
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from mamba4_amd import _lib
+from mamba4_amd.memory import _ptr, _require_device, _stream
+
+MAX_WIDTH = 128
+_MAX_TOKEN_STRIDE = (2**31 - 1) // 256
+
+
+class LinearAttentionResult(NamedTuple):
+    output: torch.Tensor
+    state: torch.Tensor
+
+
+def _f32(t):
+    return t.to(torch.float32).contiguous()
+
+
+def _strided(t):
+    """t itself where the kernels can address it: unit stride along the width,
+    tokens at least a row apart (views into a fused projection, say); else a
+    contiguous copy."""
+    unit = t.stride(-1) == 1 or t.shape[-1] == 1
+    if unit and t.dim() == 4 and t.shape[1] > 1:
+        unit = t.shape[-1] <= t.stride(1) <= _MAX_TOKEN_STRIDE
+    return t if unit else t.contiguous()
+
+
+def _rows(t):
+    """The m4rt_rows of [B,T,h,W] or [B,h,W]; strides of axes of one element are
+    never used and given as zero (the token stride, as the width)."""
+    heads, width = t.shape[-2:]
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    token = strides[1] if t.dim() == 4 and t.shape[1] > 1 else width
+    return ctypes.byref(_lib.Rows(t.data_ptr(), strides[0], token, strides[-2], heads, width))
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _forward(q, k, v, log_decay, initial, lengths, scale):
+    lib = _lib.load()
+    batch, time = q.shape[:2]
+    heads = log_decay.shape[-1]
+    n, p = k.shape[-1], v.shape[-1]
+    bf16 = int(v.dtype == torch.bfloat16)
+    output = torch.empty(batch, time, heads, p, dtype=v.dtype, device=v.device)
+    state = torch.empty(batch, heads, n, p, dtype=torch.float32, device=v.device)
+    nbytes = lib.m4rt_attention_workspace_bytes(batch, time, heads, n, p, bf16)
+    workspace = _workspace(nbytes, v.device)
+    _lib.check(
+        lib.m4rt_attention_forward(
+            _rows(q), _rows(k), _rows(v), bf16, _ptr(log_decay), int(log_decay.dim() == 3),
+            _ptr(lengths), _ptr(initial), scale, batch, time, heads, _ptr(output), _ptr(state),
+            _ptr(workspace), nbytes, _stream(),
+        )
+    )
+    return output, state
+
+
+class _Attention(torch.autograd.Function):
+    """q, k, v all bfloat16 or all float32, strided as ``_strided`` leaves them;
+    the other inputs float32 and contiguous, lengths int32."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial, lengths, scale):
+        output, state = _forward(q, k, v, log_decay, initial, lengths, scale)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, initial, lengths, state)
+        ctx.scale = scale
+        return output, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_output, d_state):
+        lib = _lib.load()
+        q, k, v, log_decay, initial, lengths, state = ctx.saved_tensors
+        batch, time = q.shape[:2]
+        heads = log_decay.shape[-1]
+        n, p = k.shape[-1], v.shape[-1]
+        bf16 = int(v.dtype == torch.bfloat16)
+        shape = (batch, time, heads, p)
+        if d_output is None:
+            d_output = torch.zeros(shape, dtype=v.dtype, device=v.device)
+        d_output = d_output.to(v.dtype).contiguous()
+        d_state = None if d_state is None else _f32(d_state)
+        d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        d_decay = torch.empty_like(log_decay) if ctx.needs_input_grad[3] else None
+        d_initial = torch.empty_like(state) if ctx.needs_input_grad[4] else None
+        nbytes = lib.m4rt_attention_backward_workspace_bytes(
+            batch, time, heads, q.shape[2], k.shape[2], v.shape[2], n, p, bf16)
+        workspace = _workspace(nbytes, v.device)
+        _lib.check(
+            lib.m4rt_attention_backward(
+                _rows(q), _rows(k), _rows(v), bf16, _ptr(log_decay), int(log_decay.dim() == 3),
+                _ptr(lengths), _ptr(initial), ctx.scale, batch, time, heads, _ptr(d_output),
+                _ptr(d_state), _ptr(state), _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_decay),
+                _ptr(d_initial), _ptr(workspace), nbytes, _stream(),
+            )
+        )
+        return d_q, d_k, d_v, d_decay, d_initial, None, None
+
+
+def _model_rows(name, queries, keys, values, dims):
+    """The heads of the call, and q, k, v in one dtype of the kernels."""
+    layout = "[B,T,h,W]" if dims == 4 else "[B,h,W]"
+    lead = dims - 2
+    if any(t.dim() != dims for t in (queries, keys, values)):
+        raise ValueError(f"{name} needs queries, keys and values {layout}")
+    if keys.shape[:lead] != queries.shape[:lead] or values.shape[:lead] != queries.shape[:lead]:
+        raise ValueError("queries, keys and values disagree")
+    if queries.shape[-1] != keys.shape[-1]:
+        raise ValueError("queries and keys disagree in width")
+    heads = max(t.shape[-2] for t in (queries, keys, values))
+    if heads == 0 or any(t.shape[-2] == 0 or heads % t.shape[-2] for t in (queries, keys, values)):
+        raise ValueError("the heads of queries, keys and values must divide the largest of them")
+    if not all(1 <= t.shape[-1] <= MAX_WIDTH for t in (keys, values)):
+        raise ValueError(f"key and value widths must be 1..{MAX_WIDTH}")
+    if not all(t.dtype == torch.bfloat16 for t in (queries, keys, values)):
+        queries, keys, values = (t.to(torch.float32) for t in (queries, keys, values))
+    return heads, queries, keys, values
+
+
+def _same_device(*tensors):
+    _require_device(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"all tensors must be on one device; got {sorted(map(str, devices))}")
+
+
+def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=None, scale=1.0):
+    """Decayed linear attention over sequences, differentiable.
+
+    queries, keys [B,T,h,N], values [B,T,h,P] with N, P <= 128; the numbers of
+    heads may differ if each divides the largest, H (consecutive heads share).
+    log_decay [B,T,H], or [H] for one constant a head (log of the factor that the
+    state keeps; -inf drops it).  initial [B,H,N,P] is the state before the first token
+    (zeros by default).  lengths [B] (integers): tokens from lengths[b] on are
+    absent, whatever their rows hold; their outputs and gradients are zero.
+
+    Returns LinearAttentionResult(output [B,T,H,P] in the values' dtype, state
+    [B,H,N,P] float32 after the last token).  A row's result does not depend on
+    the batch it is in.
+    """
+    _same_device(queries, keys, values, log_decay, initial, lengths)
+    heads, q, k, v = _model_rows("linear_attention", queries, keys, values, 4)
+    batch, time = queries.shape[:2]
+    n, p = keys.shape[-1], values.shape[-1]
+    if tuple(log_decay.shape) not in ((batch, time, heads), (heads,)):
+        raise ValueError("linear_attention needs log_decay [B,T,H] or [H]")
+    if initial is not None and tuple(initial.shape) != (batch, heads, n, p):
+        raise ValueError("linear_attention needs initial [B,H,N,P]")
+    if lengths is not None:
+        if tuple(lengths.shape) != (batch,) or lengths.dtype.is_floating_point \
+                or lengths.dtype in (torch.bool, torch.complex64, torch.complex128):
+            raise ValueError("linear_attention needs integer lengths [B]")
+        # Clamped before the narrowing, so that no length wraps around.
+        lengths = lengths.clamp(0, time).to(torch.int32).contiguous()
+    if batch == 0 or time == 0:
+        output = values.new_zeros((batch, time, heads, p))
+        state = output.new_zeros((batch, heads, n, p), dtype=torch.float32)
+        if initial is not None:
+            state = state + initial
+        return LinearAttentionResult(output, state)
+    args = (_strided(q), _strided(k), _strided(v), _f32(log_decay),
+            None if initial is None else _f32(initial), lengths, float(scale))
+    with torch.cuda.device(values.device):
+        if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in args[:5]
+        ):
+            output, state = _Attention.apply(*args)
+        else:
+            output, state = _forward(*args)
+    return LinearAttentionResult(output.to(values.dtype), state)
+
+
+def _step_checks(state, query, key, value, log_decay, active):
+    _same_device(state, query, key, value, log_decay, active)
+    heads, q, k, v = _model_rows("linear_attention_step", query, key, value, 3)
+    batch = query.shape[0]
+    n, p = key.shape[-1], value.shape[-1]
+    if tuple(state.shape) != (batch, heads, n, p):
+        raise ValueError("linear_attention_step needs state [B,H,N,P]")
+    if tuple(log_decay.shape) not in ((batch, heads), (heads,)):
+        raise ValueError("linear_attention_step needs log_decay [B,H] or [H]")
+    if active is not None and (tuple(active.shape) != (batch,) or active.dtype != torch.bool):
+        raise ValueError("linear_attention_step needs a boolean active [B]")
+    return heads, q, k, v
+
+
+def _step(state, new_state, q, k, v, log_decay, active, scale, heads, dtype):
+    lib = _lib.load()
+    batch, n, p = q.shape[0], k.shape[-1], v.shape[-1]
+    bf16 = int(v.dtype == torch.bfloat16)
+    output = torch.empty(batch, heads, p, dtype=v.dtype, device=v.device)
+    q, k, v, g = _strided(q), _strided(k), _strided(v), _f32(log_decay)
+    active = None if active is None else active.contiguous()
+    if batch:
+        with torch.cuda.device(output.device):
+            _lib.check(
+                lib.m4rt_attention_step(
+                    _rows(q), _rows(k), _rows(v), bf16, _ptr(g), int(log_decay.dim() == 2),
+                    _ptr(active), float(scale), batch, heads, _ptr(state), _ptr(new_state),
+                    _ptr(output), _stream(),
+                )
+            )
+    return LinearAttentionResult(output.to(dtype), new_state)
+
+
+def linear_attention_step(state, query, key, value, log_decay, *, active=None, scale=1.0):
+    """One token of ``linear_attention`` from a cached state.
+
+    state [B,H,N,P]; query, key [B,h,N], value [B,h,P]; log_decay [B,H] or [H].
+    active [B] (bool): rows where it is false keep their state and give zeros,
+    whatever their token holds.  Returns LinearAttentionResult(output [B,H,P],
+    new state); the state given is not modified.  Where a gradient is wanted the
+    step is ``linear_attention`` over one token.
+    """
+    heads, q, k, v = _step_checks(state, query, key, value, log_decay, active)
+    if torch.is_grad_enabled() and any(
+        t.requires_grad for t in (state, query, key, value, log_decay)
+    ):
+        decay = log_decay if log_decay.dim() == 1 else log_decay[:, None]
+        one = linear_attention(query[:, None], key[:, None], value[:, None], decay, initial=state,
+                               lengths=None if active is None else active.to(torch.int32),
+                               scale=scale)
+        return LinearAttentionResult(one.output[:, 0], one.state)
+    old = _f32(state)
+    return _step(old, torch.empty_like(old), q, k, v, log_decay, active, scale, heads, value.dtype)
+
+
+def linear_attention_step_(state, query, key, value, log_decay, *, active=None, scale=1.0):
+    """In-place ``linear_attention_step``: overwrites ``state``, which has to be
+    float32 and contiguous, with the new state.  Not differentiable."""
+    heads, q, k, v = _step_checks(state, query, key, value, log_decay, active)
+    if state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError("linear_attention_step_ needs a contiguous float32 state")
+    if torch.is_grad_enabled() and any(
+        t.requires_grad for t in (state, query, key, value, log_decay)
+    ):
+        raise ValueError("linear_attention_step_ has no gradient; use linear_attention_step")
+    # The state may be saved for a backward: the write counts as one of torch's.
+    torch.autograd.graph.increment_version(state)
+    return _step(state, state, q, k, v, log_decay, active, scale, heads, value.dtype)

@@ -17,6 +17,7 @@
 
 #include "../../include/mamba3_scan.h"
 #include "../../include/mamba4_memread.h"
+#include "api_common.hpp"
 #include "common.hpp"
 #include "scan3.hpp"
 
@@ -1873,3 +1874,16 @@ const char* m4mr_profile_kernel_name(int i) {
 }
 
 }  // extern "C"
+
+// The error message, launches and device facts for the entry points of other
+// sources.
+namespace m4 {
+
+int api_fail(int code, const std::string& msg) { return fail(code, msg); }
+void api_clear() { g_error.clear(); }
+int api_compute_units() { return compute_units(); }
+int api_launch(const char* name, hipStream_t stream, void (*body)(void*), void* context) {
+  return launch(name, stream, [&] { body(context); });
+}
+
+}  // namespace m4

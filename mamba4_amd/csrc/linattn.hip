@@ -1,0 +1,865 @@
+// Decayed linear attention for gfx950.
+//
+// Per batch row and head, with keys and queries of width n and values of p:
+//   S_t = e^{g_t} S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t.
+// In chunks of 64 tokens, P the chunk's running sum of g:
+//   O  = scale (A V + e^{P_i} Q S),   A_ij = (q_i . k_j) e^{P_i - P_j}, j <= i,
+//   S <- e^{P_L} S + (K e^{P_L - P_j})^T V.
+// The gradients are three more of the same:
+//   dQ = scale attention(dO, V, K) on the state S^T,
+//   dV = attention(K, Q, dO) and dK = attention(V, dO, Q) with time reversed,
+//        on the cotangent R of the state and R^T
+//        (R <- e^{P_L} R + scale (Q e^{P_i})^T dO, weights e^{P_i - P_j}, i >= j),
+//   dg_t = <S_T, R_T> + sum over i >= t of (q_i . dq_i - k_i . dk_i),
+// which sums (q_i . k_j)(do_i . v_j) scale e^{P_i - P_j} over pairs i >= t > j
+// (the pairs i = j are in both products and left out of both).
+// So one kernel serves all of them ("roles"); a block walks the chunks of one
+// (b, h) for 64 columns of the values, keeping the state in registers.
+//
+// Products run on bfloat16 MFMA with float32 accumulation.  An operand is a sum of
+// bfloat16 planes: a bfloat16 input is one plane; what is computed
+// in float32 (A, S, the weighted K) is two planes beside bfloat16 inputs
+// (2^-17 of the value left out, far below the rounding of a bfloat16 result and
+// near float32 for the states and dg); float32 inputs and what is computed from
+// them are three planes (all 24 bits) with the six largest plane products:
+// a sixth of the bfloat16 rate, 2.7 times that of float32 MFMA.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "linattn.hpp"
+
+namespace la {
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr unsigned kNoLoad = 0x80000000u;  // an offset past every resource
+
+__device__ __forceinline__ Rsrc rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
+}
+
+template <typename In>
+struct Type;
+template <>
+struct Type<bf16_t> {
+  static constexpr int IN = 1, MADE = 2;  // planes of an input, of a computed operand
+};
+template <>
+struct Type<float> {
+  static constexpr int IN = 3, MADE = 3;
+};
+
+// Eight consecutive elements as loaded.
+template <typename In>
+struct Piece {
+  u4 w[sizeof(In) / 2];
+};
+
+// MFMA operand fragments of 16x16x32: lane (g, r) = (lane >> 4, lane & 15)
+// holds row (or column) r at eight of the 32 k, as PLANES bfloat16 planes.
+template <int PLANES>
+struct Frag {
+  b8 p[PLANES];
+};
+
+__device__ __forceinline__ unsigned pack(float a, float b) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
+}
+__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+// Two float32 values as bfloat16 planes: each plane is what is left of them,
+// rounded to the nearest.
+template <int PLANES>
+__device__ __forceinline__ void split2(float a, float b, unsigned (&out)[PLANES]) {
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i) {
+    out[i] = pack(a, b);
+    a -= low(out[i]);
+    b -= high(out[i]);
+  }
+}
+
+template <int PLANES>
+__device__ __forceinline__ Frag<PLANES> split8(const float (&x)[8]) {
+  u4 w[PLANES];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    unsigned part[PLANES];
+    split2<PLANES>(x[2 * e], x[2 * e + 1], part);
+#pragma unroll
+    for (int i = 0; i < PLANES; ++i) w[i][e] = part[i];
+  }
+  Frag<PLANES> f;
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i) f.p[i] = __builtin_bit_cast(b8, w[i]);
+  return f;
+}
+
+__device__ __forceinline__ Frag<1> planes(const Piece<bf16_t>& x) {
+  return Frag<1>{{__builtin_bit_cast(b8, x.w[0])}};
+}
+__device__ __forceinline__ Frag<3> planes(const Piece<float>& x) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(x.w[e >> 2][e & 3]);
+  return split8<3>(v);
+}
+
+// acc += a b over the plane products that count: the sum of the planes'
+// indexes below the larger number of planes.
+template <int PA, int PB>
+__device__ __forceinline__ f4 mma(const Frag<PA>& a, const Frag<PB>& b, f4 acc) {
+  constexpr int most = PA > PB ? PA : PB;
+#pragma unroll
+  for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      if (s - i >= 0 && s - i < PB)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], acc, 0, 0, 0);
+  return acc;
+}
+
+// Elements col..col+7 of a row of `width` at byte offset `row`, zeros past the
+// width (and past the resource).
+__device__ __forceinline__ Piece<bf16_t> load_piece(Rsrc r, unsigned row, int col, int width,
+                                                    int vec, const bf16_t*) {
+  Piece<bf16_t> x;
+  const unsigned off = row + 2 * col;
+  if (vec == 8) {
+    x.w[0] = __builtin_bit_cast(
+        u4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0));
+  } else if (vec == 2) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x.w[0][e] = __builtin_amdgcn_raw_buffer_load_b32(
+          r, col + 2 * e < width ? off + 4 * e : kNoLoad, 0, 0);
+  } else {
+    unsigned v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = __builtin_amdgcn_raw_buffer_load_b16(r, col + e < width ? off + 2 * e : kNoLoad, 0,
+                                                  0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.w[0][e] = v[2 * e] | (v[2 * e + 1] << 16);
+  }
+  return x;
+}
+__device__ __forceinline__ Piece<float> load_piece(Rsrc r, unsigned row, int col, int width,
+                                                   int vec, const float*) {
+  Piece<float> x;
+  const unsigned off = row + 4 * col;
+  if (vec >= 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      x.w[i] = __builtin_bit_cast(
+          u4, __builtin_amdgcn_raw_buffer_load_b128(
+                  r, col + 4 * i < width ? off + 16 * i : kNoLoad, 0, 0));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x.w[e >> 2][e & 3] = __builtin_amdgcn_raw_buffer_load_b32(
+          r, col + e < width ? off + 4 * e : kNoLoad, 0, 0);
+  }
+  return x;
+}
+
+// The chunk's rows of (b, h): a resource that ends with row `rows` - 1.
+template <typename In>
+__device__ __forceinline__ Rsrc chunk_rows(const Rows& x, int b, int h, long t0, int rows) {
+  const In* base = static_cast<const In*>(x.base) + b * x.sb + (h / x.share) * x.sh + t0 * x.st;
+  const int bytes = rows > 0 ? (int)(((rows - 1) * x.st + x.width) * sizeof(In)) : 0;
+  return rsrc(base, bytes);
+}
+
+// LDS rows: 64 NT or 64 bfloat16 and 16 bytes of padding, so that the rows
+// 0..15 of a fragment start in distinct 16-byte bank groups.
+template <int NT>
+__host__ __device__ constexpr int row_elems() {
+  return 64 * NT + 8;
+}
+
+template <typename In, int NT>
+struct Shared {
+  bf16_t k[Type<In>::IN][C * row_elems<NT>()];        // K [token][n]
+  bf16_t v[Type<In>::IN][C * row_elems<1>()];         // V [token][column]
+  bf16_t s[Type<In>::MADE][TILE * row_elems<NT>()];   // S^T [column][n]
+  float ph[C], pl[C];  // running log2 decay, high and low parts
+  float inter[C];      // weights of the state's part of each output
+  float update[C];     // weights of each token's part of the next state
+  float decay;         // the chunk's decay of the state
+};
+
+__device__ __forceinline__ Frag<1> cat(s4 a, s4 b) {
+  typedef short s8 __attribute__((ext_vector_type(8)));
+  return Frag<1>{{__builtin_bit_cast(b8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]})}};
+}
+
+// Column fragments of a row-major tile by transposing reads: lane (g, r)
+// receives column c0 + r at the tokens 32 s + 4 g + (0..3) and 32 s + 16 + 4 g
+// + (0..3).  That is the order in which the scores' accumulators hold the
+// tokens, so those are operands as they are.
+template <int PLANES, int STRIDE>
+__device__ __forceinline__ Frag<PLANES> columns(const bf16_t (&tile)[PLANES][C * STRIDE], int s,
+                                                int c0, int g, int r) {
+  typedef __attribute__((address_space(3))) s4* lds4;
+  Frag<PLANES> f;
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i) {
+    const bf16_t* p = &tile[i][(32 * s + 4 * g + (r >> 2)) * STRIDE + c0 + 4 * (r & 3)];
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * STRIDE));
+    f.p[i] = cat(a, b).p[0];
+  }
+  return f;
+}
+
+// Row fragments: lane (g, r) receives row r0 + r at n = 32 kk + 8 g + (0..7).
+template <int PLANES, int ROWS, int STRIDE>
+__device__ __forceinline__ Frag<PLANES> rows(const bf16_t (&tile)[PLANES][ROWS * STRIDE], int r0,
+                                             int kk, int g, int r) {
+  Frag<PLANES> f;
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i)
+    f.p[i] = __builtin_bit_cast(
+        b8, *reinterpret_cast<const u4*>(&tile[i][(r0 + r) * STRIDE + 32 * kk + 8 * g]));
+  return f;
+}
+
+// The eight values of a fragment, times eight weights, as computed planes.
+template <int MADE>
+__device__ __forceinline__ Frag<MADE> weighted(const Frag<1>& f, const float (&w)[8]) {
+  const u4 u = __builtin_bit_cast(u4, f.p[0]);
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = low(u[e]) * w[2 * e];
+    x[2 * e + 1] = high(u[e]) * w[2 * e + 1];
+  }
+  return split8<MADE>(x);
+}
+template <int MADE>
+__device__ __forceinline__ Frag<MADE> weighted(const Frag<3>& f, const float (&w)[8]) {
+  const u4 a = __builtin_bit_cast(u4, f.p[0]), b = __builtin_bit_cast(u4, f.p[1]),
+           c = __builtin_bit_cast(u4, f.p[2]);
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = (low(a[e]) + (low(b[e]) + low(c[e]))) * w[2 * e];
+    x[2 * e + 1] = (high(a[e]) + (high(b[e]) + high(c[e]))) * w[2 * e + 1];
+  }
+  return split8<MADE>(x);
+}
+
+// x of the lanes below, DPP row shifts and broadcasts on both halves of a
+// double; zero where there is none.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_double(double x) {
+  const u2 u = __builtin_bit_cast(u2, x);
+  const unsigned a = __builtin_amdgcn_update_dpp(0, u[0], CTRL, ROW_MASK, 0xf, true);
+  const unsigned b = __builtin_amdgcn_update_dpp(0, u[1], CTRL, ROW_MASK, 0xf, true);
+  return __builtin_bit_cast(double, u2{a, b});
+}
+__device__ __forceinline__ double wave_prefix(double x) {
+  x += dpp_double<0x111, 0xf>(x);
+  x += dpp_double<0x112, 0xf>(x);
+  x += dpp_double<0x114, 0xf>(x);
+  x += dpp_double<0x118, 0xf>(x);
+  x += dpp_double<0x142, 0xa>(x);
+  x += dpp_double<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ double lane_double(double x, int lane) {
+  const u2 u = __builtin_bit_cast(u2, x);
+  const unsigned a = __builtin_amdgcn_readlane(u[0], lane);
+  const unsigned b = __builtin_amdgcn_readlane(u[1], lane);
+  return __builtin_bit_cast(double, u2{a, b});
+}
+
+// Sum over the four lanes that share r.
+__device__ __forceinline__ float sum_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A chunk's decays, by one wave (lane = token).  The running sum is in
+// float64 and kept as two float32, so that e^{P_i - P_j} of near tokens is exact
+// to float32 after any decay before them.  A log decay below -2000 (-infinity, a
+// type's lowest value) counts as -2000: its exponential is zero either way and
+// the differences behind it stay finite.
+template <typename S>
+__device__ __forceinline__ void chunk_decays(S& sh, float g, int lane, bool rev, float inter,
+                                             float update) {
+  const double p = wave_prefix((double)(g < -2000.f ? -2000.f : g) * 1.4426950408889634);
+  const double last = lane_double(p, 63);
+  const float ph = (float)p;
+  sh.ph[lane] = ph;
+  sh.pl[lane] = (float)(p - ph);
+  const float head = __builtin_amdgcn_exp2f((float)p);
+  const float tail = __builtin_amdgcn_exp2f((float)(last - p));
+  sh.inter[lane] = inter * (rev ? tail : head);
+  sh.update[lane] = update * (rev ? head : tail);
+  if (lane == 63) sh.decay = head;
+}
+
+__device__ __forceinline__ void store_out(void* base, long at, f4 v, int left, bool f32,
+                                          bool vec) {
+  if (f32) {
+    float* p = static_cast<float*>(base) + at;
+    if (vec) {
+      *reinterpret_cast<f4*>(p) = v;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < left) p[q] = v[q];
+    }
+  } else {
+    bf16_t* p = static_cast<bf16_t*>(base) + at;
+    const u2 u{pack(v[0], v[1]), pack(v[2], v[3])};
+    if (vec) {
+      *reinterpret_cast<u2*>(p) = u;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < left) p[q] = (bf16_t)(u[q >> 1] >> (16 * (q & 1)));
+    }
+  }
+}
+
+// One block: 64 value columns of one (b, h), the chunks c0..c1-1 (in reverse
+// if role.rev).  OUT: outputs from the state at the first chunk; else only the
+// segment's own state from zero, for split runs.
+//
+// A segment of SEG chunks keeps its own state (from zero) apart from the
+// state at its start; the state in use is decay * start + own.  So a split run, whose
+// blocks take one segment each, has the bits of a walk over all of them.
+template <typename In, int NT, bool OUT>
+__device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int b, int h, int c0,
+                                     int c1, int seg, Shared<In, NT>& sh) {
+  constexpr int IN = Type<In>::IN, MADE = Type<In>::MADE;
+  constexpr int KROW = row_elems<NT>(), VROW = row_elems<1>();
+  constexpr int KP = 2 * NT;  // pieces of K a thread loads
+  const In* tag = nullptr;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col0 = TILE * tile, bh = b * a.H + h;
+  const int length = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const bool rev = R.rev;
+  const int count = c1 - c0;
+
+  // The state's accumulators: n = 64 nt + 16 w + 4 g + q, column 16 pb + r.
+  f4 start[NT][4], own[NT][4];
+  float since = 1.f;  // decay since the segment's start
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int pb = 0; pb < 4; ++pb) {
+      own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
+      start[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (OUT) {
+        if (seg >= 0) {
+          const long slot = ((long)(tile * a.B * a.H + bh) * a.NS + seg) * (NT * 4096);
+          start[nt][pb] = *reinterpret_cast<const f4*>(
+              R.starts + slot + ((nt * 4 + pb) * THREADS + tid) * 4);
+        } else if (R.initial.base) {
+          const float* s = R.initial.base + (long)bh * R.n * R.p;
+          const int p = col0 + 16 * pb + r;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = 64 * nt + 16 * w + 4 * g + q;
+            if (n < R.n && p < R.p) start[nt][pb][q] = s[(long)n * R.initial.sn + (long)p * R.initial.sp];
+          }
+        }
+      }
+    }
+
+  Piece<In> kraw[KP], vraw[2], qraw[2 * NT];
+  float graw = 0.f;
+  const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
+  const int vcol = 8 * (tid & 7), vrow = tid >> 3;
+  auto fetch = [&](int c) {
+    const long t0 = (long)c * C;
+    const int have = min(length - (int)t0, C);
+    const Rsrc kr = chunk_rows<In>(R.k, b, h, t0, have);
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      kraw[i] = load_piece(kr, (unsigned)((krow + 32 / NT * i) * R.k.st * sizeof(In)), kcol, R.n,
+                           R.k.vec, tag);
+    const Rsrc vr = chunk_rows<In>(R.v, b, h, t0, have);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      vraw[i] = load_piece(vr, (unsigned)((vrow + 32 * i) * R.v.st * sizeof(In)), col0 + vcol, R.p,
+                           R.v.vec, tag);
+    if constexpr (OUT) {
+      const Rsrc qr = chunk_rows<In>(R.q, b, h, t0, have);
+#pragma unroll
+      for (int kk = 0; kk < 2 * NT; ++kk)
+        qraw[kk] = load_piece(qr, (unsigned)((16 * w + r) * R.q.st * sizeof(In)), 32 * kk + 8 * g,
+                              R.n, R.q.vec, tag);
+    }
+    if (w == 0) graw = lane < have ? a.g[b * a.gb + (t0 + lane) * a.gt + h] : 0.f;
+  };
+
+  if (count > 0) fetch(rev ? c1 - 1 : c0);
+  for (int it = 0; it < count; ++it) {
+    const int c = rev ? c1 - 1 - it : c0 + it;
+    const long t0 = (long)c * C;
+    const int have = min(length - (int)t0, C);
+    Frag<IN> qf[2 * NT];
+    if (have > 0) {
+      // K, V, the state and the decays to LDS.
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const Frag<IN> f = planes(kraw[i]);
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+          *reinterpret_cast<u4*>(&sh.k[j][(krow + 32 / NT * i) * KROW + kcol]) =
+              __builtin_bit_cast(u4, f.p[j]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Frag<IN> f = planes(vraw[i]);
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+          *reinterpret_cast<u4*>(&sh.v[j][(vrow + 32 * i) * VROW + vcol]) =
+              __builtin_bit_cast(u4, f.p[j]);
+      }
+      if constexpr (OUT) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb) {
+            float s[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] = fmaf(since, start[nt][pb][q], own[nt][pb][q]);
+            unsigned lo[MADE], hi[MADE];
+            split2<MADE>(s[0], s[1], lo);
+            split2<MADE>(s[2], s[3], hi);
+#pragma unroll
+            for (int j = 0; j < MADE; ++j)
+              *reinterpret_cast<u2*>(
+                  &sh.s[j][(16 * pb + r) * KROW + 64 * nt + 16 * w + 4 * g]) = u2{lo[j], hi[j]};
+          }
+#pragma unroll
+        for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
+      }
+      if (w == 0) chunk_decays(sh, graw, lane, rev, R.inter, R.update);
+    }
+    __syncthreads();
+    if (it + 1 < count) fetch(rev ? c - 1 : c + 1);
+    if (have > 0) {
+      f4 out[4];
+      Frag<MADE> score[2];
+      float diagonal;  // with dots: a token's score with itself, kept out of score
+      if constexpr (OUT) {
+        // The state's part, transposed: columns 16 pb + 4 g + q of token 16 w + r.
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb) out[pb] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 2 * NT; ++kk)
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb)
+            out[pb] = mma(rows<MADE, TILE, KROW>(sh.s, 16 * pb, kk, g, r), qf[kk], out[pb]);
+        const float inter = sh.inter[16 * w + r];
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb) out[pb] *= inter;
+        // Scores, transposed: keys 16 jb + 4 g + q of query 16 w + r.
+        const float ph = sh.ph[16 * w + r], pl = sh.pl[16 * w + r];
+        diagonal = 0.f;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float x[8];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int jb = 2 * s + half;
+            f4 acc{0.f, 0.f, 0.f, 0.f};
+            if (rev ? jb >= w : jb <= w) {
+#pragma unroll
+              for (int kk = 0; kk < 2 * NT; ++kk)
+                acc = mma(rows<IN, C, KROW>(sh.k, 16 * jb, kk, g, r), qf[kk], acc);
+              const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[16 * jb + 4 * g]);
+              const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[16 * jb + 4 * g]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float gap = (ph - kh[q]) + (pl - kl[q]);
+                const int ahead = 16 * (w - jb) + r - 4 * g - q;  // query - key
+                const float d = __builtin_amdgcn_exp2f(rev ? -gap : gap) * R.intra;
+                acc[q] = (rev ? ahead <= 0 : ahead >= 0) ? acc[q] * d : 0.f;
+                if (R.dots && ahead == 0) {
+                  diagonal = acc[q];
+                  acc[q] = 0.f;
+                }
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[4 * half + q] = acc[q];
+          }
+          score[s] = split8<MADE>(x);
+        }
+      }
+      // The next state, and the scores' part of the output.
+      const float decay = sh.decay;
+      since *= decay;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb) own[nt][pb] *= decay;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float wt[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const f4 u = *reinterpret_cast<const f4*>(&sh.update[32 * s + 16 * half + 4 * g]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) wt[4 * half + q] = u[q];
+        }
+        Frag<MADE> kw[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          kw[nt] = weighted<MADE>(columns<IN, KROW>(sh.k, s, 64 * nt + 16 * w, g, r), wt);
+        const bool scores = OUT && (rev ? 2 * s + 1 >= w : 2 * s <= w);
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb) {
+          const Frag<IN> vf = columns<IN, VROW>(sh.v, s, 16 * pb, g, r);
+          if constexpr (OUT) {
+            if (scores) out[pb] = mma(vf, score[s], out[pb]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) own[nt][pb] = mma(kw[nt], vf, own[nt][pb]);
+        }
+      }
+      if constexpr (OUT) {
+        const int t = 16 * w + r;
+        if (R.dots) {
+          const Rsrc er = chunk_rows<In>(R.e, b, h, t0, have);
+          float dot = 0.f;
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb) {
+            const int p = col0 + 16 * pb + 4 * g;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const unsigned off = (unsigned)((t * R.e.st + p + q) * sizeof(In));
+              float e;
+              if constexpr (sizeof(In) == 2)
+                e = __uint_as_float((unsigned)__builtin_amdgcn_raw_buffer_load_b16(
+                                        er, p + q < R.p ? off : kNoLoad, 0, 0)
+                                    << 16);
+              else
+                e = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                    er, p + q < R.p ? off : kNoLoad, 0, 0));
+              dot = fmaf(out[pb][q], e, dot);
+            }
+          }
+          dot = sum_groups(dot);
+          if (g == 0 && t < have)
+            R.dots[((long)(tile * a.B + b) * a.H + h) * a.T + t0 + t] = dot;
+          // The token's own term, which the dots leave out.
+          const float own_score = sum_groups(diagonal);
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb)
+#pragma unroll
+            for (int i = IN - 1; i >= 0; --i) {
+              const u2 u = *reinterpret_cast<const u2*>(&sh.v[i][t * VROW + 16 * pb + 4 * g]);
+              out[pb] += own_score * f4{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
+            }
+        }
+        if (t0 + t < a.T) {
+          const bool here = t < have;
+          const long at = (((long)b * a.T + t0 + t) * a.H + h) * R.p;
+          const bool vec = (R.p & 3) == 0, f32 = R.out_f32;
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb) {
+            const int p = col0 + 16 * pb + 4 * g;
+            if (p < R.p)
+              store_out(R.out, at + p, here ? out[pb] : f4{0.f, 0.f, 0.f, 0.f}, R.p - p, f32,
+                        vec);
+          }
+        }
+      }
+    } else if constexpr (OUT) {
+      // Past the row's length: zeros.
+      for (int i = tid; i < C * TILE; i += THREADS) {
+        const long t = t0 + (i >> 6);
+        const int p = col0 + (i & 63);
+        if (t < a.T && p < R.p) {
+          const long at = (((long)b * a.T + t) * a.H + h) * R.p + p;
+          if (R.out_f32) static_cast<float*>(R.out)[at] = 0.f;
+          else static_cast<bf16_t*>(R.out)[at] = 0;
+        }
+      }
+    }
+    __syncthreads();
+    // A segment ends: its state joins the start.
+    if (OUT && (rev ? c % SEG == 0 : c % SEG == SEG - 1 || c == a.NC - 1)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            start[nt][pb][q] = fmaf(since, start[nt][pb][q], own[nt][pb][q]);
+          own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+      since = 1.f;
+    }
+  }
+
+  if constexpr (OUT) {
+    if (R.final.base && (rev ? c0 == 0 : c1 == a.NC)) {
+      float* s = R.final.base + (long)bh * R.n * R.p;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = 64 * nt + 16 * w + 4 * g + q, p = col0 + 16 * pb + r;
+            if (n < R.n && p < R.p)
+              s[(long)n * R.final.sn + (long)p * R.final.sp] = start[nt][pb][q];
+          }
+    }
+  } else {
+    const long slot = (long)(tile * a.B * a.H + bh) * a.NS + seg;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb)
+        *reinterpret_cast<f4*>(R.starts + slot * (NT * 4096) +
+                               ((nt * 4 + pb) * THREADS + tid) * 4) = own[nt][pb];
+    if (tid == 0) R.decays[slot] = since;
+  }
+}
+
+// Blocks of one (b, h) (its roles' tiles) differ by 8 in the grid: with
+// consecutive blocks on the 8 XCDs in turn they share an L2, and so the rows.
+__device__ __forceinline__ bool block_of(const Args& a, int x, int* which, int* b, int* h) {
+  const int group = x / (8 * a.blocks), rest = x - group * 8 * a.blocks;
+  const int bh = group * 8 + (rest & 7);
+  *which = rest >> 3;
+  *b = bh / a.H;
+  *h = bh - *b * a.H;
+  return bh < a.B * a.H;
+}
+
+template <typename In, int NT, bool OUT>
+__global__ __launch_bounds__(THREADS, 2) void attention_kernel(Args a) {
+  __shared__ Shared<In, NT> sh;
+  int which, b, h, i = 0;
+  if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
+  while (which >= a.role[i].tiles) which -= a.role[i++].tiles;
+  const Role& R = a.role[i];
+  // Split runs take a segment per block (blockIdx.y), others the sequence.
+  const bool split = !OUT || gridDim.y > 1;
+  const int seg = split ? (int)blockIdx.y : -1;
+  const int c0 = split ? seg * SEG : 0, c1 = split ? min(a.NC, c0 + SEG) : a.NC;
+  if constexpr (NT == 2) {
+    if (R.n <= 64) {
+      walk<In, 1, OUT>(a, R, which, b, h, c0, c1, seg, reinterpret_cast<Shared<In, 1>&>(sh));
+      return;
+    }
+  }
+  walk<In, NT, OUT>(a, R, which, b, h, c0, c1, seg, sh);
+}
+
+// Split runs: each segment's start state from the segments' own states and
+// decays, in place.  One thread per state element.
+__global__ void carry_kernel(Args a) {
+  int which, b, h, i = 0;
+  if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
+  while (which >= a.role[i].tiles) which -= a.role[i++].tiles;
+  const Role& R = a.role[i];
+  const int nts = R.n > 64 ? 2 : 1, part = blockIdx.y;  // part = (nt * 4 + pb)
+  if (part >= 4 * nts) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, r = lane & 15;
+  const int bh = b * a.H + h, nt = part >> 2, p = TILE * which + 16 * (part & 3) + r;
+  f4 x{0.f, 0.f, 0.f, 0.f};
+  if (R.initial.base) {
+    const float* s = R.initial.base + (long)bh * R.n * R.p;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = 64 * nt + 16 * w + 4 * g + q;
+      if (n < R.n && p < R.p) x[q] = s[(long)n * R.initial.sn + (long)p * R.initial.sp];
+    }
+  }
+  const long first = (long)(which * a.B * a.H + bh) * a.NS;
+  float* own = R.starts + first * (nts * 4096) + (part * THREADS + tid) * 4;
+  const float* decays = R.decays + first;
+  constexpr int AHEAD = 8;  // segments loaded together
+  for (int s0 = 0; s0 < a.NS; s0 += AHEAD) {
+    f4 l[AHEAD];
+    float d[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int s = min(s0 + k, a.NS - 1), at = R.rev ? a.NS - 1 - s : s;
+      l[k] = *reinterpret_cast<const f4*>(own + (long)at * (nts * 4096));
+      d[k] = decays[at];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (s0 + k >= a.NS) break;
+      const int at = R.rev ? a.NS - 1 - s0 - k : s0 + k;
+      *reinterpret_cast<f4*>(own + (long)at * (nts * 4096)) = x;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = fmaf(d[k], x[q], l[k][q]);
+    }
+  }
+}
+
+// d log_decay: one block per (b, h), from the last token to the first, sums
+// in float64.
+__global__ __launch_bounds__(1024) void decay_grad_kernel(DecayGrad a) {
+  __shared__ double part[16], total[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+  const int length = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const long bh = blockIdx.x, slab = (long)a.B * a.H * a.T;
+  auto block_sum = [&](double x, double* at) {
+    x = lane_double(wave_prefix(x), 63);
+    if (lane == 0) at[w] = x;
+    __syncthreads();
+    double s = 0.0;
+    for (int i = 0; i < 16; ++i) s += at[i];
+    __syncthreads();
+    return s;
+  };
+  double carry = 0.0;
+  if (a.state) {
+    const long count = (long)a.n * a.p;
+    double x = 0.0;
+    for (long i = tid; i < count; i += 1024)
+      x += (double)a.state[bh * count + i] * (double)a.d_state[bh * count + i];
+    carry = block_sum(x, total);
+  }
+  double sum = 0.0;
+  for (int end = a.T; end > 0; end -= 1024) {
+    // Thread i takes token end - 1 - i: a suffix sum is a prefix sum here.
+    const int t = end - 1 - tid;
+    double x = 0.0;
+    if (t >= 0 && t < length) {
+      for (int i = 0; i < a.tiles_q; ++i) x += (double)a.dots_q[i * slab + bh * a.T + t];
+      for (int i = 0; i < a.tiles_k; ++i) x -= (double)a.dots_k[i * slab + bh * a.T + t];
+    }
+    x = wave_prefix(x);
+    const double all = lane_double(x, 63);
+    if (lane == 0) part[w] = all;
+    __syncthreads();
+    double before = carry;
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) before += part[i];
+      carry += part[i];
+    }
+    __syncthreads();
+    x += before;
+    if (t >= 0) {
+      // No gradient past the length, nor where the decay is exactly zero.
+      const float g = t < length ? a.g[b * a.gb + t * a.gt + h] : 0.f;
+      if (t >= length || g < -2000.f) x = 0.0;
+      if (a.d_g) a.d_g[((long)b * a.T + t) * a.H + h] = (float)x;
+      sum += x;
+    }
+  }
+  if (a.head) {
+    sum = block_sum(sum, total);
+    if (tid == 0) a.head[bh] = sum;
+  }
+}
+
+__global__ void decay_heads_kernel(const double* head, int B, int H, float* d_g) {
+  const int h = blockIdx.x * blockDim.x + threadIdx.x;
+  if (h >= H) return;
+  double s = 0.0;
+  for (int b = 0; b < B; ++b) s += head[(long)b * H + h];
+  d_g[h] = (float)s;
+}
+
+// Gradients of shared heads: out[b,t,j,:] = sum over the heads h of group j
+// of part[b,t,h,:], float32 rounded once.
+template <typename Out>
+__global__ void share_sum_kernel(const float* part, long tokens, int heads, int share, int width,
+                                 Out* out) {
+  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int own = heads / share;
+  if (i >= tokens * own * width) return;
+  const int x = (int)(i % width);
+  const long row = i / width;
+  const long t = row / own;
+  const int j = (int)(row - t * own);
+  const float* p = part + ((t * heads) + (long)j * share) * width + x;
+  float s = 0.f;
+  for (int k = 0; k < share; ++k) s += p[(long)k * width];
+  if constexpr (sizeof(Out) == 2)
+    out[i] = (bf16_t)pack(s, 0.f);
+  else
+    out[i] = s;
+}
+
+// One token: S' = e^g S + k v^T, o = scale S'^T q.  The state is read and
+// written once; a block holds one (b, h), thread (row group, column quad).
+template <typename In>
+__device__ __forceinline__ float load_one(const void* p, long i) {
+  if constexpr (sizeof(In) == 2)
+    return __uint_as_float((unsigned)static_cast<const bf16_t*>(p)[i] << 16);
+  else
+    return static_cast<const float*>(p)[i];
+}
+
+template <typename In>
+__global__ __launch_bounds__(256) void step_kernel(Step a) {
+  __shared__ float q[MAX_WIDTH], k[MAX_WIDTH], v[MAX_WIDTH], part[4][MAX_WIDTH];
+  const int tid = threadIdx.x, b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+  const bool on = !a.active || a.active[b];
+  const long bh = blockIdx.x, at = bh * a.N * a.P;
+  if (tid < a.N) {
+    q[tid] = load_one<In>(a.q, b * a.qb + (h / a.q_share) * a.qh + tid);
+    k[tid] = load_one<In>(a.k, b * a.kb + (h / a.k_share) * a.kh + tid);
+  }
+  if (tid < a.P) v[tid] = load_one<In>(a.v, b * a.vb + (h / a.v_share) * a.vh + tid);
+  const float g = a.g[b * a.gb + h];
+  const float lam = expf(g);
+  __syncthreads();
+  const int lane = tid & 63, w = tid >> 6;
+  for (int p = lane; p < a.P; p += 64) {
+    float o = 0.f;
+    for (int n = w; n < a.N; n += 4) {
+      const float s = a.state[at + (long)n * a.P + p];
+      const float x = on ? fmaf(lam, s, k[n] * v[p]) : s;
+      if (on || a.new_state != a.state) a.new_state[at + (long)n * a.P + p] = x;
+      o = fmaf(q[n], x, o);
+    }
+    part[w][p] = o;
+  }
+  __syncthreads();
+  if (tid < a.P) {
+    const float o =
+        on ? a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])) : 0.f;
+    if constexpr (sizeof(In) == 2)
+      static_cast<bf16_t*>(a.out)[bh * a.P + tid] = (bf16_t)pack(o, 0.f);
+    else
+      static_cast<float*>(a.out)[bh * a.P + tid] = o;
+  }
+}
+
+#define LA_INSTANCES(In)                                          \
+  template __global__ void attention_kernel<In, 1, true>(Args);   \
+  template __global__ void attention_kernel<In, 1, false>(Args);  \
+  template __global__ void attention_kernel<In, 2, true>(Args);   \
+  template __global__ void attention_kernel<In, 2, false>(Args);  \
+  template __global__ void step_kernel<In>(Step);                 \
+  template __global__ void share_sum_kernel<In>(const float*, long, int, int, int, In*);
+LA_INSTANCES(float)
+LA_INSTANCES(bf16_t)
+#undef LA_INSTANCES
+
+}  // namespace la

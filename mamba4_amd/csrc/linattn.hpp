@@ -1,0 +1,90 @@
+// Shapes and arguments of the decayed linear attention's kernels, shared by
+// the host entry points and linattn.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+namespace la {
+
+constexpr int C = 64;        // tokens of a chunk
+constexpr int SEG = 4;       // chunks of a segment
+constexpr int TILE = 64;     // value columns of a block
+constexpr int WAVES = 4;     // one 16-token strip of the chunk each
+constexpr int MAX_WIDTH = 128;
+constexpr int THREADS = 64 * WAVES;
+
+typedef unsigned short bf16_t;
+
+// Rows [B,T,h,W] of one operand: unit stride along W, element strides along
+// the others, `share` attention heads to each of its own, `vec` consecutive
+// elements that may be loaded at once.
+struct Rows {
+  const void* base;
+  long sb, st, sh;
+  int share, width, vec;
+};
+
+// States [B,H,.,.] float32 with element strides of the key and value axes
+// (a transposed state swaps them); NULL: zeros, or not wanted.
+struct States {
+  float* base;
+  int sn, sp;
+};
+
+// One linear attention over the tokens (in reverse, if rev): scores q.k,
+// values v, state [n, p] with n the width of q and k and p that of v.
+//   out_i = intra * sum_j D_ij (q_i.k_j) v_j + inter * E_i q_i^T S
+//   S'    = D_L S + update * sum_j F_j k_j v_j^T
+struct Role {
+  Rows q, k, v;
+  States initial, final;
+  void* out;           // [B,T,H,p] contiguous
+  int out_f32;         // out is float32 (else the operands' type)
+  int rev;
+  float intra, inter, update;
+  Rows e;              // dots_i = (out_i less its term j = i) . e_i over the
+                       // tile's columns, if dots
+  float* dots;         // [tiles][B,H,T], or NULL
+  int n, p, tiles;
+  float* starts;       // split runs: [tiles][B*H][NS][NT * 4096] segment states
+  float* decays;       // split runs: [tiles][B*H][NS]
+};
+
+struct Args {
+  Role role[3];
+  int roles, blocks;       // blocks of one (b, h): the roles' tiles together
+  const float* g;          // log decays, element strides gb, gt (zero: per head)
+  long gb, gt;
+  const int* lengths;      // [B], or NULL
+  int B, T, H, NC, NS;
+};
+
+// d log_decay from the roles' dots.
+struct DecayGrad {
+  const float *dots_q, *dots_k;  // [tiles_q / tiles_k][B,H,T]
+  int tiles_q, tiles_k;
+  const float *g;
+  long gb, gt;
+  const int* lengths;
+  const float *state, *d_state;  // [B,H,n,p], or both NULL
+  int n, p;
+  float* d_g;                    // [B,T,H], or NULL
+  double* head;                  // [B,H] sums over the tokens, or NULL
+  int B, T, H;
+};
+
+struct Step {
+  const void *q, *k, *v;
+  long qb, qh, kb, kh, vb, vh;
+  int q_share, k_share, v_share;
+  const float* g;
+  long gb;
+  const unsigned char* active;   // [B], or NULL
+  const float* state;
+  float* new_state;
+  void* out;
+  float scale;
+  int B, H, N, P;
+};
+
+}  // namespace la
