@@ -1,8 +1,9 @@
 /*
  * mamba4_retention.h -- C ABI of the MI355X (gfx950) retention layer's
  * operators: decayed linear attention over prompts and training batches, its
- * gradient, and its step for single tokens (the library that also holds
- * mamba4_memread.h).
+ * gradient, and its step for single tokens; group normalisation with an
+ * activation or a gate; the scaled embedding lookup (the library that also
+ * holds mamba4_memread.h).
  *
  * Plain pointers and sizes only; every buffer is on the device and owned by
  * the caller.  `stream` is a hipStream_t passed as void* (NULL = the null
@@ -89,6 +90,56 @@ int m4rt_attention_step(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows*
                         const float* log_decay, int per_token, const uint8_t* active, float scale,
                         int B, int H, const float* state, float* new_state, void* output,
                         void* stream);
+
+#define M4RT_NONE 0
+#define M4RT_SILU 1
+#define M4RT_GELU 2 /* z Phi(z), by the error function */
+
+/*
+ * Group normalisation, channels last: x [M,L,C] in float32, or bfloat16 if
+ * `bf16` is not zero; G groups of C/G channels.  Over a sample's L positions and
+ * a group's channels n = (x - mean) / sqrt(variance + eps);
+ * z = n weight + bias (weight, bias float32 [C], or NULL: ones, zeros).
+ * output [M,L,C] in x's type: act(z), or z act(gate) with a gate [M,L,C] in x's
+ * type (NULL: none).  stats: [M][G][2] float32, mean and 1 / sqrt(variance +
+ * eps), for the gradient (NULL: not wanted).  Statistics and sums are float32, the
+ * variance about the mean.
+ */
+size_t m4rt_norm_workspace_bytes(long M, int L, int C, int G, int bf16, int backward);
+int m4rt_norm_forward(const void* x, const float* weight, const float* bias, const void* gate,
+                      int bf16, long M, int L, int C, int G, int activation, float eps,
+                      void* output, float* stats, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
+ * Its gradient, from d_output [M,L,C] in x's type and the forward's stats: d_x and
+ * d_gate (with a gate) in x's type, d_weight and d_bias float32 [C], each NULL if
+ * not wanted.
+ */
+int m4rt_norm_backward(const void* x, const float* weight, const float* bias, const void* gate,
+                       const void* d_output, const float* stats, int bf16, long M, int L, int C,
+                       int G, int activation, float eps, void* d_x, float* d_weight,
+                       float* d_bias, void* d_gate, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * Embedding: output [n,width] = scale * table[ids[i]], float32 or bfloat16 each;
+ * table [rows,width].  ids int32, or int64 if `ids_int64`.  An id outside
+ * 0..rows-1 (-1 for padding, say) gives a row of zeros.
+ */
+int m4rt_embedding_forward(const void* ids, int ids_int64, const void* table, int table_bf16,
+                           long n, int rows, int width, float scale, void* output,
+                           int output_bf16, void* stream);
+
+/*
+ * Its gradient: d_table [rows,width] = scale * the sums of d_output's rows by
+ * id, every row written (ids outside the table add to none).  Sums are float32 in a
+ * fixed order and rounded once.
+ */
+size_t m4rt_embedding_workspace_bytes(long n, int rows, int width);
+int m4rt_embedding_backward(const void* ids, int ids_int64, const void* d_output, int output_bf16,
+                            long n, int rows, int width, float scale, void* d_table,
+                            int table_bf16, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

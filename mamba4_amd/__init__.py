@@ -9,7 +9,8 @@ implemented by hand-written HIP kernels behind the C ABI in
 (``memory_inputs``, ``gated_read``; lm/models/mamba4.py:183-237, 266-273)
 and the order head's gated scan (``order_memory_chunked``, ``order_memory``;
 lm/models/mamba4.py:46-95).  Beside them, the retention layer's operators
-(``linear_attention``, ``linear_attention_step``).
+(``linear_attention``, ``linear_attention_step``, ``group_norm``,
+``embedding``).
 """
 
 from mamba4_amd.attention import (  # noqa: F401
@@ -37,7 +38,9 @@ from mamba4_amd.mixer import (  # noqa: F401
     memory_inputs,
     mixer_read,
 )
+from mamba4_amd.embedding import embedding  # noqa: F401
 from mamba4_amd.flashmamba import mamba3_fused  # noqa: F401
+from mamba4_amd.norm import group_norm  # noqa: F401
 from mamba4_amd.order import order_memory, order_memory_chunked  # noqa: F401
 
 __all__ = [
@@ -48,11 +51,13 @@ __all__ = [
     "SOLVERS",
     "SelectiveResult",
     "SelectiveState",
+    "embedding",
     "linear_attention",
     "linear_attention_step",
     "linear_attention_step_",
     "mamba3_fused",
     "gated_read",
+    "group_norm",
     "memory_inputs",
     "mixer_read",
     "order_memory",

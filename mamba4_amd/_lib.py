@@ -147,6 +147,13 @@ SIGNATURES = {
         _I, [_R] * 3 + [_I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 9 + [_S, _P]),
     "m4rt_attention_step": (
         _I, [_R] * 3 + [_I, _P, _I, _P, _F] + [_I] * 2 + [_P] * 3 + [_P]),
+    "m4rt_norm_workspace_bytes": (_S, [_L] + [_I] * 5),
+    "m4rt_norm_forward": (_I, [_P] * 4 + [_I, _L] + [_I] * 4 + [_F] + [_P] * 3 + [_S, _P]),
+    "m4rt_norm_backward": (_I, [_P] * 6 + [_I, _L] + [_I] * 4 + [_F] + [_P] * 5 + [_S, _P]),
+    "m4rt_embedding_forward": (_I, [_P, _I, _P, _I, _L, _I, _I, _F, _P, _I, _P]),
+    "m4rt_embedding_workspace_bytes": (_S, [_L, _I, _I]),
+    "m4rt_embedding_backward": (
+        _I, [_P, _I, _P, _I, _L, _I, _I, _F, _P, _I, _P, _S, _P]),
     "m4mr_profile_enable": (None, [_I]),
     "m4mr_profile_select": (None, [ctypes.c_char_p]),
     "m4mr_profile_reset": (None, []),

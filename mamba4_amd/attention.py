@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.memory import _ptr, _require_device, _stream
+from mamba4_amd.memory import _ptr, _stream
 
 MAX_WIDTH = 128
 _MAX_TOKEN_STRIDE = (2**31 - 1) // 256
@@ -145,10 +145,10 @@ def _model_rows(name, queries, keys, values, dims):
 
 
 def _same_device(*tensors):
-    _require_device(*tensors)
     devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"all tensors must be on one device; got {sorted(map(str, devices))}")
+    if len(devices) > 1 or any(d.type != "cuda" for d in devices):
+        raise ValueError("all tensors must be ROCm device tensors on one device; got "
+                         + ", ".join(sorted(map(str, devices))))
 
 
 def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=None, scale=1.0):

@@ -20,7 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBRARY = os.path.join(HERE, "libmamba4_memread.so")
 SOURCES = ["api.hip", "states.hip", "factor.hip", "chunk.hip", "mixer.hip", "order.hip",
            "scan3.hip", "diag.hip", "spd_wide.hip", "resize.hip", "api_retention.hip",
-           "linattn.hip"]
+           "linattn.hip", "norm.hip", "embed.hip"]
 ARCH = "gfx950"
 
 FLAGS = [

@@ -1,12 +1,16 @@
 // C ABI of the retention layer's operators (include/mamba4_retention.h): the
 // checks of the arguments and the launches.
+#include <algorithm>
 #include <climits>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/mamba4_retention.h"
 #include "api_common.hpp"
+#include "embed.hpp"
 #include "linattn.hpp"
+#include "norm.hpp"
 
 namespace la {
 template <typename In, int NT, bool OUT>
@@ -19,6 +23,25 @@ __global__ void share_sum_kernel(const float*, long, int, int, int, Out*);
 template <typename In>
 __global__ void step_kernel(Step);
 }  // namespace la
+
+namespace gn {
+template <typename In, int V, int IT, bool BWD>
+__global__ void norm_rows_kernel(Norm);
+template <typename In, int V, bool BWD, int PHASE>
+__global__ void norm_positions_kernel(Norm);
+__global__ void norm_columns_kernel(const float*, int, int, float*, float*);
+}  // namespace gn
+
+namespace em {
+template <typename In, typename Out, int V>
+__global__ void lookup_kernel(Lookup);
+__global__ void count_kernel(Sort, unsigned*, Clear);
+__global__ void scatter_kernel(Sort);
+template <typename In, typename Out, int V>
+__global__ void sum_kernel(Sum, unsigned);
+template <typename Out, int V>
+__global__ void join_kernel(Sum);
+}  // namespace em
 
 namespace {
 
@@ -406,6 +429,468 @@ int m4rt_attention_step(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows*
         hipLaunchKernelGGL(la::step_kernel<la::bf16_t>, dim3(B * H), dim3(256), 0, st, a);
       else
         hipLaunchKernelGGL(la::step_kernel<float>, dim3(B * H), dim3(256), 0, st, a);
+    });
+  });
+}
+
+}  // extern "C"
+
+// -------------------------------------------------------------- group norm --
+
+namespace {
+
+bool bad_norm(long M, int L, int C, int G, int act, std::string* why) {
+  if (M <= 0 || L <= 0 || C <= 0 || G <= 0 || C % G) {
+    *why = "M, L and C must be positive and G must divide C";
+    return true;
+  }
+  if ((double)M * L * C > 1e15 || (long)L * C > INT_MAX || C > 1 << 23) {
+    *why = "problem too large";
+    return true;
+  }
+  if (act < gn::NONE || act > gn::GELU) {
+    *why = "unknown activation";
+    return true;
+  }
+  return false;
+}
+
+// Widest piece, in elements, that the channels of a group and the arrays'
+// addresses allow.
+int norm_vec(int D, int bf16, std::initializer_list<const void*> arrays) {
+  uintptr_t at = 0;
+  for (const void* p : arrays) at |= reinterpret_cast<uintptr_t>(p);
+  const int size = bf16 ? 2 : 4;
+  int vec = 16 / size;
+  while (vec > 1 && (D % vec || at % (vec * size))) vec >>= 1;
+  return vec;
+}
+
+// The route of a call: groups within a wave (one position, at most IT pieces a
+// lane), or blocks over positions.  Grids depend on the sizes and the card.
+struct NormPlan {
+  int vec, pieces;  // pieces a lane holds; 0: position kernels
+  dim3 grid;
+  int threads, part_rows;
+  size_t sums;      // floats of the position kernels' partial statistics
+};
+
+NormPlan norm_plan(long M, int L, int C, int G, int vec, gn::Norm* a) {
+  NormPlan p{};
+  p.vec = vec;
+  a->M = M;
+  a->L = L;
+  a->C = C;
+  a->G = G;
+  a->D = C / G;
+  const int vecs = a->D / vec, cus = m4::api_compute_units();
+  if (L == 1) {
+    // Fewest idle lanes, then fewest pieces; at most 16 elements a lane.
+    int best = 0;
+    for (int lanes = 64; lanes >= 1; lanes >>= 1) {
+      int pieces = (vecs + lanes - 1) / lanes;
+      if (pieces == 3) pieces = 4;
+      if (pieces > 4 || pieces * vec > 16) break;
+      if (best == 0 || lanes * pieces < a->lanes * best) {
+        a->lanes = lanes;
+        best = pieces;
+      }
+    }
+    if (best) {
+      p.pieces = best;
+      a->groups = std::min(G, gn::ROW_THREADS / a->lanes);
+      const int across = a->groups * a->lanes;
+      a->rows = (int)std::min<long>(gn::ROW_THREADS / across, M);
+      p.threads = (a->rows * across + 63) / 64 * 64;
+      const long most = (M + a->rows - 1) / a->rows;
+      p.grid = dim3((unsigned)std::min<long>(most, 4L * cus), (G + a->groups - 1) / a->groups);
+      p.part_rows = (int)p.grid.x;
+      return p;
+    }
+  }
+  a->vecs = vecs;
+  a->subs = (vecs + gn::POS_THREADS - 1) / gn::POS_THREADS;
+  a->span = a->subs > 1 ? 1 : std::min(G, gn::POS_THREADS / vecs);
+  a->rows = a->subs > 1 ? 1 : std::max(1, std::min(L, gn::POS_THREADS / (vecs * a->span)));
+  const int slots = (G * a->subs + a->span - 1) / a->span;
+  // Enough blocks for the card, each with some rows for each thread.
+  const long want = (4L * cus + M * slots - 1) / (M * slots);
+  a->blocks = (int)std::max<long>(1, std::min<long>(want, L / (8L * a->rows)));
+  if (a->subs > 1 && a->blocks == 1) a->blocks = std::min(L, 2);
+  const bool whole = a->blocks == 1 && a->subs == 1;
+  // Blocks walk over samples past these (the column sums have a part for each).
+  const long samples = std::min<long>(M, std::max(1L, 8L * cus / ((long)slots * a->blocks)));
+  p.grid = dim3(a->blocks, (unsigned)samples, slots);
+  p.threads = gn::POS_THREADS;
+  p.part_rows = (int)samples * a->blocks;
+  p.sums = whole ? 0 : (size_t)M * a->blocks * a->subs * G * 4;
+  return p;
+}
+
+template <typename In, int V, int IT, bool BWD>
+void start_rows(const gn::Norm& a, const NormPlan& p, hipStream_t st) {
+  if constexpr (V * IT <= 16)
+    hipLaunchKernelGGL((gn::norm_rows_kernel<In, V, IT, BWD>), p.grid, dim3(p.threads), 0, st, a);
+}
+
+template <typename In, int V, bool BWD>
+void start_norm(const gn::Norm& a, const NormPlan& p, int phase, hipStream_t st) {
+  if (p.pieces == 1) return start_rows<In, V, 1, BWD>(a, p, st);
+  if (p.pieces == 2) return start_rows<In, V, 2, BWD>(a, p, st);
+  if (p.pieces == 4) return start_rows<In, V, 4, BWD>(a, p, st);
+  const dim3 block(p.threads);
+  if (phase == gn::SUMS)
+    hipLaunchKernelGGL((gn::norm_positions_kernel<In, V, BWD, gn::SUMS>), p.grid, block, 0, st, a);
+  else if (phase == gn::APPLY)
+    hipLaunchKernelGGL((gn::norm_positions_kernel<In, V, BWD, gn::APPLY>), p.grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((gn::norm_positions_kernel<In, V, BWD, gn::BOTH>), p.grid, block, 0, st, a);
+}
+
+template <bool BWD>
+void launch_norm(const gn::Norm& a, const NormPlan& p, int bf16, int phase, hipStream_t st) {
+  if (bf16) {
+    if (p.vec == 8) return start_norm<gn::bf16_t, 8, BWD>(a, p, phase, st);
+    if (p.vec == 4) return start_norm<gn::bf16_t, 4, BWD>(a, p, phase, st);
+    if (p.vec == 2) return start_norm<gn::bf16_t, 2, BWD>(a, p, phase, st);
+    return start_norm<gn::bf16_t, 1, BWD>(a, p, phase, st);
+  }
+  if (p.vec == 4) return start_norm<float, 4, BWD>(a, p, phase, st);
+  if (p.vec == 2) return start_norm<float, 2, BWD>(a, p, phase, st);
+  return start_norm<float, 1, BWD>(a, p, phase, st);
+}
+
+template <bool BWD>
+int run_norm(const gn::Norm& a, const NormPlan& p, int bf16, hipStream_t st) {
+  const char* name = BWD ? "norm_backward" : "norm";
+  if (p.pieces || p.sums == 0)
+    return api_launch(name, st, [&] { launch_norm<BWD>(a, p, bf16, gn::BOTH, st); });
+  int rc = api_launch(BWD ? "norm_backward_sums" : "norm_sums", st,
+                      [&] { launch_norm<BWD>(a, p, bf16, gn::SUMS, st); });
+  if (rc) return rc;
+  return api_launch(name, st, [&] { launch_norm<BWD>(a, p, bf16, gn::APPLY, st); });
+}
+
+bool misaligned(int bf16, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % (bf16 ? 2 : 4)) return true;
+  return false;
+}
+
+// The largest workspace over the widths of the pieces, which depend on
+// addresses.
+size_t norm_workspace(long M, int L, int C, int G, int bf16, bool backward) {
+  size_t most = 0;
+  for (int vec = bf16 ? 8 : 4; vec >= 1; vec >>= 1) {
+    if ((C / G) % vec) continue;
+    gn::Norm a{};
+    const NormPlan p = norm_plan(M, L, C, G, vec, &a);
+    const size_t part = backward ? align256((size_t)p.part_rows * 2 * C * sizeof(float)) : 0;
+    most = std::max(most, part + align256(p.sums * sizeof(float)));
+  }
+  return most;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t m4rt_norm_workspace_bytes(long M, int L, int C, int G, int bf16, int backward) {
+  std::string why;
+  if (bad_norm(M, L, C, G, gn::NONE, &why)) return 0;
+  return norm_workspace(M, L, C, G, bf16, backward);
+}
+
+int m4rt_norm_forward(const void* x, const float* weight, const float* bias, const void* gate,
+                      int bf16, long M, int L, int C, int G, int activation, float eps, void* y,
+                      float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "m4rt_norm_forward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_norm(M, L, C, G, activation, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!x || !y)
+      return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(bf16, {x, gate, y}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    if (bad_workspace(workspace, workspace_bytes, norm_workspace(M, L, C, G, bf16, false), &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    gn::Norm a{};
+    const NormPlan p = norm_plan(M, L, C, G, norm_vec(C / G, bf16, {x, gate, y}), &a);
+    a.x = x;
+    a.gate = gate;
+    a.weight = weight;
+    a.bias = bias;
+    a.y = y;
+    a.eps = eps;
+    a.act = activation;
+    a.stats = stats;
+    a.sums = static_cast<float*>(workspace);
+    return run_norm<false>(a, p, bf16, static_cast<hipStream_t>(stream));
+  });
+}
+
+int m4rt_norm_backward(const void* x, const float* weight, const float* bias, const void* gate,
+                       const void* d_output, const float* stats, int bf16, long M, int L, int C,
+                       int G, int activation, float eps, void* d_x, float* d_weight, float* d_bias,
+                       void* d_gate, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "m4rt_norm_backward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_norm(M, L, C, G, activation, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!x || !d_output || !d_x || !stats || (gate && !d_gate))
+      return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(bf16, {x, gate, d_output, d_x, d_gate}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    if (bad_workspace(workspace, workspace_bytes, norm_workspace(M, L, C, G, bf16, true), &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    gn::Norm a{};
+    const NormPlan p =
+        norm_plan(M, L, C, G, norm_vec(C / G, bf16, {x, gate, d_output, d_x, d_gate}), &a);
+    Carver c{static_cast<char*>(workspace)};
+    const bool columns = d_weight || d_bias;
+    a.x = x;
+    a.gate = gate;
+    a.dy = d_output;
+    a.weight = weight;
+    a.bias = bias;
+    a.dx = d_x;
+    a.dgate = gate ? d_gate : nullptr;
+    a.eps = eps;
+    a.act = activation;
+    a.stats = const_cast<float*>(stats);
+    float* part = c.take<float>((size_t)p.part_rows * 2 * C);
+    a.part = columns ? part : nullptr;
+    a.sums = c.take<float>(p.sums);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int rc = run_norm<true>(a, p, bf16, st);
+    if (rc || !columns) return rc;
+    return api_launch("norm_columns", st, [&] {
+      hipLaunchKernelGGL(gn::norm_columns_kernel, dim3((2 * C + 63) / 64), dim3(1024), 0, st, part,
+                         p.part_rows, C, d_weight, d_bias);
+    });
+  });
+}
+
+}  // extern "C"
+
+// --------------------------------------------------------------- embedding --
+
+namespace {
+
+bool bad_embedding(long n, int rows, int width, std::string* why) {
+  if (n <= 0 || rows <= 0 || width <= 0) {
+    *why = "the tokens, rows and width must be positive";
+    return true;
+  }
+  if (n > INT_MAX - (1 << 24) || rows > INT_MAX - 1 || (double)n * width > 1e12 ||
+      (double)rows * width > 1e12) {
+    *why = "problem too large";
+    return true;
+  }
+  return false;
+}
+
+int embedding_vec(int width, std::initializer_list<const void*> arrays) {
+  uintptr_t at = 0;
+  for (const void* p : arrays) at |= reinterpret_cast<uintptr_t>(p);
+  int vec = 8;
+  // 16-byte pieces of bfloat16, two of float32.
+  while (vec > 1 && (width % vec || at % std::min(16, 4 * vec))) vec >>= 1;
+  return vec;
+}
+
+// The backward's sort and chunks, and its workspace.
+struct EmbeddingPlan {
+  int passes, bits, tile, tiles, chunk, chunks;
+  unsigned* counts[4];
+  unsigned char* present;
+  unsigned *keys[2], *tokens[2];
+  float *head, *tail;
+  size_t cleared;  // words from counts[1] on that the passes add up
+};
+
+size_t embedding_plan(long n, int rows, int width, void* base, EmbeddingPlan* p) {
+  int bits = 1;
+  while (bits < 32 && (unsigned)rows >> bits) ++bits;  // keys are 0..rows
+  p->passes = (bits + em::MAX_DIGIT - 1) / em::MAX_DIGIT;
+  p->bits = (bits + p->passes - 1) / p->passes;
+  // Every tile reads all tiles' counts: at most 128 of them.
+  p->tile = 2048;
+  while ((n + p->tile - 1) / p->tile > 128) p->tile *= 2;
+  p->tiles = (int)((n + p->tile - 1) / p->tile);
+  // Short chunks fill the card, long ones leave fewer parts to join.
+  p->chunk = n >= 65536 ? 32 : 16;
+  p->chunks = (int)((n + p->chunk - 1) / p->chunk);
+  Carver c{static_cast<char*>(base)};
+  size_t first = 0;
+  for (int i = 0; i < p->passes; ++i) {
+    p->counts[i] = c.take<unsigned>((size_t)p->tiles << p->bits);
+    if (i == 0) first = c.used;
+  }
+  p->present = c.take<unsigned char>(rows);
+  p->cleared = (c.used - first) / sizeof(unsigned);
+  for (int i = 0; i < 2; ++i) {
+    p->keys[i] = c.take<unsigned>(n);
+    p->tokens[i] = c.take<unsigned>(n);
+  }
+  p->head = c.take<float>((size_t)p->chunks * width);
+  p->tail = c.take<float>((size_t)p->chunks * width);
+  return c.used;
+}
+
+template <typename In, typename Out, int V>
+void start_lookup(const em::Lookup& a, hipStream_t st) {
+  const long items = a.n * (a.width / V);
+  hipLaunchKernelGGL((em::lookup_kernel<In, Out, V>),
+                     dim3((unsigned)((items + 4 * em::THREADS - 1) / (4 * em::THREADS))),
+                     dim3(em::THREADS), 0, st, a);
+}
+
+template <int V>
+void launch_lookup(const em::Lookup& a, int table_bf16, int out_bf16, hipStream_t st) {
+  if (table_bf16)
+    out_bf16 ? start_lookup<em::bf16_t, em::bf16_t, V>(a, st)
+             : start_lookup<em::bf16_t, float, V>(a, st);
+  else
+    out_bf16 ? start_lookup<float, em::bf16_t, V>(a, st) : start_lookup<float, float, V>(a, st);
+}
+
+template <typename In, typename Out, int V>
+void start_sums(const em::Sum& a, hipStream_t st) {
+  const long vecs = a.width / V, sums = (a.chunks * vecs + em::THREADS - 1) / em::THREADS;
+  const long zeros = (a.rows * vecs + 4 * em::THREADS - 1) / (4 * em::THREADS);
+  hipLaunchKernelGGL((em::sum_kernel<In, Out, V>), dim3((unsigned)(sums + zeros)),
+                     dim3(em::THREADS), 0, st, a, (unsigned)sums);
+}
+
+template <int V>
+void launch_sums(const em::Sum& a, int table_bf16, int out_bf16, hipStream_t st) {
+  if (table_bf16)
+    out_bf16 ? start_sums<em::bf16_t, em::bf16_t, V>(a, st)
+             : start_sums<float, em::bf16_t, V>(a, st);
+  else
+    out_bf16 ? start_sums<em::bf16_t, float, V>(a, st) : start_sums<float, float, V>(a, st);
+}
+
+template <int V>
+void launch_join(const em::Sum& a, int table_bf16, hipStream_t st) {
+  const dim3 grid((unsigned)(((long)a.chunks * (a.width / V) + em::THREADS - 1) / em::THREADS));
+  if (table_bf16)
+    hipLaunchKernelGGL((em::join_kernel<em::bf16_t, V>), grid, dim3(em::THREADS), 0, st, a);
+  else
+    hipLaunchKernelGGL((em::join_kernel<float, V>), grid, dim3(em::THREADS), 0, st, a);
+}
+
+#define EM_BY_VEC(vec, call)                 \
+  do {                                       \
+    if ((vec) == 8) call<8> EM_ARGS;         \
+    else if ((vec) == 4) call<4> EM_ARGS;    \
+    else if ((vec) == 2) call<2> EM_ARGS;    \
+    else call<1> EM_ARGS;                    \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int m4rt_embedding_forward(const void* ids, int ids_int64, const void* table, int table_bf16,
+                           long n, int rows, int width, float scale, void* output, int output_bf16,
+                           void* stream) {
+  const char* name = "m4rt_embedding_forward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_embedding(n, rows, width, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!ids || !table || !output)
+      return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(table_bf16, {table}) || misaligned(output_bf16, {output}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    const em::Lookup a{ids, ids_int64, table, output, n, rows, width, scale};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int vec = embedding_vec(width, {table, output});
+    return api_launch("embedding", st, [&] {
+#define EM_ARGS (a, table_bf16, output_bf16, st)
+      EM_BY_VEC(vec, launch_lookup);
+#undef EM_ARGS
+    });
+  });
+}
+
+size_t m4rt_embedding_workspace_bytes(long n, int rows, int width) {
+  std::string why;
+  if (bad_embedding(n, rows, width, &why)) return 0;
+  EmbeddingPlan p{};
+  return embedding_plan(n, rows, width, nullptr, &p);
+}
+
+int m4rt_embedding_backward(const void* ids, int ids_int64, const void* d_output, int output_bf16,
+                            long n, int rows, int width, float scale, void* d_table,
+                            int table_bf16, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  const char* name = "m4rt_embedding_backward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_embedding(n, rows, width, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!ids || !d_output || !d_table)
+      return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(table_bf16, {d_table}) || misaligned(output_bf16, {d_output}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    EmbeddingPlan p{};
+    if (bad_workspace(workspace, workspace_bytes, embedding_plan(n, rows, width, workspace, &p),
+                      &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    em::Sort sort{};
+    sort.ids = ids;
+    sort.wide = ids_int64;
+    sort.n = n;
+    sort.rows = rows;
+    sort.tile = p.tile;
+    sort.tiles = p.tiles;
+    sort.bits = p.bits;
+    const em::Clear clear{reinterpret_cast<unsigned*>(p.passes > 1
+                                                          ? reinterpret_cast<char*>(p.counts[1])
+                                                          : reinterpret_cast<char*>(p.present)),
+                          (long)p.cleared};
+    int rc = api_launch("embedding_count", st, [&] {
+      hipLaunchKernelGGL(em::count_kernel, dim3(p.tiles), dim3(em::THREADS), 0, st, sort,
+                         p.counts[0], clear);
+    });
+    if (rc) return rc;
+    for (int i = 0; i < p.passes; ++i) {
+      const bool last = i + 1 == p.passes;
+      sort.keys = i ? p.keys[(i - 1) & 1] : nullptr;
+      sort.tokens = i ? p.tokens[(i - 1) & 1] : nullptr;
+      sort.out_keys = p.keys[i & 1];
+      sort.out_tokens = p.tokens[i & 1];
+      sort.counts = p.counts[i];
+      sort.next = last ? nullptr : p.counts[i + 1];
+      sort.present = last ? p.present : nullptr;
+      sort.shift = i * p.bits;
+      sort.next_shift = sort.shift + p.bits;
+      sort.next_bits = p.bits;
+      rc = api_launch("embedding_scatter", st, [&] {
+        hipLaunchKernelGGL(em::scatter_kernel, dim3(p.tiles), dim3(em::THREADS), 0, st, sort);
+      });
+      if (rc) return rc;
+    }
+    const int sorted = (p.passes - 1) & 1;
+    const em::Sum sum{p.keys[sorted], p.tokens[sorted], p.present, d_output, d_table,
+                      p.head, p.tail, n, rows, width, p.chunk, p.chunks, scale};
+    const int vec = embedding_vec(width, {d_output, d_table});
+    rc = api_launch("embedding_sums", st, [&] {
+#define EM_ARGS (sum, table_bf16, output_bf16, st)
+      EM_BY_VEC(vec, launch_sums);
+#undef EM_ARGS
+    });
+    if (rc) return rc;
+    return api_launch("embedding_join", st, [&] {
+#define EM_ARGS (sum, table_bf16, st)
+      EM_BY_VEC(vec, launch_join);
+#undef EM_ARGS
     });
   });
 }

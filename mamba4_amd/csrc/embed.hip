@@ -1,0 +1,339 @@
+// Embedding lookup with a scale, and its gradient by sorted tokens, for gfx950.
+//
+//   out_i = scale table[id_i],   dtable[r] = scale * sum of dy_i over id_i = r.
+// An id outside the table gives a zero row and adds to none.
+//
+// The lookup moves rows in 16-byte pieces.  The gradient sorts the tokens by
+// id (stable, so that a row's terms are added in the order of the tokens and the
+// bits are the same on every run), then cuts the sorted tokens into chunks of
+// equal length, however often an id occurs: each chunk sums its runs of equal
+// ids in float32 and stores the rows that begin and end in it; parts of rows
+// that span chunks are joined by a last kernel in order.  Rows of ids that do
+// not occur are zeroed by the same launch as the sums.
+//
+// Sort: passes of at most 9 bits over tiles of tokens.  A pass's tile counts are
+// complete before it starts (the first pass's by the counting kernel, the next
+// one's added up by the scatter before it, integers, so in any order); each
+// tile sums the counts that precede it itself, which spares the scans their own
+// launches.
+#include <hip/hip_runtime.h>
+
+#include "embed.hpp"
+
+namespace em {
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ unsigned pack(float a, float b) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
+}
+__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+// V consecutive elements, read as float32 and rounded as they are stored.
+template <int V>
+__device__ __forceinline__ void read(const float* p, float (&v)[V]) {
+  typedef float raw __attribute__((ext_vector_type(V)));
+  const raw r = *reinterpret_cast<const raw*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = r[i];
+}
+template <int V>
+__device__ __forceinline__ void read(const bf16_t* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = __uint_as_float((unsigned)*p << 16);
+  } else {
+    typedef unsigned raw __attribute__((ext_vector_type(V / 2)));
+    const raw r = *reinterpret_cast<const raw*>(p);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      v[i] = low(r[i / 2]);
+      v[i + 1] = high(r[i / 2]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void write(float* p, const float (&v)[V]) {
+  typedef float raw __attribute__((ext_vector_type(V)));
+  raw r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = v[i];
+  *reinterpret_cast<raw*>(p) = r;
+}
+template <int V>
+__device__ __forceinline__ void write(bf16_t* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = (bf16_t)pack(v[0], 0.f);
+  } else {
+    typedef unsigned raw __attribute__((ext_vector_type(V / 2)));
+    raw r;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) r[i / 2] = pack(v[i], v[i + 1]);
+    *reinterpret_cast<raw*>(p) = r;
+  }
+}
+
+// The id of token i, or `rows` for one outside the table.
+__device__ __forceinline__ unsigned key_of(const void* ids, int wide, long i, int rows) {
+  const long id = wide ? static_cast<const long*>(ids)[i] : (long)static_cast<const int*>(ids)[i];
+  return id >= 0 && id < rows ? (unsigned)id : (unsigned)rows;
+}
+
+// Each thread moves four pieces, 256 apart, of the block's 1024.
+template <typename In, typename Out, int V>
+__global__ __launch_bounds__(THREADS) void lookup_kernel(Lookup a) {
+  const int vecs = a.width / V;
+  const long first = (long)blockIdx.x * (4 * THREADS), row0 = first / vecs;
+  const unsigned rest = (unsigned)(first - row0 * vecs);
+  const In* table = static_cast<const In*>(a.table);
+  Out* out = static_cast<Out*>(a.out);
+  float x[4][V];
+  long at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned item = rest + threadIdx.x + THREADS * j, step = item / vecs;
+    const unsigned v = item - step * vecs;
+    const long i = row0 + step;
+    at[j] = i < a.n ? i * a.width + v * V : -1;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[j][e] = 0.f;
+    if (i < a.n) {
+      const unsigned key = key_of(a.ids, a.wide, i, a.rows);
+      if (key < (unsigned)a.rows) read<V>(table + (long)key * a.width + v * V, x[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (at[j] < 0) continue;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[j][e] *= a.scale;
+    write<V>(out + at[j], x[j]);
+  }
+}
+
+// Tile counts of the first pass's digits; clears what the passes add up.
+__global__ __launch_bounds__(THREADS) void count_kernel(Sort a, unsigned* counts, Clear clear) {
+  __shared__ unsigned bins[BINS];
+  const int size = 1 << a.bits;
+  for (int d = threadIdx.x; d < size; d += THREADS) bins[d] = 0;
+  for (long i = (long)blockIdx.x * THREADS + threadIdx.x; i < clear.count;
+       i += (long)gridDim.x * THREADS)
+    clear.words[i] = 0;
+  __syncthreads();
+  const long first = (long)blockIdx.x * a.tile;
+  for (int k = threadIdx.x; k < a.tile; k += THREADS)
+    if (first + k < a.n) {
+      const unsigned key = key_of(a.ids, a.wide, first + k, a.rows);
+      atomicAdd(&bins[(key >> a.shift) & (size - 1)], 1u);
+    }
+  __syncthreads();
+  for (int d = threadIdx.x; d < size; d += THREADS) counts[(long)blockIdx.x * size + d] = bins[d];
+}
+
+// Lanes whose digit is this lane's, among the lanes that have one.
+__device__ __forceinline__ unsigned long peers(unsigned digit, int bits, bool have) {
+  unsigned long mask = __ballot(have);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned long set = __ballot((digit >> b) & 1);
+    mask &= (digit >> b) & 1 ? set : ~set;
+  }
+  return mask;
+}
+
+// One pass: each wave ranks a quarter of the tile in order, 64 pairs at a
+// time; equal digits keep their order.
+__global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
+  __shared__ unsigned place[THREADS / 64][BINS], total[2][BINS], before[BINS];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, size = 1 << a.bits;
+  for (int d = tid; d < (THREADS / 64) * BINS; d += THREADS) (&place[0][0])[d] = 0;
+  for (int d = tid; d < size; d += THREADS) {
+    unsigned all = 0, mine = 0;
+#pragma unroll 8
+    for (int t = 0; t < a.tiles; ++t) {
+      const unsigned c = a.counts[(long)t * size + d];
+      all += c;
+      mine += t < (int)blockIdx.x ? c : 0;
+    }
+    total[0][d] = all;
+    before[d] = mine;
+  }
+  __syncthreads();
+  const long first = (long)blockIdx.x * a.tile + w * (a.tile / 4);
+  const unsigned long below = (1ul << lane) - 1;
+  auto fetch = [&](int k, bool* have) {
+    const long i = first + k + lane;
+    *have = i < a.n;
+    if (!*have) return 0u;
+    return a.keys ? a.keys[i] : key_of(a.ids, a.wide, i, a.rows);
+  };
+  for (int k = 0; k < a.tile / 4; k += 64) {
+    bool have;
+    const unsigned digit = (fetch(k, &have) >> a.shift) & (size - 1);
+    const unsigned long mask = peers(digit, a.bits, have);
+    if (have && (mask & below) == 0) place[w][digit] += __popcll(mask);
+  }
+  // Exclusive sums of the totals over the digits.
+  int from = 0;
+  for (int s = 1; s < size; s <<= 1) {
+    for (int d = tid; d < size; d += THREADS)
+      total[from ^ 1][d] = total[from][d] + (d >= s ? total[from][d - s] : 0);
+    from ^= 1;
+    __syncthreads();
+  }
+  for (int d = tid; d < size; d += THREADS) {
+    unsigned at = (d > 0 ? total[from][d - 1] : 0) + before[d];
+    for (int i = 0; i < THREADS / 64; ++i) {
+      const unsigned c = place[i][d];
+      place[i][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < a.tile / 4; k += 64) {
+    bool have;
+    const unsigned key = fetch(k, &have), digit = (key >> a.shift) & (size - 1);
+    const unsigned long mask = peers(digit, a.bits, have);
+    const unsigned rank = __popcll(mask & below);
+    if (have) {
+      const unsigned at = place[w][digit] + rank;
+      const long i = first + k + lane;
+      a.out_keys[at] = key;
+      a.out_tokens[at] = a.tokens ? a.tokens[i] : (unsigned)i;
+      if (a.next)
+        atomicAdd(&a.next[((long)(at / a.tile) << a.next_bits) +
+                          ((key >> a.next_shift) & ((1 << a.next_bits) - 1))], 1u);
+      if (a.present && key < (unsigned)a.rows) a.present[key] = 1;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (have && rank == 0) place[w][digit] += __popcll(mask);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Sums of runs: a thread takes one piece of the columns of one chunk.  The
+// blocks from `sum_blocks` on zero the rows that do not occur.
+template <typename In, typename Out, int V>
+__global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks) {
+  const int vecs = a.width / V;
+  const unsigned rows = (unsigned)a.rows;
+  Out* dw = static_cast<Out*>(a.dw);
+  if (blockIdx.x >= sum_blocks) {
+    const long first = (long)(blockIdx.x - sum_blocks) * (4 * THREADS), row0 = first / vecs;
+    const unsigned rest = (unsigned)(first - row0 * vecs);
+    const float zero[V] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned item = rest + threadIdx.x + THREADS * j, step = item / vecs;
+      const long r = row0 + step;
+      if (r < a.rows && !a.present[r]) write<V>(dw + r * a.width + (item - step * vecs) * V, zero);
+    }
+    return;
+  }
+  const long thread = (long)blockIdx.x * THREADS + threadIdx.x;
+  const long chunk = thread / vecs;
+  if (chunk >= a.chunks) return;
+  const int column = (int)(thread - chunk * vecs) * V;
+  const In* dy = static_cast<const In*>(a.dy) + column;
+  const long s = chunk * a.chunk, e = min(s + a.chunk, a.n);
+  unsigned current = a.keys[s];
+  bool from_before = s > 0 && a.keys[s - 1] == current;
+  float acc[V] = {};
+  auto store = [&](unsigned key) {
+    float x[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = a.scale * acc[i];
+    write<V>(dw + (long)key * a.width + column, x);
+  };
+  constexpr int AHEAD = 8;
+  for (long i = s; i < e; i += AHEAD) {
+    unsigned key[AHEAD];
+    float x[AHEAD][V];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      key[j] = i + j < e ? a.keys[i + j] : rows;
+      const long token = i + j < e ? a.tokens[i + j] : 0;
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[j][k] = 0.f;
+      if (key[j] < rows) read<V>(dy + token * a.width, x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (i + j < e && key[j] != current) {
+        if (from_before)
+          write<V>(a.head + chunk * a.width + column, acc);
+        else
+          store(current);
+        from_before = false;
+        current = key[j];
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += x[j][k];
+    }
+  }
+  if (current >= rows) return;
+  if (from_before)
+    write<V>(a.head + chunk * a.width + column, acc);
+  else if (e < a.n && a.keys[e] == current)
+    write<V>(a.tail + chunk * a.width + column, acc);
+  else
+    store(current);
+}
+
+// Rows whose run goes on past the chunk it begins in: its parts in order.
+template <typename Out, int V>
+__global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
+  const int vecs = a.width / V;
+  const long thread = (long)blockIdx.x * THREADS + threadIdx.x;
+  const long chunk = thread / vecs;
+  if (chunk >= a.chunks) return;
+  const int column = (int)(thread - chunk * vecs) * V;
+  const long s = chunk * a.chunk, e = s + a.chunk;
+  if (e >= a.n) return;
+  const unsigned key = a.keys[e - 1];
+  if (key >= (unsigned)a.rows || a.keys[e] != key) return;
+  if (s > 0 && a.keys[s - 1] == key) return;
+  float acc[V];
+  read<V>(a.tail + chunk * a.width + column, acc);
+  constexpr int AHEAD = 16;
+  bool more = true;
+  for (long c = chunk + 1; more; c += AHEAD) {
+    float x[AHEAD][V];
+    bool goes_on[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const long at = min(c + j, (long)a.chunks - 1), end = (c + j + 1) * a.chunk;
+      read<V>(a.head + at * a.width + column, x[j]);
+      goes_on[j] = end < a.n && a.keys[end] == key;
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (more) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += x[j][k];
+        more = goes_on[j];
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] *= a.scale;
+  write<V>(static_cast<Out*>(a.dw) + (long)key * a.width + column, acc);
+}
+
+#define EM_TYPES(In, Out, V)                                         \
+  template __global__ void lookup_kernel<In, Out, V>(Lookup);        \
+  template __global__ void sum_kernel<In, Out, V>(Sum, unsigned);
+#define EM_ALL(V)                                            \
+  EM_TYPES(float, float, V)                                  \
+  EM_TYPES(float, bf16_t, V)                                 \
+  EM_TYPES(bf16_t, float, V)                                 \
+  EM_TYPES(bf16_t, bf16_t, V)                                \
+  template __global__ void join_kernel<float, V>(Sum);       \
+  template __global__ void join_kernel<bf16_t, V>(Sum);
+EM_ALL(8)
+EM_ALL(4)
+EM_ALL(2)
+EM_ALL(1)
+
+}  // namespace em
