@@ -13,7 +13,7 @@
 #include "norm.hpp"
 
 namespace la {
-template <typename In, int NT, bool OUT>
+template <typename In, int NT, bool OUT, bool WHOLE>
 __global__ void attention_kernel(Args);
 __global__ void carry_kernel(Args);
 __global__ void decay_grad_kernel(DecayGrad);
@@ -121,20 +121,15 @@ void take_states(Carver& c, const Shape& s, int n, int tiles, bool split, la::Ro
   role->decays = c.take<float>(slots);
 }
 
-// Rows as the kernels take them: how many elements a load may take at once
-// (16 bytes, or the 4 of a bfloat16 pair, else one element).
+// Rows as the kernels take them: whole, where every row consists of 16-byte
+// pieces at multiples of 16 bytes.
 la::Rows rows_of(const m4rt_rows& r, int H, int bf16) {
-  la::Rows x{r.data, r.batch_stride, r.token_stride, r.head_stride, H / r.heads, r.width, 1};
-  const uintptr_t at = reinterpret_cast<uintptr_t>(r.data);
-  const int size = bf16 ? 2 : 4;
-  for (int vec : {16 / size, 4 / size}) {
-    if (at % (vec * size) == 0 && r.batch_stride % vec == 0 && r.token_stride % vec == 0 &&
-        r.head_stride % vec == 0 && r.width % vec == 0) {
-      x.vec = vec;
-      break;
-    }
-  }
-  return x;
+  const int piece = bf16 ? 8 : 4;
+  const bool whole = reinterpret_cast<uintptr_t>(r.data) % 16 == 0 &&
+                     r.batch_stride % piece == 0 && r.token_stride % piece == 0 &&
+                     r.head_stride % piece == 0 && r.width % piece == 0;
+  return la::Rows{r.data, r.batch_stride, r.token_stride, r.head_stride, H / r.heads, r.width,
+                  whole};
 }
 
 bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why) {
@@ -169,7 +164,17 @@ int wide_keys(const la::Args& a) {
 
 template <typename In, int NT, bool OUT>
 void start_attention(const la::Args& a, dim3 grid, hipStream_t st) {
-  hipLaunchKernelGGL((la::attention_kernel<In, NT, OUT>), grid, dim3(la::THREADS), 0, st, a);
+  bool whole = true;
+  for (int i = 0; i < a.roles; ++i) {
+    const la::Role& r = a.role[i];
+    whole = whole && r.q.whole && r.k.whole && r.v.whole && (!r.dots || r.e.whole);
+  }
+  if (whole)
+    hipLaunchKernelGGL((la::attention_kernel<In, NT, OUT, true>), grid, dim3(la::THREADS), 0, st,
+                       a);
+  else
+    hipLaunchKernelGGL((la::attention_kernel<In, NT, OUT, false>), grid, dim3(la::THREADS), 0, st,
+                       a);
 }
 
 template <bool OUT>

@@ -129,19 +129,16 @@ __device__ __forceinline__ f4 mma(const Frag<PA>& a, const Frag<PB>& b, f4 acc) 
 }
 
 // Elements col..col+7 of a row of `width` at byte offset `row`, zeros past the
-// width (and past the resource).
+// width (and past the resource).  WHOLE: in 16-byte pieces, as the rows' addresses
+// and width allow; one load each, so that nothing waits for it before its use.
+template <bool WHOLE>
 __device__ __forceinline__ Piece<bf16_t> load_piece(Rsrc r, unsigned row, int col, int width,
-                                                    int vec, const bf16_t*) {
+                                                    const bf16_t*) {
   Piece<bf16_t> x;
   const unsigned off = row + 2 * col;
-  if (vec == 8) {
+  if constexpr (WHOLE) {
     x.w[0] = __builtin_bit_cast(
         u4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0));
-  } else if (vec == 2) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      x.w[0][e] = __builtin_amdgcn_raw_buffer_load_b32(
-          r, col + 2 * e < width ? off + 4 * e : kNoLoad, 0, 0);
   } else {
     unsigned v[8];
 #pragma unroll
@@ -153,11 +150,12 @@ __device__ __forceinline__ Piece<bf16_t> load_piece(Rsrc r, unsigned row, int co
   }
   return x;
 }
+template <bool WHOLE>
 __device__ __forceinline__ Piece<float> load_piece(Rsrc r, unsigned row, int col, int width,
-                                                   int vec, const float*) {
+                                                   const float*) {
   Piece<float> x;
   const unsigned off = row + 4 * col;
-  if (vec >= 4) {
+  if constexpr (WHOLE) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       x.w[i] = __builtin_bit_cast(
@@ -172,30 +170,55 @@ __device__ __forceinline__ Piece<float> load_piece(Rsrc r, unsigned row, int col
   return x;
 }
 
-// The chunk's rows of (b, h): a resource that ends with row `rows` - 1.
-template <typename In>
-__device__ __forceinline__ Rsrc chunk_rows(const Rows& x, int b, int h, long t0, int rows) {
-  const In* base = static_cast<const In*>(x.base) + b * x.sb + (h / x.share) * x.sh + t0 * x.st;
-  const int bytes = rows > 0 ? (int)(((rows - 1) * x.st + x.width) * sizeof(In)) : 0;
-  return rsrc(base, bytes);
+// Elements col..col+3 as float32.
+template <bool WHOLE>
+__device__ __forceinline__ f4 load_quad(Rsrc r, unsigned row, int col, int width, const bf16_t*) {
+  u2 u;
+  const unsigned off = row + 2 * col;
+  if constexpr (WHOLE) {
+    u = __builtin_bit_cast(
+        u2, __builtin_amdgcn_raw_buffer_load_b64(r, col < width ? off : kNoLoad, 0, 0));
+  } else {
+    unsigned v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e] = __builtin_amdgcn_raw_buffer_load_b16(r, col + e < width ? off + 2 * e : kNoLoad, 0,
+                                                  0);
+    u = u2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)};
+  }
+  return f4{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
+}
+template <bool WHOLE>
+__device__ __forceinline__ f4 load_quad(Rsrc r, unsigned row, int col, int width, const float*) {
+  const unsigned off = row + 4 * col;
+  if constexpr (WHOLE) {
+    return __builtin_bit_cast(
+        f4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0));
+  } else {
+    f4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+          r, col + e < width ? off + 4 * e : kNoLoad, 0, 0));
+    return x;
+  }
 }
 
-// LDS rows: 64 NT or 64 bfloat16 and 16 bytes of padding, so that the rows
-// 0..15 of a fragment start in distinct 16-byte bank groups.
-template <int NT>
-__host__ __device__ constexpr int row_elems() {
-  return 64 * NT + 8;
-}
+// LDS tiles of bfloat16, 64 columns wide (wider ones are side by side): the
+// 16-byte units of a row change places by the row's low bits, with which the
+// transposing reads and the row reads below are free of bank conflicts (with
+// rows padded by 16 bytes instead, both took twice the cycles).
+__device__ __forceinline__ int unit(int row, int u) { return 64 * row + 8 * (u ^ (row & 7)); }
 
 template <typename In, int NT>
 struct Shared {
-  bf16_t k[Type<In>::IN][C * row_elems<NT>()];        // K [token][n]
-  bf16_t v[Type<In>::IN][C * row_elems<1>()];         // V [token][column]
-  bf16_t s[Type<In>::MADE][TILE * row_elems<NT>()];   // S^T [column][n]
-  float ph[C], pl[C];  // running log2 decay, high and low parts
-  float inter[C];      // weights of the state's part of each output
-  float update[C];     // weights of each token's part of the next state
-  float decay;         // the chunk's decay of the state
+  bf16_t k[Type<In>::IN][NT][C * 64];       // K [token][n]
+  bf16_t v[Type<In>::IN][1][C * TILE];      // V [token][column]
+  bf16_t s[Type<In>::MADE][NT][TILE * 64];  // S^T [column][n]
+  // Each wave's own, of the chunk's tokens.
+  float ph[WAVES][C], pl[WAVES][C];  // running log2 decay, high and low parts
+  float far[WAVES][C];     // decays between a token and the wave's strip
+  float update[WAVES][C];  // weights of each token's part of the next state
 };
 
 __device__ __forceinline__ Frag<1> cat(s4 a, s4 b) {
@@ -204,33 +227,35 @@ __device__ __forceinline__ Frag<1> cat(s4 a, s4 b) {
 }
 
 // Column fragments of a row-major tile by transposing reads: lane (g, r)
-// receives column c0 + r at the tokens 32 s + 4 g + (0..3) and 32 s + 16 + 4 g
-// + (0..3).  That is the order in which the scores' accumulators hold the
-// tokens, so those are operands as they are.
-template <int PLANES, int STRIDE>
-__device__ __forceinline__ Frag<PLANES> columns(const bf16_t (&tile)[PLANES][C * STRIDE], int s,
-                                                int c0, int g, int r) {
+// receives column 16 cb + r of its 64 at the tokens 32 s + 4 g + (0..3) and 32 s
+// + 16 + 4 g + (0..3).  That is the order in which the scores' accumulators hold
+// the tokens, so those are operands as they are.
+template <int PLANES, int NT>
+__device__ __forceinline__ Frag<PLANES> columns(const bf16_t (&tile)[PLANES][NT][C * 64], int nt,
+                                                int s, int cb, int g, int r) {
   typedef __attribute__((address_space(3))) s4* lds4;
   Frag<PLANES> f;
+  const int at = unit(4 * g + (r >> 2), 2 * cb + ((r >> 1) & 1)) + 4 * (r & 1);
 #pragma unroll
   for (int i = 0; i < PLANES; ++i) {
-    const bf16_t* p = &tile[i][(32 * s + 4 * g + (r >> 2)) * STRIDE + c0 + 4 * (r & 3)];
+    const bf16_t* p = &tile[i][nt][at + 32 * 64 * s];
     const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * STRIDE));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * 64));
     f.p[i] = cat(a, b).p[0];
   }
   return f;
 }
 
 // Row fragments: lane (g, r) receives row r0 + r at n = 32 kk + 8 g + (0..7).
-template <int PLANES, int ROWS, int STRIDE>
-__device__ __forceinline__ Frag<PLANES> rows(const bf16_t (&tile)[PLANES][ROWS * STRIDE], int r0,
+template <int PLANES, int NT>
+__device__ __forceinline__ Frag<PLANES> rows(const bf16_t (&tile)[PLANES][NT][C * 64], int r0,
                                              int kk, int g, int r) {
   Frag<PLANES> f;
 #pragma unroll
   for (int i = 0; i < PLANES; ++i)
     f.p[i] = __builtin_bit_cast(
-        b8, *reinterpret_cast<const u4*>(&tile[i][(r0 + r) * STRIDE + 32 * kk + 8 * g]));
+        b8, *reinterpret_cast<const u4*>(
+                &tile[i][kk >> 1][64 * r0 + unit(r, 4 * (kk & 1) + g)]));
   return f;
 }
 
@@ -294,24 +319,35 @@ __device__ __forceinline__ float sum_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// A chunk's decays, by one wave (lane = token).  The running sum is in
-// float64 and kept as two float32, so that e^{P_i - P_j} of near tokens is exact
-// to float32 after any decay before them.  A log decay below -2000 (-infinity, a
-// type's lowest value) counts as -2000: its exponential is zero either way and
-// the differences behind it stay finite.
-template <typename S>
-__device__ __forceinline__ void chunk_decays(S& sh, float g, int lane, bool rev, float inter,
-                                             float update) {
+// A chunk's decays, by each wave for itself (lane = token): P, the running sum
+// of log decays, in base 2.  The sum is in float64 and kept as two float32, so
+// that e^{P_i - P_j} of near tokens is exact to float32 after any decay before them.
+// A log decay below -2000 (-infinity, a type's lowest value) counts as -2000: its
+// exponential is zero either way and the differences behind it stay finite.
+//
+// Between strips of 16 tokens the decay is taken in two factors, from the key to
+// the near end of the query's strip (`far`, a table) and on to the query (`near`):
+// for decays below one neither can overflow, and the product costs two
+// multiplications a score instead of an exponential.
+struct Decays {
+  float head, tail;  // of this lane's token, from the chunk's start and to its end
+  float chunk;       // of the whole chunk
+};
+__device__ __forceinline__ Decays chunk_decays(float (&ph)[C], float (&pl)[C], float (&far)[C],
+                                               float (&weights)[C], float g, int lane, int w,
+                                               bool rev, float update) {
   const double p = wave_prefix((double)(g < -2000.f ? -2000.f : g) * 1.4426950408889634);
-  const double last = lane_double(p, 63);
-  const float ph = (float)p;
-  sh.ph[lane] = ph;
-  sh.pl[lane] = (float)(p - ph);
-  const float head = __builtin_amdgcn_exp2f((float)p);
-  const float tail = __builtin_amdgcn_exp2f((float)(last - p));
-  sh.inter[lane] = inter * (rev ? tail : head);
-  sh.update[lane] = update * (rev ? head : tail);
-  if (lane == 63) sh.decay = head;
+  const double last = lane_double(p, 63), edge = lane_double(p, rev ? 16 * w + 15 : 16 * w);
+  Decays d;
+  const float high = (float)p;
+  ph[lane] = high;
+  pl[lane] = (float)(p - high);
+  d.head = __builtin_amdgcn_exp2f((float)p);
+  d.tail = __builtin_amdgcn_exp2f((float)(last - p));
+  d.chunk = __builtin_amdgcn_exp2f((float)last);
+  far[lane] = __builtin_amdgcn_exp2f((float)(rev ? p - edge : edge - p));
+  weights[lane] = update * (rev ? d.head : d.tail);
+  return d;
 }
 
 __device__ __forceinline__ void store_out(void* base, long at, f4 v, int left, bool f32,
@@ -338,6 +374,24 @@ __device__ __forceinline__ void store_out(void* base, long at, f4 v, int left, b
   }
 }
 
+// Where an operand's rows of (b, h) begin, and their token stride in bytes.
+struct Source {
+  const char* base;
+  unsigned stride;
+  int bytes;  // of one row
+};
+template <typename In>
+__device__ __forceinline__ Source source(const Rows& x, int b, int h) {
+  return Source{static_cast<const char*>(x.base) +
+                    (b * x.sb + (h / x.share) * x.sh) * (long)sizeof(In),
+                (unsigned)(x.st * sizeof(In)), (int)(x.width * sizeof(In))};
+}
+// Chunk c's rows: a resource that ends with row `rows` - 1.
+__device__ __forceinline__ Rsrc chunk_rows(const Source& x, int c, int rows) {
+  return rsrc(x.base + (long)c * (C * (long)x.stride),
+              rows > 0 ? (rows - 1) * (int)x.stride + x.bytes : 0);
+}
+
 // One block: 64 value columns of one (b, h), the chunks c0..c1-1 (in reverse
 // if role.rev).  OUT: outputs from the state at the first chunk; else only the
 // segment's own state from zero, for split runs.
@@ -345,11 +399,10 @@ __device__ __forceinline__ void store_out(void* base, long at, f4 v, int left, b
 // A segment of SEG chunks keeps its own state (from zero) apart from the
 // state at its start; the state in use is decay * start + own.  So a split run, whose
 // blocks take one segment each, has the bits of a walk over all of them.
-template <typename In, int NT, bool OUT>
+template <typename In, int NT, bool OUT, bool WHOLE>
 __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int b, int h, int c0,
                                      int c1, int seg, Shared<In, NT>& sh) {
   constexpr int IN = Type<In>::IN, MADE = Type<In>::MADE;
-  constexpr int KROW = row_elems<NT>(), VROW = row_elems<1>();
   constexpr int KP = 2 * NT;  // pieces of K a thread loads
   const In* tag = nullptr;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
@@ -379,53 +432,54 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int n = 64 * nt + 16 * w + 4 * g + q;
-            if (n < R.n && p < R.p) start[nt][pb][q] = s[(long)n * R.initial.sn + (long)p * R.initial.sp];
+            if (n < R.n && p < R.p)
+              start[nt][pb][q] = s[(long)n * R.initial.sn + (long)p * R.initial.sp];
           }
         }
       }
     }
 
+  const Source ks = source<In>(R.k, b, h), vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h);
+  const float* gs = a.g + b * a.gb + h;
+  const long gt = a.gt;
   Piece<In> kraw[KP], vraw[2], qraw[2 * NT];
   float graw = 0.f;
   const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
   const int vcol = 8 * (tid & 7), vrow = tid >> 3;
   auto fetch = [&](int c) {
-    const long t0 = (long)c * C;
-    const int have = min(length - (int)t0, C);
-    const Rsrc kr = chunk_rows<In>(R.k, b, h, t0, have);
+    const int have = min(length - c * C, C);
+    const Rsrc kr = chunk_rows(ks, c, have);
 #pragma unroll
     for (int i = 0; i < KP; ++i)
-      kraw[i] = load_piece(kr, (unsigned)((krow + 32 / NT * i) * R.k.st * sizeof(In)), kcol, R.n,
-                           R.k.vec, tag);
-    const Rsrc vr = chunk_rows<In>(R.v, b, h, t0, have);
+      kraw[i] = load_piece<WHOLE>(kr, (krow + 32 / NT * i) * ks.stride, kcol, R.n, tag);
+    const Rsrc vr = chunk_rows(vs, c, have);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      vraw[i] = load_piece(vr, (unsigned)((vrow + 32 * i) * R.v.st * sizeof(In)), col0 + vcol, R.p,
-                           R.v.vec, tag);
+      vraw[i] = load_piece<WHOLE>(vr, (vrow + 32 * i) * vs.stride, col0 + vcol, R.p, tag);
     if constexpr (OUT) {
-      const Rsrc qr = chunk_rows<In>(R.q, b, h, t0, have);
+      const Rsrc qr = chunk_rows(qs, c, have);
 #pragma unroll
       for (int kk = 0; kk < 2 * NT; ++kk)
-        qraw[kk] = load_piece(qr, (unsigned)((16 * w + r) * R.q.st * sizeof(In)), 32 * kk + 8 * g,
-                              R.n, R.q.vec, tag);
+        qraw[kk] = load_piece<WHOLE>(qr, (16 * w + r) * qs.stride, 32 * kk + 8 * g, R.n, tag);
     }
-    if (w == 0) graw = lane < have ? a.g[b * a.gb + (t0 + lane) * a.gt + h] : 0.f;
+    graw = lane < have ? gs[((long)c * C + lane) * gt] : 0.f;
   };
 
   if (count > 0) fetch(rev ? c1 - 1 : c0);
   for (int it = 0; it < count; ++it) {
     const int c = rev ? c1 - 1 - it : c0 + it;
-    const long t0 = (long)c * C;
-    const int have = min(length - (int)t0, C);
+    const int t0 = c * C, have = min(length - t0, C);
     Frag<IN> qf[2 * NT];
+    Decays d{};
     if (have > 0) {
       // K, V, the state and the decays to LDS.
 #pragma unroll
       for (int i = 0; i < KP; ++i) {
         const Frag<IN> f = planes(kraw[i]);
+        const int row = krow + 32 / NT * i;
 #pragma unroll
         for (int j = 0; j < IN; ++j)
-          *reinterpret_cast<u4*>(&sh.k[j][(krow + 32 / NT * i) * KROW + kcol]) =
+          *reinterpret_cast<u4*>(&sh.k[j][kcol >> 6][unit(row, (kcol >> 3) & 7)]) =
               __builtin_bit_cast(u4, f.p[j]);
       }
 #pragma unroll
@@ -433,7 +487,7 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
         const Frag<IN> f = planes(vraw[i]);
 #pragma unroll
         for (int j = 0; j < IN; ++j)
-          *reinterpret_cast<u4*>(&sh.v[j][(vrow + 32 * i) * VROW + vcol]) =
+          *reinterpret_cast<u4*>(&sh.v[j][0][unit(vrow + 32 * i, vcol >> 3)]) =
               __builtin_bit_cast(u4, f.p[j]);
       }
       if constexpr (OUT) {
@@ -450,19 +504,20 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
 #pragma unroll
             for (int j = 0; j < MADE; ++j)
               *reinterpret_cast<u2*>(
-                  &sh.s[j][(16 * pb + r) * KROW + 64 * nt + 16 * w + 4 * g]) = u2{lo[j], hi[j]};
+                  &sh.s[j][nt][64 * 16 * pb + unit(r, 2 * w + (g >> 1)) + 4 * (g & 1)]) =
+                  u2{lo[j], hi[j]};
           }
 #pragma unroll
         for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
       }
-      if (w == 0) chunk_decays(sh, graw, lane, rev, R.inter, R.update);
+      d = chunk_decays(sh.ph[w], sh.pl[w], sh.far[w], sh.update[w], graw, lane, w, rev, R.update);
     }
     __syncthreads();
     if (it + 1 < count) fetch(rev ? c - 1 : c + 1);
     if (have > 0) {
       f4 out[4];
       Frag<MADE> score[2];
-      float diagonal;  // with dots: a token's score with itself, kept out of score
+      float diagonal = 0.f;  // with dots: a token's score with itself, kept out of score
       if constexpr (OUT) {
         // The state's part, transposed: columns 16 pb + 4 g + q of token 16 w + r.
 #pragma unroll
@@ -471,13 +526,16 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
         for (int kk = 0; kk < 2 * NT; ++kk)
 #pragma unroll
           for (int pb = 0; pb < 4; ++pb)
-            out[pb] = mma(rows<MADE, TILE, KROW>(sh.s, 16 * pb, kk, g, r), qf[kk], out[pb]);
-        const float inter = sh.inter[16 * w + r];
+            out[pb] = mma(rows<MADE, NT>(sh.s, 16 * pb, kk, g, r), qf[kk], out[pb]);
+        // Scores, transposed: keys 16 jb + 4 g + q of query 16 w + r.
+        const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
+        const int edge = rev ? 16 * w + 15 : 16 * w;
+        const float to_edge = (ph - sh.ph[w][edge]) + (pl - sh.pl[w][edge]);
+        const float near = R.intra * __builtin_amdgcn_exp2f(rev ? -to_edge : to_edge);
+        const float inter =
+            R.inter * __shfl(rev ? d.tail : d.head, 16 * w + r);
 #pragma unroll
         for (int pb = 0; pb < 4; ++pb) out[pb] *= inter;
-        // Scores, transposed: keys 16 jb + 4 g + q of query 16 w + r.
-        const float ph = sh.ph[16 * w + r], pl = sh.pl[16 * w + r];
-        diagonal = 0.f;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float x[8];
@@ -488,19 +546,23 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
             if (rev ? jb >= w : jb <= w) {
 #pragma unroll
               for (int kk = 0; kk < 2 * NT; ++kk)
-                acc = mma(rows<IN, C, KROW>(sh.k, 16 * jb, kk, g, r), qf[kk], acc);
-              const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[16 * jb + 4 * g]);
-              const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[16 * jb + 4 * g]);
+                acc = mma(rows<IN, NT>(sh.k, 16 * jb, kk, g, r), qf[kk], acc);
+              if (jb == w) {
+                const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * jb + 4 * g]);
+                const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * jb + 4 * g]);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float gap = (ph - kh[q]) + (pl - kl[q]);
-                const int ahead = 16 * (w - jb) + r - 4 * g - q;  // query - key
-                const float d = __builtin_amdgcn_exp2f(rev ? -gap : gap) * R.intra;
-                acc[q] = (rev ? ahead <= 0 : ahead >= 0) ? acc[q] * d : 0.f;
-                if (R.dots && ahead == 0) {
-                  diagonal = acc[q];
-                  acc[q] = 0.f;
+                for (int q = 0; q < 4; ++q) {
+                  const float gap = (ph - kh[q]) + (pl - kl[q]);
+                  const int ahead = r - 4 * g - q;  // query - key
+                  const float dec = __builtin_amdgcn_exp2f(rev ? -gap : gap) * R.intra;
+                  acc[q] = (rev ? ahead <= 0 : ahead >= 0) ? acc[q] * dec : 0.f;
+                  if (R.dots && ahead == 0) {
+                    diagonal = acc[q];
+                    acc[q] = 0.f;
+                  }
                 }
+              } else {
+                acc *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * jb + 4 * g]);
               }
             }
 #pragma unroll
@@ -510,29 +572,28 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
         }
       }
       // The next state, and the scores' part of the output.
-      const float decay = sh.decay;
-      since *= decay;
+      since *= d.chunk;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int pb = 0; pb < 4; ++pb) own[nt][pb] *= decay;
+        for (int pb = 0; pb < 4; ++pb) own[nt][pb] *= d.chunk;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float wt[8];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const f4 u = *reinterpret_cast<const f4*>(&sh.update[32 * s + 16 * half + 4 * g]);
+          const f4 u = *reinterpret_cast<const f4*>(&sh.update[w][32 * s + 16 * half + 4 * g]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) wt[4 * half + q] = u[q];
         }
         Frag<MADE> kw[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-          kw[nt] = weighted<MADE>(columns<IN, KROW>(sh.k, s, 64 * nt + 16 * w, g, r), wt);
+          kw[nt] = weighted<MADE>(columns<IN, NT>(sh.k, nt, s, w, g, r), wt);
         const bool scores = OUT && (rev ? 2 * s + 1 >= w : 2 * s <= w);
 #pragma unroll
         for (int pb = 0; pb < 4; ++pb) {
-          const Frag<IN> vf = columns<IN, VROW>(sh.v, s, 16 * pb, g, r);
+          const Frag<IN> vf = columns<IN, 1>(sh.v, 0, s, pb, g, r);
           if constexpr (OUT) {
             if (scores) out[pb] = mma(vf, score[s], out[pb]);
           }
@@ -543,24 +604,15 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
       if constexpr (OUT) {
         const int t = 16 * w + r;
         if (R.dots) {
-          const Rsrc er = chunk_rows<In>(R.e, b, h, t0, have);
+          const Source es = source<In>(R.e, b, h);
+          const Rsrc er = chunk_rows(es, c, have);
           float dot = 0.f;
 #pragma unroll
           for (int pb = 0; pb < 4; ++pb) {
             const int p = col0 + 16 * pb + 4 * g;
+            const f4 e = load_quad<WHOLE>(er, t * es.stride, p, R.p, tag);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const unsigned off = (unsigned)((t * R.e.st + p + q) * sizeof(In));
-              float e;
-              if constexpr (sizeof(In) == 2)
-                e = __uint_as_float((unsigned)__builtin_amdgcn_raw_buffer_load_b16(
-                                        er, p + q < R.p ? off : kNoLoad, 0, 0)
-                                    << 16);
-              else
-                e = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                    er, p + q < R.p ? off : kNoLoad, 0, 0));
-              dot = fmaf(out[pb][q], e, dot);
-            }
+            for (int q = 0; q < 4; ++q) dot = fmaf(out[pb][q], e[q], dot);
           }
           dot = sum_groups(dot);
           if (g == 0 && t < have)
@@ -571,7 +623,8 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
           for (int pb = 0; pb < 4; ++pb)
 #pragma unroll
             for (int i = IN - 1; i >= 0; --i) {
-              const u2 u = *reinterpret_cast<const u2*>(&sh.v[i][t * VROW + 16 * pb + 4 * g]);
+              const u2 u = *reinterpret_cast<const u2*>(
+                  &sh.v[i][0][unit(t, 2 * pb + (g >> 1)) + 4 * (g & 1)]);
               out[pb] += own_score * f4{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
             }
         }
@@ -591,8 +644,7 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
     } else if constexpr (OUT) {
       // Past the row's length: zeros.
       for (int i = tid; i < C * TILE; i += THREADS) {
-        const long t = t0 + (i >> 6);
-        const int p = col0 + (i & 63);
+        const int t = t0 + (i >> 6), p = col0 + (i & 63);
         if (t < a.T && p < R.p) {
           const long at = (((long)b * a.T + t) * a.H + h) * R.p + p;
           if (R.out_f32) static_cast<float*>(R.out)[at] = 0.f;
@@ -653,7 +705,7 @@ __device__ __forceinline__ bool block_of(const Args& a, int x, int* which, int* 
   return bh < a.B * a.H;
 }
 
-template <typename In, int NT, bool OUT>
+template <typename In, int NT, bool OUT, bool WHOLE>
 __global__ __launch_bounds__(THREADS, 2) void attention_kernel(Args a) {
   __shared__ Shared<In, NT> sh;
   int which, b, h, i = 0;
@@ -666,11 +718,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_kernel(Args a) {
   const int c0 = split ? seg * SEG : 0, c1 = split ? min(a.NC, c0 + SEG) : a.NC;
   if constexpr (NT == 2) {
     if (R.n <= 64) {
-      walk<In, 1, OUT>(a, R, which, b, h, c0, c1, seg, reinterpret_cast<Shared<In, 1>&>(sh));
+      walk<In, 1, OUT, WHOLE>(a, R, which, b, h, c0, c1, seg, reinterpret_cast<Shared<In, 1>&>(sh));
       return;
     }
   }
-  walk<In, NT, OUT>(a, R, which, b, h, c0, c1, seg, sh);
+  walk<In, NT, OUT, WHOLE>(a, R, which, b, h, c0, c1, seg, sh);
 }
 
 // Split runs: each segment's start state from the segments' own states and
@@ -851,15 +903,19 @@ __global__ __launch_bounds__(256) void step_kernel(Step a) {
   }
 }
 
-#define LA_INSTANCES(In)                                          \
-  template __global__ void attention_kernel<In, 1, true>(Args);   \
-  template __global__ void attention_kernel<In, 1, false>(Args);  \
-  template __global__ void attention_kernel<In, 2, true>(Args);   \
-  template __global__ void attention_kernel<In, 2, false>(Args);  \
-  template __global__ void step_kernel<In>(Step);                 \
+#define LA_ATTENTION(In, NT)                                            \
+  template __global__ void attention_kernel<In, NT, true, true>(Args);  \
+  template __global__ void attention_kernel<In, NT, true, false>(Args); \
+  template __global__ void attention_kernel<In, NT, false, true>(Args); \
+  template __global__ void attention_kernel<In, NT, false, false>(Args);
+#define LA_INSTANCES(In)                                                       \
+  LA_ATTENTION(In, 1)                                                          \
+  LA_ATTENTION(In, 2)                                                          \
+  template __global__ void step_kernel<In>(Step);                              \
   template __global__ void share_sum_kernel<In>(const float*, long, int, int, int, In*);
 LA_INSTANCES(float)
 LA_INSTANCES(bf16_t)
 #undef LA_INSTANCES
+#undef LA_ATTENTION
 
 }  // namespace la

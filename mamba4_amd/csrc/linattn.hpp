@@ -16,12 +16,11 @@ constexpr int THREADS = 64 * WAVES;
 typedef unsigned short bf16_t;
 
 // Rows [B,T,h,W] of one operand: unit stride along W, element strides along
-// the others, `share` attention heads to each of its own, `vec` consecutive
-// elements that may be loaded at once.
+// the others, `share` attention heads to each of its own; whole: 16-byte pieces.
 struct Rows {
   const void* base;
   long sb, st, sh;
-  int share, width, vec;
+  int share, width, whole;
 };
 
 // States [B,H,.,.] float32 with element strides of the key and value axes
