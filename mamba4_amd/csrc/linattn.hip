@@ -114,18 +114,33 @@ __device__ __forceinline__ Frag<3> planes(const Piece<float>& x) {
   return split8<3>(v);
 }
 
-// acc += a b over the plane products that count: the sum of the planes'
-// indexes below the larger number of planes.
-template <int PA, int PB>
-__device__ __forceinline__ f4 mma(const Frag<PA>& a, const Frag<PB>& b, f4 acc) {
+// acc[i] += a[i] b over the plane products that count: the sum of the planes'
+// indexes below the larger number of planes.  Products of different accumulators
+// follow each other, so that none waits for the one before.
+template <int N, int PA, int PB>
+__device__ __forceinline__ void mma(const Frag<PA> (&a)[N], const Frag<PB>& b, f4* acc) {
   constexpr int most = PA > PB ? PA : PB;
 #pragma unroll
   for (int s = most - 1; s >= 0; --s)
 #pragma unroll
     for (int i = 0; i < PA; ++i)
       if (s - i >= 0 && s - i < PB)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], acc, 0, 0, 0);
-  return acc;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n].p[i], b.p[s - i], acc[n], 0, 0, 0);
+}
+// acc[i] += a b[i].
+template <int N, int PA, int PB>
+__device__ __forceinline__ void mma(const Frag<PA>& a, const Frag<PB> (&b)[N], f4* acc) {
+  constexpr int most = PA > PB ? PA : PB;
+#pragma unroll
+  for (int s = most - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      if (s - i >= 0 && s - i < PB)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b[n].p[s - i], acc[n], 0, 0, 0);
 }
 
 // Elements col..col+7 of a row of `width` at byte offset `row`, zeros past the
@@ -170,37 +185,51 @@ __device__ __forceinline__ Piece<float> load_piece(Rsrc r, unsigned row, int col
   return x;
 }
 
-// Elements col..col+3 as float32.
-template <bool WHOLE>
-__device__ __forceinline__ f4 load_quad(Rsrc r, unsigned row, int col, int width, const bf16_t*) {
+// Elements col..col+3 as loaded, and as float32.
+template <typename In>
+struct Quad;
+template <>
+struct Quad<bf16_t> {
   u2 u;
+  __device__ __forceinline__ f4 get() const {
+    return f4{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
+  }
+};
+template <>
+struct Quad<float> {
+  f4 u;
+  __device__ __forceinline__ f4 get() const { return u; }
+};
+template <bool WHOLE>
+__device__ __forceinline__ Quad<bf16_t> load_quad(Rsrc r, unsigned row, int col, int width,
+                                                  const bf16_t*) {
   const unsigned off = row + 2 * col;
   if constexpr (WHOLE) {
-    u = __builtin_bit_cast(
-        u2, __builtin_amdgcn_raw_buffer_load_b64(r, col < width ? off : kNoLoad, 0, 0));
+    return {__builtin_bit_cast(
+        u2, __builtin_amdgcn_raw_buffer_load_b64(r, col < width ? off : kNoLoad, 0, 0))};
   } else {
     unsigned v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       v[e] = __builtin_amdgcn_raw_buffer_load_b16(r, col + e < width ? off + 2 * e : kNoLoad, 0,
                                                   0);
-    u = u2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)};
+    return {u2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)}};
   }
-  return f4{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
 }
 template <bool WHOLE>
-__device__ __forceinline__ f4 load_quad(Rsrc r, unsigned row, int col, int width, const float*) {
+__device__ __forceinline__ Quad<float> load_quad(Rsrc r, unsigned row, int col, int width,
+                                                 const float*) {
   const unsigned off = row + 4 * col;
   if constexpr (WHOLE) {
-    return __builtin_bit_cast(
-        f4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0));
+    return {__builtin_bit_cast(
+        f4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0))};
   } else {
     f4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
           r, col + e < width ? off + 4 * e : kNoLoad, 0, 0));
-    return x;
+    return {x};
   }
 }
 
@@ -210,15 +239,15 @@ __device__ __forceinline__ f4 load_quad(Rsrc r, unsigned row, int col, int width
 // rows padded by 16 bytes instead, both took twice the cycles).
 __device__ __forceinline__ int unit(int row, int u) { return 64 * row + 8 * (u ^ (row & 7)); }
 
-template <typename In, int NT>
+template <typename In, int NT, bool OUT>
 struct Shared {
-  bf16_t k[Type<In>::IN][NT][C * 64];       // K [token][n]
-  bf16_t v[Type<In>::IN][1][C * TILE];      // V [token][column]
-  bf16_t s[Type<In>::MADE][NT][TILE * 64];  // S^T [column][n]
-  // Each wave's own, of the chunk's tokens.
-  float ph[WAVES][C], pl[WAVES][C];  // running log2 decay, high and low parts
-  float far[WAVES][C];     // decays between a token and the wave's strip
-  float update[WAVES][C];  // weights of each token's part of the next state
+  alignas(16) bf16_t k[Type<In>::IN][NT][C * 64];       // K [token][n]
+  alignas(16) bf16_t v[Type<In>::IN][1][C * TILE];      // V [token][column]
+  alignas(16) bf16_t s[Type<In>::MADE][NT][OUT ? TILE * 64 : 8];  // S^T [column][n]
+  // Each wave's own, of the chunk's tokens: the running log2 decay in two
+  // parts, the decays between a token and the wave's strip, and the weights of the
+  // tokens in the next state.
+  alignas(16) float ph[WAVES][C], pl[WAVES][C], far[WAVES][C], update[WAVES][C];
 };
 
 __device__ __forceinline__ Frag<1> cat(s4 a, s4 b) {
@@ -227,20 +256,19 @@ __device__ __forceinline__ Frag<1> cat(s4 a, s4 b) {
 }
 
 // Column fragments of a row-major tile by transposing reads: lane (g, r)
-// receives column 16 cb + r of its 64 at the tokens 32 s + 4 g + (0..3) and 32 s
-// + 16 + 4 g + (0..3).  That is the order in which the scores' accumulators hold
-// the tokens, so those are operands as they are.
+// receives column 16 cb + r of its 64 at the tokens 16 ja + 4 g + (0..3) and 16 jb
+// + 4 g + (0..3).  That is the order in which the scores' accumulators hold the
+// tokens of two blocks, so those are operands as they are.
 template <int PLANES, int NT>
 __device__ __forceinline__ Frag<PLANES> columns(const bf16_t (&tile)[PLANES][NT][C * 64], int nt,
-                                                int s, int cb, int g, int r) {
+                                                int ja, int jb, int cb, int g, int r) {
   typedef __attribute__((address_space(3))) s4* lds4;
   Frag<PLANES> f;
   const int at = unit(4 * g + (r >> 2), 2 * cb + ((r >> 1) & 1)) + 4 * (r & 1);
 #pragma unroll
   for (int i = 0; i < PLANES; ++i) {
-    const bf16_t* p = &tile[i][nt][at + 32 * 64 * s];
-    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * 64));
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&tile[i][nt][at + 16 * 64 * ja]));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&tile[i][nt][at + 16 * 64 * jb]));
     f.p[i] = cat(a, b).p[0];
   }
   return f;
@@ -330,48 +358,49 @@ __device__ __forceinline__ float sum_groups(float x) {
 // for decays below one neither can overflow, and the product costs two
 // multiplications a score instead of an exponential.
 struct Decays {
-  float head, tail;  // of this lane's token, from the chunk's start and to its end
-  float chunk;       // of the whole chunk
+  float inter;  // of this lane's token: the state's part in its output
+  float near;   // from the near end of the wave's strip (tokens of the strip)
+  float chunk;  // of the whole chunk
 };
+template <bool REV>
 __device__ __forceinline__ Decays chunk_decays(float (&ph)[C], float (&pl)[C], float (&far)[C],
                                                float (&weights)[C], float g, int lane, int w,
-                                               bool rev, float update) {
+                                               float update) {
   const double p = wave_prefix((double)(g < -2000.f ? -2000.f : g) * 1.4426950408889634);
-  const double last = lane_double(p, 63), edge = lane_double(p, rev ? 16 * w + 15 : 16 * w);
-  Decays d;
-  const float high = (float)p;
+  const double last = lane_double(p, 63), edge = lane_double(p, REV ? 16 * w + 15 : 16 * w);
+  const float high = (float)p, to_edge = (float)(REV ? p - edge : edge - p);
+  const float head = __builtin_amdgcn_exp2f(high);
+  const float tail = __builtin_amdgcn_exp2f((float)(last - p));
   ph[lane] = high;
   pl[lane] = (float)(p - high);
-  d.head = __builtin_amdgcn_exp2f((float)p);
-  d.tail = __builtin_amdgcn_exp2f((float)(last - p));
-  d.chunk = __builtin_amdgcn_exp2f((float)last);
-  far[lane] = __builtin_amdgcn_exp2f((float)(rev ? p - edge : edge - p));
-  weights[lane] = update * (rev ? d.head : d.tail);
-  return d;
+  far[lane] = __builtin_amdgcn_exp2f(to_edge);
+  weights[lane] = update * (REV ? head : tail);
+  return Decays{REV ? tail : head, __builtin_amdgcn_exp2f(-to_edge),
+                __builtin_amdgcn_exp2f((float)last)};
 }
 
-__device__ __forceinline__ void store_out(void* base, long at, f4 v, int left, bool f32,
-                                          bool vec) {
+// Four consecutive columns of a token's output, `left` of them within the width.
+__device__ __forceinline__ void store_some(void* base, long at, f4 v, int left, bool f32) {
   if (f32) {
     float* p = static_cast<float*>(base) + at;
-    if (vec) {
-      *reinterpret_cast<f4*>(p) = v;
-    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (q < left) p[q] = v[q];
-    }
+    for (int q = 0; q < 4; ++q)
+      if (q < left) p[q] = v[q];
   } else {
     bf16_t* p = static_cast<bf16_t*>(base) + at;
     const u2 u{pack(v[0], v[1]), pack(v[2], v[3])};
-    if (vec) {
-      *reinterpret_cast<u2*>(p) = u;
-    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (q < left) p[q] = (bf16_t)(u[q >> 1] >> (16 * (q & 1)));
-    }
+    for (int q = 0; q < 4; ++q)
+      if (q < left) p[q] = (bf16_t)(u[q >> 1] >> (16 * (q & 1)));
   }
+}
+
+// The thread's index, opaque to the compiler: what is computed from it inside a
+// loop is computed there, instead of keeping registers over the whole loop.
+__device__ __forceinline__ int thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
 }
 
 // Where an operand's rows of (b, h) begin, and their token stride in bytes.
@@ -383,7 +412,7 @@ struct Source {
 template <typename In>
 __device__ __forceinline__ Source source(const Rows& x, int b, int h) {
   return Source{static_cast<const char*>(x.base) +
-                    (b * x.sb + (h / x.share) * x.sh) * (long)sizeof(In),
+                    (b * x.sb + (x.share > 1 ? h / x.share : h) * x.sh) * (long)sizeof(In),
                 (unsigned)(x.st * sizeof(In)), (int)(x.width * sizeof(In))};
 }
 // Chunk c's rows: a resource that ends with row `rows` - 1.
@@ -399,21 +428,22 @@ __device__ __forceinline__ Rsrc chunk_rows(const Source& x, int c, int rows) {
 // A segment of SEG chunks keeps its own state (from zero) apart from the
 // state at its start; the state in use is decay * start + own.  So a split run, whose
 // blocks take one segment each, has the bits of a walk over all of them.
-template <typename In, int NT, bool OUT, bool WHOLE>
+template <typename In, int NT, bool OUT, bool WHOLE, bool REV>
 __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int b, int h, int c0,
-                                     int c1, int seg, Shared<In, NT>& sh) {
+                                     int c1, int seg, Shared<In, NT, OUT>& sh) {
   constexpr int IN = Type<In>::IN, MADE = Type<In>::MADE;
   constexpr int KP = 2 * NT;  // pieces of K a thread loads
+  constexpr int GROUP = IN > 1 ? 2 : 4;  // products between which no wait is needed
   const In* tag = nullptr;
-  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col0 = TILE * tile, bh = b * a.H + h;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-  const bool rev = R.rev;
   const int count = c1 - c0;
 
   // The state's accumulators: n = 64 nt + 16 w + 4 g + q, column 16 pb + r.
   f4 start[NT][4], own[NT][4];
+  int tid = thread();
+  int lane = tid & 63, g = lane >> 4, r = lane & 15;
   float since = 1.f;  // decay since the segment's start
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -439,15 +469,16 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
       }
     }
 
-  const Source ks = source<In>(R.k, b, h), vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h);
+  const Source ks = source<In>(R.k, b, h), vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h),
+               es = source<In>(R.e, b, h);
   const float* gs = a.g + b * a.gb + h;
   const long gt = a.gt;
   Piece<In> kraw[KP], vraw[2], qraw[2 * NT];
   float graw = 0.f;
-  const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
-  const int vcol = 8 * (tid & 7), vrow = tid >> 3;
   auto fetch = [&](int c) {
     const int have = min(length - c * C, C);
+    const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
+    const int vcol = 8 * (tid & 7), vrow = tid >> 3;
     const Rsrc kr = chunk_rows(ks, c, have);
 #pragma unroll
     for (int i = 0; i < KP; ++i)
@@ -465,14 +496,19 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
     graw = lane < have ? gs[((long)c * C + lane) * gt] : 0.f;
   };
 
-  if (count > 0) fetch(rev ? c1 - 1 : c0);
+  if (count > 0) fetch(REV ? c1 - 1 : c0);
   for (int it = 0; it < count; ++it) {
-    const int c = rev ? c1 - 1 - it : c0 + it;
+    const int c = REV ? c1 - 1 - it : c0 + it;
     const int t0 = c * C, have = min(length - t0, C);
+    tid = thread();
+    lane = tid & 63, g = lane >> 4, r = lane & 15;
     Frag<IN> qf[2 * NT];
     Decays d{};
+    Quad<In> e[4];
     if (have > 0) {
       // K, V, the state and the decays to LDS.
+      const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
+      const int vcol = 8 * (tid & 7), vrow = tid >> 3;
 #pragma unroll
       for (int i = 0; i < KP; ++i) {
         const Frag<IN> f = planes(kraw[i]);
@@ -510,11 +546,28 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
 #pragma unroll
         for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
       }
-      d = chunk_decays(sh.ph[w], sh.pl[w], sh.far[w], sh.update[w], graw, lane, w, rev, R.update);
+      d = chunk_decays<REV>(sh.ph[w], sh.pl[w], sh.far[w], sh.update[w], graw, lane, w, R.update);
+      if constexpr (OUT) {
+        // Before the next chunk's loads, so that their wait does not include those.
+        if (R.dots) {
+          const Rsrc er = chunk_rows(es, c, have);
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb)
+            e[pb] = load_quad<WHOLE>(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p, tag);
+        }
+      }
     }
     __syncthreads();
-    if (it + 1 < count) fetch(rev ? c - 1 : c + 1);
+    if (it + 1 < count) fetch(REV ? c - 1 : c + 1);
     if (have > 0) {
+      // The blocks of 16 keys in turn from the wave's own strip, into the past (REV:
+      // the future) and round: the first `seen` of them reach the strip's queries.
+      // (Opaque, so that the addresses that follow from it are not kept in registers
+      // over the loop.)
+      int strip = w;
+      asm volatile("" : "+s"(strip));
+      const int seen = REV ? WAVES - strip : strip + 1;
+      auto block = [&](int i) { return (REV ? strip + i : strip - i) & 3; };
       f4 out[4];
       Frag<MADE> score[2];
       float diagonal = 0.f;  // with dots: a token's score with itself, kept out of score
@@ -525,49 +578,53 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
 #pragma unroll
         for (int kk = 0; kk < 2 * NT; ++kk)
 #pragma unroll
-          for (int pb = 0; pb < 4; ++pb)
-            out[pb] = mma(rows<MADE, NT>(sh.s, 16 * pb, kk, g, r), qf[kk], out[pb]);
-        // Scores, transposed: keys 16 jb + 4 g + q of query 16 w + r.
-        const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
-        const int edge = rev ? 16 * w + 15 : 16 * w;
-        const float to_edge = (ph - sh.ph[w][edge]) + (pl - sh.pl[w][edge]);
-        const float near = R.intra * __builtin_amdgcn_exp2f(rev ? -to_edge : to_edge);
-        const float inter =
-            R.inter * __shfl(rev ? d.tail : d.head, 16 * w + r);
+          for (int p0 = 0; p0 < 4; p0 += GROUP) {
+            Frag<MADE> sf[GROUP];
+#pragma unroll
+            for (int pb = 0; pb < GROUP; ++pb)
+              sf[pb] = rows<MADE, NT>(sh.s, 16 * (p0 + pb), kk, g, r);
+            mma(sf, qf[kk], &out[p0]);
+          }
+        const float inter = R.inter * __shfl(d.inter, 16 * w + r);
+        const float near = R.intra * __shfl(d.near, 16 * w + r);
 #pragma unroll
         for (int pb = 0; pb < 4; ++pb) out[pb] *= inter;
+        // Scores, transposed: keys 16 block(i) + 4 g + q of query 16 w + r.
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          float x[8];
+          f4 acc[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+          if (2 * s < seen) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int jb = 2 * s + half;
-            f4 acc{0.f, 0.f, 0.f, 0.f};
-            if (rev ? jb >= w : jb <= w) {
-#pragma unroll
-              for (int kk = 0; kk < 2 * NT; ++kk)
-                acc = mma(rows<IN, NT>(sh.k, 16 * jb, kk, g, r), qf[kk], acc);
-              if (jb == w) {
-                const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * jb + 4 * g]);
-                const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * jb + 4 * g]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const float gap = (ph - kh[q]) + (pl - kl[q]);
-                  const int ahead = r - 4 * g - q;  // query - key
-                  const float dec = __builtin_amdgcn_exp2f(rev ? -gap : gap) * R.intra;
-                  acc[q] = (rev ? ahead <= 0 : ahead >= 0) ? acc[q] * dec : 0.f;
-                  if (R.dots && ahead == 0) {
-                    diagonal = acc[q];
-                    acc[q] = 0.f;
-                  }
-                }
-              } else {
-                acc *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * jb + 4 * g]);
-              }
+            for (int kk = 0; kk < 2 * NT; ++kk) {
+              const Frag<IN> kf[2] = {rows<IN, NT>(sh.k, 16 * block(2 * s), kk, g, r),
+                                      rows<IN, NT>(sh.k, 16 * block(2 * s + 1), kk, g, r)};
+              mma(kf, qf[kk], acc);
             }
+            if (s == 0) {
+              const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
+              const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * w + 4 * g]);
+              const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * w + 4 * g]);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) x[4 * half + q] = acc[q];
+              for (int q = 0; q < 4; ++q) {
+                const float gap = (ph - kh[q]) + (pl - kl[q]);
+                const int ahead = REV ? 4 * g + q - r : r - 4 * g - q;  // query - key
+                const float dec = __builtin_amdgcn_exp2f(REV ? -gap : gap) * R.intra;
+                const float x = acc[0][q] * dec;
+                acc[0][q] = ahead > 0 ? x : 0.f;
+                if (ahead == 0) diagonal = x;
+                if (ahead == 0 && !R.dots) acc[0][q] = x;
+              }
+            } else {
+              acc[0] *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * block(2 * s) + 4 * g]);
+            }
+            // A block past the last one seen gives no scores.
+            const f4 far =
+                near * *reinterpret_cast<const f4*>(&sh.far[w][16 * block(2 * s + 1) + 4 * g]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[1][q] = 2 * s + 1 < seen ? acc[1][q] * far[q] : 0.f;
           }
+          const float x[8] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3],
+                              acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
           score[s] = split8<MADE>(x);
         }
       }
@@ -579,41 +636,35 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
         for (int pb = 0; pb < 4; ++pb) own[nt][pb] *= d.chunk;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        float wt[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const f4 u = *reinterpret_cast<const f4*>(&sh.update[w][32 * s + 16 * half + 4 * g]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) wt[4 * half + q] = u[q];
-        }
+        const int ja = block(2 * s), jb = block(2 * s + 1);
+        const f4 ua = *reinterpret_cast<const f4*>(&sh.update[w][16 * ja + 4 * g]);
+        const f4 ub = *reinterpret_cast<const f4*>(&sh.update[w][16 * jb + 4 * g]);
+        const float wt[8] = {ua[0], ua[1], ua[2], ua[3], ub[0], ub[1], ub[2], ub[3]};
         Frag<MADE> kw[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-          kw[nt] = weighted<MADE>(columns<IN, NT>(sh.k, nt, s, w, g, r), wt);
-        const bool scores = OUT && (rev ? 2 * s + 1 >= w : 2 * s <= w);
+          kw[nt] = weighted<MADE>(columns<IN, NT>(sh.k, nt, ja, jb, w, g, r), wt);
 #pragma unroll
-        for (int pb = 0; pb < 4; ++pb) {
-          const Frag<IN> vf = columns<IN, 1>(sh.v, 0, s, pb, g, r);
+        for (int p0 = 0; p0 < 4; p0 += GROUP) {
+          Frag<IN> vf[GROUP];
+#pragma unroll
+          for (int pb = 0; pb < GROUP; ++pb)
+            vf[pb] = columns<IN, 1>(sh.v, 0, ja, jb, p0 + pb, g, r);
           if constexpr (OUT) {
-            if (scores) out[pb] = mma(vf, score[s], out[pb]);
+            if (2 * s < seen) mma(vf, score[s], &out[p0]);
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) own[nt][pb] = mma(kw[nt], vf, own[nt][pb]);
+          for (int nt = 0; nt < NT; ++nt) mma(kw[nt], vf, &own[nt][p0]);
         }
       }
       if constexpr (OUT) {
         const int t = 16 * w + r;
         if (R.dots) {
-          const Source es = source<In>(R.e, b, h);
-          const Rsrc er = chunk_rows(es, c, have);
           float dot = 0.f;
 #pragma unroll
-          for (int pb = 0; pb < 4; ++pb) {
-            const int p = col0 + 16 * pb + 4 * g;
-            const f4 e = load_quad<WHOLE>(er, t * es.stride, p, R.p, tag);
+          for (int pb = 0; pb < 4; ++pb)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) dot = fmaf(out[pb][q], e[q], dot);
-          }
+            for (int q = 0; q < 4; ++q) dot = fmaf(out[pb][q], e[pb].get()[q], dot);
           dot = sum_groups(dot);
           if (g == 0 && t < have)
             R.dots[((long)(tile * a.B + b) * a.H + h) * a.T + t0 + t] = dot;
@@ -630,14 +681,27 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
         }
         if (t0 + t < a.T) {
           const bool here = t < have;
-          const long at = (((long)b * a.T + t0 + t) * a.H + h) * R.p;
-          const bool vec = (R.p & 3) == 0, f32 = R.out_f32;
+          const long at = (((long)b * a.T + t0 + t) * a.H + h) * R.p + col0 + 4 * g;
 #pragma unroll
-          for (int pb = 0; pb < 4; ++pb) {
-            const int p = col0 + 16 * pb + 4 * g;
-            if (p < R.p)
-              store_out(R.out, at + p, here ? out[pb] : f4{0.f, 0.f, 0.f, 0.f}, R.p - p, f32,
-                        vec);
+          for (int pb = 0; pb < 4; ++pb)
+            if (!here) out[pb] = f4{0.f, 0.f, 0.f, 0.f};
+          const int left = R.p - col0 - 4 * g;
+          if (R.p & 3) {
+#pragma unroll
+            for (int pb = 0; pb < 4; ++pb)
+              store_some(R.out, at + 16 * pb, out[pb], left - 16 * pb, R.out_f32);
+          } else if (R.out_f32) {
+            float* p = static_cast<float*>(R.out) + at;
+#pragma unroll
+            for (int pb = 0; pb < 4; ++pb)
+              if (16 * pb < left) *reinterpret_cast<f4*>(p + 16 * pb) = out[pb];
+          } else {
+            bf16_t* p = static_cast<bf16_t*>(R.out) + at;
+#pragma unroll
+            for (int pb = 0; pb < 4; ++pb)
+              if (16 * pb < left)
+                *reinterpret_cast<u2*>(p + 16 * pb) =
+                    u2{pack(out[pb][0], out[pb][1]), pack(out[pb][2], out[pb][3])};
           }
         }
       }
@@ -654,7 +718,7 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
     }
     __syncthreads();
     // A segment ends: its state joins the start.
-    if (OUT && (rev ? c % SEG == 0 : c % SEG == SEG - 1 || c == a.NC - 1)) {
+    if (OUT && (REV ? c % SEG == 0 : c % SEG == SEG - 1 || c == a.NC - 1)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -669,7 +733,7 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
   }
 
   if constexpr (OUT) {
-    if (R.final.base && (rev ? c0 == 0 : c1 == a.NC)) {
+    if (R.final.base && (REV ? c0 == 0 : c1 == a.NC)) {
       float* s = R.final.base + (long)bh * R.n * R.p;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -706,8 +770,8 @@ __device__ __forceinline__ bool block_of(const Args& a, int x, int* which, int* 
 }
 
 template <typename In, int NT, bool OUT, bool WHOLE>
-__global__ __launch_bounds__(THREADS, 2) void attention_kernel(Args a) {
-  __shared__ Shared<In, NT> sh;
+__global__ __launch_bounds__(THREADS, sizeof(In) == 2 && NT == 1 ? 3 : sizeof(In) == 4 && NT == 2 ? 1 : 2) void attention_kernel(Args a) {
+  __shared__ Shared<In, NT, OUT> sh;
   int which, b, h, i = 0;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   while (which >= a.role[i].tiles) which -= a.role[i++].tiles;
@@ -718,11 +782,18 @@ __global__ __launch_bounds__(THREADS, 2) void attention_kernel(Args a) {
   const int c0 = split ? seg * SEG : 0, c1 = split ? min(a.NC, c0 + SEG) : a.NC;
   if constexpr (NT == 2) {
     if (R.n <= 64) {
-      walk<In, 1, OUT, WHOLE>(a, R, which, b, h, c0, c1, seg, reinterpret_cast<Shared<In, 1>&>(sh));
+      Shared<In, 1, OUT>& narrow = reinterpret_cast<Shared<In, 1, OUT>&>(sh);
+      if (R.rev)
+        walk<In, 1, OUT, WHOLE, true>(a, R, which, b, h, c0, c1, seg, narrow);
+      else
+        walk<In, 1, OUT, WHOLE, false>(a, R, which, b, h, c0, c1, seg, narrow);
       return;
     }
   }
-  walk<In, NT, OUT, WHOLE>(a, R, which, b, h, c0, c1, seg, sh);
+  if (R.rev)
+    walk<In, NT, OUT, WHOLE, true>(a, R, which, b, h, c0, c1, seg, sh);
+  else
+    walk<In, NT, OUT, WHOLE, false>(a, R, which, b, h, c0, c1, seg, sh);
 }
 
 // Split runs: each segment's start state from the segments' own states and
