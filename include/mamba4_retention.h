@@ -37,6 +37,11 @@ typedef struct {
   int heads, width;
 } m4rt_rows;
 
+/* The queries, keys and values of a call, in this order. */
+typedef struct {
+  m4rt_rows q, k, v;
+} m4rt_qkv;
+
 /*
  * Linear attention with a decay for each head.
  *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t
@@ -57,10 +62,10 @@ typedef struct {
  * that is present spreads to the outputs of its chunk of 64 tokens and after it.
  */
 size_t m4rt_attention_workspace_bytes(int B, int T, int H, int N, int P, int bf16);
-int m4rt_attention_forward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
-                           const float* log_decay, int per_token, const int* lengths,
-                           const float* initial, float scale, int B, int T, int H, void* output,
-                           float* state, void* workspace, size_t workspace_bytes, void* stream);
+int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
+                           const int* lengths, const float* initial, float scale, int B, int T,
+                           int H, void* output, float* state, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 /*
  * Its gradient, from the cotangents d_output [B,T,H,P] in the inputs' type and
@@ -72,10 +77,9 @@ int m4rt_attention_forward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_ro
  */
 size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads, int k_heads,
                                                int v_heads, int N, int P, int bf16);
-int m4rt_attention_backward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
-                            const float* log_decay, int per_token, const int* lengths,
-                            const float* initial, float scale, int B, int T, int H,
-                            const void* d_output, const float* d_state, const float* state,
+int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_decay,
+                            int per_token, const int* lengths, const float* initial, float scale,
+                            int B, int T, int H, const void* d_output, const float* d_state, const float* state,
                             void* d_q, void* d_k, void* d_v, float* d_log_decay,
                             float* d_initial, void* workspace, size_t workspace_bytes,
                             void* stream);
@@ -86,10 +90,9 @@ int m4rt_attention_backward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_r
  * else [H].  active [B] bytes, or NULL: a row whose byte is zero keeps its
  * state and its output is zero.
  */
-int m4rt_attention_step(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
-                        const float* log_decay, int per_token, const uint8_t* active, float scale,
-                        int B, int H, const float* state, float* new_state, void* output,
-                        void* stream);
+int m4rt_attention_step(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
+                        const uint8_t* active, float scale, int B, int H, const float* state,
+                        float* new_state, void* output, void* stream);
 
 #define M4RT_NONE 0
 #define M4RT_SILU 1

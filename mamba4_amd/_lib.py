@@ -7,6 +7,7 @@ missing: there is no fallback implementation.
 import ctypes
 import os
 import re
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = os.path.join(HERE, "libmamba4_memread.so")
@@ -62,20 +63,10 @@ class ResizeArray(ctypes.Structure):
     ]
 
 
-class Rows(ctypes.Structure):
-    """m4rt_rows (include/mamba4_retention.h)."""
+# m4rt_rows (include/mamba4_retention.h) three times: an m4rt_qkv, packed into
+# bytes (a fraction of the time of filling a ctypes.Structure).
+pack_qkv = struct.Struct("@" + 3 * "Plllii").pack
 
-    _fields_ = [
-        ("data", ctypes.c_void_p),
-        ("batch_stride", ctypes.c_long),
-        ("token_stride", ctypes.c_long),
-        ("head_stride", ctypes.c_long),
-        ("heads", ctypes.c_int),
-        ("width", ctypes.c_int),
-    ]
-
-
-_R = ctypes.POINTER(Rows)
 _F = ctypes.c_float
 
 SIGNATURES = {
@@ -141,12 +132,12 @@ SIGNATURES = {
     "m3s_backward_bf16": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P] * 9 + [_P, _S, _P]),
     "m4rt_attention_workspace_bytes": (_S, [_I] * 6),
     "m4rt_attention_forward": (
-        _I, [_R] * 3 + [_I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 3 + [_S, _P]),
+        _I, [_P, _I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 3 + [_S, _P]),
     "m4rt_attention_backward_workspace_bytes": (_S, [_I] * 9),
     "m4rt_attention_backward": (
-        _I, [_R] * 3 + [_I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 9 + [_S, _P]),
+        _I, [_P, _I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 9 + [_S, _P]),
     "m4rt_attention_step": (
-        _I, [_R] * 3 + [_I, _P, _I, _P, _F] + [_I] * 2 + [_P] * 3 + [_P]),
+        _I, [_P, _I, _P, _I, _P, _F] + [_I] * 2 + [_P] * 3 + [_P]),
     "m4rt_norm_workspace_bytes": (_S, [_L] + [_I] * 5),
     "m4rt_norm_forward": (_I, [_P] * 4 + [_I, _L] + [_I] * 4 + [_F] + [_P] * 3 + [_S, _P]),
     "m4rt_norm_backward": (_I, [_P] * 6 + [_I, _L] + [_I] * 4 + [_F] + [_P] * 5 + [_S, _P]),

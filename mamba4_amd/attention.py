@@ -17,16 +17,17 @@ them as they are and return bfloat16; any other mix is computed in float32 and
 returned in the values' dtype.  States, decays and sums are float32 or wider.
 """
 
-import ctypes
 from typing import NamedTuple
 
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.memory import _ptr, _stream
+from mamba4_amd.memory import _ptr
 
 MAX_WIDTH = 128
 _MAX_TOKEN_STRIDE = (2**31 - 1) // 256
+_BF16 = torch.bfloat16
+_F32 = torch.float32
 
 
 class LinearAttentionResult(NamedTuple):
@@ -35,26 +36,57 @@ class LinearAttentionResult(NamedTuple):
 
 
 def _f32(t):
-    return t.to(torch.float32).contiguous()
+    return t.to(_F32).contiguous()
+
+
+def _on(device):
+    """Makes the device the current one."""
+    return torch.cuda.device(device)
+
+
+def _same_device(*tensors):
+    device = None
+    for t in tensors:
+        if t is not None and t.device != device:
+            if device is not None or t.device.type != "cuda":
+                devices = sorted({str(u.device) for u in tensors if u is not None})
+                raise ValueError("all tensors must be ROCm device tensors on one device; got "
+                                 + ", ".join(devices))
+            device = t.device
+    return device
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _strided(t):
     """t itself where the kernels can address it: unit stride along the width,
     tokens at least a row apart (views into a fused projection, say); else a
     contiguous copy."""
+    if t.is_contiguous():
+        return t
     unit = t.stride(-1) == 1 or t.shape[-1] == 1
     if unit and t.dim() == 4 and t.shape[1] > 1:
         unit = t.shape[-1] <= t.stride(1) <= _MAX_TOKEN_STRIDE
     return t if unit else t.contiguous()
 
 
-def _rows(t):
+def _row(t):
     """The m4rt_rows of [B,T,h,W] or [B,h,W]; strides of axes of one element are
     never used and given as zero (the token stride, as the width)."""
-    heads, width = t.shape[-2:]
-    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    token = strides[1] if t.dim() == 4 and t.shape[1] > 1 else width
-    return ctypes.byref(_lib.Rows(t.data_ptr(), strides[0], token, strides[-2], heads, width))
+    shape, stride = t.shape, t.stride()
+    width = shape[-1]
+    if len(shape) == 4:
+        token = stride[1] if shape[1] > 1 else width
+    else:
+        token = width
+    return (t.data_ptr(), stride[0] if shape[0] > 1 else 0, token,
+            stride[-2] if shape[-2] > 1 else 0, shape[-2], width)
+
+
+def _qkv(q, k, v):
+    return _lib.pack_qkv(*_row(q), *_row(k), *_row(v))
 
 
 def _workspace(nbytes, device):
@@ -63,21 +95,20 @@ def _workspace(nbytes, device):
 
 def _forward(q, k, v, log_decay, initial, lengths, scale):
     lib = _lib.load()
-    batch, time = q.shape[:2]
-    heads = log_decay.shape[-1]
-    n, p = k.shape[-1], v.shape[-1]
-    bf16 = int(v.dtype == torch.bfloat16)
-    output = torch.empty(batch, time, heads, p, dtype=v.dtype, device=v.device)
-    state = torch.empty(batch, heads, n, p, dtype=torch.float32, device=v.device)
+    batch, time, _, n = q.shape
+    heads, p, device = log_decay.shape[-1], v.shape[-1], v.device
+    bf16 = 1 if v.dtype == _BF16 else 0
+    output = torch.empty((batch, time, heads, p), dtype=v.dtype, device=device)
+    state = torch.empty((batch, heads, n, p), dtype=_F32, device=device)
     nbytes = lib.m4rt_attention_workspace_bytes(batch, time, heads, n, p, bf16)
-    workspace = _workspace(nbytes, v.device)
-    _lib.check(
-        lib.m4rt_attention_forward(
-            _rows(q), _rows(k), _rows(v), bf16, _ptr(log_decay), int(log_decay.dim() == 3),
-            _ptr(lengths), _ptr(initial), scale, batch, time, heads, _ptr(output), _ptr(state),
-            _ptr(workspace), nbytes, _stream(),
-        )
+    workspace = _workspace(nbytes, device)
+    rc = lib.m4rt_attention_forward(
+        _qkv(q, k, v), bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
+        _ptr(initial), scale, batch, time, heads, output.data_ptr(), state.data_ptr(),
+        _ptr(workspace), nbytes, _stream(device),
     )
+    if rc:
+        _lib.check(rc)
     return output, state
 
 
@@ -98,57 +129,50 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, d_output, d_state):
         lib = _lib.load()
         q, k, v, log_decay, initial, lengths, state = ctx.saved_tensors
-        batch, time = q.shape[:2]
-        heads = log_decay.shape[-1]
-        n, p = k.shape[-1], v.shape[-1]
-        bf16 = int(v.dtype == torch.bfloat16)
-        shape = (batch, time, heads, p)
+        batch, time, _, n = q.shape
+        heads, p, device = log_decay.shape[-1], v.shape[-1], v.device
+        bf16 = 1 if v.dtype == _BF16 else 0
         if d_output is None:
-            d_output = torch.zeros(shape, dtype=v.dtype, device=v.device)
+            d_output = torch.zeros((batch, time, heads, p), dtype=v.dtype, device=device)
         d_output = d_output.to(v.dtype).contiguous()
         d_state = None if d_state is None else _f32(d_state)
-        d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
         d_decay = torch.empty_like(log_decay) if ctx.needs_input_grad[3] else None
         d_initial = torch.empty_like(state) if ctx.needs_input_grad[4] else None
         nbytes = lib.m4rt_attention_backward_workspace_bytes(
             batch, time, heads, q.shape[2], k.shape[2], v.shape[2], n, p, bf16)
-        workspace = _workspace(nbytes, v.device)
-        _lib.check(
-            lib.m4rt_attention_backward(
-                _rows(q), _rows(k), _rows(v), bf16, _ptr(log_decay), int(log_decay.dim() == 3),
-                _ptr(lengths), _ptr(initial), ctx.scale, batch, time, heads, _ptr(d_output),
-                _ptr(d_state), _ptr(state), _ptr(d_q), _ptr(d_k), _ptr(d_v), _ptr(d_decay),
-                _ptr(d_initial), _ptr(workspace), nbytes, _stream(),
-            )
+        workspace = _workspace(nbytes, device)
+        rc = lib.m4rt_attention_backward(
+            _qkv(q, k, v), bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
+            _ptr(initial), ctx.scale, batch, time, heads, d_output.data_ptr(), _ptr(d_state),
+            state.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), _ptr(d_decay),
+            _ptr(d_initial), _ptr(workspace), nbytes, _stream(device),
         )
+        if rc:
+            _lib.check(rc)
         return d_q, d_k, d_v, d_decay, d_initial, None, None
 
 
 def _model_rows(name, queries, keys, values, dims):
     """The heads of the call, and q, k, v in one dtype of the kernels."""
-    layout = "[B,T,h,W]" if dims == 4 else "[B,h,W]"
-    lead = dims - 2
-    if any(t.dim() != dims for t in (queries, keys, values)):
+    qs, ks, vs = queries.shape, keys.shape, values.shape
+    if len(qs) != dims or len(ks) != dims or len(vs) != dims:
+        layout = "[B,T,h,W]" if dims == 4 else "[B,h,W]"
         raise ValueError(f"{name} needs queries, keys and values {layout}")
-    if keys.shape[:lead] != queries.shape[:lead] or values.shape[:lead] != queries.shape[:lead]:
+    lead = dims - 2
+    if ks[:lead] != qs[:lead] or vs[:lead] != qs[:lead]:
         raise ValueError("queries, keys and values disagree")
-    if queries.shape[-1] != keys.shape[-1]:
+    if qs[-1] != ks[-1]:
         raise ValueError("queries and keys disagree in width")
-    heads = max(t.shape[-2] for t in (queries, keys, values))
-    if heads == 0 or any(t.shape[-2] == 0 or heads % t.shape[-2] for t in (queries, keys, values)):
+    hq, hk, hv = qs[-2], ks[-2], vs[-2]
+    heads = max(hq, hk, hv)
+    if min(hq, hk, hv) == 0 or heads % hq or heads % hk or heads % hv:
         raise ValueError("the heads of queries, keys and values must divide the largest of them")
-    if not all(1 <= t.shape[-1] <= MAX_WIDTH for t in (keys, values)):
+    if not (1 <= ks[-1] <= MAX_WIDTH and 1 <= vs[-1] <= MAX_WIDTH):
         raise ValueError(f"key and value widths must be 1..{MAX_WIDTH}")
-    if not all(t.dtype == torch.bfloat16 for t in (queries, keys, values)):
-        queries, keys, values = (t.to(torch.float32) for t in (queries, keys, values))
-    return heads, queries, keys, values
-
-
-def _same_device(*tensors):
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1 or any(d.type != "cuda" for d in devices):
-        raise ValueError("all tensors must be ROCm device tensors on one device; got "
-                         + ", ".join(sorted(map(str, devices))))
+    if queries.dtype != _BF16 or keys.dtype != _BF16 or values.dtype != _BF16:
+        queries, keys, values = queries.to(_F32), keys.to(_F32), values.to(_F32)
+    return heads, _strided(queries), _strided(keys), _strided(values)
 
 
 def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=None, scale=1.0):
@@ -165,11 +189,11 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
     [B,H,N,P] float32 after the last token).  A row's result does not depend on
     the batch it is in.
     """
-    _same_device(queries, keys, values, log_decay, initial, lengths)
+    device = _same_device(queries, keys, values, log_decay, initial, lengths)
     heads, q, k, v = _model_rows("linear_attention", queries, keys, values, 4)
     batch, time = queries.shape[:2]
     n, p = keys.shape[-1], values.shape[-1]
-    if tuple(log_decay.shape) not in ((batch, time, heads), (heads,)):
+    if log_decay.shape not in ((batch, time, heads), (heads,)):
         raise ValueError("linear_attention needs log_decay [B,T,H] or [H]")
     if initial is not None and tuple(initial.shape) != (batch, heads, n, p):
         raise ValueError("linear_attention needs initial [B,H,N,P]")
@@ -185,15 +209,17 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
         if initial is not None:
             state = state + initial
         return LinearAttentionResult(output, state)
-    args = (_strided(q), _strided(k), _strided(v), _f32(log_decay),
-            None if initial is None else _f32(initial), lengths, float(scale))
-    with torch.cuda.device(values.device):
-        if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in args[:5]
+    g = _f32(log_decay)
+    s0 = None if initial is None else _f32(initial)
+    scale = float(scale)
+    with _on(device):
+        if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+            or (s0 is not None and s0.requires_grad)
         ):
-            output, state = _Attention.apply(*args)
+            output, state = _Attention.apply(q, k, v, g, s0, lengths, scale)
         else:
-            output, state = _forward(*args)
+            output, state = _forward(q, k, v, g, s0, lengths, scale)
     return LinearAttentionResult(output.to(values.dtype), state)
 
 
@@ -202,9 +228,9 @@ def _step_checks(state, query, key, value, log_decay, active):
     heads, q, k, v = _model_rows("linear_attention_step", query, key, value, 3)
     batch = query.shape[0]
     n, p = key.shape[-1], value.shape[-1]
-    if tuple(state.shape) != (batch, heads, n, p):
+    if state.shape != (batch, heads, n, p):
         raise ValueError("linear_attention_step needs state [B,H,N,P]")
-    if tuple(log_decay.shape) not in ((batch, heads), (heads,)):
+    if log_decay.shape not in ((batch, heads), (heads,)):
         raise ValueError("linear_attention_step needs log_decay [B,H] or [H]")
     if active is not None and (tuple(active.shape) != (batch,) or active.dtype != torch.bool):
         raise ValueError("linear_attention_step needs a boolean active [B]")
@@ -212,21 +238,19 @@ def _step_checks(state, query, key, value, log_decay, active):
 
 
 def _step(state, new_state, q, k, v, log_decay, active, scale, heads, dtype):
-    lib = _lib.load()
-    batch, n, p = q.shape[0], k.shape[-1], v.shape[-1]
-    bf16 = int(v.dtype == torch.bfloat16)
-    output = torch.empty(batch, heads, p, dtype=v.dtype, device=v.device)
-    q, k, v, g = _strided(q), _strided(k), _strided(v), _f32(log_decay)
-    active = None if active is None else active.contiguous()
+    batch, p, device = q.shape[0], v.shape[-1], v.device
+    output = torch.empty((batch, heads, p), dtype=v.dtype, device=device)
     if batch:
-        with torch.cuda.device(output.device):
-            _lib.check(
-                lib.m4rt_attention_step(
-                    _rows(q), _rows(k), _rows(v), bf16, _ptr(g), int(log_decay.dim() == 2),
-                    _ptr(active), float(scale), batch, heads, _ptr(state), _ptr(new_state),
-                    _ptr(output), _stream(),
-                )
+        g = _f32(log_decay)
+        active = None if active is None else active.contiguous()
+        with _on(device):
+            rc = _lib.load().m4rt_attention_step(
+                _qkv(q, k, v), v.dtype == _BF16, g.data_ptr(), g.dim() == 2, _ptr(active),
+                float(scale), batch, heads, state.data_ptr(), new_state.data_ptr(),
+                output.data_ptr(), _stream(device),
             )
+        if rc:
+            _lib.check(rc)
     return LinearAttentionResult(output.to(dtype), new_state)
 
 
@@ -240,8 +264,9 @@ def linear_attention_step(state, query, key, value, log_decay, *, active=None, s
     step is ``linear_attention`` over one token.
     """
     heads, q, k, v = _step_checks(state, query, key, value, log_decay, active)
-    if torch.is_grad_enabled() and any(
-        t.requires_grad for t in (state, query, key, value, log_decay)
+    if torch.is_grad_enabled() and (
+        state.requires_grad or query.requires_grad or key.requires_grad or value.requires_grad
+        or log_decay.requires_grad
     ):
         decay = log_decay if log_decay.dim() == 1 else log_decay[:, None]
         one = linear_attention(query[:, None], key[:, None], value[:, None], decay, initial=state,
@@ -258,8 +283,9 @@ def linear_attention_step_(state, query, key, value, log_decay, *, active=None, 
     heads, q, k, v = _step_checks(state, query, key, value, log_decay, active)
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("linear_attention_step_ needs a contiguous float32 state")
-    if torch.is_grad_enabled() and any(
-        t.requires_grad for t in (state, query, key, value, log_decay)
+    if torch.is_grad_enabled() and (
+        state.requires_grad or query.requires_grad or key.requires_grad or value.requires_grad
+        or log_decay.requires_grad
     ):
         raise ValueError("linear_attention_step_ has no gradient; use linear_attention_step")
     # The state may be saved for a backward: the write counts as one of torch's.

@@ -13,8 +13,12 @@
 #include "norm.hpp"
 
 namespace la {
-template <typename In, int NT, bool OUT, bool WHOLE>
+template <typename In, int NT, bool WHOLE>
 __global__ void attention_kernel(Args);
+template <typename In, int NT, bool WHOLE>
+__global__ void attention_states_kernel(Args);
+template <typename In, int NP, int NN, bool DOTS, bool WHOLE>
+__global__ void attention_backward_kernel(Args);
 __global__ void carry_kernel(Args);
 __global__ void decay_grad_kernel(DecayGrad);
 __global__ void decay_heads_kernel(const double*, int, int, float*);
@@ -80,8 +84,23 @@ bool bad_workspace(const void* base, size_t given, size_t need, std::string* why
 struct Shape {
   int B, T, H, N, P, bf16;
   int chunks() const { return (T + la::C - 1) / la::C; }
-  int segments() const { return (chunks() + la::SEG - 1) / la::SEG; }
 };
+
+int tiles_of(int width) { return (width + la::TILE - 1) / la::TILE; }
+
+// Chunks of a segment, by the chunk-tiles of one row (`blocks` tiles a head):
+// 4 while a segment is latency, up to 16 where the segments' states are traffic.
+// It does not depend on the batch (segments decide the bits).  Forward, 4 / 8 / 16:
+// T2000 H12 N64 P128 34 / 37 / 58 us, T32768 H16 N128 P128 342 / 299 / 292.
+int segment(const Shape& s, int blocks) {
+  const long each = (long)s.chunks() * s.H * blocks / 768;
+  return each >= 16 ? 16 : each >= 8 ? 8 : 4;
+}
+
+int segments(const Shape& s, int blocks) {
+  const int seg = segment(s, blocks);
+  return (s.chunks() + seg - 1) / seg;
+}
 
 bool bad_shape(const Shape& s, std::string* why) {
   if (s.B <= 0 || s.T <= 0 || s.H <= 0) {
@@ -93,30 +112,40 @@ bool bad_shape(const Shape& s, std::string* why) {
     return true;
   }
   // Grids: blocks of at most six tiles a (b, h), segments along y.
-  if ((double)s.B * s.H * 6 + 64 > INT_MAX / 2 || s.segments() > 65535 || s.T > INT_MAX - 4096) {
+  if ((double)s.B * s.H * 6 + 64 > INT_MAX / 2 || s.T > INT_MAX / 16) {
     *why = "problem too large";
     return true;
   }
   return false;
 }
 
-int tiles_of(int width) { return (width + la::TILE - 1) / la::TILE; }
-
 // Whether the sequences are split into segments (their states formed first,
-// then carried, then all walked at once) instead of walked from end to end.
-// M4RT_ATTENTION = "walk" or "split" overrides the choice; the bits are the same.
+// then carried, then all walked at once) instead of walked from end to end.  A walk
+// takes a step's latency a chunk, and more once the card has more than a block a
+// compute unit; a split run three launches, a segment's latency twice, and about
+// 1.6 times the steps' throughput.  Forward, walk / split: bfloat16 N64 P128 H12 B4
+// T2000 68 / 46 us, B8 T1024 37 / 46, B16 T1024 53 / 78; float32 B4 T1024 69 / 51, B8
+// T1024 72 / 81.  M4RT_ATTENTION = "walk" or "split" overrides the choice; the bits are
+// the same.
 bool attention_splits(const Shape& s, int blocks) {
-  if (s.segments() < 2) return false;
+  if (segments(s, blocks) < 2) return false;
   if (const char* mode = std::getenv("M4RT_ATTENTION")) {
     if (std::strcmp(mode, "walk") == 0) return false;
     if (std::strcmp(mode, "split") == 0) return true;
   }
-  return (long)s.B * s.H * blocks < 2L * m4::api_compute_units();
+  const bool wide = s.N > 64 || (blocks > tiles_of(s.P) && s.P > 64);
+  const double step = (s.bf16 ? 2.1 : 4.1) * (wide ? 1.5 : 1.0);  // us a chunk
+  const double units = m4::api_compute_units(), walks = (double)s.B * s.H * blocks;
+  const double walk = s.chunks() * step * std::max(1.0, 0.95 * walks / units);
+  const double split =
+      8.0 + 1.6 * step * std::max<double>(segment(s, blocks), s.chunks() * walks / (1.05 * units));
+  return split < walk;
 }
 
-// A split run's states of one role (n keys wide, `tiles` blocks of values).
-void take_states(Carver& c, const Shape& s, int n, int tiles, bool split, la::Role* role) {
-  const size_t slots = split ? (size_t)tiles * s.B * s.H * s.segments() : 0;
+// A split run's states of one role (n keys wide, `tiles` blocks of values); no
+// segments: not split.
+void take_states(Carver& c, const Shape& s, int n, int tiles, int segments, la::Role* role) {
+  const size_t slots = (size_t)tiles * s.B * s.H * segments;
   role->starts = c.take<float>(slots * tiles_of(n) * la::TILE * la::TILE);
   role->decays = c.take<float>(slots);
 }
@@ -133,7 +162,7 @@ la::Rows rows_of(const m4rt_rows& r, int H, int bf16) {
 }
 
 bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why) {
-  if (!r || !r->data) {
+  if (!r->data) {
     *why = "a required pointer is NULL";
     return true;
   }
@@ -162,54 +191,81 @@ int wide_keys(const la::Args& a) {
   return 1;
 }
 
-template <typename In, int NT, bool OUT>
-void start_attention(const la::Args& a, dim3 grid, hipStream_t st) {
-  bool whole = true;
-  for (int i = 0; i < a.roles; ++i) {
-    const la::Role& r = a.role[i];
-    whole = whole && r.q.whole && r.k.whole && r.v.whole && (!r.dots || r.e.whole);
-  }
-  if (whole)
-    hipLaunchKernelGGL((la::attention_kernel<In, NT, OUT, true>), grid, dim3(la::THREADS), 0, st,
-                       a);
+template <typename In, bool WHOLE>
+void start_states(const la::Args& a, dim3 grid, hipStream_t st) {
+  const dim3 block(64 * la::WAVES);
+  if (wide_keys(a) == 1)
+    hipLaunchKernelGGL((la::attention_states_kernel<In, 1, WHOLE>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((la::attention_kernel<In, NT, OUT, false>), grid, dim3(la::THREADS), 0, st,
-                       a);
+    hipLaunchKernelGGL((la::attention_states_kernel<In, 2, WHOLE>), grid, block, 0, st, a);
 }
 
-template <bool OUT>
-void launch_attention(const la::Args& a, int bf16, dim3 grid, hipStream_t st) {
-  const int nt = wide_keys(a);
-  if (bf16) {
-    nt == 1 ? start_attention<la::bf16_t, 1, OUT>(a, grid, st)
-            : start_attention<la::bf16_t, 2, OUT>(a, grid, st);
-  } else {
-    nt == 1 ? start_attention<float, 1, OUT>(a, grid, st)
-            : start_attention<float, 2, OUT>(a, grid, st);
+template <typename In, int NP, int NN, bool WHOLE>
+void start_backward(const la::Args& a, dim3 grid, hipStream_t st) {
+  const dim3 block(128 * la::WAVES);
+  if (a.role[0].dots)
+    hipLaunchKernelGGL((la::attention_backward_kernel<In, NP, NN, true, WHOLE>), grid, block, 0,
+                       st, a);
+  else
+    hipLaunchKernelGGL((la::attention_backward_kernel<In, NP, NN, false, WHOLE>), grid, block, 0,
+                       st, a);
+}
+
+template <typename In, bool WHOLE>
+void start_outputs(const la::Args& a, dim3 grid, hipStream_t st) {
+  const dim3 block(128 * la::WAVES);
+  if (a.roles == 1) {
+    if (a.role[0].n <= 64)
+      hipLaunchKernelGGL((la::attention_kernel<In, 1, WHOLE>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((la::attention_kernel<In, 2, WHOLE>), grid, block, 0, st, a);
+    return;
   }
+  const bool wide_p = a.role[0].n > 64, wide_n = a.role[2].n > 64;
+  if (wide_p)
+    wide_n ? start_backward<In, 2, 2, WHOLE>(a, grid, st)
+           : start_backward<In, 2, 1, WHOLE>(a, grid, st);
+  else
+    wide_n ? start_backward<In, 1, 2, WHOLE>(a, grid, st)
+           : start_backward<In, 1, 1, WHOLE>(a, grid, st);
+}
+
+template <typename In, bool WHOLE>
+int start_attention(const la::Args& a, hipStream_t st) {
+  const unsigned x = (unsigned)((a.B * a.H + 7) / 8 * 8 * a.blocks);
+  if (a.split) {
+    int rc = api_launch("attention_states", st,
+                        [&] { start_states<In, WHOLE>(a, dim3(x, a.NS), st); });
+    if (rc) return rc;
+    rc = api_launch("attention_carry", st, [&] {
+      hipLaunchKernelGGL(la::carry_kernel, dim3(x, 4 * wide_keys(a)), dim3(64 * la::WAVES), 0, st,
+                         a);
+    });
+    if (rc) return rc;
+  }
+  return api_launch("attention", st,
+                    [&] { start_outputs<In, WHOLE>(a, dim3(x, a.split ? a.NS : 1), st); });
 }
 
 int run_attention(la::Args& a, const Shape& s, bool split, hipStream_t st) {
   a.blocks = 0;
-  for (int i = 0; i < a.roles; ++i) a.blocks += a.role[i].tiles;
+  bool whole = true;
+  for (int i = 0; i < a.roles; ++i) {
+    const la::Role& r = a.role[i];
+    a.blocks += r.tiles;
+    whole = whole && r.q.whole && r.k.whole && r.v.whole && (!r.dots || r.e.whole);
+  }
   a.B = s.B;
   a.T = s.T;
   a.H = s.H;
   a.NC = s.chunks();
-  a.NS = s.segments();
-  const unsigned x = (unsigned)((s.B * s.H + 7) / 8 * 8 * a.blocks);
-  if (split) {
-    int rc = api_launch("attention_states", st,
-                        [&] { launch_attention<false>(a, s.bf16, dim3(x, a.NS), st); });
-    if (rc) return rc;
-    rc = api_launch("attention_carry", st, [&] {
-      hipLaunchKernelGGL(la::carry_kernel, dim3(x, 4 * wide_keys(a)), dim3(la::THREADS), 0, st, a);
-    });
-    if (rc) return rc;
-  }
-  return api_launch("attention", st, [&] {
-    launch_attention<true>(a, s.bf16, dim3(x, split ? a.NS : 1), st);
-  });
+  a.seg = segment(s, a.blocks);
+  a.NS = segments(s, a.blocks);
+  a.split = split;
+  if (s.bf16)
+    return whole ? start_attention<la::bf16_t, true>(a, st)
+                 : start_attention<la::bf16_t, false>(a, st);
+  return whole ? start_attention<float, true>(a, st) : start_attention<float, false>(a, st);
 }
 
 struct Backward {
@@ -226,7 +282,8 @@ size_t backward_workspace(const Shape& s, const int heads[3], void* base, Backwa
   Carver c{static_cast<char*>(base)};
   const int n[3] = {s.P, s.P, s.N}, p[3] = {s.N, s.N, s.P};
   const size_t rows = (size_t)s.B * s.T * s.H;
-  const bool split = attention_splits(s, backward_tiles(s));
+  const int blocks = backward_tiles(s);
+  const int split = attention_splits(s, blocks) ? segments(s, blocks) : 0;
   for (int i = 0; i < 3; ++i) {
     take_states(c, s, n[i], tiles_of(p[i]), split, &out->role[i]);
     out->part[i] = c.take<float>(heads[i] == s.H ? 0 : rows * p[i]);
@@ -247,18 +304,21 @@ size_t m4rt_attention_workspace_bytes(int B, int T, int H, int N, int P, int bf1
   if (bad_shape(s, &why)) return 0;
   Carver c{nullptr};
   la::Role role{};
-  take_states(c, s, N, tiles_of(P), attention_splits(s, tiles_of(P)), &role);
+  const int blocks = tiles_of(P);
+  take_states(c, s, N, blocks, attention_splits(s, blocks) ? segments(s, blocks) : 0, &role);
   return c.used;
 }
 
-int m4rt_attention_forward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
-                           const float* log_decay, int per_token, const int* lengths,
-                           const float* initial, float scale, int B, int T, int H, void* output,
-                           float* state, void* workspace, size_t workspace_bytes, void* stream) {
+int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
+                           const int* lengths, const float* initial, float scale, int B, int T,
+                           int H, void* output, float* state, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   const char* name = "m4rt_attention_forward";
   return m4::api_entry(name, [&] {
     const std::string at = std::string(name) + ": ";
-    const Shape s{B, T, H, q ? q->width : 0, v ? v->width : 0, bf16};
+    if (!rows) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
+    const Shape s{B, T, H, q->width, v->width, bf16};
     std::string why;
     if (bad_shape(s, &why) || bad_rows(q, H, bf16, true, &why) || bad_rows(k, H, bf16, true, &why) ||
         bad_rows(v, H, bf16, true, &why))
@@ -269,7 +329,7 @@ int m4rt_attention_forward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_ro
     la::Role& r = a.role[0];
     const bool split = attention_splits(s, tiles_of(s.P));
     Carver c{static_cast<char*>(workspace)};
-    take_states(c, s, s.N, tiles_of(s.P), split, &r);
+    take_states(c, s, s.N, tiles_of(s.P), split ? segments(s, tiles_of(s.P)) : 0, &r);
     if (bad_workspace(workspace, workspace_bytes, c.used, &why))
       return api_fail(M4MR_EINVAL, at + why);
     r.q = rows_of(*q, H, bf16);
@@ -303,16 +363,17 @@ size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads,
   return backward_workspace(s, heads, nullptr, &w);
 }
 
-int m4rt_attention_backward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
-                            const float* log_decay, int per_token, const int* lengths,
-                            const float* initial, float scale, int B, int T, int H,
-                            const void* d_output, const float* d_state, const float* state,
+int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_decay,
+                            int per_token, const int* lengths, const float* initial, float scale,
+                            int B, int T, int H, const void* d_output, const float* d_state, const float* state,
                             void* d_q, void* d_k, void* d_v, float* d_log_decay, float* d_initial,
                             void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "m4rt_attention_backward";
   return m4::api_entry(name, [&] {
     const std::string at = std::string(name) + ": ";
-    const Shape s{B, T, H, q ? q->width : 0, v ? v->width : 0, bf16};
+    if (!rows) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
+    const Shape s{B, T, H, q->width, v->width, bf16};
     std::string why;
     if (bad_shape(s, &why) || bad_rows(q, H, bf16, true, &why) || bad_rows(k, H, bf16, true, &why) ||
         bad_rows(v, H, bf16, true, &why))
@@ -409,14 +470,15 @@ int m4rt_attention_backward(const m4rt_rows* q, const m4rt_rows* k, const m4rt_r
   });
 }
 
-int m4rt_attention_step(const m4rt_rows* q, const m4rt_rows* k, const m4rt_rows* v, int bf16,
-                        const float* log_decay, int per_token, const uint8_t* active, float scale,
-                        int B, int H, const float* state, float* new_state, void* output,
-                        void* stream) {
+int m4rt_attention_step(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
+                        const uint8_t* active, float scale, int B, int H, const float* state,
+                        float* new_state, void* output, void* stream) {
   const char* name = "m4rt_attention_step";
   return m4::api_entry(name, [&] {
     const std::string at = std::string(name) + ": ";
-    const Shape s{B, 1, H, q ? q->width : 0, v ? v->width : 0, bf16};
+    if (!rows) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
+    const Shape s{B, 1, H, q->width, v->width, bf16};
     std::string why;
     if (bad_shape(s, &why) || bad_rows(q, H, bf16, false, &why) ||
         bad_rows(k, H, bf16, false, &why) || bad_rows(v, H, bf16, false, &why))

@@ -13,15 +13,16 @@
 //   dg_t = <S_T, R_T> + sum over i >= t of (q_i . dq_i - k_i . dk_i),
 // which sums (q_i . k_j)(do_i . v_j) scale e^{P_i - P_j} over pairs i >= t > j
 // (the pairs i = j are in both products and left out of both).
-// So one kernel serves all of them ("roles"); a block walks the chunks of one
+// So one body serves all of them ("roles"); a block walks the chunks of one
 // (b, h) for 64 columns of the values, keeping the state in registers.
 //
 // Products run on bfloat16 MFMA with float32 accumulation.  An operand is a sum of
 // bfloat16 planes: a bfloat16 input is one plane; what is computed
 // in float32 (A, S, the weighted K) is two planes beside bfloat16 inputs
-// (2^-17 of the value left out, far below the rounding of a bfloat16 result and
-// near float32 for the states and dg); float32 inputs and what is computed from
-// them are three planes (all 24 bits) with the six largest plane products:
+// (2^-17 of the value left out: below the rounding of a bfloat16 result and near
+// float32 for the states and dg; one plane for A and S saved a tenth of the time and
+// left an error like that rounding's own); float32 inputs and what is computed
+// from them are three planes (all 24 bits) with the six largest plane products:
 // a sixth of the bfloat16 rate, 2.7 times that of float32 MFMA.
 #include <hip/hip_runtime.h>
 
@@ -239,15 +240,17 @@ __device__ __forceinline__ Quad<float> load_quad(Rsrc r, unsigned row, int col, 
 // rows padded by 16 bytes instead, both took twice the cycles).
 __device__ __forceinline__ int unit(int row, int u) { return 64 * row + 8 * (u ^ (row & 7)); }
 
+// OUT: outputs are formed (else only states).
 template <typename In, int NT, bool OUT>
 struct Shared {
-  alignas(16) bf16_t k[Type<In>::IN][NT][C * 64];       // K [token][n]
-  alignas(16) bf16_t v[Type<In>::IN][1][C * TILE];      // V [token][column]
+  alignas(16) bf16_t k[Type<In>::IN][NT][C * 64];                 // K [token][n]
+  alignas(16) bf16_t v[Type<In>::IN][1][C * TILE];                // V [token][column]
   alignas(16) bf16_t s[Type<In>::MADE][NT][OUT ? TILE * 64 : 8];  // S^T [column][n]
   // Each wave's own, of the chunk's tokens: the running log2 decay in two
-  // parts, the decays between a token and the wave's strip, and the weights of the
-  // tokens in the next state.
-  alignas(16) float ph[WAVES][C], pl[WAVES][C], far[WAVES][C], update[WAVES][C];
+  // parts and the decays between a token and the wave's strip (outputs), and the
+  // weights of the tokens in the next state (states).
+  alignas(16) float ph[OUT ? WAVES : 1][C], pl[OUT ? WAVES : 1][C], far[OUT ? WAVES : 1][C];
+  alignas(16) float update[WAVES][C];
 };
 
 __device__ __forceinline__ Frag<1> cat(s4 a, s4 b) {
@@ -352,31 +355,36 @@ __device__ __forceinline__ float sum_groups(float x) {
 // that e^{P_i - P_j} of near tokens is exact to float32 after any decay before them.
 // A log decay below -2000 (-infinity, a type's lowest value) counts as -2000: its
 // exponential is zero either way and the differences behind it stay finite.
-//
-// Between strips of 16 tokens the decay is taken in two factors, from the key to
-// the near end of the query's strip (`far`, a table) and on to the query (`near`):
-// for decays below one neither can overflow, and the product costs two
-// multiplications a score instead of an exponential.
-struct Decays {
+__device__ __forceinline__ double running(float g) {
+  return wave_prefix((double)(g < -2000.f ? -2000.f : g) * 1.4426950408889634);
+}
+
+// For the outputs of strip w.  Between strips of 16 tokens the decay is taken in
+// two factors, from the key to the near end of the query's strip (`far`, a table)
+// and on to the query (`near`): for decays below one neither can overflow, and the
+// product costs two multiplications a score instead of an exponential.
+struct Reach {
   float inter;  // of this lane's token: the state's part in its output
   float near;   // from the near end of the wave's strip (tokens of the strip)
-  float chunk;  // of the whole chunk
 };
 template <bool REV>
-__device__ __forceinline__ Decays chunk_decays(float (&ph)[C], float (&pl)[C], float (&far)[C],
-                                               float (&weights)[C], float g, int lane, int w,
-                                               float update) {
-  const double p = wave_prefix((double)(g < -2000.f ? -2000.f : g) * 1.4426950408889634);
-  const double last = lane_double(p, 63), edge = lane_double(p, REV ? 16 * w + 15 : 16 * w);
+__device__ __forceinline__ Reach reach(float (&ph)[C], float (&pl)[C], float (&far)[C], float g,
+                                       int lane, int w) {
+  const double p = running(g), edge = lane_double(p, REV ? 16 * w + 15 : 16 * w);
   const float high = (float)p, to_edge = (float)(REV ? p - edge : edge - p);
-  const float head = __builtin_amdgcn_exp2f(high);
-  const float tail = __builtin_amdgcn_exp2f((float)(last - p));
   ph[lane] = high;
   pl[lane] = (float)(p - high);
   far[lane] = __builtin_amdgcn_exp2f(to_edge);
-  weights[lane] = update * (REV ? head : tail);
-  return Decays{REV ? tail : head, __builtin_amdgcn_exp2f(-to_edge),
-                __builtin_amdgcn_exp2f((float)last)};
+  return Reach{__builtin_amdgcn_exp2f(REV ? (float)(lane_double(p, 63) - p) : high),
+               __builtin_amdgcn_exp2f(-to_edge)};
+}
+
+// For the state: the tokens' weights; returns the chunk's decay.
+template <bool REV>
+__device__ __forceinline__ float weigh(float (&weights)[C], float g, int lane, float update) {
+  const double p = running(g), last = lane_double(p, 63);
+  weights[lane] = update * __builtin_amdgcn_exp2f((float)(REV ? p : last - p));
+  return __builtin_amdgcn_exp2f((float)last);
 }
 
 // Four consecutive columns of a token's output, `left` of them within the width.
@@ -421,112 +429,219 @@ __device__ __forceinline__ Rsrc chunk_rows(const Source& x, int c, int rows) {
               rows > 0 ? (rows - 1) * (int)x.stride + x.bytes : 0);
 }
 
-// One block: 64 value columns of one (b, h), the chunks c0..c1-1 (in reverse
-// if role.rev).  OUT: outputs from the state at the first chunk; else only the
-// segment's own state from zero, for split runs.
+// What a block does: 64 value columns of one (b, h), the chunks c0..c1-1 (in
+// reverse if REV).
 //
-// A segment of SEG chunks keeps its own state (from zero) apart from the
+// A segment of a.seg chunks keeps its own state (from zero) apart from the
 // state at its start; the state in use is decay * start + own.  So a split run, whose
 // blocks take one segment each, has the bits of a walk over all of them.
-template <typename In, int NT, bool OUT, bool WHOLE, bool REV>
-__device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int b, int h, int c0,
-                                     int c1, int seg, Shared<In, NT, OUT>& sh) {
-  constexpr int IN = Type<In>::IN, MADE = Type<In>::MADE;
-  constexpr int KP = 2 * NT;  // pieces of K a thread loads
-  constexpr int GROUP = IN > 1 ? 2 : 4;  // products between which no wait is needed
-  const In* tag = nullptr;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col0 = TILE * tile, bh = b * a.H + h;
-  const int length = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-  const int count = c1 - c0;
+template <typename In, int NT, bool WHOLE, bool REV>
+struct Block {
+  static constexpr int IN = Type<In>::IN, MADE = Type<In>::MADE;
+  static constexpr int KP = 2 * NT;               // pieces of K a thread loads
+  static constexpr int GROUP = IN > 1 ? 2 : 4;    // products between which no wait is needed
+  const Args& a;
+  const Role& R;
+  int tile, b, h, w;
+  int col0, bh, length;
+  const float* gs;
 
-  // The state's accumulators: n = 64 nt + 16 w + 4 g + q, column 16 pb + r.
-  f4 start[NT][4], own[NT][4];
-  int tid = thread();
-  int lane = tid & 63, g = lane >> 4, r = lane & 15;
-  float since = 1.f;  // decay since the segment's start
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int pb = 0; pb < 4; ++pb) {
-      own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
-      start[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (OUT) {
-        if (seg >= 0) {
-          const long slot = ((long)(tile * a.B * a.H + bh) * a.NS + seg) * (NT * 4096);
-          start[nt][pb] = *reinterpret_cast<const f4*>(
-              R.starts + slot + ((nt * 4 + pb) * THREADS + tid) * 4);
-        } else if (R.initial.base) {
-          const float* s = R.initial.base + (long)bh * R.n * R.p;
-          const int p = col0 + 16 * pb + r;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int n = 64 * nt + 16 * w + 4 * g + q;
-            if (n < R.n && p < R.p)
-              start[nt][pb][q] = s[(long)n * R.initial.sn + (long)p * R.initial.sp];
-          }
-        }
-      }
-    }
-
-  const Source ks = source<In>(R.k, b, h), vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h),
-               es = source<In>(R.e, b, h);
-  const float* gs = a.g + b * a.gb + h;
-  const long gt = a.gt;
-  Piece<In> kraw[KP], vraw[2], qraw[2 * NT];
-  float graw = 0.f;
-  auto fetch = [&](int c) {
-    const int have = min(length - c * C, C);
-    const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
-    const int vcol = 8 * (tid & 7), vrow = tid >> 3;
-    const Rsrc kr = chunk_rows(ks, c, have);
+  __device__ __forceinline__ Block(const Args& args, const Role& role, int tile_, int b_, int h_)
+      : a(args), R(role), tile(tile_), b(b_), h(h_) {
+    w = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & (WAVES - 1));
+    col0 = TILE * tile;
+    bh = b * a.H + h;
+    length = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    gs = a.g + b * a.gb + h;
+  }
+  __device__ __forceinline__ int have(int c) const { return min(length - c * C, C); }
+  __device__ __forceinline__ float decay(int c, int lane) const {
+    return lane < have(c) ? gs[((long)c * C + lane) * a.gt] : 0.f;
+  }
+  __device__ __forceinline__ void fetch_k(Piece<In> (&raw)[KP], const Source& src, int c, int t) {
+    const int col = 8 * (t & (8 * NT - 1)), row = t / (8 * NT);
+    const Rsrc r = chunk_rows(src, c, have(c));
 #pragma unroll
     for (int i = 0; i < KP; ++i)
-      kraw[i] = load_piece<WHOLE>(kr, (krow + 32 / NT * i) * ks.stride, kcol, R.n, tag);
-    const Rsrc vr = chunk_rows(vs, c, have);
+      raw[i] = load_piece<WHOLE>(r, (row + 32 / NT * i) * src.stride, col, R.n, (const In*)nullptr);
+  }
+  __device__ __forceinline__ void fetch_v(Piece<In> (&raw)[2], const Source& src, int c, int t) {
+    const int col = 8 * (t & 7), row = t >> 3;
+    const Rsrc r = chunk_rows(src, c, have(c));
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      vraw[i] = load_piece<WHOLE>(vr, (vrow + 32 * i) * vs.stride, col0 + vcol, R.p, tag);
-    if constexpr (OUT) {
-      const Rsrc qr = chunk_rows(qs, c, have);
+      raw[i] = load_piece<WHOLE>(r, (row + 32 * i) * src.stride, col0 + col, R.p,
+                                 (const In*)nullptr);
+  }
+  template <typename Sh>
+  __device__ __forceinline__ void stage_k(Sh& sh, const Piece<In> (&raw)[KP], int t) {
+    const int col = 8 * (t & (8 * NT - 1)), row = t / (8 * NT);
 #pragma unroll
-      for (int kk = 0; kk < 2 * NT; ++kk)
-        qraw[kk] = load_piece<WHOLE>(qr, (16 * w + r) * qs.stride, 32 * kk + 8 * g, R.n, tag);
+    for (int i = 0; i < KP; ++i) {
+      const Frag<IN> f = planes(raw[i]);
+#pragma unroll
+      for (int j = 0; j < IN; ++j)
+        *reinterpret_cast<u4*>(&sh.k[j][col >> 6][unit(row + 32 / NT * i, (col >> 3) & 7)]) =
+            __builtin_bit_cast(u4, f.p[j]);
     }
-    graw = lane < have ? gs[((long)c * C + lane) * gt] : 0.f;
-  };
+  }
+  template <typename Sh>
+  __device__ __forceinline__ void stage_v(Sh& sh, const Piece<In> (&raw)[2], int t) {
+    const int col = 8 * (t & 7), row = t >> 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Frag<IN> f = planes(raw[i]);
+#pragma unroll
+      for (int j = 0; j < IN; ++j)
+        *reinterpret_cast<u4*>(&sh.v[j][0][unit(row + 32 * i, col >> 3)]) =
+            __builtin_bit_cast(u4, f.p[j]);
+    }
+  }
 
-  if (count > 0) fetch(REV ? c1 - 1 : c0);
-  for (int it = 0; it < count; ++it) {
-    const int c = REV ? c1 - 1 - it : c0 + it;
-    const int t0 = c * C, have = min(length - t0, C);
-    tid = thread();
-    lane = tid & 63, g = lane >> 4, r = lane & 15;
-    Frag<IN> qf[2 * NT];
-    Decays d{};
-    Quad<In> e[4];
-    if (have > 0) {
-      // K, V, the state and the decays to LDS.
-      const int kcol = 8 * (tid & (8 * NT - 1)), krow = tid / (8 * NT);
-      const int vcol = 8 * (tid & 7), vrow = tid >> 3;
+  // The blocks of 16 keys in turn from a wave's own strip, into the past (REV:
+  // the future) and round: the first `seen` of them reach the strip's queries.
+  __device__ __forceinline__ static int seen(int strip) { return REV ? WAVES - strip : strip + 1; }
+  __device__ __forceinline__ static int block(int strip, int i) {
+    return (REV ? strip + i : strip - i) & (WAVES - 1);
+  }
+  // The strip, opaque, so that the addresses that follow from it are not kept in
+  // registers over the loop.
+  __device__ __forceinline__ int opaque_strip() const {
+    int strip = w;
+    asm volatile("" : "+s"(strip));
+    return strip;
+  }
+
+  // State rows n = 64 nt + 16 w + 4 g + q, columns 16 pb + r: own <- decay own +
+  // weighted K^T V.
+  template <typename Sh>
+  __device__ __forceinline__ void advance(Sh& sh, f4 (&own)[NT][4], float decay, int g, int r) {
+    const int strip = opaque_strip();
 #pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const Frag<IN> f = planes(kraw[i]);
-        const int row = krow + 32 / NT * i;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < IN; ++j)
-          *reinterpret_cast<u4*>(&sh.k[j][kcol >> 6][unit(row, (kcol >> 3) & 7)]) =
-              __builtin_bit_cast(u4, f.p[j]);
+      for (int pb = 0; pb < 4; ++pb) own[nt][pb] *= decay;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int ja = block(strip, 2 * s), jb = block(strip, 2 * s + 1);
+      const f4 ua = *reinterpret_cast<const f4*>(&sh.update[w][16 * ja + 4 * g]);
+      const f4 ub = *reinterpret_cast<const f4*>(&sh.update[w][16 * jb + 4 * g]);
+      const float wt[8] = {ua[0], ua[1], ua[2], ua[3], ub[0], ub[1], ub[2], ub[3]};
+      Frag<MADE> kw[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        kw[nt] = weighted<MADE>(columns<IN, NT>(sh.k, nt, ja, jb, w, g, r), wt);
+#pragma unroll
+      for (int p0 = 0; p0 < 4; p0 += GROUP) {
+        Frag<IN> vf[GROUP];
+#pragma unroll
+        for (int pb = 0; pb < GROUP; ++pb)
+          vf[pb] = columns<IN, 1>(sh.v, 0, ja, jb, p0 + pb, g, r);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma(kw[nt], vf, &own[nt][p0]);
       }
+    }
+  }
+
+  __device__ __forceinline__ float* slot(int seg) const {
+    return R.starts + ((long)(tile * a.B * a.H + bh) * a.NS + seg) * (NT * 4096);
+  }
+
+  // Split runs: the segment's own state, from zero, and its decay.  Four waves.
+  __device__ __forceinline__ void states(int seg, int c0, int c1, Shared<In, NT, false>& sh) {
+    f4 own[NT][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Frag<IN> f = planes(vraw[i]);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < IN; ++j)
-          *reinterpret_cast<u4*>(&sh.v[j][0][unit(vrow + 32 * i, vcol >> 3)]) =
-              __builtin_bit_cast(u4, f.p[j]);
+      for (int pb = 0; pb < 4; ++pb) own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
+    float since = 1.f;
+    const Source ks = source<In>(R.k, b, h), vs = source<In>(R.v, b, h);
+    Piece<In> kraw[KP], vraw[2];
+    float graw;
+    auto fetch = [&](int c) {
+      const int t = thread();
+      fetch_k(kraw, ks, c, t);
+      fetch_v(vraw, vs, c, t);
+      graw = decay(c, t & 63);
+    };
+    fetch(REV ? c1 - 1 : c0);
+    for (int it = 0; it < c1 - c0; ++it) {
+      const int c = REV ? c1 - 1 - it : c0 + it;
+      const int t = thread(), lane = t & 63;
+      float whole = 1.f;
+      if (have(c) > 0) {
+        stage_k(sh, kraw, t);
+        stage_v(sh, vraw, t);
+        whole = weigh<REV>(sh.update[w], graw, lane, R.update);
       }
-      if constexpr (OUT) {
+      __syncthreads();
+      if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
+      if (have(c) > 0) {
+        since *= whole;
+        advance(sh, own, whole, lane >> 4, lane & 15);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb)
+        *reinterpret_cast<f4*>(slot(seg) + ((nt * 4 + pb) * 64 * WAVES + threadIdx.x) * 4) =
+            own[nt][pb];
+    if (threadIdx.x == 0) R.decays[(long)(tile * a.B * a.H + bh) * a.NS + seg] = since;
+  }
+
+  // Outputs from the state at the first chunk.  Eight waves: four form the
+  // outputs of a strip of 16 tokens each, four keep the state (16 rows of its n
+  // and of every 64 each), so that a chunk's two halves run beside each other.
+  template <bool DOTS>
+  __device__ __forceinline__ void outputs(int seg, int c0, int c1, Shared<In, NT, true>& sh) {
+    if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < WAVES)
+      write_outputs<DOTS>(c0, c1, sh);
+    else
+      keep_state(seg, c0, c1, sh);
+  }
+
+  __device__ __forceinline__ void keep_state(int seg, int c0, int c1, Shared<In, NT, true>& sh) {
+    f4 start[NT][4], own[NT][4];
+    float since = 1.f;  // decay since the segment's start
+    {
+      const int t = thread() & (64 * WAVES - 1), g = (t >> 4) & 3, r = t & 15;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb) {
+          own[nt][pb] = start[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
+          if (seg >= 0) {
+            start[nt][pb] = *reinterpret_cast<const f4*>(
+                slot(seg) + ((nt * 4 + pb) * 64 * WAVES + t) * 4);
+          } else if (R.initial.base) {
+            const float* s = R.initial.base + (long)bh * R.n * R.p;
+            const int p = col0 + 16 * pb + r;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int n = 64 * nt + 16 * w + 4 * g + q;
+              if (n < R.n && p < R.p)
+                start[nt][pb][q] = s[(long)n * R.initial.sn + (long)p * R.initial.sp];
+            }
+          }
+        }
+    }
+    const Source ks = source<In>(R.k, b, h);
+    Piece<In> kraw[KP];
+    float graw;
+    auto fetch = [&](int c) {
+      const int t = thread() & (64 * WAVES - 1);
+      fetch_k(kraw, ks, c, t);
+      graw = decay(c, t & 63);
+    };
+    fetch(REV ? c1 - 1 : c0);
+    for (int it = 0; it < c1 - c0; ++it) {
+      const int c = REV ? c1 - 1 - it : c0 + it;
+      const int t = thread() & (64 * WAVES - 1), lane = t & 63, g = lane >> 4, r = lane & 15;
+      float whole = 1.f;
+      if (have(c) > 0) {
+        stage_k(sh, kraw, t);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -543,36 +658,88 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
                   &sh.s[j][nt][64 * 16 * pb + unit(r, 2 * w + (g >> 1)) + 4 * (g & 1)]) =
                   u2{lo[j], hi[j]};
           }
-#pragma unroll
-        for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
+        whole = weigh<REV>(sh.update[w], graw, lane, R.update);
       }
-      d = chunk_decays<REV>(sh.ph[w], sh.pl[w], sh.far[w], sh.update[w], graw, lane, w, R.update);
-      if constexpr (OUT) {
-        // Before the next chunk's loads, so that their wait does not include those.
-        if (R.dots) {
-          const Rsrc er = chunk_rows(es, c, have);
+      __syncthreads();
+      if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
+      if (have(c) > 0) {
+        since *= whole;
+        advance(sh, own, whole, g, r);
+      }
+      __syncthreads();
+      // A segment ends: its state joins the start.
+      if (REV ? c % a.seg == 0 : c % a.seg == a.seg - 1 || c == a.NC - 1) {
 #pragma unroll
-          for (int pb = 0; pb < 4; ++pb)
-            e[pb] = load_quad<WHOLE>(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p, tag);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              start[nt][pb][q] = fmaf(since, start[nt][pb][q], own[nt][pb][q]);
+            own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
+          }
+        since = 1.f;
       }
     }
-    __syncthreads();
-    if (it + 1 < count) fetch(REV ? c - 1 : c + 1);
-    if (have > 0) {
-      // The blocks of 16 keys in turn from the wave's own strip, into the past (REV:
-      // the future) and round: the first `seen` of them reach the strip's queries.
-      // (Opaque, so that the addresses that follow from it are not kept in registers
-      // over the loop.)
-      int strip = w;
-      asm volatile("" : "+s"(strip));
-      const int seen = REV ? WAVES - strip : strip + 1;
-      auto block = [&](int i) { return (REV ? strip + i : strip - i) & 3; };
-      f4 out[4];
-      Frag<MADE> score[2];
-      float diagonal = 0.f;  // with dots: a token's score with itself, kept out of score
-      if constexpr (OUT) {
+    if (R.final.base && (REV ? c0 == 0 : c1 == a.NC)) {
+      const int t = thread() & (64 * WAVES - 1), g = (t >> 4) & 3, r = t & 15;
+      float* s = R.final.base + (long)bh * R.n * R.p;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pb = 0; pb < 4; ++pb)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = 64 * nt + 16 * w + 4 * g + q, p = col0 + 16 * pb + r;
+            if (n < R.n && p < R.p)
+              s[(long)n * R.final.sn + (long)p * R.final.sp] = start[nt][pb][q];
+          }
+    }
+  }
+
+  template <bool DOTS>
+  __device__ __forceinline__ void write_outputs(int c0, int c1, Shared<In, NT, true>& sh) {
+    const Source vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h);
+    Piece<In> vraw[2], qraw[2 * NT];
+    float graw;
+    auto fetch = [&](int c) {
+      const int t = thread(), lane = t & 63;
+      fetch_v(vraw, vs, c, t);
+      const Rsrc qr = chunk_rows(qs, c, have(c));
+#pragma unroll
+      for (int kk = 0; kk < 2 * NT; ++kk)
+        qraw[kk] = load_piece<WHOLE>(qr, (16 * w + (lane & 15)) * qs.stride,
+                                     32 * kk + 8 * (lane >> 4), R.n, (const In*)nullptr);
+      graw = decay(c, lane);
+    };
+    fetch(REV ? c1 - 1 : c0);
+    for (int it = 0; it < c1 - c0; ++it) {
+      const int c = REV ? c1 - 1 - it : c0 + it, t0 = c * C;
+      const int tid = thread(), lane = tid & 63, g = lane >> 4, r = lane & 15;
+      Frag<IN> qf[2 * NT];
+      Reach d{};
+      Quad<In> e[4];
+      if (have(c) > 0) {
+        stage_v(sh, vraw, tid);
+#pragma unroll
+        for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
+        d = reach<REV>(sh.ph[w], sh.pl[w], sh.far[w], graw, lane, w);
+        if constexpr (DOTS) {
+          // Before the next chunk's loads, so that their wait does not include those.
+          const Source es = source<In>(R.e, b, h);
+          const Rsrc er = chunk_rows(es, c, have(c));
+#pragma unroll
+          for (int pb = 0; pb < 4; ++pb)
+            e[pb] = load_quad<WHOLE>(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p,
+                                     (const In*)nullptr);
+        }
+      }
+      __syncthreads();
+      if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
+      if (have(c) > 0) {
+        const int strip = opaque_strip(), reached = seen(strip);
         // The state's part, transposed: columns 16 pb + 4 g + q of token 16 w + r.
+        f4 out[4];
 #pragma unroll
         for (int pb = 0; pb < 4; ++pb) out[pb] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -589,84 +756,59 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
         const float near = R.intra * __shfl(d.near, 16 * w + r);
 #pragma unroll
         for (int pb = 0; pb < 4; ++pb) out[pb] *= inter;
-        // Scores, transposed: keys 16 block(i) + 4 g + q of query 16 w + r.
+        float diagonal = 0.f;  // with dots: a token's score with itself, kept out of score
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
+          if (2 * s >= reached) continue;
+          const int ja = block(strip, 2 * s), jb = block(strip, 2 * s + 1);
+          // Scores, transposed: keys 16 ja (jb) + 4 g + q of query 16 w + r.
           f4 acc[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
-          if (2 * s < seen) {
 #pragma unroll
-            for (int kk = 0; kk < 2 * NT; ++kk) {
-              const Frag<IN> kf[2] = {rows<IN, NT>(sh.k, 16 * block(2 * s), kk, g, r),
-                                      rows<IN, NT>(sh.k, 16 * block(2 * s + 1), kk, g, r)};
-              mma(kf, qf[kk], acc);
-            }
-            if (s == 0) {
-              const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
-              const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * w + 4 * g]);
-              const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * w + 4 * g]);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float gap = (ph - kh[q]) + (pl - kl[q]);
-                const int ahead = REV ? 4 * g + q - r : r - 4 * g - q;  // query - key
-                const float dec = __builtin_amdgcn_exp2f(REV ? -gap : gap) * R.intra;
-                const float x = acc[0][q] * dec;
-                acc[0][q] = ahead > 0 ? x : 0.f;
-                if (ahead == 0) diagonal = x;
-                if (ahead == 0 && !R.dots) acc[0][q] = x;
-              }
-            } else {
-              acc[0] *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * block(2 * s) + 4 * g]);
-            }
-            // A block past the last one seen gives no scores.
-            const f4 far =
-                near * *reinterpret_cast<const f4*>(&sh.far[w][16 * block(2 * s + 1) + 4 * g]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[1][q] = 2 * s + 1 < seen ? acc[1][q] * far[q] : 0.f;
+          for (int kk = 0; kk < 2 * NT; ++kk) {
+            const Frag<IN> kf[2] = {rows<IN, NT>(sh.k, 16 * ja, kk, g, r),
+                                    rows<IN, NT>(sh.k, 16 * jb, kk, g, r)};
+            mma(kf, qf[kk], acc);
           }
+          if (s == 0) {
+            const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
+            const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * w + 4 * g]);
+            const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * w + 4 * g]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float gap = (ph - kh[q]) + (pl - kl[q]);
+              const int ahead = REV ? 4 * g + q - r : r - 4 * g - q;  // query - key
+              const float x = acc[0][q] * (__builtin_amdgcn_exp2f(REV ? -gap : gap) * R.intra);
+              acc[0][q] = ahead > (DOTS ? 0 : -1) ? x : 0.f;
+              if (DOTS && ahead == 0) diagonal = x;
+            }
+          } else {
+            acc[0] *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * ja + 4 * g]);
+          }
+          // A block past the last one seen gives no scores.
+          const f4 far = near * *reinterpret_cast<const f4*>(&sh.far[w][16 * jb + 4 * g]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[1][q] = 2 * s + 1 < reached ? acc[1][q] * far[q] : 0.f;
           const float x[8] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3],
                               acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
-          score[s] = split8<MADE>(x);
-        }
-      }
-      // The next state, and the scores' part of the output.
-      since *= d.chunk;
+          const Frag<MADE> score = split8<MADE>(x);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+          for (int p0 = 0; p0 < 4; p0 += GROUP) {
+            Frag<IN> vf[GROUP];
 #pragma unroll
-        for (int pb = 0; pb < 4; ++pb) own[nt][pb] *= d.chunk;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int ja = block(2 * s), jb = block(2 * s + 1);
-        const f4 ua = *reinterpret_cast<const f4*>(&sh.update[w][16 * ja + 4 * g]);
-        const f4 ub = *reinterpret_cast<const f4*>(&sh.update[w][16 * jb + 4 * g]);
-        const float wt[8] = {ua[0], ua[1], ua[2], ua[3], ub[0], ub[1], ub[2], ub[3]};
-        Frag<MADE> kw[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          kw[nt] = weighted<MADE>(columns<IN, NT>(sh.k, nt, ja, jb, w, g, r), wt);
-#pragma unroll
-        for (int p0 = 0; p0 < 4; p0 += GROUP) {
-          Frag<IN> vf[GROUP];
-#pragma unroll
-          for (int pb = 0; pb < GROUP; ++pb)
-            vf[pb] = columns<IN, 1>(sh.v, 0, ja, jb, p0 + pb, g, r);
-          if constexpr (OUT) {
-            if (2 * s < seen) mma(vf, score[s], &out[p0]);
+            for (int pb = 0; pb < GROUP; ++pb)
+              vf[pb] = columns<IN, 1>(sh.v, 0, ja, jb, p0 + pb, g, r);
+            mma(vf, score, &out[p0]);
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(kw[nt], vf, &own[nt][p0]);
         }
-      }
-      if constexpr (OUT) {
         const int t = 16 * w + r;
-        if (R.dots) {
+        if constexpr (DOTS) {
           float dot = 0.f;
 #pragma unroll
           for (int pb = 0; pb < 4; ++pb)
 #pragma unroll
             for (int q = 0; q < 4; ++q) dot = fmaf(out[pb][q], e[pb].get()[q], dot);
           dot = sum_groups(dot);
-          if (g == 0 && t < have)
+          if (g == 0 && t < have(c))
             R.dots[((long)(tile * a.B + b) * a.H + h) * a.T + t0 + t] = dot;
           // The token's own term, which the dots leave out.
           const float own_score = sum_groups(diagonal);
@@ -679,84 +821,42 @@ __device__ __forceinline__ void walk(const Args& a, const Role& R, int tile, int
               out[pb] += own_score * f4{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
             }
         }
-        if (t0 + t < a.T) {
-          const bool here = t < have;
-          const long at = (((long)b * a.T + t0 + t) * a.H + h) * R.p + col0 + 4 * g;
+        if (t0 + t < a.T) store(out, t0 + t, t < have(c), g);
+      } else {
+        // Past the row's length: zeros.
+        const f4 zero[4] = {};
 #pragma unroll
-          for (int pb = 0; pb < 4; ++pb)
-            if (!here) out[pb] = f4{0.f, 0.f, 0.f, 0.f};
-          const int left = R.p - col0 - 4 * g;
-          if (R.p & 3) {
-#pragma unroll
-            for (int pb = 0; pb < 4; ++pb)
-              store_some(R.out, at + 16 * pb, out[pb], left - 16 * pb, R.out_f32);
-          } else if (R.out_f32) {
-            float* p = static_cast<float*>(R.out) + at;
-#pragma unroll
-            for (int pb = 0; pb < 4; ++pb)
-              if (16 * pb < left) *reinterpret_cast<f4*>(p + 16 * pb) = out[pb];
-          } else {
-            bf16_t* p = static_cast<bf16_t*>(R.out) + at;
-#pragma unroll
-            for (int pb = 0; pb < 4; ++pb)
-              if (16 * pb < left)
-                *reinterpret_cast<u2*>(p + 16 * pb) =
-                    u2{pack(out[pb][0], out[pb][1]), pack(out[pb][2], out[pb][3])};
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          if (t0 + 16 * i + r < a.T && (i & 3) == w) store(zero, t0 + 16 * i + r, false, g);
       }
-    } else if constexpr (OUT) {
-      // Past the row's length: zeros.
-      for (int i = tid; i < C * TILE; i += THREADS) {
-        const int t = t0 + (i >> 6), p = col0 + (i & 63);
-        if (t < a.T && p < R.p) {
-          const long at = (((long)b * a.T + t) * a.H + h) * R.p + p;
-          if (R.out_f32) static_cast<float*>(R.out)[at] = 0.f;
-          else static_cast<bf16_t*>(R.out)[at] = 0;
-        }
-      }
-    }
-    __syncthreads();
-    // A segment ends: its state joins the start.
-    if (OUT && (REV ? c % SEG == 0 : c % SEG == SEG - 1 || c == a.NC - 1)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int pb = 0; pb < 4; ++pb) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            start[nt][pb][q] = fmaf(since, start[nt][pb][q], own[nt][pb][q]);
-          own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
-        }
-      since = 1.f;
+      __syncthreads();
     }
   }
 
-  if constexpr (OUT) {
-    if (R.final.base && (REV ? c0 == 0 : c1 == a.NC)) {
-      float* s = R.final.base + (long)bh * R.n * R.p;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int pb = 0; pb < 4; ++pb)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int n = 64 * nt + 16 * w + 4 * g + q, p = col0 + 16 * pb + r;
-            if (n < R.n && p < R.p)
-              s[(long)n * R.final.sn + (long)p * R.final.sp] = start[nt][pb][q];
-          }
-    }
-  } else {
-    const long slot = (long)(tile * a.B * a.H + bh) * a.NS + seg;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+  // A token's output, columns 16 pb + 4 g + q; zeros past the row's length.
+  __device__ __forceinline__ void store(const f4 (&out)[4], int t, bool here, int g) {
+    const long at = (((long)b * a.T + t) * a.H + h) * R.p + col0 + 4 * g;
+    const int left = R.p - col0 - 4 * g;
+    const f4 zero{0.f, 0.f, 0.f, 0.f};
+    if (R.p & 3) {
 #pragma unroll
       for (int pb = 0; pb < 4; ++pb)
-        *reinterpret_cast<f4*>(R.starts + slot * (NT * 4096) +
-                               ((nt * 4 + pb) * THREADS + tid) * 4) = own[nt][pb];
-    if (tid == 0) R.decays[slot] = since;
+        store_some(R.out, at + 16 * pb, here ? out[pb] : zero, left - 16 * pb, R.out_f32);
+    } else if (R.out_f32) {
+      float* p = static_cast<float*>(R.out) + at;
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb)
+        if (16 * pb < left) *reinterpret_cast<f4*>(p + 16 * pb) = here ? out[pb] : zero;
+    } else {
+      bf16_t* p = static_cast<bf16_t*>(R.out) + at;
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb)
+        if (16 * pb < left)
+          *reinterpret_cast<u2*>(p + 16 * pb) =
+              here ? u2{pack(out[pb][0], out[pb][1]), pack(out[pb][2], out[pb][3])} : u2{0u, 0u};
+    }
   }
-}
+};
 
 // Blocks of one (b, h) (its roles' tiles) differ by 8 in the grid: with
 // consecutive blocks on the 8 XCDs in turn they share an L2, and so the rows.
@@ -769,31 +869,68 @@ __device__ __forceinline__ bool block_of(const Args& a, int x, int* which, int* 
   return bh < a.B * a.H;
 }
 
-template <typename In, int NT, bool OUT, bool WHOLE>
-__global__ __launch_bounds__(THREADS, sizeof(In) == 2 && NT == 1 ? 3 : sizeof(In) == 4 && NT == 2 ? 1 : 2) void attention_kernel(Args a) {
-  __shared__ Shared<In, NT, OUT> sh;
-  int which, b, h, i = 0;
+// A block's chunks: of one segment (blockIdx.y) in split runs, else all.
+__device__ __forceinline__ int chunks_of(const Args& a, int* c0, int* c1) {
+  const bool split = a.split;
+  *c0 = split ? (int)blockIdx.y * a.seg : 0;
+  *c1 = split ? min(a.NC, *c0 + a.seg) : a.NC;
+  return split ? (int)blockIdx.y : -1;
+}
+
+// Eight waves a block: two blocks a compute unit need no more than 128 registers
+// (float32 with wide keys: one block, by its LDS).
+constexpr int waves_per_simd(int bytes, int nt) { return bytes == 4 && nt == 2 ? 2 : 4; }
+
+template <typename In, int NT, bool WHOLE>
+__global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void attention_kernel(Args a) {
+  __shared__ Shared<In, NT, true> sh;
+  int which, b, h, c0, c1;
+  if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
+  const int seg = chunks_of(a, &c0, &c1);
+  Block<In, NT, WHOLE, false>(a, a.role[0], which, b, h).template outputs<false>(seg, c0, c1, sh);
+}
+
+// The gradients: dQ forward in time, dK and dV in reverse; NP and NN 64s of the
+// value and key widths, DOTS with what the decays' gradient needs.
+template <typename In, int NP, int NN, bool DOTS, bool WHOLE>
+__global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NP > NN ? NP : NN)) void
+attention_backward_kernel(Args a) {
+  __shared__ union {
+    Shared<In, NP, true> p;
+    Shared<In, NN, true> n;
+  } sh;
+  int which, b, h, c0, c1;
+  if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
+  const int seg = chunks_of(a, &c0, &c1);
+  if (which < a.role[0].tiles)
+    return Block<In, NP, WHOLE, false>(a, a.role[0], which, b, h)
+        .template outputs<DOTS>(seg, c0, c1, sh.p);
+  which -= a.role[0].tiles;
+  if (which < a.role[1].tiles)
+    return Block<In, NP, WHOLE, true>(a, a.role[1], which, b, h)
+        .template outputs<DOTS>(seg, c0, c1, sh.p);
+  Block<In, NN, WHOLE, true>(a, a.role[2], which - a.role[1].tiles, b, h)
+      .template outputs<false>(seg, c0, c1, sh.n);
+}
+
+// Split runs: the segments' own states, of all roles.
+template <typename In, int NT, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
+  __shared__ Shared<In, NT, false> sh;
+  int which, b, h, i = 0, c0, c1;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   while (which >= a.role[i].tiles) which -= a.role[i++].tiles;
   const Role& R = a.role[i];
-  // Split runs take a segment per block (blockIdx.y), others the sequence.
-  const bool split = !OUT || gridDim.y > 1;
-  const int seg = split ? (int)blockIdx.y : -1;
-  const int c0 = split ? seg * SEG : 0, c1 = split ? min(a.NC, c0 + SEG) : a.NC;
+  const int seg = chunks_of(a, &c0, &c1);
   if constexpr (NT == 2) {
     if (R.n <= 64) {
-      Shared<In, 1, OUT>& narrow = reinterpret_cast<Shared<In, 1, OUT>&>(sh);
-      if (R.rev)
-        walk<In, 1, OUT, WHOLE, true>(a, R, which, b, h, c0, c1, seg, narrow);
-      else
-        walk<In, 1, OUT, WHOLE, false>(a, R, which, b, h, c0, c1, seg, narrow);
-      return;
+      Shared<In, 1, false>& narrow = reinterpret_cast<Shared<In, 1, false>&>(sh);
+      if (R.rev) return Block<In, 1, WHOLE, true>(a, R, which, b, h).states(seg, c0, c1, narrow);
+      return Block<In, 1, WHOLE, false>(a, R, which, b, h).states(seg, c0, c1, narrow);
     }
   }
-  if (R.rev)
-    walk<In, NT, OUT, WHOLE, true>(a, R, which, b, h, c0, c1, seg, sh);
-  else
-    walk<In, NT, OUT, WHOLE, false>(a, R, which, b, h, c0, c1, seg, sh);
+  if (R.rev) return Block<In, NT, WHOLE, true>(a, R, which, b, h).states(seg, c0, c1, sh);
+  Block<In, NT, WHOLE, false>(a, R, which, b, h).states(seg, c0, c1, sh);
 }
 
 // Split runs: each segment's start state from the segments' own states and
@@ -817,7 +954,7 @@ __global__ void carry_kernel(Args a) {
     }
   }
   const long first = (long)(which * a.B * a.H + bh) * a.NS;
-  float* own = R.starts + first * (nts * 4096) + (part * THREADS + tid) * 4;
+  float* own = R.starts + first * (nts * 4096) + (part * 64 * WAVES + tid) * 4;
   const float* decays = R.decays + first;
   constexpr int AHEAD = 8;  // segments loaded together
   for (int s0 = 0; s0 < a.NS; s0 += AHEAD) {
@@ -974,19 +1111,27 @@ __global__ __launch_bounds__(256) void step_kernel(Step a) {
   }
 }
 
-#define LA_ATTENTION(In, NT)                                            \
-  template __global__ void attention_kernel<In, NT, true, true>(Args);  \
-  template __global__ void attention_kernel<In, NT, true, false>(Args); \
-  template __global__ void attention_kernel<In, NT, false, true>(Args); \
-  template __global__ void attention_kernel<In, NT, false, false>(Args);
+#define LA_WHOLE(In, W)                                                       \
+  template __global__ void attention_kernel<In, 1, W>(Args);                 \
+  template __global__ void attention_kernel<In, 2, W>(Args);                 \
+  template __global__ void attention_states_kernel<In, 1, W>(Args);          \
+  template __global__ void attention_states_kernel<In, 2, W>(Args);          \
+  template __global__ void attention_backward_kernel<In, 1, 1, false, W>(Args); \
+  template __global__ void attention_backward_kernel<In, 1, 1, true, W>(Args);  \
+  template __global__ void attention_backward_kernel<In, 1, 2, false, W>(Args); \
+  template __global__ void attention_backward_kernel<In, 1, 2, true, W>(Args);  \
+  template __global__ void attention_backward_kernel<In, 2, 1, false, W>(Args); \
+  template __global__ void attention_backward_kernel<In, 2, 1, true, W>(Args);  \
+  template __global__ void attention_backward_kernel<In, 2, 2, false, W>(Args); \
+  template __global__ void attention_backward_kernel<In, 2, 2, true, W>(Args);
 #define LA_INSTANCES(In)                                                       \
-  LA_ATTENTION(In, 1)                                                          \
-  LA_ATTENTION(In, 2)                                                          \
+  LA_WHOLE(In, true)                                                           \
+  LA_WHOLE(In, false)                                                          \
   template __global__ void step_kernel<In>(Step);                              \
   template __global__ void share_sum_kernel<In>(const float*, long, int, int, int, In*);
 LA_INSTANCES(float)
 LA_INSTANCES(bf16_t)
 #undef LA_INSTANCES
-#undef LA_ATTENTION
+#undef LA_WHOLE
 
 }  // namespace la

@@ -7,11 +7,10 @@
 namespace la {
 
 constexpr int C = 64;        // tokens of a chunk
-constexpr int SEG = 4;       // chunks of a segment
+constexpr int MAX_SEG = 16;  // most chunks of a segment
 constexpr int TILE = 64;     // value columns of a block
-constexpr int WAVES = 4;     // one 16-token strip of the chunk each
+constexpr int WAVES = 4;     // strips of 16 tokens in a chunk, each a wave's
 constexpr int MAX_WIDTH = 128;
-constexpr int THREADS = 64 * WAVES;
 
 typedef unsigned short bf16_t;
 
@@ -56,6 +55,7 @@ struct Args {
   long gb, gt;
   const int* lengths;      // [B], or NULL
   int B, T, H, NC, NS;
+  int seg, split;          // chunks of a segment; split: a segment a block
 };
 
 // d log_decay from the roles' dots.

@@ -11,8 +11,8 @@ library (``m4rt_embedding_*``, include/mamba4_retention.h) on the current stream
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _same_device, _workspace
-from mamba4_amd.memory import _ptr, _stream
+from mamba4_amd.attention import _on, _same_device, _stream, _workspace
+from mamba4_amd.memory import _ptr
 
 _DTYPES = (torch.float32, torch.bfloat16)
 
@@ -28,7 +28,7 @@ class _Embedding(torch.autograd.Function):
             _lib.load().m4rt_embedding_forward(
                 _ptr(ids), int(ids.dtype == torch.int64), _ptr(table),
                 int(table.dtype == torch.bfloat16), ids.numel(), rows, width, scale, _ptr(out),
-                int(dtype == torch.bfloat16), _stream(),
+                int(dtype == torch.bfloat16), _stream(ids.device),
             )
         )
         ctx.save_for_backward(ids)
@@ -49,7 +49,7 @@ class _Embedding(torch.autograd.Function):
             lib.m4rt_embedding_backward(
                 _ptr(ids), int(ids.dtype == torch.int64), _ptr(d_out),
                 int(dtype == torch.bfloat16), ids.numel(), rows, width, scale, _ptr(d_table),
-                int(table_dtype == torch.bfloat16), _ptr(workspace), nbytes, _stream(),
+                int(table_dtype == torch.bfloat16), _ptr(workspace), nbytes, _stream(ids.device),
             )
         )
         return None, d_table, None, None
@@ -71,5 +71,5 @@ def embedding(ids, table, *, scale=1.0, dtype=None):
         raise ValueError("embedding takes float32 and bfloat16")
     if ids.numel() == 0:
         return table[:0].to(dtype).reshape(*ids.shape, table.shape[1])
-    with torch.cuda.device(table.device):
+    with _on(table.device):
         return _Embedding.apply(ids.contiguous(), table.contiguous(), float(scale), dtype)

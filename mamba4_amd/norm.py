@@ -14,8 +14,8 @@ usual norm over space or time.  Runs on the gfx950 HIP library
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _f32, _same_device, _workspace
-from mamba4_amd.memory import _ptr, _stream
+from mamba4_amd.attention import _f32, _on, _same_device, _stream, _workspace
+from mamba4_amd.memory import _ptr
 
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2}
 
@@ -43,7 +43,7 @@ class _GroupNorm(torch.autograd.Function):
         _lib.check(
             lib.m4rt_norm_forward(
                 _ptr(x), _ptr(weight), _ptr(bias), _ptr(gate), bf16, samples, positions, channels,
-                groups, activation, eps, _ptr(y), _ptr(stats), _ptr(workspace), nbytes, _stream(),
+                groups, activation, eps, _ptr(y), _ptr(stats), _ptr(workspace), nbytes, _stream(x.device),
             )
         )
         ctx.save_for_backward(x, weight, bias, gate, stats)
@@ -69,7 +69,7 @@ class _GroupNorm(torch.autograd.Function):
             lib.m4rt_norm_backward(
                 _ptr(x), _ptr(weight), _ptr(bias), _ptr(gate), _ptr(d_y), _ptr(stats), bf16,
                 samples, positions, channels, groups, activation, eps, _ptr(d_x), _ptr(d_weight),
-                _ptr(d_bias), _ptr(d_gate), _ptr(workspace), nbytes, _stream(),
+                _ptr(d_bias), _ptr(d_gate), _ptr(workspace), nbytes, _stream(x.device),
             )
         )
         return d_x, d_weight, d_bias, d_gate, None, None, None
@@ -107,7 +107,7 @@ def group_norm(x, groups, weight=None, bias=None, *, gate=None, activation="none
     x = x.to(rows).contiguous()
     gate = None if gate is None else gate.to(rows).contiguous()
     weight, bias = (None if t is None else _f32(t) for t in (weight, bias))
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         y = _GroupNorm.apply(x, weight, bias, gate, int(groups), ACTIVATIONS[activation],
                              float(eps))
     return y.to(dtype)
