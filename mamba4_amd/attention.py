@@ -17,6 +17,7 @@ them as they are and return bfloat16; any other mix is computed in float32 and
 returned in the values' dtype.  States, decays and sums are float32 or wider.
 """
 
+import contextlib
 from typing import NamedTuple
 
 import torch
@@ -39,9 +40,13 @@ def _f32(t):
     return t.to(_F32).contiguous()
 
 
+_NOTHING = contextlib.nullcontext()
+
+
 def _on(device):
-    """Makes the device the current one."""
-    return torch.cuda.device(device)
+    """Makes the device the current one (torch.cuda.device costs microseconds
+    where it already is)."""
+    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _same_device(*tensors):
@@ -57,7 +62,7 @@ def _same_device(*tensors):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _strided(t):

@@ -24,7 +24,7 @@ __global__ void decay_grad_kernel(DecayGrad);
 __global__ void decay_heads_kernel(const double*, int, int, float*);
 template <typename Out>
 __global__ void share_sum_kernel(const float*, long, int, int, int, Out*);
-template <typename In>
+template <typename In, int V, int PASSES>
 __global__ void step_kernel(Step);
 }  // namespace la
 
@@ -268,6 +268,21 @@ int run_attention(la::Args& a, const Shape& s, bool split, hipStream_t st) {
   return whole ? start_attention<float, true>(a, st) : start_attention<float, false>(a, st);
 }
 
+// The step with as many loads in flight as its rows need.
+template <typename In>
+void start_step(const la::Step& a, bool whole, hipStream_t st) {
+  const dim3 grid(a.B * a.H), block(la::STEP_THREADS);
+  const int rows = la::STEP_THREADS >> a.span, passes = (a.N + rows - 1) / rows;
+  if (!whole)
+    hipLaunchKernelGGL((la::step_kernel<In, 1, 16>), grid, block, 0, st, a);
+  else if (passes <= 4)
+    hipLaunchKernelGGL((la::step_kernel<In, 4, 4>), grid, block, 0, st, a);
+  else if (passes <= 8)
+    hipLaunchKernelGGL((la::step_kernel<In, 4, 8>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((la::step_kernel<In, 4, 16>), grid, block, 0, st, a);
+}
+
 struct Backward {
   la::Role role[3];
   float *part[3], *dots_q, *dots_k;
@@ -486,16 +501,18 @@ int m4rt_attention_step(const m4rt_qkv* rows, int bf16, const float* log_decay, 
     if (q->width != k->width) return api_fail(M4MR_EINVAL, at + "q and k disagree in width");
     if (!log_decay || !state || !new_state || !output)
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
-    const la::Step a{q->data, k->data, v->data, q->batch_stride, q->head_stride, k->batch_stride,
+    la::Step a{q->data, k->data, v->data, q->batch_stride, q->head_stride, k->batch_stride,
                      k->head_stride, v->batch_stride, v->head_stride, H / q->heads, H / k->heads,
                      H / v->heads, log_decay, per_token ? H : 0, active, state, new_state, output,
-                     scale, B, H, s.N, s.P};
+                     scale, B, H, s.N, s.P, 0};
+    const uintptr_t states = reinterpret_cast<uintptr_t>(state) |
+                             reinterpret_cast<uintptr_t>(new_state);
+    if (states % 4) return api_fail(M4MR_EINVAL, at + "states must be aligned to 4 bytes");
+    const bool whole = s.P % 4 == 0 && states % 16 == 0;
+    while ((1 << a.span) < (whole ? s.P / 4 : s.P)) ++a.span;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return api_launch("attention_step", st, [&] {
-      if (bf16)
-        hipLaunchKernelGGL(la::step_kernel<la::bf16_t>, dim3(B * H), dim3(256), 0, st, a);
-      else
-        hipLaunchKernelGGL(la::step_kernel<float>, dim3(B * H), dim3(256), 0, st, a);
+      bf16 ? start_step<la::bf16_t>(a, whole, st) : start_step<float>(a, whole, st);
     });
   });
 }
@@ -734,7 +751,7 @@ int m4rt_norm_backward(const void* x, const float* weight, const float* bias, co
     const int rc = run_norm<true>(a, p, bf16, st);
     if (rc || !columns) return rc;
     return api_launch("norm_columns", st, [&] {
-      hipLaunchKernelGGL(gn::norm_columns_kernel, dim3((2 * C + 63) / 64), dim3(1024), 0, st, part,
+      hipLaunchKernelGGL(gn::norm_columns_kernel, dim3((2 * C + 15) / 16), dim3(1024), 0, st, part,
                          p.part_rows, C, d_weight, d_bias);
     });
   });
@@ -784,11 +801,13 @@ size_t embedding_plan(long n, int rows, int width, void* base, EmbeddingPlan* p)
   p->passes = (bits + em::MAX_DIGIT - 1) / em::MAX_DIGIT;
   p->bits = (bits + p->passes - 1) / p->passes;
   // Every tile reads all tiles' counts: at most 128 of them.
-  p->tile = 2048;
+  p->tile = 1024;
   while ((n + p->tile - 1) / p->tile > 128) p->tile *= 2;
   p->tiles = (int)((n + p->tile - 1) / p->tile);
-  // Short chunks fill the card, long ones leave fewer parts to join.
-  p->chunk = n >= 65536 ? 32 : 16;
+  // Short chunks fill the card, long ones leave fewer parts to join: sums and
+  // joins of 16,384 tokens of 768 23 + 11 us in chunks of 16, 53 + 4 in 64s; of
+  // 131,071 tokens of 1,024 120 + 66 and 118 + 17 us.
+  p->chunk = n >= 65536 ? 64 : 16;
   p->chunks = (int)((n + p->chunk - 1) / p->chunk);
   Carver c{static_cast<char*>(base)};
   size_t first = 0;

@@ -142,14 +142,30 @@ __device__ __forceinline__ unsigned long peers(unsigned digit, int bits, bool ha
 }
 
 // One pass: each wave ranks a quarter of the tile in order, 64 pairs at a
-// time; equal digits keep their order.
+// time; equal digits keep their order.  A tile of 64 ROUNDS pairs a wave holds
+// them in registers; longer ones repeat that.
+constexpr int ROUNDS = 4;
+
 __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
   __shared__ unsigned place[THREADS / 64][BINS], total[2][BINS], before[BINS];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, size = 1 << a.bits;
+  const int per = a.tile / (THREADS / 64);
+  const long first = (long)blockIdx.x * a.tile + w * per;
+  const unsigned long below = (1ul << lane) - 1;
+  auto fetch = [&](int k, unsigned (&key)[ROUNDS]) {
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j) {
+      const long i = min(first + k + 64 * j + lane, a.n - 1);
+      key[j] = a.keys ? a.keys[i] : key_of(a.ids, a.wide, i, a.rows);
+    }
+  };
+  unsigned key[ROUNDS], rank[ROUNDS];
+  fetch(0, key);
   for (int d = tid; d < (THREADS / 64) * BINS; d += THREADS) (&place[0][0])[d] = 0;
+  // This tile's part in the digits: all tiles' counts, and those before it.
   for (int d = tid; d < size; d += THREADS) {
     unsigned all = 0, mine = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int t = 0; t < a.tiles; ++t) {
       const unsigned c = a.counts[(long)t * size + d];
       all += c;
@@ -159,19 +175,23 @@ __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
     before[d] = mine;
   }
   __syncthreads();
-  const long first = (long)blockIdx.x * a.tile + w * (a.tile / 4);
-  const unsigned long below = (1ul << lane) - 1;
-  auto fetch = [&](int k, bool* have) {
-    const long i = first + k + lane;
-    *have = i < a.n;
-    if (!*have) return 0u;
-    return a.keys ? a.keys[i] : key_of(a.ids, a.wide, i, a.rows);
+  // Ranks within the wave's quarter.
+  auto count = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j) {
+      const bool have = first + k + 64 * j + lane < a.n;
+      const unsigned digit = (key[j] >> a.shift) & (size - 1);
+      const unsigned long mask = peers(digit, a.bits, have);
+      const unsigned seen = __popcll(mask & below);
+      rank[j] = place[w][digit] + seen;
+      __builtin_amdgcn_wave_barrier();
+      if (have && seen == 0) place[w][digit] += __popcll(mask);
+      __builtin_amdgcn_wave_barrier();
+    }
   };
-  for (int k = 0; k < a.tile / 4; k += 64) {
-    bool have;
-    const unsigned digit = (fetch(k, &have) >> a.shift) & (size - 1);
-    const unsigned long mask = peers(digit, a.bits, have);
-    if (have && (mask & below) == 0) place[w][digit] += __popcll(mask);
+  for (int k = 0; k < per; k += 64 * ROUNDS) {
+    if (k) fetch(k, key);
+    count(k);
   }
   // Exclusive sums of the totals over the digits.
   int from = 0;
@@ -190,29 +210,31 @@ __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
     }
   }
   __syncthreads();
-  for (int k = 0; k < a.tile / 4; k += 64) {
-    bool have;
-    const unsigned key = fetch(k, &have), digit = (key >> a.shift) & (size - 1);
-    const unsigned long mask = peers(digit, a.bits, have);
-    const unsigned rank = __popcll(mask & below);
-    if (have) {
-      const unsigned at = place[w][digit] + rank;
-      const long i = first + k + lane;
-      a.out_keys[at] = key;
+  const bool once = per == 64 * ROUNDS;  // the ranks are still at hand
+  for (int k = 0; k < per; k += 64 * ROUNDS) {
+    if (!once) {
+      fetch(k, key);
+      count(k);
+    }
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j) {
+      const long i = first + k + 64 * j + lane;
+      if (i >= a.n) continue;
+      const unsigned digit = (key[j] >> a.shift) & (size - 1);
+      const unsigned at = once ? place[w][digit] + rank[j] : rank[j];
+      a.out_keys[at] = key[j];
       a.out_tokens[at] = a.tokens ? a.tokens[i] : (unsigned)i;
       if (a.next)
         atomicAdd(&a.next[((long)(at / a.tile) << a.next_bits) +
-                          ((key >> a.next_shift) & ((1 << a.next_bits) - 1))], 1u);
-      if (a.present && key < (unsigned)a.rows) a.present[key] = 1;
+                          ((key[j] >> a.next_shift) & ((1 << a.next_bits) - 1))], 1u);
+      if (a.present && key[j] < (unsigned)a.rows) a.present[key[j]] = 1;
     }
-    __builtin_amdgcn_wave_barrier();
-    if (have && rank == 0) place[w][digit] += __popcll(mask);
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // Sums of runs: a thread takes one piece of the columns of one chunk.  The
-// blocks from `sum_blocks` on zero the rows that do not occur.
+// blocks from `sum_blocks` on zero the rows that do not occur (blocks of both kinds
+// in turn took longer).
 template <typename In, typename Out, int V>
 __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks) {
   const int vecs = a.width / V;
@@ -304,9 +326,11 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
     bool goes_on[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
+      // Loads without a condition, so that they are in flight together.
       const long at = min(c + j, (long)a.chunks - 1), end = (c + j + 1) * a.chunk;
       read<V>(a.head + at * a.width + column, x[j]);
-      goes_on[j] = end < a.n && a.keys[end] == key;
+      const unsigned then = a.keys[min(end, a.n - 1)];
+      goes_on[j] = (end < a.n) & (then == key);
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)

@@ -1066,7 +1066,9 @@ __global__ void share_sum_kernel(const float* part, long tokens, int heads, int 
 }
 
 // One token: S' = e^g S + k v^T, o = scale S'^T q.  The state is read and
-// written once; a block holds one (b, h), thread (row group, column quad).
+// written once, which is all the time there is: a block takes one (b, h), its
+// threads a piece of V columns of every R-th row each, and all of a thread's loads are
+// issued (after those of q, k and v) before the first is used.
 template <typename In>
 __device__ __forceinline__ float load_one(const void* p, long i) {
   if constexpr (sizeof(In) == 2)
@@ -1075,39 +1077,73 @@ __device__ __forceinline__ float load_one(const void* p, long i) {
     return static_cast<const float*>(p)[i];
 }
 
-template <typename In>
-__global__ __launch_bounds__(256) void step_kernel(Step a) {
-  __shared__ float q[MAX_WIDTH], k[MAX_WIDTH], v[MAX_WIDTH], part[4][MAX_WIDTH];
+template <typename In, int V, int PASSES>
+__global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
+  typedef float piece __attribute__((ext_vector_type(V)));
+  __shared__ float q[MAX_WIDTH], k[MAX_WIDTH], v[MAX_WIDTH], part[STEP_THREADS * V];
   const int tid = threadIdx.x, b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
   const bool on = !a.active || a.active[b];
   const long bh = blockIdx.x, at = bh * a.N * a.P;
-  if (tid < a.N) {
-    q[tid] = load_one<In>(a.q, b * a.qb + (h / a.q_share) * a.qh + tid);
-    k[tid] = load_one<In>(a.k, b * a.kb + (h / a.k_share) * a.kh + tid);
-  }
-  if (tid < a.P) v[tid] = load_one<In>(a.v, b * a.vb + (h / a.v_share) * a.vh + tid);
   const float g = a.g[b * a.gb + h];
-  const float lam = expf(g);
-  __syncthreads();
-  const int lane = tid & 63, w = tid >> 6;
-  for (int p = lane; p < a.P; p += 64) {
-    float o = 0.f;
-    for (int n = w; n < a.N; n += 4) {
-      const float s = a.state[at + (long)n * a.P + p];
-      const float x = on ? fmaf(lam, s, k[n] * v[p]) : s;
-      if (on || a.new_state != a.state) a.new_state[at + (long)n * a.P + p] = x;
-      o = fmaf(q[n], x, o);
-    }
-    part[w][p] = o;
+  float qx = 0.f, kx = 0.f, vx = 0.f;
+  if (tid < a.N) {
+    qx = load_one<In>(a.q, b * a.qb + (h / a.q_share) * a.qh + tid);
+    kx = load_one<In>(a.k, b * a.kb + (h / a.k_share) * a.kh + tid);
   }
+  if (tid < a.P) vx = load_one<In>(a.v, b * a.vb + (h / a.v_share) * a.vh + tid);
+  // Thread (row, column) of the 2^span threads along a row.
+  const int p = (tid & ((1 << a.span) - 1)) * V, row = tid >> a.span;
+  const int step = STEP_THREADS >> a.span;
+  piece s[PASSES];
+  piece o(0.f);
+  for (int n0 = 0; n0 < a.N; n0 += PASSES * step) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int n = n0 + i * step + row;
+      s[i] = piece(0.f);
+      if (n < a.N && p < a.P)
+        s[i] = __builtin_nontemporal_load(
+            reinterpret_cast<const piece*>(a.state + at + (long)n * a.P + p));
+    }
+    if (n0 == 0) {
+      if (tid < a.N) q[tid] = qx, k[tid] = kx;
+      if (tid < a.P) v[tid] = vx;
+      __syncthreads();
+    }
+    const float lam = expf(g);
+    if (p < a.P) {
+      piece vp;
+#pragma unroll
+      for (int c = 0; c < V; ++c) vp[c] = v[p + c];
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int n = n0 + i * step + row;
+        if (n >= a.N) continue;
+        const float kn = k[n], qn = q[n];
+        piece x = s[i];
+        if (on) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) x[c] = fmaf(lam, s[i][c], kn * vp[c]);
+        }
+        if (on || a.new_state != a.state)
+          __builtin_nontemporal_store(
+              x, reinterpret_cast<piece*>(a.new_state + at + (long)n * a.P + p));
+#pragma unroll
+        for (int c = 0; c < V; ++c) o[c] = fmaf(qn, x[c], o[c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < V; ++c) part[tid * V + c] = o[c];
   __syncthreads();
   if (tid < a.P) {
-    const float o =
-        on ? a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])) : 0.f;
+    float x = 0.f;
+    for (int r = 0; r < step; ++r) x += part[(r << a.span) * V + tid];
+    x = on ? a.scale * x : 0.f;
     if constexpr (sizeof(In) == 2)
-      static_cast<bf16_t*>(a.out)[bh * a.P + tid] = (bf16_t)pack(o, 0.f);
+      static_cast<bf16_t*>(a.out)[bh * a.P + tid] = (bf16_t)pack(x, 0.f);
     else
-      static_cast<float*>(a.out)[bh * a.P + tid] = o;
+      static_cast<float*>(a.out)[bh * a.P + tid] = x;
   }
 }
 
@@ -1127,7 +1163,10 @@ __global__ __launch_bounds__(256) void step_kernel(Step a) {
 #define LA_INSTANCES(In)                                                       \
   LA_WHOLE(In, true)                                                           \
   LA_WHOLE(In, false)                                                          \
-  template __global__ void step_kernel<In>(Step);                              \
+  template __global__ void step_kernel<In, 4, 4>(Step);                        \
+  template __global__ void step_kernel<In, 4, 8>(Step);                        \
+  template __global__ void step_kernel<In, 4, 16>(Step);                       \
+  template __global__ void step_kernel<In, 1, 16>(Step);                       \
   template __global__ void share_sum_kernel<In>(const float*, long, int, int, int, In*);
 LA_INSTANCES(float)
 LA_INSTANCES(bf16_t)

@@ -11,6 +11,7 @@ constexpr int MAX_SEG = 16;  // most chunks of a segment
 constexpr int TILE = 64;     // value columns of a block
 constexpr int WAVES = 4;     // strips of 16 tokens in a chunk, each a wave's
 constexpr int MAX_WIDTH = 128;
+constexpr int STEP_THREADS = 256;  // block of the step's kernel
 
 typedef unsigned short bf16_t;
 
@@ -84,6 +85,7 @@ struct Step {
   void* out;
   float scale;
   int B, H, N, P;
+  int span;                      // 2^span threads hold a row of the state
 };
 
 }  // namespace la

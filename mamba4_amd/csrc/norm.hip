@@ -278,24 +278,28 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
   }
 }
 
-// Sums of `rows` partials [rows][2][C] in order: 64 columns a block, 16
-// threads of a column each every 16th row.
+// Sums of `rows` partials [rows][2][C]: 16 columns a block, 64 threads of a
+// column each every 64th row, joined in order.
 __global__ __launch_bounds__(1024) void norm_columns_kernel(const float* part, int rows, int C,
                                                             float* dweight, float* dbias) {
-  __shared__ float fold[16][64];
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const int column = blockIdx.x * 64 + x;
+  __shared__ float fold[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const int column = blockIdx.x * 16 + x;
   float s = 0.f;
-  if (column < 2 * C)
-    for (int r = y; r < rows; r += 16) s += part[(long)r * 2 * C + column];
+  if (column < 2 * C) {
+#pragma unroll 8
+    for (int r = y; r < rows; r += 64) s += part[(long)r * 2 * C + column];
+  }
   fold[y][x] = s;
-  __syncthreads();
+  for (int h = 32; h > 0; h >>= 1) {
+    __syncthreads();
+    if (y < h) fold[y][x] += fold[y + h][x];
+  }
   if (y == 0 && column < 2 * C) {
-    for (int j = 1; j < 16; ++j) s += fold[j][x];
     if (column < C) {
-      if (dweight) dweight[column] = s;
+      if (dweight) dweight[column] = fold[0][x];
     } else if (dbias) {
-      dbias[column - C] = s;
+      dbias[column - C] = fold[0][x];
     }
   }
 }

@@ -17,23 +17,27 @@ from mamba4_amd.memory import _ptr
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
+def _forward(ids, table, scale, dtype):
+    rows, width = table.shape
+    out = torch.empty((*ids.shape, width), dtype=dtype, device=table.device)
+    rc = _lib.load().m4rt_embedding_forward(
+        ids.data_ptr(), ids.dtype == torch.int64, table.data_ptr(), table.dtype == torch.bfloat16,
+        ids.numel(), rows, width, scale, out.data_ptr(), dtype == torch.bfloat16,
+        _stream(table.device),
+    )
+    if rc:
+        _lib.check(rc)
+    return out
+
+
 class _Embedding(torch.autograd.Function):
     """ids int32 or int64, table float32 or bfloat16, both contiguous."""
 
     @staticmethod
     def forward(ctx, ids, table, scale, dtype):
-        rows, width = table.shape
-        out = torch.empty(*ids.shape, width, dtype=dtype, device=table.device)
-        _lib.check(
-            _lib.load().m4rt_embedding_forward(
-                _ptr(ids), int(ids.dtype == torch.int64), _ptr(table),
-                int(table.dtype == torch.bfloat16), ids.numel(), rows, width, scale, _ptr(out),
-                int(dtype == torch.bfloat16), _stream(ids.device),
-            )
-        )
         ctx.save_for_backward(ids)
         ctx.args = (tuple(table.shape), table.dtype, scale, dtype)
-        return out
+        return _forward(ids, table, scale, dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -71,5 +75,8 @@ def embedding(ids, table, *, scale=1.0, dtype=None):
         raise ValueError("embedding takes float32 and bfloat16")
     if ids.numel() == 0:
         return table[:0].to(dtype).reshape(*ids.shape, table.shape[1])
+    ids, table = ids.contiguous(), table.contiguous()
     with _on(table.device):
-        return _Embedding.apply(ids.contiguous(), table.contiguous(), float(scale), dtype)
+        if torch.is_grad_enabled() and table.requires_grad:
+            return _Embedding.apply(ids, table, float(scale), dtype)
+        return _forward(ids, table, float(scale), dtype)

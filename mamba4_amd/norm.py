@@ -26,26 +26,33 @@ def _sizes(x):
     return x.shape[0], x.numel() // (x.shape[0] * channels), channels
 
 
+def _forward(x, weight, bias, gate, groups, activation, eps, keep):
+    """The result, and with ``keep`` the statistics that the gradient needs."""
+    lib = _lib.load()
+    samples, positions, channels = _sizes(x)
+    bf16 = 1 if x.dtype == torch.bfloat16 else 0
+    y = torch.empty_like(x)
+    stats = None
+    if keep:
+        stats = torch.empty((samples, groups, 2), dtype=torch.float32, device=x.device)
+    nbytes = lib.m4rt_norm_workspace_bytes(samples, positions, channels, groups, bf16, 0)
+    workspace = _workspace(nbytes, x.device)
+    rc = lib.m4rt_norm_forward(
+        x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(gate), bf16, samples, positions, channels,
+        groups, activation, eps, y.data_ptr(), _ptr(stats), _ptr(workspace), nbytes,
+        _stream(x.device),
+    )
+    if rc:
+        _lib.check(rc)
+    return y, stats
+
+
 class _GroupNorm(torch.autograd.Function):
     """x, gate contiguous and of one dtype; weight and bias float32."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, gate, groups, activation, eps):
-        lib = _lib.load()
-        samples, positions, channels = _sizes(x)
-        bf16 = int(x.dtype == torch.bfloat16)
-        y = torch.empty_like(x)
-        stats = None
-        if any(ctx.needs_input_grad):
-            stats = torch.empty(samples, groups, 2, dtype=torch.float32, device=x.device)
-        nbytes = lib.m4rt_norm_workspace_bytes(samples, positions, channels, groups, bf16, 0)
-        workspace = _workspace(nbytes, x.device)
-        _lib.check(
-            lib.m4rt_norm_forward(
-                _ptr(x), _ptr(weight), _ptr(bias), _ptr(gate), bf16, samples, positions, channels,
-                groups, activation, eps, _ptr(y), _ptr(stats), _ptr(workspace), nbytes, _stream(x.device),
-            )
-        )
+        y, stats = _forward(x, weight, bias, gate, groups, activation, eps, True)
         ctx.save_for_backward(x, weight, bias, gate, stats)
         ctx.args = (groups, activation, eps)
         return y
@@ -107,7 +114,10 @@ def group_norm(x, groups, weight=None, bias=None, *, gate=None, activation="none
     x = x.to(rows).contiguous()
     gate = None if gate is None else gate.to(rows).contiguous()
     weight, bias = (None if t is None else _f32(t) for t in (weight, bias))
+    args = (x, weight, bias, gate, int(groups), ACTIVATIONS[activation], float(eps))
     with _on(x.device):
-        y = _GroupNorm.apply(x, weight, bias, gate, int(groups), ACTIVATIONS[activation],
-                             float(eps))
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+            y = _GroupNorm.apply(*args)
+        else:
+            y = _forward(*args, False)[0]
     return y.to(dtype)
