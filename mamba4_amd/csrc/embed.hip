@@ -31,28 +31,31 @@ __device__ __forceinline__ unsigned pack(float a, float b) {
 __device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 
-// V consecutive elements, read as float32 and rounded as they are stored.
+// V consecutive elements: as loaded, and as float32; written rounded.
+template <typename T, int V>
+struct Piece;
 template <int V>
-__device__ __forceinline__ void read(const float* p, float (&v)[V]) {
+struct Piece<float, V> {
   typedef float raw __attribute__((ext_vector_type(V)));
-  const raw r = *reinterpret_cast<const raw*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = r[i];
-}
+  raw r;
+  __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const raw*>(p); }
+  __device__ __forceinline__ float get(int i) const { return r[i]; }
+};
 template <int V>
-__device__ __forceinline__ void read(const bf16_t* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = __uint_as_float((unsigned)*p << 16);
-  } else {
-    typedef unsigned raw __attribute__((ext_vector_type(V / 2)));
-    const raw r = *reinterpret_cast<const raw*>(p);
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      v[i] = low(r[i / 2]);
-      v[i + 1] = high(r[i / 2]);
-    }
+struct Piece<bf16_t, V> {
+  typedef unsigned raw __attribute__((ext_vector_type(V / 2)));
+  raw r;
+  __device__ __forceinline__ void load(const bf16_t* p) { r = *reinterpret_cast<const raw*>(p); }
+  __device__ __forceinline__ float get(int i) const {
+    return i & 1 ? high(r[i / 2]) : low(r[i / 2]);
   }
-}
+};
+template <>
+struct Piece<bf16_t, 1> {
+  bf16_t r;
+  __device__ __forceinline__ void load(const bf16_t* p) { r = *p; }
+  __device__ __forceinline__ float get(int) const { return __uint_as_float((unsigned)r << 16); }
+};
 template <int V>
 __device__ __forceinline__ void write(float* p, const float (&v)[V]) {
   typedef float raw __attribute__((ext_vector_type(V)));
@@ -88,27 +91,27 @@ __global__ __launch_bounds__(THREADS) void lookup_kernel(Lookup a) {
   const unsigned rest = (unsigned)(first - row0 * vecs);
   const In* table = static_cast<const In*>(a.table);
   Out* out = static_cast<Out*>(a.out);
-  float x[4][V];
+  // Every load is issued before the first use, unknown ids' from row 0.
+  Piece<In, V> x[4];
   long at[4];
+  bool known[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const unsigned item = rest + threadIdx.x + THREADS * j, step = item / vecs;
     const unsigned v = item - step * vecs;
     const long i = row0 + step;
     at[j] = i < a.n ? i * a.width + v * V : -1;
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[j][e] = 0.f;
-    if (i < a.n) {
-      const unsigned key = key_of(a.ids, a.wide, i, a.rows);
-      if (key < (unsigned)a.rows) read<V>(table + (long)key * a.width + v * V, x[j]);
-    }
+    const unsigned key = key_of(a.ids, a.wide, min(i, a.n - 1), a.rows);
+    known[j] = key < (unsigned)a.rows;
+    x[j].load(table + (long)(known[j] ? key : 0) * a.width + v * V);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (at[j] < 0) continue;
+    float y[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x[j][e] *= a.scale;
-    write<V>(out + at[j], x[j]);
+    for (int e = 0; e < V; ++e) y[e] = known[j] ? x[j].get(e) * a.scale : 0.f;
+    write<V>(out + at[j], y);
   }
 }
 
@@ -267,21 +270,22 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
     for (int i = 0; i < V; ++i) x[i] = a.scale * acc[i];
     write<V>(dw + (long)key * a.width + column, x);
   };
+  // Loads without a condition, so that they are in flight together; what they
+  // read past the chunk or for unknown ids is not added.
   constexpr int AHEAD = 8;
   for (long i = s; i < e; i += AHEAD) {
     unsigned key[AHEAD];
-    float x[AHEAD][V];
+    Piece<In, V> x[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      key[j] = i + j < e ? a.keys[i + j] : rows;
-      const long token = i + j < e ? a.tokens[i + j] : 0;
-#pragma unroll
-      for (int k = 0; k < V; ++k) x[j][k] = 0.f;
-      if (key[j] < rows) read<V>(dy + token * a.width, x[j]);
+      const long at = min(i + j, e - 1);
+      key[j] = a.keys[at];
+      x[j].load(dy + (long)a.tokens[at] * a.width);
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      if (i + j < e && key[j] != current) {
+      if (i + j >= e) break;
+      if (key[j] != current) {
         if (from_before)
           write<V>(a.head + chunk * a.width + column, acc);
         else
@@ -291,8 +295,10 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] = 0.f;
       }
+      if (current < rows) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] += x[j][k];
+        for (int k = 0; k < V; ++k) acc[k] += x[j].get(k);
+      }
     }
   }
   if (current >= rows) return;
@@ -317,18 +323,21 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
   const unsigned key = a.keys[e - 1];
   if (key >= (unsigned)a.rows || a.keys[e] != key) return;
   if (s > 0 && a.keys[s - 1] == key) return;
+  Piece<float, V> tail;
+  tail.load(a.tail + chunk * a.width + column);
   float acc[V];
-  read<V>(a.tail + chunk * a.width + column, acc);
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = tail.get(k);
   constexpr int AHEAD = 16;
   bool more = true;
   for (long c = chunk + 1; more; c += AHEAD) {
-    float x[AHEAD][V];
+    Piece<float, V> x[AHEAD];
     bool goes_on[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       // Loads without a condition, so that they are in flight together.
       const long at = min(c + j, (long)a.chunks - 1), end = (c + j + 1) * a.chunk;
-      read<V>(a.head + at * a.width + column, x[j]);
+      x[j].load(a.head + at * a.width + column);
       const unsigned then = a.keys[min(end, a.n - 1)];
       goes_on[j] = (end < a.n) & (then == key);
     }
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
     for (int j = 0; j < AHEAD; ++j)
       if (more) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += x[j][k];
+        for (int k = 0; k < V; ++k) acc[k] += x[j].get(k);
         more = goes_on[j];
       }
   }
