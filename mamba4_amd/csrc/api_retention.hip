@@ -587,7 +587,7 @@ NormPlan norm_plan(long M, int L, int C, int G, int vec, gn::Norm* a) {
       a->rows = (int)std::min<long>(gn::ROW_THREADS / across, M);
       p.threads = (a->rows * across + 63) / 64 * 64;
       const long most = (M + a->rows - 1) / a->rows;
-      p.grid = dim3((unsigned)std::min<long>(most, 4L * cus), (G + a->groups - 1) / a->groups);
+      p.grid = dim3((unsigned)std::min<long>(most, 3L * cus), (G + a->groups - 1) / a->groups);
       p.part_rows = (int)p.grid.x;
       return p;
     }
@@ -598,12 +598,12 @@ NormPlan norm_plan(long M, int L, int C, int G, int vec, gn::Norm* a) {
   a->rows = a->subs > 1 ? 1 : std::max(1, std::min(L, gn::POS_THREADS / (vecs * a->span)));
   const int slots = (G * a->subs + a->span - 1) / a->span;
   // Enough blocks for the card, each with some rows for each thread.
-  const long want = (4L * cus + M * slots - 1) / (M * slots);
+  const long want = (2L * cus + M * slots - 1) / (M * slots);
   a->blocks = (int)std::max<long>(1, std::min<long>(want, L / (8L * a->rows)));
   if (a->subs > 1 && a->blocks == 1) a->blocks = std::min(L, 2);
   const bool whole = a->blocks == 1 && a->subs == 1;
   // Blocks walk over samples past these (the column sums have a part for each).
-  const long samples = std::min<long>(M, std::max(1L, 8L * cus / ((long)slots * a->blocks)));
+  const long samples = std::min<long>(M, std::max(1L, 4L * cus / ((long)slots * a->blocks)));
   p.grid = dim3(a->blocks, (unsigned)samples, slots);
   p.threads = gn::POS_THREADS;
   p.part_rows = (int)samples * a->blocks;

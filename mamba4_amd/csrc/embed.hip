@@ -163,6 +163,7 @@ __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
     }
   };
   unsigned key[ROUNDS], rank[ROUNDS];
+  unsigned long same[ROUNDS];  // lanes with this lane's digit
   fetch(0, key);
   for (int d = tid; d < (THREADS / 64) * BINS; d += THREADS) (&place[0][0])[d] = 0;
   // This tile's part in the digits: all tiles' counts, and those before it.
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
       const unsigned digit = (key[j] >> a.shift) & (size - 1);
       const unsigned long mask = peers(digit, a.bits, have);
       const unsigned seen = __popcll(mask & below);
+      same[j] = mask;
       rank[j] = place[w][digit] + seen;
       __builtin_amdgcn_wave_barrier();
       if (have && seen == 0) place[w][digit] += __popcll(mask);
@@ -222,14 +224,25 @@ __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j) {
       const long i = first + k + 64 * j + lane;
-      if (i >= a.n) continue;
+      const bool have = i < a.n;
       const unsigned digit = (key[j] >> a.shift) & (size - 1);
-      const unsigned at = once ? place[w][digit] + rank[j] : rank[j];
+      const unsigned at = once && have ? place[w][digit] + rank[j] : rank[j];
+      if (a.next) {
+        // One addition for the lanes that share the first one's id and tile: a
+        // frequent id's would meet at one address.
+        const unsigned tile = at / a.tile;
+        const int lead = __ffsll((unsigned long long)same[j]) - 1;
+        const unsigned lead_key = __shfl(key[j], lead), lead_tile = __shfl(tile, lead);
+        const bool with = have && key[j] == lead_key && tile == lead_tile;
+        const unsigned long group = __ballot(with) & same[j];
+        unsigned* counter = &a.next[((long)tile << a.next_bits) +
+                                    ((key[j] >> a.next_shift) & ((1 << a.next_bits) - 1))];
+        if (have && lane == lead) atomicAdd(counter, (unsigned)__popcll(group));
+        if (have && !with) atomicAdd(counter, 1u);
+      }
+      if (!have) continue;
       a.out_keys[at] = key[j];
       a.out_tokens[at] = a.tokens ? a.tokens[i] : (unsigned)i;
-      if (a.next)
-        atomicAdd(&a.next[((long)(at / a.tile) << a.next_bits) +
-                          ((key[j] >> a.next_shift) & ((1 << a.next_bits) - 1))], 1u);
       if (a.present && key[j] < (unsigned)a.rows) a.present[key[j]] = 1;
     }
   }

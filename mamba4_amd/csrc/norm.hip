@@ -156,22 +156,36 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
     }
   }
   const float scale = 1.f / a.D;
-  for (long base = (long)blockIdx.x * a.rows; base < a.M; base += (long)gridDim.x * a.rows) {
+  const long stride = (long)gridDim.x * a.rows;
+  // The next row's pieces are on their way while a row is computed.
+  Vec<In, V> xn[IT], gn[IT], dn_[IT];
+  auto fetch = [&](long m) {
+    const long at = m * a.C + group * a.D + lane * V;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      xn[i].zero();
+      gn[i].zero();
+      dn_[i].zero();
+      if (m < a.M && on[i]) {
+        xn[i].load(a.x, at + i * a.lanes * V);
+        if (a.gate) gn[i].load(a.gate, at + i * a.lanes * V);
+        if (BWD) dn_[i].load(a.dy, at + i * a.lanes * V);
+      }
+    }
+  };
+  fetch((long)blockIdx.x * a.rows + rr);
+  for (long base = (long)blockIdx.x * a.rows; base < a.M; base += stride) {
     const long m = base + rr;
     const bool here = m < a.M;
     const long at = m * a.C + group * a.D + lane * V;
     Vec<In, V> xv[IT], gv[IT], dv[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      xv[i].zero();
-      gv[i].zero();
-      dv[i].zero();
-      if (here && on[i]) {
-        xv[i].load(a.x, at + i * a.lanes * V);
-        if (a.gate) gv[i].load(a.gate, at + i * a.lanes * V);
-        if (BWD) dv[i].load(a.dy, at + i * a.lanes * V);
-      }
+      xv[i] = xn[i];
+      gv[i] = gn[i];
+      dv[i] = dn_[i];
     }
+    fetch(m + stride);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < IT; ++i)

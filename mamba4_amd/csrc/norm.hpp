@@ -9,7 +9,7 @@ namespace gn {
 typedef unsigned short bf16_t;
 
 constexpr int ROW_THREADS = 512;   // largest block of the row kernels
-constexpr int POS_THREADS = 256;   // block of the position kernels
+constexpr int POS_THREADS = 512;   // block of the position kernels
 enum Activation { NONE = 0, SILU = 1, GELU = 2 };
 // What a launch over positions does: partial sums, what follows from them, or
 // both (a block holds whole samples).
