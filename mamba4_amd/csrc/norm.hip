@@ -130,6 +130,22 @@ __device__ __forceinline__ float activate(float z, int act, float* slope) {
   return z;
 }
 
+// The same of several values, with one choice of the activation.
+template <int V>
+__device__ __forceinline__ void activate(const float (&z)[V], int act, float (&y)[V],
+                                         float (&slope)[V]) {
+  if (act == SILU) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) y[k] = activate(z[k], SILU, &slope[k]);
+  } else if (act == GELU) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) y[k] = activate(z[k], GELU, &slope[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) y[k] = activate(z[k], NONE, &slope[k]);
+  }
+}
+
 // ---------------------------------------------------------------- one position
 
 template <typename In, int V, int IT, bool BWD>
@@ -186,28 +202,40 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
       dv[i] = dn_[i];
     }
     fetch(m + stride);
+    float n[IT][V];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
-      for (int k = 0; k < V; ++k) s += xv[i].get(k);
+      for (int k = 0; k < V; ++k) {
+        n[i][k] = xv[i].get(k);
+        s += n[i][k];
+      }
     const float mean = group_sum(s, a.lanes) * scale;
-    // The mean's own rounding, which a small deviation about a large mean feels.
+    // Again, for the mean's own rounding, which a small deviation about a large
+    // mean feels.
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
-      for (int k = 0; k < V; ++k) s += on[i] ? xv[i].get(k) - mean : 0.f;
+      for (int k = 0; k < V; ++k) {
+        n[i][k] = on[i] ? n[i][k] - mean : 0.f;
+        s += n[i][k];
+      }
     const float rest = group_sum(s, a.lanes) * scale;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float d = on[i] ? (xv[i].get(k) - mean) - rest : 0.f;
-        s = fmaf(d, d, s);
+        n[i][k] = on[i] ? n[i][k] - rest : 0.f;
+        s = fmaf(n[i][k], n[i][k], s);
       }
-    const float inv = 1.f / sqrtf(fmaf(group_sum(s, a.lanes), scale, a.eps));
+    const float inv = __builtin_amdgcn_rsqf(fmaf(group_sum(s, a.lanes), scale, a.eps));
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) n[i][k] *= inv;
     if constexpr (!BWD) {
       if (a.stats && here && member && lane == 0) {
         a.stats[(m * a.G + group) * 2] = mean + rest;
@@ -215,12 +243,16 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
       }
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        float y[V];
+        float z[V], u[V], y[V], slope[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float z = fmaf(((xv[i].get(k) - mean) - rest) * inv, w[i][k], bias[i][k]);
-          float slope;
-          y[k] = a.gate ? z * activate(gv[i].get(k), a.act, &slope) : activate(z, a.act, &slope);
+          z[k] = fmaf(n[i][k], w[i][k], bias[i][k]);
+          u[k] = a.gate ? gv[i].get(k) : z[k];
+        }
+        activate<V>(u, a.act, y, slope);
+        if (a.gate) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) y[k] *= z[k];
         }
         if (here && on[i]) Vec<In, V>::store(a.y, at + i * a.lanes * V, y);
       }
@@ -229,30 +261,38 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        float dg[V];
+        float z[V], u[V], y[V], slope[V], dz[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float n = ((xv[i].get(k) - mean) - rest) * inv, dy = dv[i].get(k);
-          const float z = fmaf(n, w[i][k], bias[i][k]);
-          float slope, dz;
-          if (a.gate) {
-            const float act = activate(gv[i].get(k), a.act, &slope);
-            dz = dy * act;
-            dg[k] = dy * z * slope;
-          } else {
-            activate(z, a.act, &slope);
-            dz = dy * slope;
+          z[k] = fmaf(n[i][k], w[i][k], bias[i][k]);
+          u[k] = a.gate ? gv[i].get(k) : z[k];
+        }
+        activate<V>(u, a.act, y, slope);
+        if (a.gate) {
+          float dg[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            dz[k] = dv[i].get(k) * y[k];
+            dg[k] = dv[i].get(k) * z[k] * slope[k];
           }
-          if (!on[i]) dz = 0.f;
-          dn[i][k] = dz * w[i][k];
+          if (here && on[i]) Vec<In, V>::store(a.dgate, at + i * a.lanes * V, dg);
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) dz[k] = dv[i].get(k) * slope[k];
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          dn[i][k] = dz[k] * w[i][k];
           s1 += dn[i][k];
-          s2 = on[i] ? fmaf(dn[i][k], n, s2) : s2;
-          if (here && on[i]) {
-            dw[i][k] = fmaf(dz, n, dw[i][k]);
-            db[i][k] += dz;
+          s2 = fmaf(dn[i][k], n[i][k], s2);
+        }
+        if (here) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            dw[i][k] = fmaf(dz[k], n[i][k], dw[i][k]);
+            db[i][k] += dz[k];
           }
         }
-        if (a.gate && here && on[i]) Vec<In, V>::store(a.dgate, at + i * a.lanes * V, dg);
       }
       s1 = group_sum(s1, a.lanes) * scale;
       s2 = group_sum(s2, a.lanes) * scale;
@@ -260,10 +300,7 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
       for (int i = 0; i < IT; ++i) {
         float dx[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float n = ((xv[i].get(k) - mean) - rest) * inv;
-          dx[k] = inv * (dn[i][k] - s1 - n * s2);
-        }
+        for (int k = 0; k < V; ++k) dx[k] = inv * (dn[i][k] - s1 - n[i][k] * s2);
         if (here && on[i]) Vec<In, V>::store(a.dx, at + i * a.lanes * V, dx);
       }
     }
@@ -455,12 +492,16 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i)
             if (l + i * a.rows < l1) {
-              float y[V];
+              float z[V], u[V], y[V], slope[V];
 #pragma unroll
               for (int e = 0; e < V; ++e) {
-                const float z = fmaf((x[i].get(e) - mean) * inv, w[e], bias[e]);
-                float slope;
-                y[e] = a.gate ? z * activate(g[i].get(e), a.act, &slope) : activate(z, a.act, &slope);
+                z[e] = fmaf((x[i].get(e) - mean) * inv, w[e], bias[e]);
+                u[e] = a.gate ? g[i].get(e) : z[e];
+              }
+              activate<V>(u, a.act, y, slope);
+              if (a.gate) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] *= z[e];
               }
               Vec<In, V>::store(a.y, at + (long)(l + i * a.rows) * a.C, y);
             }
@@ -488,20 +529,21 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
               }
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
-              if (l + i * a.rows < l1)
+              if (l + i * a.rows < l1) {
+                float n[V], u[V], y[V], slope[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                  const float n = (x[i].get(e) - mean) * inv;
-                  float slope, dz = d[i].get(e);
-                  if (a.gate) {
-                    dz *= activate(g[i].get(e), a.act, &slope);
-                  } else {
-                    activate(fmaf(n, w[e], bias[e]), a.act, &slope);
-                    dz *= slope;
-                  }
-                  dws[e] = fmaf(dz, n, dws[e]);
+                  n[e] = (x[i].get(e) - mean) * inv;
+                  u[e] = a.gate ? g[i].get(e) : fmaf(n[e], w[e], bias[e]);
+                }
+                activate<V>(u, a.act, y, slope);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                  const float dz = d[i].get(e) * (a.gate ? y[e] : slope[e]);
+                  dws[e] = fmaf(dz, n[e], dws[e]);
                   dbs[e] += dz;
                 }
+              }
           }
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -543,20 +585,19 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
           for (int i = 0; i < AHEAD; ++i)
             if (l + i * a.rows < l1) {
               const long p = at + (long)(l + i * a.rows) * a.C;
-              float dx[V], dg[V];
+              float n[V], z[V], u[V], y[V], slope[V], dx[V], dg[V];
 #pragma unroll
               for (int e = 0; e < V; ++e) {
-                const float n = (x[i].get(e) - mean) * inv, dy = d[i].get(e);
-                const float z = fmaf(n, w[e], bias[e]);
-                float slope, dz;
-                if (a.gate) {
-                  dz = dy * activate(g[i].get(e), a.act, &slope);
-                  dg[e] = dy * z * slope;
-                } else {
-                  activate(z, a.act, &slope);
-                  dz = dy * slope;
-                }
-                dx[e] = inv * (dz * w[e] - s1 - n * s2);
+                n[e] = (x[i].get(e) - mean) * inv;
+                z[e] = fmaf(n[e], w[e], bias[e]);
+                u[e] = a.gate ? g[i].get(e) : z[e];
+              }
+              activate<V>(u, a.act, y, slope);
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float dy = d[i].get(e), dz = dy * (a.gate ? y[e] : slope[e]);
+                dg[e] = dy * z[e] * slope[e];
+                dx[e] = inv * (dz * w[e] - s1 - n[e] * s2);
               }
               Vec<In, V>::store(a.dx, p, dx);
               if (a.gate) Vec<In, V>::store(a.dgate, p, dg);
