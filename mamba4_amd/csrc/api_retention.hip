@@ -860,8 +860,10 @@ void launch_sums(const em::Sum& a, int table_bf16, int out_bf16, hipStream_t st)
     out_bf16 ? start_sums<em::bf16_t, float, V>(a, st) : start_sums<float, float, V>(a, st);
 }
 
-template <int V>
+// (Pieces of at most four: the parts are float32.)
+template <int W>
 void launch_join(const em::Sum& a, int table_bf16, hipStream_t st) {
+  constexpr int V = W < 4 ? W : 4;
   const dim3 grid((unsigned)(((long)a.chunks * (a.width / V) + em::THREADS - 1) / em::THREADS));
   if (table_bf16)
     hipLaunchKernelGGL((em::join_kernel<em::bf16_t, V>), grid, dim3(em::THREADS), 0, st, a);

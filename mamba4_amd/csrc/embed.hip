@@ -286,15 +286,26 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
   // Loads without a condition, so that they are in flight together; what they
   // read past the chunk or for unknown ids is not added.
   constexpr int AHEAD = 8;
+  unsigned next_key[AHEAD], next_token[AHEAD];
+  auto fetch = [&](long i) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const long at = min(i + j, e - 1);
+      next_key[j] = a.keys[at];
+      next_token[j] = a.tokens[at];
+    }
+  };
+  fetch(s);
   for (long i = s; i < e; i += AHEAD) {
     unsigned key[AHEAD];
     Piece<In, V> x[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const long at = min(i + j, e - 1);
-      key[j] = a.keys[at];
-      x[j].load(dy + (long)a.tokens[at] * a.width);
+      key[j] = next_key[j];
+      x[j].load(dy + (long)next_token[j] * a.width);
     }
+    fetch(i + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);  // all of them before the first sum
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (i + j >= e) break;
@@ -341,7 +352,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
   float acc[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = tail.get(k);
-  constexpr int AHEAD = 16;
+  constexpr int AHEAD = 128 / V < 32 ? 128 / V : 32;
   bool more = true;
   for (long c = chunk + 1; more; c += AHEAD) {
     Piece<float, V> x[AHEAD];
@@ -354,13 +365,14 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
       const unsigned then = a.keys[min(end, a.n - 1)];
       goes_on[j] = (end < a.n) & (then == key);
     }
+    __builtin_amdgcn_sched_barrier(0);  // all of them before the first sum
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (more) {
+    for (int j = 0; j < AHEAD; ++j) {
+      // (Selected, not branched around: the loads would move into the branches.)
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += x[j].get(k);
-        more = goes_on[j];
-      }
+      for (int k = 0; k < V; ++k) acc[k] = more ? acc[k] + x[j].get(k) : acc[k];
+      more = more & goes_on[j];
+    }
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] *= a.scale;
@@ -374,12 +386,16 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
   EM_TYPES(float, float, V)                                  \
   EM_TYPES(float, bf16_t, V)                                 \
   EM_TYPES(bf16_t, float, V)                                 \
-  EM_TYPES(bf16_t, bf16_t, V)                                \
+  EM_TYPES(bf16_t, bf16_t, V)
+#define EM_JOIN(V)                                           \
   template __global__ void join_kernel<float, V>(Sum);       \
   template __global__ void join_kernel<bf16_t, V>(Sum);
 EM_ALL(8)
 EM_ALL(4)
 EM_ALL(2)
 EM_ALL(1)
+EM_JOIN(4)
+EM_JOIN(2)
+EM_JOIN(1)
 
 }  // namespace em
