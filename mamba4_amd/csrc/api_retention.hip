@@ -818,8 +818,9 @@ size_t embedding_plan(long n, int rows, int width, void* base, EmbeddingPlan* p)
   p->present = c.take<unsigned char>(rows);
   p->cleared = (c.used - first) / sizeof(unsigned);
   for (int i = 0; i < 2; ++i) {
-    p->keys[i] = c.take<unsigned>(n);
-    p->tokens[i] = c.take<unsigned>(n);
+    // (Padded: a batch of rows may end past the last.)
+    p->keys[i] = c.take<unsigned>(n + em::AHEAD);
+    p->tokens[i] = c.take<unsigned>(n + em::AHEAD);
   }
   p->head = c.take<float>((size_t)p->chunks * width);
   p->tail = c.take<float>((size_t)p->chunks * width);
@@ -843,9 +844,15 @@ void launch_lookup(const em::Lookup& a, int table_bf16, int out_bf16, hipStream_
     out_bf16 ? start_lookup<float, em::bf16_t, V>(a, st) : start_lookup<float, float, V>(a, st);
 }
 
+// Blocks of waves that take 64 pieces of a chunk's columns each.
+long chunk_blocks(const em::Sum& a, int V) {
+  constexpr int waves = em::THREADS / 64;
+  return ((long)a.chunks * ((a.width / V + 63) / 64) + waves - 1) / waves;
+}
+
 template <typename In, typename Out, int V>
 void start_sums(const em::Sum& a, hipStream_t st) {
-  const long vecs = a.width / V, sums = (a.chunks * vecs + em::THREADS - 1) / em::THREADS;
+  const long vecs = a.width / V, sums = chunk_blocks(a, V);
   const long zeros = (a.rows * vecs + 4 * em::THREADS - 1) / (4 * em::THREADS);
   hipLaunchKernelGGL((em::sum_kernel<In, Out, V>), dim3((unsigned)(sums + zeros)),
                      dim3(em::THREADS), 0, st, a, (unsigned)sums);
@@ -860,11 +867,9 @@ void launch_sums(const em::Sum& a, int table_bf16, int out_bf16, hipStream_t st)
     out_bf16 ? start_sums<em::bf16_t, float, V>(a, st) : start_sums<float, float, V>(a, st);
 }
 
-// (Pieces of at most four: the parts are float32.)
-template <int W>
+template <int V>
 void launch_join(const em::Sum& a, int table_bf16, hipStream_t st) {
-  constexpr int V = W < 4 ? W : 4;
-  const dim3 grid((unsigned)(((long)a.chunks * (a.width / V) + em::THREADS - 1) / em::THREADS));
+  const dim3 grid((unsigned)chunk_blocks(a, V));
   if (table_bf16)
     hipLaunchKernelGGL((em::join_kernel<em::bf16_t, V>), grid, dim3(em::THREADS), 0, st, a);
   else

@@ -40,6 +40,14 @@ struct Piece<float, V> {
   raw r;
   __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const raw*>(p); }
   __device__ __forceinline__ float get(int i) const { return r[i]; }
+  __device__ __forceinline__ void touch() {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float x = r[i];
+      asm volatile("" : "+v"(x));
+      r[i] = x;
+    }
+  }
 };
 template <int V>
 struct Piece<bf16_t, V> {
@@ -49,12 +57,25 @@ struct Piece<bf16_t, V> {
   __device__ __forceinline__ float get(int i) const {
     return i & 1 ? high(r[i / 2]) : low(r[i / 2]);
   }
+  __device__ __forceinline__ void touch() {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      unsigned x = r[i];
+      asm volatile("" : "+v"(x));
+      r[i] = x;
+    }
+  }
 };
 template <>
 struct Piece<bf16_t, 1> {
   bf16_t r;
   __device__ __forceinline__ void load(const bf16_t* p) { r = *p; }
   __device__ __forceinline__ float get(int) const { return __uint_as_float((unsigned)r << 16); }
+  __device__ __forceinline__ void touch() {
+    unsigned x = r;
+    asm volatile("" : "+v"(x));
+    r = (bf16_t)x;
+  }
 };
 template <int V>
 __device__ __forceinline__ void write(float* p, const float (&v)[V]) {
@@ -248,7 +269,30 @@ __global__ __launch_bounds__(THREADS) void scatter_kernel(Sort a) {
   }
 }
 
-// Sums of runs: a thread takes one piece of the columns of one chunk.  The
+// The sorted ids and tokens, which no kernel that reads them so writes.
+typedef const __attribute__((address_space(4))) unsigned* Scalars;
+
+// Every load of x is issued before this point: without it the compiler moves
+// them to their uses behind branches, one wait each.
+template <typename P, int N>
+__device__ __forceinline__ void in_flight(P (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i].touch();
+}
+
+// A wave's chunk, and the lane's piece of the columns.
+struct Place {
+  int chunk, piece;
+};
+__device__ __forceinline__ Place place_of(int vecs) {
+  const unsigned slices = (vecs + 63) / 64;
+  const unsigned wave =
+      __builtin_amdgcn_readfirstlane(blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6));
+  const unsigned chunk = wave / slices;
+  return Place{(int)chunk, (int)(64 * (wave - chunk * slices) + (threadIdx.x & 63))};
+}
+
+// Sums of runs: a wave takes 64 pieces of the columns of one chunk.  The
 // blocks from `sum_blocks` on zero the rows that do not occur (blocks of both kinds
 // in turn took longer).
 template <typename In, typename Out, int V>
@@ -268,50 +312,44 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
     }
     return;
   }
-  const long thread = (long)blockIdx.x * THREADS + threadIdx.x;
-  const long chunk = thread / vecs;
-  if (chunk >= a.chunks) return;
-  const int column = (int)(thread - chunk * vecs) * V;
-  const In* dy = static_cast<const In*>(a.dy) + column;
+  // A wave: 64 pieces of one chunk's columns, so that ids and tokens are scalars.
+  const Place at = place_of(vecs);
+  if (at.chunk >= a.chunks) return;
+  const long chunk = at.chunk;
+  const int column = at.piece * V;
+  const bool on = at.piece < vecs;
+  const In* dy = static_cast<const In*>(a.dy) + (on ? column : 0);
+  const Scalars keys = (Scalars)a.keys, tokens = (Scalars)a.tokens;
   const long s = chunk * a.chunk, e = min(s + a.chunk, a.n);
-  unsigned current = a.keys[s];
-  bool from_before = s > 0 && a.keys[s - 1] == current;
+  unsigned current = keys[s];
+  bool from_before = s > 0 && keys[s - 1] == current;
   float acc[V] = {};
   auto store = [&](unsigned key) {
     float x[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = a.scale * acc[i];
-    write<V>(dw + (long)key * a.width + column, x);
+    if (on) write<V>(dw + (long)key * a.width + column, x);
+  };
+  auto keep = [&](float* parts) {
+    if (on) write<V>(parts + chunk * a.width + column, acc);
   };
   // Loads without a condition, so that they are in flight together; what they
-  // read past the chunk or for unknown ids is not added.
-  constexpr int AHEAD = 8;
-  unsigned next_key[AHEAD], next_token[AHEAD];
-  auto fetch = [&](long i) {
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const long at = min(i + j, e - 1);
-      next_key[j] = a.keys[at];
-      next_token[j] = a.tokens[at];
-    }
-  };
-  fetch(s);
+  // read past the chunk (the arrays are padded) or for unknown ids is not added.
   for (long i = s; i < e; i += AHEAD) {
     unsigned key[AHEAD];
     Piece<In, V> x[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      key[j] = next_key[j];
-      x[j].load(dy + (long)next_token[j] * a.width);
+      key[j] = keys[i + j];
+      const long token = key[j] < rows ? tokens[i + j] : 0u;
+      x[j].load(dy + min(token, a.n - 1) * a.width);
     }
-    fetch(i + AHEAD);
-    __builtin_amdgcn_sched_barrier(0);  // all of them before the first sum
+    in_flight(x);
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      if (i + j >= e) break;
-      if (key[j] != current) {
+      if (i + j < e && key[j] != current) {
         if (from_before)
-          write<V>(a.head + chunk * a.width + column, acc);
+          keep(a.head);
         else
           store(current);
         from_before = false;
@@ -319,7 +357,7 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] = 0.f;
       }
-      if (current < rows) {
+      if (i + j < e && current < rows) {
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] += x[j].get(k);
       }
@@ -327,9 +365,9 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
   }
   if (current >= rows) return;
   if (from_before)
-    write<V>(a.head + chunk * a.width + column, acc);
-  else if (e < a.n && a.keys[e] == current)
-    write<V>(a.tail + chunk * a.width + column, acc);
+    keep(a.head);
+  else if (e < a.n && keys[e] == current)
+    keep(a.tail);
   else
     store(current);
 }
@@ -338,42 +376,45 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(Sum a, unsigned sum_blocks
 template <typename Out, int V>
 __global__ __launch_bounds__(THREADS) void join_kernel(Sum a) {
   const int vecs = a.width / V;
-  const long thread = (long)blockIdx.x * THREADS + threadIdx.x;
-  const long chunk = thread / vecs;
-  if (chunk >= a.chunks) return;
-  const int column = (int)(thread - chunk * vecs) * V;
+  const Place at = place_of(vecs);
+  if (at.chunk >= a.chunks) return;
+  const long chunk = at.chunk;
+  const bool on = at.piece < vecs;
+  const int column = on ? at.piece * V : 0;
+  const Scalars keys = (Scalars)a.keys;
   const long s = chunk * a.chunk, e = s + a.chunk;
   if (e >= a.n) return;
-  const unsigned key = a.keys[e - 1];
-  if (key >= (unsigned)a.rows || a.keys[e] != key) return;
-  if (s > 0 && a.keys[s - 1] == key) return;
+  const unsigned key = keys[e - 1];
+  if (key >= (unsigned)a.rows || keys[e] != key) return;
+  if (s > 0 && keys[s - 1] == key) return;
   Piece<float, V> tail;
   tail.load(a.tail + chunk * a.width + column);
   float acc[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = tail.get(k);
-  constexpr int AHEAD = 128 / V < 32 ? 128 / V : 32;
+  // The run's parts, 64 at a time: where it ends, then the sums.
+  constexpr int PARTS = 16;
   bool more = true;
-  for (long c = chunk + 1; more; c += AHEAD) {
-    Piece<float, V> x[AHEAD];
-    bool goes_on[AHEAD];
+  for (long c = chunk + 1; more; c += 64) {
+    const long end = (c + (threadIdx.x & 63) + 1) * a.chunk;
+    const unsigned then = a.keys[min(end, a.n - 1)];
+    const unsigned long goes_on = __ballot(end < a.n && then == key);
+    more = ~goes_on == 0;
+    const int parts = more ? 64 : __ffsll((unsigned long long)~goes_on);
+    for (int first = 0; first < parts; first += PARTS) {
+      Piece<float, V> x[PARTS];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      // Loads without a condition, so that they are in flight together.
-      const long at = min(c + j, (long)a.chunks - 1), end = (c + j + 1) * a.chunk;
-      x[j].load(a.head + at * a.width + column);
-      const unsigned then = a.keys[min(end, a.n - 1)];
-      goes_on[j] = (end < a.n) & (then == key);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // all of them before the first sum
+      for (int j = 0; j < PARTS; ++j)
+        x[j].load(a.head + min(c + first + j, (long)a.chunks - 1) * a.width + column);
+      in_flight(x);
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      // (Selected, not branched around: the loads would move into the branches.)
+      for (int j = 0; j < PARTS; ++j)
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] = more ? acc[k] + x[j].get(k) : acc[k];
-      more = more & goes_on[j];
+        for (int k = 0; k < V; ++k)
+          acc[k] = first + j < parts ? acc[k] + x[j].get(k) : acc[k];
     }
   }
+  if (!on) return;
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] *= a.scale;
   write<V>(static_cast<Out*>(a.dw) + (long)key * a.width + column, acc);
@@ -394,6 +435,7 @@ EM_ALL(8)
 EM_ALL(4)
 EM_ALL(2)
 EM_ALL(1)
+EM_JOIN(8)
 EM_JOIN(4)
 EM_JOIN(2)
 EM_JOIN(1)

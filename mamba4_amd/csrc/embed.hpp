@@ -9,6 +9,7 @@ namespace em {
 typedef unsigned short bf16_t;
 
 constexpr int THREADS = 256;
+constexpr int AHEAD = 8;               // rows a thread loads at a time
 constexpr int MAX_DIGIT = 9;          // bits of a sorting pass
 constexpr int BINS = 1 << MAX_DIGIT;  // most bins of a pass
 
