@@ -54,10 +54,11 @@ typedef struct {
  * output [B,T,H,P] in v's type; state [B,H,N,P] float32, after the last
  * token, or NULL.
  *
- * Sums, states and decays are held in float32 or more (bfloat16 operands that are
- * computed on the way, the scores, the state and the weighted keys, enter the
- * products as two bfloat16 parts, those of float32 calls as three).  A row's result
- * does not depend on the batch size.  A log decay of -infinity (or any that
+ * Sums, states and decays are held in float32 or more.  What is computed on the way
+ * and multiplied again (the scores, the state, the weighted keys) enters the products
+ * as three bfloat16 parts, all its bits, where the result is float32, and as two
+ * where it is rounded to bfloat16.  A row's result does not depend on the batch
+ * size.  A log decay of -infinity (or any that
  * underflows) drops what came before exactly.  An infinity or NaN in a row
  * that is present spreads to the outputs of its chunk of 64 tokens and after it.
  */
@@ -73,10 +74,11 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
  * where both d_state and d_log_decay are given.  d_q, d_k, d_v:
  * [B,T,heads,width] in the inputs' type, contiguous; d_log_decay float32,
  * [B,T,H] if per_token else [H], or NULL; d_initial [B,H,N,P], or NULL.
- * Gradients of shared heads are summed in float32 and rounded once.
+ * Gradients of shared heads are summed in float32 and rounded once.  `decays` of
+ * the workspace's size: whether d_log_decay is wanted.
  */
 size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads, int k_heads,
-                                               int v_heads, int N, int P, int bf16);
+                                               int v_heads, int N, int P, int bf16, int decays);
 int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_decay,
                             int per_token, const int* lengths, const float* initial, float scale,
                             int B, int T, int H, const void* d_output, const float* d_state, const float* state,

@@ -133,7 +133,7 @@ SIGNATURES = {
     "m4rt_attention_workspace_bytes": (_S, [_I] * 6),
     "m4rt_attention_forward": (
         _I, [_P, _I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 3 + [_S, _P]),
-    "m4rt_attention_backward_workspace_bytes": (_S, [_I] * 9),
+    "m4rt_attention_backward_workspace_bytes": (_S, [_I] * 10),
     "m4rt_attention_backward": (
         _I, [_P, _I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 9 + [_S, _P]),
     "m4rt_attention_step": (

@@ -145,7 +145,8 @@ class _Attention(torch.autograd.Function):
         d_decay = torch.empty_like(log_decay) if ctx.needs_input_grad[3] else None
         d_initial = torch.empty_like(state) if ctx.needs_input_grad[4] else None
         nbytes = lib.m4rt_attention_backward_workspace_bytes(
-            batch, time, heads, q.shape[2], k.shape[2], v.shape[2], n, p, bf16)
+            batch, time, heads, q.shape[2], k.shape[2], v.shape[2], n, p, bf16,
+            d_decay is not None)
         workspace = _workspace(nbytes, device)
         rc = lib.m4rt_attention_backward(
             _qkv(q, k, v), bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),

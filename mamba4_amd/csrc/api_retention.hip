@@ -21,7 +21,7 @@ template <typename In, int NP, int NN, bool DOTS, bool WHOLE>
 __global__ void attention_backward_kernel(Args);
 __global__ void carry_kernel(Args);
 __global__ void decay_grad_kernel(DecayGrad);
-__global__ void decay_heads_kernel(const double*, int, int, float*);
+__global__ void decay_heads_kernel(const double*, int, int, int, float*);
 template <typename Out>
 __global__ void share_sum_kernel(const float*, long, int, int, int, Out*);
 template <typename In, int V, int PASSES>
@@ -133,8 +133,9 @@ bool attention_splits(const Shape& s, int blocks) {
     if (std::strcmp(mode, "walk") == 0) return false;
     if (std::strcmp(mode, "split") == 0) return true;
   }
-  const bool wide = s.N > 64 || (blocks > tiles_of(s.P) && s.P > 64);
-  const double step = (s.bf16 ? 2.1 : 4.1) * (wide ? 1.5 : 1.0);  // us a chunk
+  const bool backward = blocks > tiles_of(s.P), wide = s.N > 64 || (backward && s.P > 64);
+  const double step = (s.bf16 ? 2.1 : 4.1) * (wide ? 1.5 : 1.0) *
+                      (backward ? (s.bf16 ? 1.2 : 1.6) : 1.0);  // us a chunk
   const double units = m4::api_compute_units(), walks = (double)s.B * s.H * blocks;
   const double walk = s.chunks() * step * std::max(1.0, 0.95 * walks / units);
   const double split =
@@ -142,8 +143,8 @@ bool attention_splits(const Shape& s, int blocks) {
   return split < walk;
 }
 
-// A split run's states of one role (n keys wide, `tiles` blocks of values); no
-// segments: not split.
+// The segments' states of one role (n keys wide, `tiles` blocks of values); no
+// segments: none are kept.
 void take_states(Carver& c, const Shape& s, int n, int tiles, int segments, la::Role* role) {
   const size_t slots = (size_t)tiles * s.B * s.H * segments;
   role->starts = c.take<float>(slots * tiles_of(n) * la::TILE * la::TILE);
@@ -291,21 +292,24 @@ struct Backward {
 
 int backward_tiles(const Shape& s) { return 2 * tiles_of(s.N) + tiles_of(s.P); }
 
-// The backward's workspace: split states, float32 gradients of shared heads
-// before their sums, the dots, the heads' sums.
-size_t backward_workspace(const Shape& s, const int heads[3], void* base, Backward* out) {
+// The backward's workspace: the segments' states (of dQ and dK for the decays'
+// gradient too), float32 gradients of shared heads before their sums, the dots, the
+// heads' sums.
+size_t backward_workspace(const Shape& s, const int heads[3], bool decays, void* base,
+                          Backward* out) {
   Carver c{static_cast<char*>(base)};
   const int n[3] = {s.P, s.P, s.N}, p[3] = {s.N, s.N, s.P};
   const size_t rows = (size_t)s.B * s.T * s.H;
-  const int blocks = backward_tiles(s);
-  const int split = attention_splits(s, blocks) ? segments(s, blocks) : 0;
+  const int blocks = backward_tiles(s), count = segments(s, blocks);
+  const bool split = attention_splits(s, blocks);
   for (int i = 0; i < 3; ++i) {
-    take_states(c, s, n[i], tiles_of(p[i]), split, &out->role[i]);
+    take_states(c, s, n[i], tiles_of(p[i]), split || (decays && i < 2) ? count : 0,
+                &out->role[i]);
     out->part[i] = c.take<float>(heads[i] == s.H ? 0 : rows * p[i]);
   }
-  out->dots_q = c.take<float>(rows * tiles_of(s.N));
-  out->dots_k = c.take<float>(rows * tiles_of(s.N));
-  out->head = c.take<double>((size_t)s.B * s.H);
+  out->dots_q = c.take<float>(decays ? rows * tiles_of(s.N) : 0);
+  out->dots_k = c.take<float>(decays ? rows * tiles_of(s.N) : 0);
+  out->head = c.take<double>(decays ? (size_t)s.B * s.H * count : 0);
   return c.used;
 }
 
@@ -369,13 +373,13 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
 }
 
 size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads, int k_heads,
-                                               int v_heads, int N, int P, int bf16) {
+                                               int v_heads, int N, int P, int bf16, int decays) {
   const Shape s{B, T, H, N, P, bf16};
   const int heads[3] = {q_heads, k_heads, v_heads};
   std::string why;
   if (bad_shape(s, &why)) return 0;
   Backward w{};
-  return backward_workspace(s, heads, nullptr, &w);
+  return backward_workspace(s, heads, decays, nullptr, &w);
 }
 
 int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_decay,
@@ -398,7 +402,7 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     const int heads[3] = {q->heads, k->heads, v->heads};
     Backward w{};
-    const size_t need = backward_workspace(s, heads, workspace, &w);
+    const size_t need = backward_workspace(s, heads, d_log_decay != nullptr, workspace, &w);
     if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
     const m4rt_rows cot = dense(d_output, T, H, s.P);
@@ -460,7 +464,12 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
     la::DecayGrad d{};
     d.dots_q = w.dots_q;
     d.dots_k = w.dots_k;
-    d.tiles_q = d.tiles_k = tiles_of(s.N);
+    d.starts_q = w.role[0].starts;
+    d.starts_k = w.role[1].starts;
+    d.tiles = tiles_of(s.N);
+    d.slot = tiles_of(s.P) * la::TILE * la::TILE;
+    d.seg = a.seg;
+    d.NS = a.NS;
     d.g = log_decay;
     d.gb = a.gb;
     d.gt = a.gt;
@@ -475,11 +484,12 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
     d.T = T;
     d.H = H;
     rc = api_launch("attention_decay", st, [&] {
-      hipLaunchKernelGGL(la::decay_grad_kernel, dim3(B * H), dim3(1024), 0, st, d);
+      hipLaunchKernelGGL(la::decay_grad_kernel, dim3(B * H, a.NS), dim3(la::GRAD_THREADS), 0, st,
+                         d);
     });
     if (rc || per_token) return rc;
     return api_launch("attention_heads", st, [&] {
-      hipLaunchKernelGGL(la::decay_heads_kernel, dim3((H + 63) / 64), dim3(64), 0, st, w.head, B, H,
+      hipLaunchKernelGGL(la::decay_heads_kernel, dim3(H), dim3(64), 0, st, w.head, B, H, a.NS,
                          d_log_decay);
     });
   });

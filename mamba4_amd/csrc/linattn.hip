@@ -12,18 +12,20 @@
 //        (R <- e^{P_L} R + scale (Q e^{P_i})^T dO, weights e^{P_i - P_j}, i >= j),
 //   dg_t = <S_T, R_T> + sum over i >= t of (q_i . dq_i - k_i . dk_i),
 // which sums (q_i . k_j)(do_i . v_j) scale e^{P_i - P_j} over pairs i >= t > j
-// (the pairs i = j are in both products and left out of both).
+// (the pairs i = j are in both products and left out of both).  The sums start
+// anew at each segment's end with <S, R> there, so that they do not cancel over
+// the whole sequence.
 // So one body serves all of them ("roles"); a block walks the chunks of one
 // (b, h) for 64 columns of the values, keeping the state in registers.
 //
 // Products run on bfloat16 MFMA with float32 accumulation.  An operand is a sum of
-// bfloat16 planes: a bfloat16 input is one plane; what is computed
-// in float32 (A, S, the weighted K) is two planes beside bfloat16 inputs
-// (2^-17 of the value left out: below the rounding of a bfloat16 result and near
-// float32 for the states and dg; one plane for A and S saved a tenth of the time and
-// left an error like that rounding's own); float32 inputs and what is computed
-// from them are three planes (all 24 bits) with the six largest plane products:
-// a sixth of the bfloat16 rate, 2.7 times that of float32 MFMA.
+// bfloat16 planes: a bfloat16 input is one plane; what is computed in float32 is
+// three planes (all 24 bits) where the result is float32 (the weighted K of the
+// states, A and S where dg follows from the output), and two beside bfloat16
+// inputs where it is rounded to bfloat16 (2^-17 of A and S left out; one plane saved
+// a tenth of the time and left an error like that rounding's own).  Float32 inputs
+// are three planes, with the six largest plane products: a sixth of the bfloat16
+// rate, 2.7 times that of float32 MFMA.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -51,12 +53,13 @@ template <typename In>
 struct Type;
 template <>
 struct Type<bf16_t> {
-  static constexpr int IN = 1, MADE = 2;  // planes of an input, of a computed operand
+  static constexpr int IN = 1, ROUGH = 2;  // planes of an input, of an operand of rounded results
 };
 template <>
 struct Type<float> {
-  static constexpr int IN = 3, MADE = 3;
+  static constexpr int IN = 3, ROUGH = 3;
 };
+constexpr int FINE = 3;  // planes of a computed operand of a float32 result
 
 // Eight consecutive elements as loaded.
 template <typename In>
@@ -240,16 +243,16 @@ __device__ __forceinline__ Quad<float> load_quad(Rsrc r, unsigned row, int col, 
 // rows padded by 16 bytes instead, both took twice the cycles).
 __device__ __forceinline__ int unit(int row, int u) { return 64 * row + 8 * (u ^ (row & 7)); }
 
-// OUT: outputs are formed (else only states).
-template <typename In, int NT, bool OUT>
+// SP planes of the state (0: only states are formed).
+template <typename In, int NT, int SP>
 struct Shared {
   alignas(16) bf16_t k[Type<In>::IN][NT][C * 64];                 // K [token][n]
   alignas(16) bf16_t v[Type<In>::IN][1][C * TILE];                // V [token][column]
-  alignas(16) bf16_t s[Type<In>::MADE][NT][OUT ? TILE * 64 : 8];  // S^T [column][n]
+  alignas(16) bf16_t s[SP ? SP : 1][NT][SP ? TILE * 64 : 8];      // S^T [column][n]
   // Each wave's own, of the chunk's tokens: the running log2 decay in two
   // parts and the decays between a token and the wave's strip (outputs), and the
   // weights of the tokens in the next state (states).
-  alignas(16) float ph[OUT ? WAVES : 1][C], pl[OUT ? WAVES : 1][C], far[OUT ? WAVES : 1][C];
+  alignas(16) float ph[SP ? WAVES : 1][C], pl[SP ? WAVES : 1][C], far[SP ? WAVES : 1][C];
   alignas(16) float update[WAVES][C];
 };
 
@@ -437,7 +440,7 @@ __device__ __forceinline__ Rsrc chunk_rows(const Source& x, int c, int rows) {
 // blocks take one segment each, has the bits of a walk over all of them.
 template <typename In, int NT, bool WHOLE, bool REV>
 struct Block {
-  static constexpr int IN = Type<In>::IN, MADE = Type<In>::MADE;
+  static constexpr int IN = Type<In>::IN;
   static constexpr int KP = 2 * NT;               // pieces of K a thread loads
   static constexpr int GROUP = IN > 1 ? 2 : 4;    // products between which no wait is needed
   const Args& a;
@@ -527,10 +530,10 @@ struct Block {
       const f4 ua = *reinterpret_cast<const f4*>(&sh.update[w][16 * ja + 4 * g]);
       const f4 ub = *reinterpret_cast<const f4*>(&sh.update[w][16 * jb + 4 * g]);
       const float wt[8] = {ua[0], ua[1], ua[2], ua[3], ub[0], ub[1], ub[2], ub[3]};
-      Frag<MADE> kw[NT];
+      Frag<FINE> kw[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        kw[nt] = weighted<MADE>(columns<IN, NT>(sh.k, nt, ja, jb, w, g, r), wt);
+        kw[nt] = weighted<FINE>(columns<IN, NT>(sh.k, nt, ja, jb, w, g, r), wt);
 #pragma unroll
       for (int p0 = 0; p0 < 4; p0 += GROUP) {
         Frag<IN> vf[GROUP];
@@ -548,7 +551,7 @@ struct Block {
   }
 
   // Split runs: the segment's own state, from zero, and its decay.  Four waves.
-  __device__ __forceinline__ void states(int seg, int c0, int c1, Shared<In, NT, false>& sh) {
+  __device__ __forceinline__ void states(int seg, int c0, int c1, Shared<In, NT, 0>& sh) {
     f4 own[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -594,15 +597,16 @@ struct Block {
   // Outputs from the state at the first chunk.  Eight waves: four form the
   // outputs of a strip of 16 tokens each, four keep the state (16 rows of its n
   // and of every 64 each), so that a chunk's two halves run beside each other.
-  template <bool DOTS>
-  __device__ __forceinline__ void outputs(int seg, int c0, int c1, Shared<In, NT, true>& sh) {
+  template <int SP, bool DOTS>
+  __device__ __forceinline__ void outputs(int seg, int c0, int c1, Shared<In, NT, SP>& sh) {
     if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < WAVES)
-      write_outputs<DOTS>(c0, c1, sh);
+      write_outputs<SP, DOTS>(c0, c1, sh);
     else
-      keep_state(seg, c0, c1, sh);
+      keep_state<SP, DOTS>(seg, c0, c1, sh);
   }
 
-  __device__ __forceinline__ void keep_state(int seg, int c0, int c1, Shared<In, NT, true>& sh) {
+  template <int SP, bool DOTS>
+  __device__ __forceinline__ void keep_state(int seg, int c0, int c1, Shared<In, NT, SP>& sh) {
     f4 start[NT][4], own[NT][4];
     float since = 1.f;  // decay since the segment's start
     {
@@ -649,11 +653,11 @@ struct Block {
             float s[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) s[q] = fmaf(since, start[nt][pb][q], own[nt][pb][q]);
-            unsigned lo[MADE], hi[MADE];
-            split2<MADE>(s[0], s[1], lo);
-            split2<MADE>(s[2], s[3], hi);
+            unsigned lo[SP], hi[SP];
+            split2<SP>(s[0], s[1], lo);
+            split2<SP>(s[2], s[3], hi);
 #pragma unroll
-            for (int j = 0; j < MADE; ++j)
+            for (int j = 0; j < SP; ++j)
               *reinterpret_cast<u2*>(
                   &sh.s[j][nt][64 * 16 * pb + unit(r, 2 * w + (g >> 1)) + 4 * (g & 1)]) =
                   u2{lo[j], hi[j]};
@@ -679,6 +683,16 @@ struct Block {
             own[nt][pb] = f4{0.f, 0.f, 0.f, 0.f};
           }
         since = 1.f;
+        // What the carries of a split run leave: the next segment's start state.
+        const int next = c / a.seg + (REV ? -1 : 1);
+        if (DOTS && seg < 0 && next >= 0 && next < a.NS) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pb = 0; pb < 4; ++pb)
+              *reinterpret_cast<f4*>(slot(next) + ((nt * 4 + pb) * 64 * WAVES + t) * 4) =
+                  start[nt][pb];
+        }
       }
     }
     if (R.final.base && (REV ? c0 == 0 : c1 == a.NC)) {
@@ -697,8 +711,8 @@ struct Block {
     }
   }
 
-  template <bool DOTS>
-  __device__ __forceinline__ void write_outputs(int c0, int c1, Shared<In, NT, true>& sh) {
+  template <int SP, bool DOTS>
+  __device__ __forceinline__ void write_outputs(int c0, int c1, Shared<In, NT, SP>& sh) {
     const Source vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h);
     Piece<In> vraw[2], qraw[2 * NT];
     float graw;
@@ -746,10 +760,10 @@ struct Block {
         for (int kk = 0; kk < 2 * NT; ++kk)
 #pragma unroll
           for (int p0 = 0; p0 < 4; p0 += GROUP) {
-            Frag<MADE> sf[GROUP];
+            Frag<SP> sf[GROUP];
 #pragma unroll
             for (int pb = 0; pb < GROUP; ++pb)
-              sf[pb] = rows<MADE, NT>(sh.s, 16 * (p0 + pb), kk, g, r);
+              sf[pb] = rows<SP, NT>(sh.s, 16 * (p0 + pb), kk, g, r);
             mma(sf, qf[kk], &out[p0]);
           }
         const float inter = R.inter * __shfl(d.inter, 16 * w + r);
@@ -790,7 +804,7 @@ struct Block {
           for (int q = 0; q < 4; ++q) acc[1][q] = 2 * s + 1 < reached ? acc[1][q] * far[q] : 0.f;
           const float x[8] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3],
                               acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
-          const Frag<MADE> score = split8<MADE>(x);
+          const Frag<SP> score = split8<SP>(x);
 #pragma unroll
           for (int p0 = 0; p0 < 4; p0 += GROUP) {
             Frag<IN> vf[GROUP];
@@ -883,11 +897,13 @@ constexpr int waves_per_simd(int bytes, int nt) { return bytes == 4 && nt == 2 ?
 
 template <typename In, int NT, bool WHOLE>
 __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void attention_kernel(Args a) {
-  __shared__ Shared<In, NT, true> sh;
+  constexpr int SP = Type<In>::ROUGH;
+  __shared__ Shared<In, NT, SP> sh;
   int which, b, h, c0, c1;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   const int seg = chunks_of(a, &c0, &c1);
-  Block<In, NT, WHOLE, false>(a, a.role[0], which, b, h).template outputs<false>(seg, c0, c1, sh);
+  Block<In, NT, WHOLE, false>(a, a.role[0], which, b, h).template outputs<SP, false>(seg, c0, c1,
+                                                                                     sh);
 }
 
 // The gradients: dQ forward in time, dK and dV in reverse; NP and NN 64s of the
@@ -895,28 +911,29 @@ __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void a
 template <typename In, int NP, int NN, bool DOTS, bool WHOLE>
 __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NP > NN ? NP : NN)) void
 attention_backward_kernel(Args a) {
+  constexpr int SP = DOTS ? FINE : Type<In>::ROUGH, SV = Type<In>::ROUGH;
   __shared__ union {
-    Shared<In, NP, true> p;
-    Shared<In, NN, true> n;
+    Shared<In, NP, SP> p;
+    Shared<In, NN, SV> n;
   } sh;
   int which, b, h, c0, c1;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   const int seg = chunks_of(a, &c0, &c1);
   if (which < a.role[0].tiles)
     return Block<In, NP, WHOLE, false>(a, a.role[0], which, b, h)
-        .template outputs<DOTS>(seg, c0, c1, sh.p);
+        .template outputs<SP, DOTS>(seg, c0, c1, sh.p);
   which -= a.role[0].tiles;
   if (which < a.role[1].tiles)
     return Block<In, NP, WHOLE, true>(a, a.role[1], which, b, h)
-        .template outputs<DOTS>(seg, c0, c1, sh.p);
+        .template outputs<SP, DOTS>(seg, c0, c1, sh.p);
   Block<In, NN, WHOLE, true>(a, a.role[2], which - a.role[1].tiles, b, h)
-      .template outputs<false>(seg, c0, c1, sh.n);
+      .template outputs<SV, false>(seg, c0, c1, sh.n);
 }
 
 // Split runs: the segments' own states, of all roles.
 template <typename In, int NT, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
-  __shared__ Shared<In, NT, false> sh;
+  __shared__ Shared<In, NT, 0> sh;
   int which, b, h, i = 0, c0, c1;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   while (which >= a.role[i].tiles) which -= a.role[i++].tiles;
@@ -924,7 +941,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   const int seg = chunks_of(a, &c0, &c1);
   if constexpr (NT == 2) {
     if (R.n <= 64) {
-      Shared<In, 1, false>& narrow = reinterpret_cast<Shared<In, 1, false>&>(sh);
+      Shared<In, 1, 0>& narrow = reinterpret_cast<Shared<In, 1, 0>&>(sh);
       if (R.rev) return Block<In, 1, WHOLE, true>(a, R, which, b, h).states(seg, c0, c1, narrow);
       return Block<In, 1, WHOLE, false>(a, R, which, b, h).states(seg, c0, c1, narrow);
     }
@@ -977,52 +994,62 @@ __global__ void carry_kernel(Args a) {
   }
 }
 
-// d log_decay: one block per (b, h), from the last token to the first, sums
-// in float64.
-__global__ __launch_bounds__(1024) void decay_grad_kernel(DecayGrad a) {
-  __shared__ double part[16], total[16];
+// d log_decay: one block per (b, h) and segment, from its last token to its
+// first, sums in float64.  At the segment's end they start with <S, R>, from the states
+// that the roles of dQ and dK have there (both [value][key]), at the sequence's end
+// with that of the final state and its cotangent.
+__global__ __launch_bounds__(GRAD_THREADS) void decay_grad_kernel(DecayGrad a) {
+  constexpr int W = GRAD_THREADS / 64;
+  __shared__ double part[W];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, seg = blockIdx.y;
   const int length = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-  const long bh = blockIdx.x, slab = (long)a.B * a.H * a.T;
-  auto block_sum = [&](double x, double* at) {
+  const long bh = blockIdx.x, rows = (long)a.B * a.H, slab = rows * a.T;
+  auto block_sum = [&](double x) {
     x = lane_double(wave_prefix(x), 63);
-    if (lane == 0) at[w] = x;
+    __syncthreads();
+    if (lane == 0) part[w] = x;
     __syncthreads();
     double s = 0.0;
-    for (int i = 0; i < 16; ++i) s += at[i];
-    __syncthreads();
+    for (int i = 0; i < W; ++i) s += part[i];
     return s;
   };
-  double carry = 0.0;
-  if (a.state) {
+  double x = 0.0;
+  if (seg + 1 < a.NS) {
+    for (int tile = 0; tile < a.tiles; ++tile) {
+      const long row = (tile * rows + bh) * a.NS;
+      const f4* s = reinterpret_cast<const f4*>(a.starts_q + (row + seg + 1) * a.slot);
+      const f4* r = reinterpret_cast<const f4*>(a.starts_k + (row + seg) * a.slot);
+      for (int i = tid; i < a.slot / 4; i += GRAD_THREADS)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x += (double)s[i][q] * (double)r[i][q];
+    }
+  } else if (a.state) {
     const long count = (long)a.n * a.p;
-    double x = 0.0;
-    for (long i = tid; i < count; i += 1024)
+    for (long i = tid; i < count; i += GRAD_THREADS)
       x += (double)a.state[bh * count + i] * (double)a.d_state[bh * count + i];
-    carry = block_sum(x, total);
   }
-  double sum = 0.0;
-  for (int end = a.T; end > 0; end -= 1024) {
+  double carry = block_sum(x), sum = 0.0;
+  const int first = seg * a.seg * C;
+  for (int end = min(a.T, first + a.seg * C); end > first; end -= GRAD_THREADS) {
     // Thread i takes token end - 1 - i: a suffix sum is a prefix sum here.
     const int t = end - 1 - tid;
-    double x = 0.0;
-    if (t >= 0 && t < length) {
-      for (int i = 0; i < a.tiles_q; ++i) x += (double)a.dots_q[i * slab + bh * a.T + t];
-      for (int i = 0; i < a.tiles_k; ++i) x -= (double)a.dots_k[i * slab + bh * a.T + t];
+    x = 0.0;
+    if (t >= first && t < length) {
+      for (int i = 0; i < a.tiles; ++i)
+        x += (double)a.dots_q[i * slab + bh * a.T + t] - (double)a.dots_k[i * slab + bh * a.T + t];
     }
     x = wave_prefix(x);
     const double all = lane_double(x, 63);
+    __syncthreads();
     if (lane == 0) part[w] = all;
     __syncthreads();
-    double before = carry;
-    for (int i = 0; i < 16; ++i) {
-      if (i < w) before += part[i];
+    x += carry;
+    for (int i = 0; i < W; ++i) {
+      if (i < w) x += part[i];
       carry += part[i];
     }
-    __syncthreads();
-    x += before;
-    if (t >= 0) {
+    if (t >= first) {
       // No gradient past the length, nor where the decay is exactly zero.
       const float g = t < length ? a.g[b * a.gb + t * a.gt + h] : 0.f;
       if (t >= length || g < -2000.f) x = 0.0;
@@ -1031,17 +1058,20 @@ __global__ __launch_bounds__(1024) void decay_grad_kernel(DecayGrad a) {
     }
   }
   if (a.head) {
-    sum = block_sum(sum, total);
-    if (tid == 0) a.head[bh] = sum;
+    sum = block_sum(sum);
+    if (tid == 0) a.head[bh * a.NS + seg] = sum;
   }
 }
 
-__global__ void decay_heads_kernel(const double* head, int B, int H, float* d_g) {
-  const int h = blockIdx.x * blockDim.x + threadIdx.x;
-  if (h >= H) return;
+// One block per head: the sums of its segments over the rows.
+__global__ __launch_bounds__(64) void decay_heads_kernel(const double* head, int B, int H, int NS,
+                                                         float* d_g) {
+  const int h = blockIdx.x;
   double s = 0.0;
-  for (int b = 0; b < B; ++b) s += head[(long)b * H + h];
-  d_g[h] = (float)s;
+  for (long i = threadIdx.x; i < (long)B * NS; i += 64)
+    s += head[(i / NS * H + h) * NS + i % NS];
+  s = lane_double(wave_prefix(s), 63);
+  if (threadIdx.x == 0) d_g[h] = (float)s;
 }
 
 // Gradients of shared heads: out[b,t,j,:] = sum over the heads h of group j

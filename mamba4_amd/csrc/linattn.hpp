@@ -11,6 +11,7 @@ constexpr int MAX_SEG = 16;  // most chunks of a segment
 constexpr int TILE = 64;     // value columns of a block
 constexpr int WAVES = 4;     // strips of 16 tokens in a chunk, each a wave's
 constexpr int MAX_WIDTH = 128;
+constexpr int GRAD_THREADS = 256;  // block of the decays' gradient
 constexpr int STEP_THREADS = 256;  // block of the step's kernel
 
 typedef unsigned short bf16_t;
@@ -45,7 +46,8 @@ struct Role {
                        // tile's columns, if dots
   float* dots;         // [tiles][B,H,T], or NULL
   int n, p, tiles;
-  float* starts;       // split runs: [tiles][B*H][NS][NT * 4096] segment states
+  float* starts;       // [tiles][B*H][NS][NT * 4096] segments' start states (split runs,
+                       // and with dots)
   float* decays;       // split runs: [tiles][B*H][NS]
 };
 
@@ -59,17 +61,19 @@ struct Args {
   int seg, split;          // chunks of a segment; split: a segment a block
 };
 
-// d log_decay from the roles' dots.
+// d log_decay from the dots and the segments' start states of the roles of dQ
+// and dK.
 struct DecayGrad {
-  const float *dots_q, *dots_k;  // [tiles_q / tiles_k][B,H,T]
-  int tiles_q, tiles_k;
-  const float *g;
+  const float *dots_q, *dots_k;      // [tiles][B,H,T]
+  const float *starts_q, *starts_k;  // [tiles][B*H][NS][slot]
+  int tiles, slot, seg, NS;
+  const float* g;
   long gb, gt;
   const int* lengths;
-  const float *state, *d_state;  // [B,H,n,p], or both NULL
+  const float *state, *d_state;      // [B,H,n,p], or both NULL
   int n, p;
-  float* d_g;                    // [B,T,H], or NULL
-  double* head;                  // [B,H] sums over the tokens, or NULL
+  float* d_g;                        // [B,T,H], or NULL
+  double* head;                      // [B,H,NS] sums over the tokens, or NULL
   int B, T, H;
 };
 
