@@ -2,6 +2,7 @@
 // checks of the arguments and the launches.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <initializer_list>
@@ -121,12 +122,12 @@ bool bad_shape(const Shape& s, std::string* why) {
 
 // Whether the sequences are split into segments (their states formed first,
 // then carried, then all walked at once) instead of walked from end to end.  A walk
-// takes a step's latency a chunk, and more once the card has more than a block a
-// compute unit; a split run three launches, a segment's latency twice, and about
-// 1.6 times the steps' throughput.  Forward, walk / split: bfloat16 N64 P128 H12 B4
-// T2000 68 / 46 us, B8 T1024 37 / 46, B16 T1024 53 / 78; float32 B4 T1024 69 / 51, B8
-// T1024 72 / 81.  M4RT_ATTENTION = "walk" or "split" overrides the choice; the bits are
-// the same.
+// takes a chunk's latency a chunk while the card has a block a compute unit, and the
+// chunks' throughput beyond; a split run three launches, a segment's latency twice,
+// and 1.7 times the throughput.  Walk / split in us: forward bfloat16 N64 P128
+// H12 B4 T2000 68 / 46, B8 T1024 37 / 46, B16 T1024 53 / 78; float32 B4 T1024 69 / 51,
+// B8 T1024 72 / 81; backward float32 N64 P64 H8 B8 T1000 104 / 79.  M4RT_ATTENTION =
+// "walk" or "split" overrides the choice; the bits are the same.
 bool attention_splits(const Shape& s, int blocks) {
   if (segments(s, blocks) < 2) return false;
   if (const char* mode = std::getenv("M4RT_ATTENTION")) {
@@ -134,12 +135,14 @@ bool attention_splits(const Shape& s, int blocks) {
     if (std::strcmp(mode, "split") == 0) return true;
   }
   const bool backward = blocks > tiles_of(s.P), wide = s.N > 64 || (backward && s.P > 64);
-  const double step = (s.bf16 ? 2.1 : 4.1) * (wide ? 1.5 : 1.0) *
-                      (backward ? (s.bf16 ? 1.2 : 1.6) : 1.0);  // us a chunk
+  // us a chunk: alone, and of a busy compute unit.
+  const double more = wide ? 1.5 : 1.0;
+  const double latency = more * (s.bf16 ? 2.1 : 4.1) * (backward ? (s.bf16 ? 1.2 : 1.6) : 1.0);
+  const double busy = more * (s.bf16 ? 1.9 : 3.9) * (backward ? (s.bf16 ? 1.25 : 1.1) : 1.0);
   const double units = m4::api_compute_units(), walks = (double)s.B * s.H * blocks;
-  const double walk = s.chunks() * step * std::max(1.0, 0.95 * walks / units);
-  const double split =
-      8.0 + 1.6 * step * std::max<double>(segment(s, blocks), s.chunks() * walks / (1.05 * units));
+  const double walk = s.chunks() * std::max(latency, busy * std::ceil(walks / units));
+  const double split = 8.0 + std::max(1.6 * segment(s, blocks) * latency,
+                                      1.7 * busy * s.chunks() * walks / units);
   return split < walk;
 }
 
