@@ -207,8 +207,11 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
         if tuple(lengths.shape) != (batch,) or lengths.dtype.is_floating_point \
                 or lengths.dtype in (torch.bool, torch.complex64, torch.complex128):
             raise ValueError("linear_attention needs integer lengths [B]")
-        # Clamped before the narrowing, so that no length wraps around.
-        lengths = lengths.clamp(0, time).to(torch.int32).contiguous()
+        # (The kernels clamp; wider integers before they are narrowed, so that none
+        # wraps around.)
+        if lengths.dtype != torch.int32:
+            lengths = lengths.clamp(0, time).to(torch.int32)
+        lengths = lengths.contiguous()
     if batch == 0 or time == 0:
         output = values.new_zeros((batch, time, heads, p))
         state = output.new_zeros((batch, heads, n, p), dtype=torch.float32)

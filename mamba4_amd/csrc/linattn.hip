@@ -458,6 +458,13 @@ struct Block {
     gs = a.g + b * a.gb + h;
   }
   __device__ __forceinline__ int have(int c) const { return min(length - c * C, C); }
+  // Whether the decays' tables have to be formed for chunk c: a constant decay's are
+  // those of any chunk with as many tokens.
+  __device__ __forceinline__ bool unknown(int c, int* known) const {
+    const bool fresh = a.gt != 0 || have(c) != *known;
+    *known = have(c);
+    return fresh;
+  }
   __device__ __forceinline__ float decay(int c, int lane) const {
     return lane < have(c) ? gs[((long)c * C + lane) * a.gt] : 0.f;
   }
@@ -568,14 +575,15 @@ struct Block {
       graw = decay(c, t & 63);
     };
     fetch(REV ? c1 - 1 : c0);
+    float whole = 1.f;
+    int known = -1;
     for (int it = 0; it < c1 - c0; ++it) {
       const int c = REV ? c1 - 1 - it : c0 + it;
       const int t = thread(), lane = t & 63;
-      float whole = 1.f;
       if (have(c) > 0) {
         stage_k(sh, kraw, t);
         stage_v(sh, vraw, t);
-        whole = weigh<REV>(sh.update[w], graw, lane, R.update);
+        if (unknown(c, &known)) whole = weigh<REV>(sh.update[w], graw, lane, R.update);
       }
       __syncthreads();
       if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
@@ -640,10 +648,11 @@ struct Block {
       graw = decay(c, t & 63);
     };
     fetch(REV ? c1 - 1 : c0);
+    float whole = 1.f;
+    int known = -1;
     for (int it = 0; it < c1 - c0; ++it) {
       const int c = REV ? c1 - 1 - it : c0 + it;
       const int t = thread() & (64 * WAVES - 1), lane = t & 63, g = lane >> 4, r = lane & 15;
-      float whole = 1.f;
       if (have(c) > 0) {
         stage_k(sh, kraw, t);
 #pragma unroll
@@ -662,7 +671,7 @@ struct Block {
                   &sh.s[j][nt][64 * 16 * pb + unit(r, 2 * w + (g >> 1)) + 4 * (g & 1)]) =
                   u2{lo[j], hi[j]};
           }
-        whole = weigh<REV>(sh.update[w], graw, lane, R.update);
+        if (unknown(c, &known)) whole = weigh<REV>(sh.update[w], graw, lane, R.update);
       }
       __syncthreads();
       if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
@@ -727,17 +736,18 @@ struct Block {
       graw = decay(c, lane);
     };
     fetch(REV ? c1 - 1 : c0);
+    Reach d{};
+    int known = -1;
     for (int it = 0; it < c1 - c0; ++it) {
       const int c = REV ? c1 - 1 - it : c0 + it, t0 = c * C;
       const int tid = thread(), lane = tid & 63, g = lane >> 4, r = lane & 15;
       Frag<IN> qf[2 * NT];
-      Reach d{};
       Quad<In> e[4];
       if (have(c) > 0) {
         stage_v(sh, vraw, tid);
 #pragma unroll
         for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
-        d = reach<REV>(sh.ph[w], sh.pl[w], sh.far[w], graw, lane, w);
+        if (unknown(c, &known)) d = reach<REV>(sh.ph[w], sh.pl[w], sh.far[w], graw, lane, w);
         if constexpr (DOTS) {
           // Before the next chunk's loads, so that their wait does not include those.
           const Source es = source<In>(R.e, b, h);
