@@ -40,8 +40,11 @@ HAZARD_CHECKED = ["factor.hip"]
 
 # Per-source extra flags.  The factorization accumulates its trailing blocks
 # in place with MFMA; keeping MFMA operands and results in VGPRs avoids a
-# second copy of those blocks in AGPRs (which would halve the occupancy).
-SOURCE_FLAGS = {"factor.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# second copy of those blocks in AGPRs (which would halve the occupancy).  The
+# linear attention's state kernels lose their copies between the two (85 -> 77 us
+# at T32768 H16 N128 P128).
+SOURCE_FLAGS = {"factor.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "linattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 _NOISE = "is not a recognized feature for this target"
 

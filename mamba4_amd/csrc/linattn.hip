@@ -949,6 +949,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   while (which >= a.role[i].tiles) which -= a.role[i++].tiles;
   const Role& R = a.role[i];
   const int seg = chunks_of(a, &c0, &c1);
+  if (seg == (R.rev ? 0 : a.NS - 1)) return;  // no segment starts from its end
   if constexpr (NT == 2) {
     if (R.n <= 64) {
       Shared<In, 1, 0>& narrow = reinterpret_cast<Shared<In, 1, 0>&>(sh);
@@ -961,7 +962,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
 }
 
 // Split runs: each segment's start state from the segments' own states and
-// decays, in place.  One thread per state element.
+// decays, in place (the last one's own was not formed, and is read for nothing).  Four
+// state elements a thread.
 __global__ void carry_kernel(Args a) {
   int which, b, h, i = 0;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
