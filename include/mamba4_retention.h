@@ -62,7 +62,7 @@ typedef struct {
  * underflows) drops what came before exactly.  An infinity or NaN in a row
  * that is present spreads to the outputs of its chunk of 64 tokens and after it.
  */
-size_t m4rt_attention_workspace_bytes(int B, int T, int H, int N, int P, int bf16);
+size_t m4rt_attention_workspace_bytes(const m4rt_qkv* rows, int bf16, int B, int T, int H);
 int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
                            const int* lengths, const float* initial, float scale, int B, int T,
                            int H, void* output, float* state, void* workspace,
@@ -77,12 +77,12 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
  * Gradients of shared heads are summed in float32 and rounded once.  `decays` of
  * the workspace's size: whether d_log_decay is wanted.
  */
-size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads, int k_heads,
-                                               int v_heads, int N, int P, int bf16, int decays);
+size_t m4rt_attention_backward_workspace_bytes(const m4rt_qkv* rows, const void* d_output,
+                                               int bf16, int B, int T, int H, int decays);
 int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_decay,
                             int per_token, const int* lengths, const float* initial, float scale,
-                            int B, int T, int H, const void* d_output, const float* d_state, const float* state,
-                            void* d_q, void* d_k, void* d_v, float* d_log_decay,
+                            int B, int T, int H, const void* d_output, const float* d_state,
+                            const float* state, void* d_q, void* d_k, void* d_v, float* d_log_decay,
                             float* d_initial, void* workspace, size_t workspace_bytes,
                             void* stream);
 

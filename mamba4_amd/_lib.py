@@ -130,10 +130,10 @@ SIGNATURES = {
     "m3s_backward": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P] * 9 + [_P, _S, _P]),
     "m3s_forward_bf16": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P]),
     "m3s_backward_bf16": (_I, [_P] * 9 + [_I] * 6 + [_P] * 4 + [_P] * 9 + [_P, _S, _P]),
-    "m4rt_attention_workspace_bytes": (_S, [_I] * 6),
+    "m4rt_attention_workspace_bytes": (_S, [_P] + [_I] * 4),
     "m4rt_attention_forward": (
         _I, [_P, _I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 3 + [_S, _P]),
-    "m4rt_attention_backward_workspace_bytes": (_S, [_I] * 10),
+    "m4rt_attention_backward_workspace_bytes": (_S, [_P] * 2 + [_I] * 5),
     "m4rt_attention_backward": (
         _I, [_P, _I, _P, _I, _P, _P, _F] + [_I] * 3 + [_P] * 9 + [_S, _P]),
     "m4rt_attention_step": (

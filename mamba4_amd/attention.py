@@ -105,10 +105,11 @@ def _forward(q, k, v, log_decay, initial, lengths, scale):
     bf16 = 1 if v.dtype == _BF16 else 0
     output = torch.empty((batch, time, heads, p), dtype=v.dtype, device=device)
     state = torch.empty((batch, heads, n, p), dtype=_F32, device=device)
-    nbytes = lib.m4rt_attention_workspace_bytes(batch, time, heads, n, p, bf16)
+    rows = _qkv(q, k, v)
+    nbytes = lib.m4rt_attention_workspace_bytes(rows, bf16, batch, time, heads)
     workspace = _workspace(nbytes, device)
     rc = lib.m4rt_attention_forward(
-        _qkv(q, k, v), bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
+        rows, bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
         _ptr(initial), scale, batch, time, heads, output.data_ptr(), state.data_ptr(),
         _ptr(workspace), nbytes, _stream(device),
     )
@@ -144,12 +145,12 @@ class _Attention(torch.autograd.Function):
         d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
         d_decay = torch.empty_like(log_decay) if ctx.needs_input_grad[3] else None
         d_initial = torch.empty_like(state) if ctx.needs_input_grad[4] else None
+        rows = _qkv(q, k, v)
         nbytes = lib.m4rt_attention_backward_workspace_bytes(
-            batch, time, heads, q.shape[2], k.shape[2], v.shape[2], n, p, bf16,
-            d_decay is not None)
+            rows, d_output.data_ptr(), bf16, batch, time, heads, d_decay is not None)
         workspace = _workspace(nbytes, device)
         rc = lib.m4rt_attention_backward(
-            _qkv(q, k, v), bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
+            rows, bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
             _ptr(initial), ctx.scale, batch, time, heads, d_output.data_ptr(), _ptr(d_state),
             state.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), _ptr(d_decay),
             _ptr(d_initial), _ptr(workspace), nbytes, _stream(device),

@@ -14,17 +14,19 @@
 #include "norm.hpp"
 
 namespace la {
-template <typename In, int NT, bool WHOLE>
+template <typename In, int NT>
 __global__ void attention_kernel(Args);
-template <typename In, int NT, bool WHOLE>
+template <typename In, int NT>
 __global__ void attention_states_kernel(Args);
-template <typename In, int NP, int NN, bool DOTS, bool WHOLE>
+template <typename In, int NP, int NN, bool DOTS>
 __global__ void attention_backward_kernel(Args);
 __global__ void carry_kernel(Args);
 __global__ void decay_grad_kernel(DecayGrad);
 __global__ void decay_heads_kernel(const double*, int, int, int, float*);
 template <typename Out>
 __global__ void share_sum_kernel(const float*, long, int, int, int, Out*);
+template <typename In>
+__global__ void pack_kernel(Pack);
 template <typename In, int V, int PASSES>
 __global__ void step_kernel(Step);
 }  // namespace la
@@ -165,6 +167,41 @@ la::Rows rows_of(const m4rt_rows& r, int H, int bf16) {
                   whole};
 }
 
+// The rows in the order given, those that are no 16-byte pieces copied to padded
+// rows: space for the copies, and their kernel.
+struct Packing {
+  la::Pack a{};
+  int count = 0;
+  long most = 0;  // pieces of the largest copy
+};
+
+void pack_rows(Carver& c, const Shape& s, la::Rows* r, int heads, Packing* out) {
+  if (r->whole) return;
+  const int piece = s.bf16 ? 8 : 4, i = out->count++;
+  const int width = (r->width + piece - 1) / piece * piece;
+  const size_t rows = (size_t)s.B * s.T * heads;
+  out->a.from[i] = *r;
+  out->a.to[i] = c.take<char>(rows * width * (16 / piece));
+  out->a.heads[i] = heads;
+  out->a.padded[i] = width;
+  out->most = std::max(out->most, (long)(rows * (width / piece)));
+  *r = la::Rows{out->a.to[i], (long)s.T * heads * width, (long)heads * width, width,
+                r->share, width, 1};
+}
+
+int run_packing(Packing& p, const Shape& s, hipStream_t st) {
+  if (p.count == 0) return M4MR_OK;
+  p.a.B = s.B;
+  p.a.T = s.T;
+  const dim3 grid((unsigned)((p.most + 255) / 256), p.count), block(256);
+  return api_launch("attention_pack", st, [&] {
+    if (s.bf16)
+      hipLaunchKernelGGL(la::pack_kernel<la::bf16_t>, grid, block, 0, st, p.a);
+    else
+      hipLaunchKernelGGL(la::pack_kernel<float>, grid, block, 0, st, p.a);
+  });
+}
+
 bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why) {
   if (!r->data) {
     *why = "a required pointer is NULL";
@@ -195,51 +232,51 @@ int wide_keys(const la::Args& a) {
   return 1;
 }
 
-template <typename In, bool WHOLE>
+template <typename In>
 void start_states(const la::Args& a, dim3 grid, hipStream_t st) {
   const dim3 block(64 * la::WAVES);
   if (wide_keys(a) == 1)
-    hipLaunchKernelGGL((la::attention_states_kernel<In, 1, WHOLE>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((la::attention_states_kernel<In, 1>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((la::attention_states_kernel<In, 2, WHOLE>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((la::attention_states_kernel<In, 2>), grid, block, 0, st, a);
 }
 
-template <typename In, int NP, int NN, bool WHOLE>
+template <typename In, int NP, int NN>
 void start_backward(const la::Args& a, dim3 grid, hipStream_t st) {
   const dim3 block(128 * la::WAVES);
   if (a.role[0].dots)
-    hipLaunchKernelGGL((la::attention_backward_kernel<In, NP, NN, true, WHOLE>), grid, block, 0,
+    hipLaunchKernelGGL((la::attention_backward_kernel<In, NP, NN, true>), grid, block, 0,
                        st, a);
   else
-    hipLaunchKernelGGL((la::attention_backward_kernel<In, NP, NN, false, WHOLE>), grid, block, 0,
+    hipLaunchKernelGGL((la::attention_backward_kernel<In, NP, NN, false>), grid, block, 0,
                        st, a);
 }
 
-template <typename In, bool WHOLE>
+template <typename In>
 void start_outputs(const la::Args& a, dim3 grid, hipStream_t st) {
   const dim3 block(128 * la::WAVES);
   if (a.roles == 1) {
     if (a.role[0].n <= 64)
-      hipLaunchKernelGGL((la::attention_kernel<In, 1, WHOLE>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((la::attention_kernel<In, 1>), grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL((la::attention_kernel<In, 2, WHOLE>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((la::attention_kernel<In, 2>), grid, block, 0, st, a);
     return;
   }
   const bool wide_p = a.role[0].n > 64, wide_n = a.role[2].n > 64;
   if (wide_p)
-    wide_n ? start_backward<In, 2, 2, WHOLE>(a, grid, st)
-           : start_backward<In, 2, 1, WHOLE>(a, grid, st);
+    wide_n ? start_backward<In, 2, 2>(a, grid, st)
+           : start_backward<In, 2, 1>(a, grid, st);
   else
-    wide_n ? start_backward<In, 1, 2, WHOLE>(a, grid, st)
-           : start_backward<In, 1, 1, WHOLE>(a, grid, st);
+    wide_n ? start_backward<In, 1, 2>(a, grid, st)
+           : start_backward<In, 1, 1>(a, grid, st);
 }
 
-template <typename In, bool WHOLE>
+template <typename In>
 int start_attention(const la::Args& a, hipStream_t st) {
   const unsigned x = (unsigned)((a.B * a.H + 7) / 8 * 8 * a.blocks);
   if (a.split) {
     int rc = api_launch("attention_states", st,
-                        [&] { start_states<In, WHOLE>(a, dim3(x, a.NS), st); });
+                        [&] { start_states<In>(a, dim3(x, a.NS), st); });
     if (rc) return rc;
     rc = api_launch("attention_carry", st, [&] {
       hipLaunchKernelGGL(la::carry_kernel, dim3(x, 4 * wide_keys(a)), dim3(64 * la::WAVES), 0, st,
@@ -248,17 +285,12 @@ int start_attention(const la::Args& a, hipStream_t st) {
     if (rc) return rc;
   }
   return api_launch("attention", st,
-                    [&] { start_outputs<In, WHOLE>(a, dim3(x, a.split ? a.NS : 1), st); });
+                    [&] { start_outputs<In>(a, dim3(x, a.split ? a.NS : 1), st); });
 }
 
 int run_attention(la::Args& a, const Shape& s, bool split, hipStream_t st) {
   a.blocks = 0;
-  bool whole = true;
-  for (int i = 0; i < a.roles; ++i) {
-    const la::Role& r = a.role[i];
-    a.blocks += r.tiles;
-    whole = whole && r.q.whole && r.k.whole && r.v.whole && (!r.dots || r.e.whole);
-  }
+  for (int i = 0; i < a.roles; ++i) a.blocks += a.role[i].tiles;
   a.B = s.B;
   a.T = s.T;
   a.H = s.H;
@@ -266,10 +298,7 @@ int run_attention(la::Args& a, const Shape& s, bool split, hipStream_t st) {
   a.seg = segment(s, a.blocks);
   a.NS = segments(s, a.blocks);
   a.split = split;
-  if (s.bf16)
-    return whole ? start_attention<la::bf16_t, true>(a, st)
-                 : start_attention<la::bf16_t, false>(a, st);
-  return whole ? start_attention<float, true>(a, st) : start_attention<float, false>(a, st);
+  return s.bf16 ? start_attention<la::bf16_t>(a, st) : start_attention<float>(a, st);
 }
 
 // The step with as many loads in flight as its rows need.
@@ -287,6 +316,12 @@ void start_step(const la::Step& a, bool whole, hipStream_t st) {
     hipLaunchKernelGGL((la::step_kernel<In, 4, 16>), grid, block, 0, st, a);
 }
 
+// The rows of a call as the kernels take them.
+struct Operands {
+  la::Rows q, k, v, d_output;
+  Packing packing;
+};
+
 struct Backward {
   la::Role role[3];
   float *part[3], *dots_q, *dots_k;
@@ -295,40 +330,90 @@ struct Backward {
 
 int backward_tiles(const Shape& s) { return 2 * tiles_of(s.N) + tiles_of(s.P); }
 
+// The forward's workspace: the segments' states of a split, packed rows.
+size_t forward_workspace(const Shape& s, const m4rt_qkv& rows, void* base, la::Role* role,
+                         Operands* x) {
+  Carver c{static_cast<char*>(base)};
+  const int tiles = tiles_of(s.P);
+  take_states(c, s, s.N, tiles, attention_splits(s, tiles) ? segments(s, tiles) : 0, role);
+  x->q = rows_of(rows.q, s.H, s.bf16);
+  x->k = rows_of(rows.k, s.H, s.bf16);
+  x->v = rows_of(rows.v, s.H, s.bf16);
+  pack_rows(c, s, &x->q, rows.q.heads, &x->packing);
+  pack_rows(c, s, &x->k, rows.k.heads, &x->packing);
+  pack_rows(c, s, &x->v, rows.v.heads, &x->packing);
+  return c.used;
+}
+
 // The backward's workspace: the segments' states (of dQ and dK for the decays'
 // gradient too), float32 gradients of shared heads before their sums, the dots, the
-// heads' sums.
-size_t backward_workspace(const Shape& s, const int heads[3], bool decays, void* base,
-                          Backward* out) {
+// heads' sums, packed rows.
+size_t backward_workspace(const Shape& s, const m4rt_qkv& rows, const void* d_output, bool decays,
+                          void* base, Backward* out, Operands* x) {
   Carver c{static_cast<char*>(base)};
   const int n[3] = {s.P, s.P, s.N}, p[3] = {s.N, s.N, s.P};
-  const size_t rows = (size_t)s.B * s.T * s.H;
+  const int heads[3] = {rows.q.heads, rows.k.heads, rows.v.heads};
+  const size_t tokens = (size_t)s.B * s.T * s.H;
   const int blocks = backward_tiles(s), count = segments(s, blocks);
   const bool split = attention_splits(s, blocks);
   for (int i = 0; i < 3; ++i) {
     take_states(c, s, n[i], tiles_of(p[i]), split || (decays && i < 2) ? count : 0,
                 &out->role[i]);
-    out->part[i] = c.take<float>(heads[i] == s.H ? 0 : rows * p[i]);
+    out->part[i] = c.take<float>(heads[i] == s.H ? 0 : tokens * p[i]);
   }
-  out->dots_q = c.take<float>(decays ? rows * tiles_of(s.N) : 0);
-  out->dots_k = c.take<float>(decays ? rows * tiles_of(s.N) : 0);
+  out->dots_q = c.take<float>(decays ? tokens * tiles_of(s.N) : 0);
+  out->dots_k = c.take<float>(decays ? tokens * tiles_of(s.N) : 0);
   out->head = c.take<double>(decays ? (size_t)s.B * s.H * count : 0);
+  x->q = rows_of(rows.q, s.H, s.bf16);
+  x->k = rows_of(rows.k, s.H, s.bf16);
+  x->v = rows_of(rows.v, s.H, s.bf16);
+  x->d_output = rows_of(dense(d_output, s.T, s.H, s.P), s.H, s.bf16);
+  pack_rows(c, s, &x->q, heads[0], &x->packing);
+  pack_rows(c, s, &x->k, heads[1], &x->packing);
+  pack_rows(c, s, &x->v, heads[2], &x->packing);
+  pack_rows(c, s, &x->d_output, s.H, &x->packing);
   return c.used;
+}
+
+// The attention's shape from its rows, if they and it are sound.
+bool bad_attention(const m4rt_qkv* rows, int bf16, int B, int T, int H, Shape* s,
+                   std::string* why) {
+  if (!rows) {
+    *why = "a required pointer is NULL";
+    return true;
+  }
+  *s = Shape{B, T, H, rows->q.width, rows->v.width, bf16};
+  if (bad_shape(*s, why)) return true;
+  for (const m4rt_rows* r : {&rows->q, &rows->k, &rows->v})
+    if (bad_rows(r, H, bf16, true, why)) return true;
+  if (rows->q.width != rows->k.width) {
+    *why = "q and k disagree in width";
+    return true;
+  }
+  return false;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t m4rt_attention_workspace_bytes(int B, int T, int H, int N, int P, int bf16) {
-  const Shape s{B, T, H, N, P, bf16};
+size_t m4rt_attention_workspace_bytes(const m4rt_qkv* rows, int bf16, int B, int T, int H) {
+  Shape s;
   std::string why;
-  if (bad_shape(s, &why)) return 0;
-  Carver c{nullptr};
   la::Role role{};
-  const int blocks = tiles_of(P);
-  take_states(c, s, N, blocks, attention_splits(s, blocks) ? segments(s, blocks) : 0, &role);
-  return c.used;
+  Operands x{};
+  if (bad_attention(rows, bf16, B, T, H, &s, &why)) return 0;
+  return forward_workspace(s, *rows, nullptr, &role, &x);
+}
+
+size_t m4rt_attention_backward_workspace_bytes(const m4rt_qkv* rows, const void* d_output,
+                                               int bf16, int B, int T, int H, int decays) {
+  Shape s;
+  std::string why;
+  Backward w{};
+  Operands x{};
+  if (bad_attention(rows, bf16, B, T, H, &s, &why)) return 0;
+  return backward_workspace(s, *rows, d_output, decays, nullptr, &w, &x);
 }
 
 int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
@@ -338,25 +423,19 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
   const char* name = "m4rt_attention_forward";
   return m4::api_entry(name, [&] {
     const std::string at = std::string(name) + ": ";
-    if (!rows) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
-    const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
-    const Shape s{B, T, H, q->width, v->width, bf16};
+    Shape s;
     std::string why;
-    if (bad_shape(s, &why) || bad_rows(q, H, bf16, true, &why) || bad_rows(k, H, bf16, true, &why) ||
-        bad_rows(v, H, bf16, true, &why))
-      return api_fail(M4MR_EINVAL, at + why);
-    if (q->width != k->width) return api_fail(M4MR_EINVAL, at + "q and k disagree in width");
+    if (bad_attention(rows, bf16, B, T, H, &s, &why)) return api_fail(M4MR_EINVAL, at + why);
     if (!log_decay || !output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     la::Args a{};
     la::Role& r = a.role[0];
-    const bool split = attention_splits(s, tiles_of(s.P));
-    Carver c{static_cast<char*>(workspace)};
-    take_states(c, s, s.N, tiles_of(s.P), split ? segments(s, tiles_of(s.P)) : 0, &r);
-    if (bad_workspace(workspace, workspace_bytes, c.used, &why))
+    Operands x{};
+    const size_t need = forward_workspace(s, *rows, workspace, &r, &x);
+    if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
-    r.q = rows_of(*q, H, bf16);
-    r.k = rows_of(*k, H, bf16);
-    r.v = rows_of(*v, H, bf16);
+    r.q = x.q;
+    r.k = x.k;
+    r.v = x.v;
     r.initial = la::States{const_cast<float*>(initial), s.P, 1};
     r.final = la::States{state, s.P, 1};
     r.out = output;
@@ -371,18 +450,10 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
     a.gb = per_token ? (long)T * H : 0;
     a.gt = per_token ? H : 0;
     a.lengths = lengths;
-    return run_attention(a, s, split, static_cast<hipStream_t>(stream));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int rc = run_packing(x.packing, s, st);
+    return rc ? rc : run_attention(a, s, attention_splits(s, r.tiles), st);
   });
-}
-
-size_t m4rt_attention_backward_workspace_bytes(int B, int T, int H, int q_heads, int k_heads,
-                                               int v_heads, int N, int P, int bf16, int decays) {
-  const Shape s{B, T, H, N, P, bf16};
-  const int heads[3] = {q_heads, k_heads, v_heads};
-  std::string why;
-  if (bad_shape(s, &why)) return 0;
-  Backward w{};
-  return backward_workspace(s, heads, decays, nullptr, &w);
 }
 
 int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_decay,
@@ -393,24 +464,21 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
   const char* name = "m4rt_attention_backward";
   return m4::api_entry(name, [&] {
     const std::string at = std::string(name) + ": ";
-    if (!rows) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
-    const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
-    const Shape s{B, T, H, q->width, v->width, bf16};
+    Shape s;
     std::string why;
-    if (bad_shape(s, &why) || bad_rows(q, H, bf16, true, &why) || bad_rows(k, H, bf16, true, &why) ||
-        bad_rows(v, H, bf16, true, &why))
-      return api_fail(M4MR_EINVAL, at + why);
-    if (q->width != k->width) return api_fail(M4MR_EINVAL, at + "q and k disagree in width");
+    if (bad_attention(rows, bf16, B, T, H, &s, &why)) return api_fail(M4MR_EINVAL, at + why);
     if (!log_decay || !d_output || !d_q || !d_k || !d_v || (d_state && d_log_decay && !state))
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
-    const int heads[3] = {q->heads, k->heads, v->heads};
+    const int heads[3] = {rows->q.heads, rows->k.heads, rows->v.heads};
     Backward w{};
-    const size_t need = backward_workspace(s, heads, d_log_decay != nullptr, workspace, &w);
+    Operands x{};
+    const size_t need =
+        backward_workspace(s, *rows, d_output, d_log_decay != nullptr, workspace, &w, &x);
     if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
-    const m4rt_rows cot = dense(d_output, T, H, s.P);
-    const la::Rows rq = rows_of(*q, H, bf16), rk = rows_of(*k, H, bf16),
-                   rv = rows_of(*v, H, bf16), ro = rows_of(cot, H, bf16);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    int rc = run_packing(x.packing, s, st);
+    if (rc) return rc;
     la::Args a{};
     void* outs[3] = {d_q, d_k, d_v};
     for (int i = 0; i < 3; ++i) {
@@ -429,24 +497,23 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
     }
     // dQ from the transposed state, dK and dV from the state's cotangent.
     la::Role &rdq = a.role[0], &rdk = a.role[1], &rdv = a.role[2];
-    rdq.q = ro, rdq.k = rv, rdq.v = rk;
-    rdk.q = rv, rdk.k = ro, rdk.v = rq;
-    rdv.q = rk, rdv.k = rq, rdv.v = ro;
+    rdq.q = x.d_output, rdq.k = x.v, rdq.v = x.k;
+    rdk.q = x.v, rdk.k = x.d_output, rdk.v = x.q;
+    rdv.q = x.k, rdv.k = x.q, rdv.v = x.d_output;
     rdq.initial = la::States{const_cast<float*>(initial), 1, s.P};
     rdk.initial = la::States{const_cast<float*>(d_state), 1, s.P};
     rdv.initial = la::States{const_cast<float*>(d_state), s.P, 1};
     rdv.final = la::States{d_initial, s.P, 1};
     if (d_log_decay) {
-      rdq.e = rq, rdq.dots = w.dots_q;
-      rdk.e = rk, rdk.dots = w.dots_k;
+      rdq.e = x.q, rdq.dots = w.dots_q;
+      rdk.e = x.k, rdk.dots = w.dots_k;
     }
     a.roles = 3;
     a.g = log_decay;
     a.gb = per_token ? (long)T * H : 0;
     a.gt = per_token ? H : 0;
     a.lengths = lengths;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    int rc = run_attention(a, s, attention_splits(s, backward_tiles(s)), st);
+    rc = run_attention(a, s, attention_splits(s, backward_tiles(s)), st);
     if (rc) return rc;
     for (int i = 0; i < 3; ++i) {
       if (heads[i] == H) continue;

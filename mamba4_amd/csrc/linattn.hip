@@ -148,44 +148,24 @@ __device__ __forceinline__ void mma(const Frag<PA>& a, const Frag<PB> (&b)[N], f
 }
 
 // Elements col..col+7 of a row of `width` at byte offset `row`, zeros past the
-// width (and past the resource).  WHOLE: in 16-byte pieces, as the rows' addresses
-// and width allow; one load each, so that nothing waits for it before its use.
-template <bool WHOLE>
+// width (and past the resource): rows are whole 16-byte pieces.
 __device__ __forceinline__ Piece<bf16_t> load_piece(Rsrc r, unsigned row, int col, int width,
                                                     const bf16_t*) {
   Piece<bf16_t> x;
   const unsigned off = row + 2 * col;
-  if constexpr (WHOLE) {
-    x.w[0] = __builtin_bit_cast(
-        u4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0));
-  } else {
-    unsigned v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      v[e] = __builtin_amdgcn_raw_buffer_load_b16(r, col + e < width ? off + 2 * e : kNoLoad, 0,
-                                                  0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x.w[0][e] = v[2 * e] | (v[2 * e + 1] << 16);
-  }
+  x.w[0] = __builtin_bit_cast(
+      u4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0));
   return x;
 }
-template <bool WHOLE>
 __device__ __forceinline__ Piece<float> load_piece(Rsrc r, unsigned row, int col, int width,
                                                    const float*) {
   Piece<float> x;
   const unsigned off = row + 4 * col;
-  if constexpr (WHOLE) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      x.w[i] = __builtin_bit_cast(
-          u4, __builtin_amdgcn_raw_buffer_load_b128(
-                  r, col + 4 * i < width ? off + 16 * i : kNoLoad, 0, 0));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x.w[e >> 2][e & 3] = __builtin_amdgcn_raw_buffer_load_b32(
-          r, col + e < width ? off + 4 * e : kNoLoad, 0, 0);
-  }
+  for (int i = 0; i < 2; ++i)
+    x.w[i] = __builtin_bit_cast(
+        u4, __builtin_amdgcn_raw_buffer_load_b128(
+                r, col + 4 * i < width ? off + 16 * i : kNoLoad, 0, 0));
   return x;
 }
 
@@ -204,37 +184,17 @@ struct Quad<float> {
   f4 u;
   __device__ __forceinline__ f4 get() const { return u; }
 };
-template <bool WHOLE>
 __device__ __forceinline__ Quad<bf16_t> load_quad(Rsrc r, unsigned row, int col, int width,
                                                   const bf16_t*) {
   const unsigned off = row + 2 * col;
-  if constexpr (WHOLE) {
-    return {__builtin_bit_cast(
-        u2, __builtin_amdgcn_raw_buffer_load_b64(r, col < width ? off : kNoLoad, 0, 0))};
-  } else {
-    unsigned v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[e] = __builtin_amdgcn_raw_buffer_load_b16(r, col + e < width ? off + 2 * e : kNoLoad, 0,
-                                                  0);
-    return {u2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)}};
-  }
+  return {__builtin_bit_cast(
+      u2, __builtin_amdgcn_raw_buffer_load_b64(r, col < width ? off : kNoLoad, 0, 0))};
 }
-template <bool WHOLE>
 __device__ __forceinline__ Quad<float> load_quad(Rsrc r, unsigned row, int col, int width,
                                                  const float*) {
   const unsigned off = row + 4 * col;
-  if constexpr (WHOLE) {
-    return {__builtin_bit_cast(
-        f4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0))};
-  } else {
-    f4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-          r, col + e < width ? off + 4 * e : kNoLoad, 0, 0));
-    return {x};
-  }
+  return {__builtin_bit_cast(
+      f4, __builtin_amdgcn_raw_buffer_load_b128(r, col < width ? off : kNoLoad, 0, 0))};
 }
 
 // LDS tiles of bfloat16, 64 columns wide (wider ones are side by side): the
@@ -438,7 +398,7 @@ __device__ __forceinline__ Rsrc chunk_rows(const Source& x, int c, int rows) {
 // A segment of a.seg chunks keeps its own state (from zero) apart from the
 // state at its start; the state in use is decay * start + own.  So a split run, whose
 // blocks take one segment each, has the bits of a walk over all of them.
-template <typename In, int NT, bool WHOLE, bool REV>
+template <typename In, int NT, bool REV>
 struct Block {
   static constexpr int IN = Type<In>::IN;
   static constexpr int KP = 2 * NT;               // pieces of K a thread loads
@@ -473,14 +433,14 @@ struct Block {
     const Rsrc r = chunk_rows(src, c, have(c));
 #pragma unroll
     for (int i = 0; i < KP; ++i)
-      raw[i] = load_piece<WHOLE>(r, (row + 32 / NT * i) * src.stride, col, R.n, (const In*)nullptr);
+      raw[i] = load_piece(r, (row + 32 / NT * i) * src.stride, col, R.n, (const In*)nullptr);
   }
   __device__ __forceinline__ void fetch_v(Piece<In> (&raw)[2], const Source& src, int c, int t) {
     const int col = 8 * (t & 7), row = t >> 3;
     const Rsrc r = chunk_rows(src, c, have(c));
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      raw[i] = load_piece<WHOLE>(r, (row + 32 * i) * src.stride, col0 + col, R.p,
+      raw[i] = load_piece(r, (row + 32 * i) * src.stride, col0 + col, R.p,
                                  (const In*)nullptr);
   }
   template <typename Sh>
@@ -731,7 +691,7 @@ struct Block {
       const Rsrc qr = chunk_rows(qs, c, have(c));
 #pragma unroll
       for (int kk = 0; kk < 2 * NT; ++kk)
-        qraw[kk] = load_piece<WHOLE>(qr, (16 * w + (lane & 15)) * qs.stride,
+        qraw[kk] = load_piece(qr, (16 * w + (lane & 15)) * qs.stride,
                                      32 * kk + 8 * (lane >> 4), R.n, (const In*)nullptr);
       graw = decay(c, lane);
     };
@@ -754,7 +714,7 @@ struct Block {
           const Rsrc er = chunk_rows(es, c, have(c));
 #pragma unroll
           for (int pb = 0; pb < 4; ++pb)
-            e[pb] = load_quad<WHOLE>(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p,
+            e[pb] = load_quad(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p,
                                      (const In*)nullptr);
         }
       }
@@ -905,20 +865,20 @@ __device__ __forceinline__ int chunks_of(const Args& a, int* c0, int* c1) {
 // (float32 with wide keys: one block, by its LDS).
 constexpr int waves_per_simd(int bytes, int nt) { return bytes == 4 && nt == 2 ? 2 : 4; }
 
-template <typename In, int NT, bool WHOLE>
+template <typename In, int NT>
 __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void attention_kernel(Args a) {
   constexpr int SP = Type<In>::ROUGH;
   __shared__ Shared<In, NT, SP> sh;
   int which, b, h, c0, c1;
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   const int seg = chunks_of(a, &c0, &c1);
-  Block<In, NT, WHOLE, false>(a, a.role[0], which, b, h).template outputs<SP, false>(seg, c0, c1,
+  Block<In, NT, false>(a, a.role[0], which, b, h).template outputs<SP, false>(seg, c0, c1,
                                                                                      sh);
 }
 
 // The gradients: dQ forward in time, dK and dV in reverse; NP and NN 64s of the
 // value and key widths, DOTS with what the decays' gradient needs.
-template <typename In, int NP, int NN, bool DOTS, bool WHOLE>
+template <typename In, int NP, int NN, bool DOTS>
 __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NP > NN ? NP : NN)) void
 attention_backward_kernel(Args a) {
   constexpr int SP = DOTS ? FINE : Type<In>::ROUGH, SV = Type<In>::ROUGH;
@@ -930,18 +890,18 @@ attention_backward_kernel(Args a) {
   if (!block_of(a, blockIdx.x, &which, &b, &h)) return;
   const int seg = chunks_of(a, &c0, &c1);
   if (which < a.role[0].tiles)
-    return Block<In, NP, WHOLE, false>(a, a.role[0], which, b, h)
+    return Block<In, NP, false>(a, a.role[0], which, b, h)
         .template outputs<SP, DOTS>(seg, c0, c1, sh.p);
   which -= a.role[0].tiles;
   if (which < a.role[1].tiles)
-    return Block<In, NP, WHOLE, true>(a, a.role[1], which, b, h)
+    return Block<In, NP, true>(a, a.role[1], which, b, h)
         .template outputs<SP, DOTS>(seg, c0, c1, sh.p);
-  Block<In, NN, WHOLE, true>(a, a.role[2], which - a.role[1].tiles, b, h)
+  Block<In, NN, true>(a, a.role[2], which - a.role[1].tiles, b, h)
       .template outputs<SV, false>(seg, c0, c1, sh.n);
 }
 
 // Split runs: the segments' own states, of all roles.
-template <typename In, int NT, bool WHOLE>
+template <typename In, int NT>
 __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   __shared__ Shared<In, NT, 0> sh;
   int which, b, h, i = 0, c0, c1;
@@ -953,12 +913,12 @@ __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   if constexpr (NT == 2) {
     if (R.n <= 64) {
       Shared<In, 1, 0>& narrow = reinterpret_cast<Shared<In, 1, 0>&>(sh);
-      if (R.rev) return Block<In, 1, WHOLE, true>(a, R, which, b, h).states(seg, c0, c1, narrow);
-      return Block<In, 1, WHOLE, false>(a, R, which, b, h).states(seg, c0, c1, narrow);
+      if (R.rev) return Block<In, 1, true>(a, R, which, b, h).states(seg, c0, c1, narrow);
+      return Block<In, 1, false>(a, R, which, b, h).states(seg, c0, c1, narrow);
     }
   }
-  if (R.rev) return Block<In, NT, WHOLE, true>(a, R, which, b, h).states(seg, c0, c1, sh);
-  Block<In, NT, WHOLE, false>(a, R, which, b, h).states(seg, c0, c1, sh);
+  if (R.rev) return Block<In, NT, true>(a, R, which, b, h).states(seg, c0, c1, sh);
+  Block<In, NT, false>(a, R, which, b, h).states(seg, c0, c1, sh);
 }
 
 // Split runs: each segment's start state from the segments' own states and
@@ -1107,6 +1067,28 @@ __global__ void share_sum_kernel(const float* part, long tokens, int heads, int 
     out[i] = s;
 }
 
+// Rows that are no whole 16-byte pieces (by width, stride or address), copied to
+// padded ones; a thread writes one piece.  Bound by memory: 500 MB in 134 us at B16
+// T1024 H12 N63 P127, forward and backward, whose attention then takes 302 us.  (Read
+// an element at a time where they are used, such rows took 587 us.)
+template <typename In>
+__global__ __launch_bounds__(256) void pack_kernel(Pack a) {
+  constexpr int V = 16 / sizeof(In);
+  const int which = blockIdx.y, pieces = a.padded[which] / V, heads = a.heads[which];
+  const Rows& x = a.from[which];
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long)a.B * a.T * heads * pieces) return;
+  const int piece = (int)(i % pieces);
+  const long row = i / pieces, token = row / heads;
+  const int h = (int)(row - token * heads), b = (int)(token / a.T), t = (int)(token % a.T);
+  const In* from = static_cast<const In*>(x.base) + b * x.sb + t * x.st + h * x.sh + piece * V;
+  typedef In piece_t __attribute__((ext_vector_type(V)));
+  piece_t v;
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = piece * V + e < x.width ? from[e] : (In)0;
+  *reinterpret_cast<piece_t*>(static_cast<In*>(a.to[which]) + i * V) = v;
+}
+
 // One token: S' = e^g S + k v^T, o = scale S'^T q.  The state is read and
 // written once, which is all the time there is: a block takes one (b, h), its
 // threads a piece of V columns of every R-th row each, and all of a thread's loads are
@@ -1189,30 +1171,27 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   }
 }
 
-#define LA_WHOLE(In, W)                                                       \
-  template __global__ void attention_kernel<In, 1, W>(Args);                 \
-  template __global__ void attention_kernel<In, 2, W>(Args);                 \
-  template __global__ void attention_states_kernel<In, 1, W>(Args);          \
-  template __global__ void attention_states_kernel<In, 2, W>(Args);          \
-  template __global__ void attention_backward_kernel<In, 1, 1, false, W>(Args); \
-  template __global__ void attention_backward_kernel<In, 1, 1, true, W>(Args);  \
-  template __global__ void attention_backward_kernel<In, 1, 2, false, W>(Args); \
-  template __global__ void attention_backward_kernel<In, 1, 2, true, W>(Args);  \
-  template __global__ void attention_backward_kernel<In, 2, 1, false, W>(Args); \
-  template __global__ void attention_backward_kernel<In, 2, 1, true, W>(Args);  \
-  template __global__ void attention_backward_kernel<In, 2, 2, false, W>(Args); \
-  template __global__ void attention_backward_kernel<In, 2, 2, true, W>(Args);
 #define LA_INSTANCES(In)                                                       \
-  LA_WHOLE(In, true)                                                           \
-  LA_WHOLE(In, false)                                                          \
+  template __global__ void attention_kernel<In, 1>(Args);                      \
+  template __global__ void attention_kernel<In, 2>(Args);                      \
+  template __global__ void attention_states_kernel<In, 1>(Args);               \
+  template __global__ void attention_states_kernel<In, 2>(Args);               \
+  template __global__ void attention_backward_kernel<In, 1, 1, false>(Args);   \
+  template __global__ void attention_backward_kernel<In, 1, 1, true>(Args);    \
+  template __global__ void attention_backward_kernel<In, 1, 2, false>(Args);   \
+  template __global__ void attention_backward_kernel<In, 1, 2, true>(Args);    \
+  template __global__ void attention_backward_kernel<In, 2, 1, false>(Args);   \
+  template __global__ void attention_backward_kernel<In, 2, 1, true>(Args);    \
+  template __global__ void attention_backward_kernel<In, 2, 2, false>(Args);   \
+  template __global__ void attention_backward_kernel<In, 2, 2, true>(Args);    \
   template __global__ void step_kernel<In, 4, 4>(Step);                        \
   template __global__ void step_kernel<In, 4, 8>(Step);                        \
   template __global__ void step_kernel<In, 4, 16>(Step);                       \
   template __global__ void step_kernel<In, 1, 16>(Step);                       \
+  template __global__ void pack_kernel<In>(Pack);                              \
   template __global__ void share_sum_kernel<In>(const float*, long, int, int, int, In*);
 LA_INSTANCES(float)
 LA_INSTANCES(bf16_t)
 #undef LA_INSTANCES
-#undef LA_WHOLE
 
 }  // namespace la

@@ -77,6 +77,15 @@ struct DecayGrad {
   int B, T, H;
 };
 
+// Rows to be copied to rows of `padded` columns, [B,T,heads,padded], zeros past
+// the width.
+struct Pack {
+  Rows from[4];
+  void* to[4];
+  int heads[4], padded[4];
+  int B, T;
+};
+
 struct Step {
   const void *q, *k, *v;
   long qb, qh, kb, kh, vb, vh;
