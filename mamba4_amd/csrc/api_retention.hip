@@ -93,7 +93,8 @@ int tiles_of(int width) { return (width + la::TILE - 1) / la::TILE; }
 
 // Chunks of a segment, by the chunk-tiles of one row (`blocks` tiles a head):
 // 4 while a segment is latency, up to 16 where the segments' states are traffic.
-// It does not depend on the batch (segments decide the bits).  Forward, 4 / 8 / 16:
+// It does not depend on the batch (segments decide the bits).  Forward, 4 / 8 / 16,
+// whole calls of an earlier form of the kernels (24 and 275 now, as chosen):
 // T2000 H12 N64 P128 34 / 37 / 58 us, T32768 H16 N128 P128 342 / 299 / 292.
 int segment(const Shape& s, int blocks) {
   const long each = (long)s.chunks() * s.H * blocks / 768;

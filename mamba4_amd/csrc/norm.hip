@@ -148,6 +148,8 @@ __device__ __forceinline__ void activate(const float (&z)[V], int act, float (&y
 
 // ---------------------------------------------------------------- one position
 
+// Bound by memory: 16384 x 1536 bfloat16 with a gate 35 us forward (4.3 TB/s), 64
+// backward (3.9), and 5 for the columns' sums.
 template <typename In, int V, int IT, bool BWD>
 __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
   __shared__ float fold[BWD ? ROW_THREADS : 1];
@@ -394,7 +396,8 @@ __device__ __forceinline__ T team_join(T mine, T* fold, int first, int k, int te
 // A block: positions of one sample, the channels of `span` groups (or a part
 // of one).  Thread: one vector of channels and every rows-th position.  A group's
 // threads are consecutive: thread = (group, row, vector).  Blocks that hold whole
-// samples walk them, blockIdx.y and every gridDim.y-th after it.
+// samples walk them, blockIdx.y and every gridDim.y-th after it.  Bound by memory: 8 x
+// 4000 x 512 float32 16 + 27 us forward, 25 + 33 backward (65 MB an array).
 template <typename In, int V, bool BWD, int PHASE>
 __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
   __shared__ Moments folded[POS_THREADS];
