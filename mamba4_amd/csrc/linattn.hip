@@ -863,11 +863,12 @@ __device__ __forceinline__ int chunks_of(const Args& a, int* c0, int* c1) {
 
 // Eight waves a block: two blocks a compute unit need no more than 128 registers
 // (float32 with wide keys: one block, by its LDS).  Bound by the issue of vector and
-// matrix instructions: B16 T1024 H12 N64 P128 bfloat16 61 us, its 127 MB 25 us.
+// matrix instructions: B16 T1024 H12 N64 P128 bfloat16 61 us, its 151 MB 30 us.
 constexpr int waves_per_simd(int bytes, int nt) { return bytes == 4 && nt == 2 ? 2 : 4; }
 
 template <typename In, int NT>
-__global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void attention_kernel(Args a) {
+__global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void attention_kernel(
+    Args a) {
   constexpr int SP = Type<In>::ROUGH;
   __shared__ Shared<In, NT, SP> sh;
   int which, b, h, c0, c1;
@@ -903,7 +904,7 @@ attention_backward_kernel(Args a) {
 }
 
 // Split runs: the segments' own states, of all roles.  T32768 H16 N128 P128 bfloat16
-// 78 us, by the loads' latency (K and V of each tile once, 2.6 TB/s).
+// with keys shared by four heads 78 us, 402 MB of loads, 168 MB of them from memory.
 template <typename In, int NT>
 __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   __shared__ Shared<In, NT, 0> sh;
