@@ -396,3 +396,28 @@ def test_refusals(gpu_lib):
         linear_attention_step_(s, q[:, 0].clone().requires_grad_(), q[:, 0], q[:, 0], g)
     with pytest.raises(ValueError, match="active"):
         linear_attention_step(s, q[:, 0], q[:, 0], q[:, 0], g, active=g)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("t", [1, 65, 300])
+def test_copied_rows_have_the_bits_of_whole_ones(gpu_lib, t, bf16):
+    """Rows of odd widths are copied to padded ones: the same bits as whole rows
+    with zeros in their place, whatever the absent tokens hold."""
+    announce(f"linear attention copied rows T{t} bf16={bf16}")
+    arrays, d_out, d_state = _problem(2, t, (4, 2, 1), 64, 128, bf16, initial=True, seed=11)
+    q, k, v, g, s0 = arrays
+    q[..., 63], k[..., 63], v[..., 125:] = 0, 0, 0
+    s0[:, :, 63], s0[..., 125:] = 0, 0
+    d_out[..., 125:], d_state[:, :, 63], d_state[..., 125:] = 0, 0, 0
+    lengths = [t, t // 2]
+    whole, whole_grads = _run(arrays, d_out, d_state, bf16, lengths)
+    for a in (q, k, v, g, d_out):
+        a[1, t // 2:] = np.nan
+    odd, odd_grads = _run([q[..., :63], k[..., :63], v[..., :125], g, s0[:, :, :63, :125]],
+                          d_out[..., :125], d_state[:, :, :63, :125], bf16, lengths)
+    assert torch.equal(odd.output, whole.output[..., :125])
+    assert torch.equal(odd.state, whole.state[:, :, :63, :125])
+    cuts = (np.s_[..., :63], np.s_[..., :63], np.s_[..., :125], np.s_[...],
+            np.s_[:, :, :63, :125])
+    for name, got, want, cut in zip(NAMES, odd_grads, whole_grads, cuts):
+        assert torch.equal(got, want[cut]), name
