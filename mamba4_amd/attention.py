@@ -21,6 +21,7 @@ import contextlib
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from mamba4_amd import _lib
 from mamba4_amd.memory import _ptr
@@ -63,6 +64,20 @@ def _same_device(*tensors):
 
 def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _differentiated(*tensors):
+    """Whether torch takes a derivative through any of the tensors: backwards, or
+    forwards (a dual tensor requires no gradient, and ``no_grad`` leaves it one)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
 
 
 def _strided(t):
@@ -223,10 +238,7 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
     s0 = None if initial is None else _f32(initial)
     scale = float(scale)
     with _on(device):
-        if torch.is_grad_enabled() and (
-            q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
-            or (s0 is not None and s0.requires_grad)
-        ):
+        if _differentiated(q, k, v, g, s0):
             output, state = _Attention.apply(q, k, v, g, s0, lengths, scale)
         else:
             output, state = _forward(q, k, v, g, s0, lengths, scale)
@@ -274,10 +286,7 @@ def linear_attention_step(state, query, key, value, log_decay, *, active=None, s
     step is ``linear_attention`` over one token.
     """
     heads, q, k, v = _step_checks(state, query, key, value, log_decay, active)
-    if torch.is_grad_enabled() and (
-        state.requires_grad or query.requires_grad or key.requires_grad or value.requires_grad
-        or log_decay.requires_grad
-    ):
+    if _differentiated(state, query, key, value, log_decay):
         decay = log_decay if log_decay.dim() == 1 else log_decay[:, None]
         one = linear_attention(query[:, None], key[:, None], value[:, None], decay, initial=state,
                                lengths=None if active is None else active.to(torch.int32),
@@ -293,10 +302,7 @@ def linear_attention_step_(state, query, key, value, log_decay, *, active=None, 
     heads, q, k, v = _step_checks(state, query, key, value, log_decay, active)
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("linear_attention_step_ needs a contiguous float32 state")
-    if torch.is_grad_enabled() and (
-        state.requires_grad or query.requires_grad or key.requires_grad or value.requires_grad
-        or log_decay.requires_grad
-    ):
+    if _differentiated(state, query, key, value, log_decay):
         raise ValueError("linear_attention_step_ has no gradient; use linear_attention_step")
     # The state may be saved for a backward: the write counts as one of torch's.
     torch.autograd.graph.increment_version(state)

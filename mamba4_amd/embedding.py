@@ -11,7 +11,7 @@ library (``m4rt_embedding_*``, include/mamba4_retention.h) on the current stream
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _on, _same_device, _stream, _workspace
+from mamba4_amd.attention import _differentiated, _on, _same_device, _stream, _workspace
 from mamba4_amd.memory import _ptr
 
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -77,6 +77,6 @@ def embedding(ids, table, *, scale=1.0, dtype=None):
         return table[:0].to(dtype).reshape(*ids.shape, table.shape[1])
     ids, table = ids.contiguous(), table.contiguous()
     with _on(table.device):
-        if torch.is_grad_enabled() and table.requires_grad:
+        if _differentiated(table):
             return _Embedding.apply(ids, table, float(scale), dtype)
         return _forward(ids, table, float(scale), dtype)

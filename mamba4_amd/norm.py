@@ -14,7 +14,7 @@ usual norm over space or time.  Runs on the gfx950 HIP library
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _f32, _on, _same_device, _stream, _workspace
+from mamba4_amd.attention import _differentiated, _f32, _on, _same_device, _stream, _workspace
 from mamba4_amd.memory import _ptr
 
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2}
@@ -116,7 +116,7 @@ def group_norm(x, groups, weight=None, bias=None, *, gate=None, activation="none
     weight, bias = (None if t is None else _f32(t) for t in (weight, bias))
     args = (x, weight, bias, gate, int(groups), ACTIVATIONS[activation], float(eps))
     with _on(x.device):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        if _differentiated(*args[:4]):
             y = _GroupNorm.apply(*args)
         else:
             y = _forward(*args, False)[0]
