@@ -21,10 +21,9 @@ import contextlib
 from typing import NamedTuple
 
 import torch
-import torch.autograd.forward_ad as forward_ad
 
 from mamba4_amd import _lib
-from mamba4_amd.memory import _ptr
+from mamba4_amd.memory import _differentiated, _ptr
 
 MAX_WIDTH = 128
 _MAX_TOKEN_STRIDE = (2**31 - 1) // 256
@@ -64,20 +63,6 @@ def _same_device(*tensors):
 
 def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _differentiated(*tensors):
-    """Whether torch takes a derivative through any of the tensors: backwards, or
-    forwards (a dual tensor requires no gradient, and ``no_grad`` leaves it one)."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                return True
-    return False
 
 
 def _strided(t):

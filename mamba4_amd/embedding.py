@@ -11,8 +11,8 @@ library (``m4rt_embedding_*``, include/mamba4_retention.h) on the current stream
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _differentiated, _on, _same_device, _stream, _workspace
-from mamba4_amd.memory import _ptr
+from mamba4_amd.attention import _on, _same_device, _stream, _workspace
+from mamba4_amd.memory import _differentiated, _ptr
 
 _DTYPES = (torch.float32, torch.bfloat16)
 

@@ -20,6 +20,7 @@ mode, lm/kernels/mamba4_fused.py:183-232).
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from mamba4_amd import _lib
 
@@ -59,6 +60,20 @@ def ctypes_stream(stream):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _differentiated(*tensors):
+    """Whether torch takes a derivative through any of the tensors: backwards, or
+    forwards (a dual tensor requires no gradient, and ``no_grad`` leaves it one)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
 
 
 def _require_device(*tensors):
@@ -386,9 +401,7 @@ def selective_gaussian_memory(
     beta, log_decay = beta.contiguous(), log_decay.contiguous()
     differentiable = (keys, values, queries, beta, log_decay, floor, init_s, init_c)
     with torch.cuda.device(device):
-        if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in differentiable
-        ):
+        if _differentiated(*differentiable):
             output, variance, final_s, final_c = _MemoryRead.apply(
                 k, v, q, beta, log_decay, f, init_s, init_c, chunk)
         else:
@@ -420,9 +433,7 @@ def selective_decode(state, key, value, query, beta, log_decay, floor, solver=No
     _require_device(evidence, cross)
     _check_state(evidence)
     inputs = (evidence, cross, key, value, query, beta, log_decay, floor)
-    if torch.is_grad_enabled() and any(
-        isinstance(t, torch.Tensor) and t.requires_grad for t in inputs
-    ):
+    if _differentiated(*(t for t in inputs if isinstance(t, torch.Tensor))):
         # A differentiable step is the one-token prefill from `state`: the
         # same HIP kernels with the custom VJP attached.
         one = selective_gaussian_memory(

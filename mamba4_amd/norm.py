@@ -14,8 +14,8 @@ usual norm over space or time.  Runs on the gfx950 HIP library
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _differentiated, _f32, _on, _same_device, _stream, _workspace
-from mamba4_amd.memory import _ptr
+from mamba4_amd.attention import _f32, _on, _same_device, _stream, _workspace
+from mamba4_amd.memory import _differentiated, _ptr
 
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2}
 
