@@ -206,12 +206,12 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
         raise ValueError("linear_attention needs initial [B,H,N,P]")
     if lengths is not None:
         if tuple(lengths.shape) != (batch,) or lengths.dtype.is_floating_point \
-                or lengths.dtype in (torch.bool, torch.complex64, torch.complex128):
+                or lengths.dtype.is_complex or lengths.dtype == torch.bool:
             raise ValueError("linear_attention needs integer lengths [B]")
-        # (The kernels clamp; wider integers before they are narrowed, so that none
-        # wraps around.)
+        # (The kernels clamp.  Other integers are clamped before they become int32, so
+        # that none wraps around, in a type that holds the sequence's length.)
         if lengths.dtype != torch.int32:
-            lengths = lengths.clamp(0, time).to(torch.int32)
+            lengths = lengths.to(torch.int64).clamp(0, time).to(torch.int32)
         lengths = lengths.contiguous()
     if batch == 0 or time == 0:
         output = values.new_zeros((batch, time, heads, p))
