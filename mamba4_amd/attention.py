@@ -104,6 +104,9 @@ def _forward(q, k, v, log_decay, initial, lengths, scale):
     heads, p, device = log_decay.shape[-1], v.shape[-1], v.device
     bf16 = 1 if v.dtype == _BF16 else 0
     output = torch.empty((batch, time, heads, p), dtype=v.dtype, device=device)
+    if batch == 0 or time == 0:
+        return output, output.new_zeros((batch, heads, n, p), dtype=_F32) if initial is None \
+            else initial.clone()
     state = torch.empty((batch, heads, n, p), dtype=_F32, device=device)
     rows = _qkv(q, k, v)
     nbytes = lib.m4rt_attention_workspace_bytes(rows, bf16, batch, time, heads)
@@ -138,6 +141,9 @@ class _Attention(torch.autograd.Function):
         batch, time, _, n = q.shape
         heads, p, device = log_decay.shape[-1], v.shape[-1], v.device
         bf16 = 1 if v.dtype == _BF16 else 0
+        if batch == 0 or time == 0:
+            d_initial = torch.zeros_like(state) if d_state is None else _f32(d_state)
+            return (*(torch.zeros_like(t) for t in (q, k, v, log_decay)), d_initial, None, None)
         if d_output is None:
             d_output = torch.zeros((batch, time, heads, p), dtype=v.dtype, device=device)
         d_output = d_output.to(v.dtype).contiguous()
@@ -213,12 +219,6 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
         if lengths.dtype != torch.int32:
             lengths = lengths.to(torch.int64).clamp(0, time).to(torch.int32)
         lengths = lengths.contiguous()
-    if batch == 0 or time == 0:
-        output = values.new_zeros((batch, time, heads, p))
-        state = output.new_zeros((batch, heads, n, p), dtype=torch.float32)
-        if initial is not None:
-            state = state + initial
-        return LinearAttentionResult(output, state)
     g = _f32(log_decay)
     s0 = None if initial is None else _f32(initial)
     scale = float(scale)

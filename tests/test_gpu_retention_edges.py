@@ -25,3 +25,46 @@ def test_lengths_of_every_integer_type(gpu_lib, dtype):
     got = linear_attention(q, q, v, g, lengths=torch.tensor(values, dtype=dtype).cuda())
     want = linear_attention(q, q, v, g, lengths=torch.tensor(values, device="cuda"))
     assert torch.equal(got.output, want.output) and torch.equal(got.state, want.state)
+
+
+@pytest.mark.parametrize("batch,time", [(0, 5), (2, 0), (0, 0)])
+@pytest.mark.parametrize("initial", [None, torch.float32, torch.float64, torch.bfloat16])
+@pytest.mark.parametrize("per_head", [False, True])
+def test_no_tokens(gpu_lib, batch, time, initial, per_head):
+    """The state is the initial one, in float32; every input has a gradient: zeros,
+    and the state's cotangent for the initial one."""
+    announce(f"no tokens B{batch} T{time} initial={initial} per_head={per_head}")
+    q, k = (_normal(batch, time, 2, 8).requires_grad_() for _ in range(2))
+    v = _normal(batch, time, 4, 6).to(torch.bfloat16).requires_grad_()
+    g = (torch.full((4,), -torch.inf, device="cuda") if per_head
+         else _normal(batch, time, 4)).requires_grad_()
+    s0 = None
+    if initial is not None:
+        s0 = _normal(batch, 4, 8, 6).to(initial).requires_grad_()
+    inputs = [t for t in (q, k, v, g, s0) if t is not None]
+    r = linear_attention(q, k, v, g, initial=s0)
+    assert r.output.shape == (batch, time, 4, 6) and r.output.dtype == torch.bfloat16
+    assert r.state.shape == (batch, 4, 8, 6) and r.state.dtype == torch.float32
+    want = torch.zeros(batch, 4, 8, 6, device="cuda") if s0 is None else s0.float()
+    assert torch.equal(r.state, want)
+    d_state = _normal(*r.state.shape)
+    grads = torch.autograd.grad([r.output, r.state], inputs,
+                                [torch.zeros_like(r.output), d_state])
+    for t, d in zip(inputs, grads):
+        assert d.shape == t.shape and d.dtype == t.dtype
+    for d in grads[:4]:
+        assert (d == 0).all()
+    if s0 is not None:
+        assert torch.equal(grads[4], d_state.to(initial))
+    with torch.no_grad():
+        again = linear_attention(q, k, v, g, initial=s0)
+    assert torch.equal(again.state, want) and again.output.shape == r.output.shape
+
+
+def test_no_tokens_from_the_output_alone(gpu_lib):
+    announce("no tokens, output alone")
+    x, s0 = _normal(2, 0, 2, 8).requires_grad_(), _normal(2, 2, 8, 8).requires_grad_()
+    g = torch.zeros(2, device="cuda", requires_grad=True)
+    r = linear_attention(x, x, x, g, initial=s0)
+    grads = torch.autograd.grad(r.output, (x, g, s0), torch.zeros_like(r.output))
+    assert grads[0].shape == x.shape and (grads[1] == 0).all() and (grads[2] == 0).all()
