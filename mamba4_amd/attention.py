@@ -142,7 +142,9 @@ class _Attention(torch.autograd.Function):
         heads, p, device = log_decay.shape[-1], v.shape[-1], v.device
         bf16 = 1 if v.dtype == _BF16 else 0
         if batch == 0 or time == 0:
-            d_initial = torch.zeros_like(state) if d_state is None else _f32(d_state)
+            d_initial = None
+            if initial is not None:
+                d_initial = torch.zeros_like(state) if d_state is None else _f32(d_state)
             return (*(torch.zeros_like(t) for t in (q, k, v, log_decay)), d_initial, None, None)
         if d_output is None:
             d_output = torch.zeros((batch, time, heads, p), dtype=v.dtype, device=device)
