@@ -37,6 +37,8 @@ class LinearAttentionResult(NamedTuple):
 
 
 def _f32(t):
+    if t.dtype.is_complex:
+        raise ValueError("complex numbers are not floating-point ones; take their real part first")
     return t.to(_F32).contiguous()
 
 
@@ -183,6 +185,8 @@ def _model_rows(name, queries, keys, values, dims):
     heads = max(hq, hk, hv)
     if min(hq, hk, hv) == 0 or heads % hq or heads % hk or heads % hv:
         raise ValueError("the heads of queries, keys and values must divide the largest of them")
+    if queries.dtype.is_complex or keys.dtype.is_complex or not values.dtype.is_floating_point:
+        raise ValueError(f"{name} needs floating-point values, and real queries and keys")
     if not (1 <= ks[-1] <= MAX_WIDTH and 1 <= vs[-1] <= MAX_WIDTH):
         raise ValueError(f"key and value widths must be 1..{MAX_WIDTH}")
     if queries.dtype != _BF16 or keys.dtype != _BF16 or values.dtype != _BF16:

@@ -97,6 +97,8 @@ def group_norm(x, groups, weight=None, bias=None, *, gate=None, activation="none
         raise ValueError(f"Unknown activation {activation}")
     if x.dim() < 2:
         raise ValueError("group_norm needs x [M, ..., C]")
+    if not x.dtype.is_floating_point or (gate is not None and gate.dtype.is_complex):
+        raise ValueError("group_norm needs a floating-point x, and a real gate")
     channels = x.shape[-1]
     if groups < 1 or channels == 0 or channels % groups:
         raise ValueError("the groups must divide the channels")

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mamba4_amd import linear_attention
+from mamba4_amd import group_norm, linear_attention, linear_attention_step
 from tests.gpu_helpers import announce
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,49 @@ def test_no_tokens_from_the_output_alone(gpu_lib):
     r = linear_attention(x, x, x, g, initial=s0)
     grads = torch.autograd.grad(r.output, (x, g, s0), torch.zeros_like(r.output))
     assert grads[0].shape == x.shape and (grads[1] == 0).all() and (grads[2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.bool, torch.complex64])
+def test_results_of_no_floating_type_are_refused(gpu_lib, dtype):
+    """Results come in the type of the values, or of x: whole numbers would cut
+    them, complex ones are no inputs at all."""
+    announce(f"results in {dtype}")
+    x = torch.ones(2, 3, 1, 8, device="cuda")
+    bad, g = x.to(dtype), torch.zeros(1, device="cuda")
+    state = torch.zeros(2, 1, 8, 8, device="cuda")
+    with pytest.raises(ValueError, match="floating"):
+        linear_attention(x, x, bad, g)
+    with pytest.raises(ValueError, match="floating"):
+        linear_attention_step(state, x[:, 0], x[:, 0], bad[:, 0], g)
+    with pytest.raises(ValueError, match="floating"):
+        group_norm(bad, 1)
+
+
+def test_complex_inputs_are_refused(gpu_lib):
+    """Their imaginary parts would be dropped."""
+    announce("complex inputs")
+    x, g = torch.ones(2, 3, 1, 8, device="cuda"), torch.zeros(1, device="cuda")
+    state, w = torch.zeros(2, 1, 8, 8, device="cuda"), torch.ones(8, device="cuda")
+
+    def z(t):
+        return t.to(torch.complex64)
+
+    for args, initial in (((z(x), x, x, g), None), ((x, z(x), x, g), None), ((x, x, x, z(g)), None),
+                          ((x, x, x, g), z(state))):
+        with pytest.raises(ValueError, match="floating|real"):
+            linear_attention(*args, initial=initial)
+    with pytest.raises(ValueError, match="floating|real"):
+        linear_attention_step(z(state), x[:, 0], x[:, 0], x[:, 0], g)
+    for weight, bias, gate in ((z(w), None, None), (w, z(w), None), (w, w, z(x))):
+        with pytest.raises(ValueError, match="floating|real"):
+            group_norm(x, 1, weight, bias, gate=gate)
+
+
+def test_whole_numbers_beside_floating_values(gpu_lib):
+    """Queries, keys, decays and states of whole numbers are numbers like others."""
+    announce("whole numbers")
+    q, v = torch.randint(-2, 3, (1, 5, 1, 8), device="cuda"), _normal(1, 5, 1, 8)
+    g, s = torch.tensor([-1], device="cuda"), torch.randint(-2, 3, (1, 1, 8, 8), device="cuda")
+    got = linear_attention(q, q, v, g, initial=s)
+    want = linear_attention(q.float(), q.float(), v, g.float(), initial=s.float())
+    assert torch.equal(got.output, want.output) and torch.equal(got.state, want.state)
