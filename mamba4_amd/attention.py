@@ -131,7 +131,12 @@ class _Attention(torch.autograd.Function):
     def forward(ctx, q, k, v, log_decay, initial, lengths, scale):
         output, state = _forward(q, k, v, log_decay, initial, lengths, scale)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, log_decay, initial, lengths, state)
+        ctx.save_for_backward(q, k, v, log_decay, initial, lengths)
+        # The final state is needed for the decays' gradient from a cotangent of the
+        # state alone, which only the backward knows: until then it may be stepped in
+        # place, so it is no saved tensor but an alias with its version.
+        ctx.state = state.detach() if ctx.needs_input_grad[3] else None
+        ctx.version = state._version
         ctx.scale = scale
         return output, state
 
@@ -139,14 +144,14 @@ class _Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_output, d_state):
         lib = _lib.load()
-        q, k, v, log_decay, initial, lengths, state = ctx.saved_tensors
+        q, k, v, log_decay, initial, lengths = ctx.saved_tensors
         batch, time, _, n = q.shape
         heads, p, device = log_decay.shape[-1], v.shape[-1], v.device
         bf16 = 1 if v.dtype == _BF16 else 0
         if batch == 0 or time == 0:
             d_initial = None
             if initial is not None:
-                d_initial = torch.zeros_like(state) if d_state is None else _f32(d_state)
+                d_initial = torch.zeros_like(initial) if d_state is None else _f32(d_state)
             return (*(torch.zeros_like(t) for t in (q, k, v, log_decay)), d_initial, None, None)
         if d_output is None:
             d_output = torch.zeros((batch, time, heads, p), dtype=v.dtype, device=device)
@@ -154,7 +159,14 @@ class _Attention(torch.autograd.Function):
         d_state = None if d_state is None else _f32(d_state)
         d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
         d_decay = torch.empty_like(log_decay) if ctx.needs_input_grad[3] else None
-        d_initial = torch.empty_like(state) if ctx.needs_input_grad[4] else None
+        d_initial = torch.empty_like(initial) if ctx.needs_input_grad[4] else None
+        state = None
+        if d_state is not None and d_decay is not None:
+            state = ctx.state
+            if state._version != ctx.version:
+                raise RuntimeError(
+                    "one of the variables needed for gradient computation has been modified by "
+                    "an inplace operation: the final state of linear_attention")
         rows = _qkv(q, k, v)
         nbytes = lib.m4rt_attention_backward_workspace_bytes(
             rows, d_output.data_ptr(), bf16, batch, time, heads, d_decay is not None)
@@ -162,7 +174,7 @@ class _Attention(torch.autograd.Function):
         rc = lib.m4rt_attention_backward(
             rows, bf16, log_decay.data_ptr(), log_decay.dim() == 3, _ptr(lengths),
             _ptr(initial), ctx.scale, batch, time, heads, d_output.data_ptr(), _ptr(d_state),
-            state.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), _ptr(d_decay),
+            _ptr(state), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), _ptr(d_decay),
             _ptr(d_initial), _ptr(workspace), nbytes, _stream(device),
         )
         if rc:

@@ -70,3 +70,50 @@ def test_forward_mode_derivatives_of_the_step_in_place_are_refused(gpu_lib):
             linear_attention_step_(s, q, k, dual, g)
         assert torch.equal(s, before)
         linear_attention_step_(s, q, k, v, g)
+
+
+def _prompt(decay_grad):
+    q, k, v = (_normal(2, 70, 2, 8).requires_grad_() for _ in range(3))
+    g = (-torch.rand(2, 70, 2, device="cuda")).requires_grad_(decay_grad)
+    return q, k, v, g
+
+
+def _advance(state):
+    """One token more, in place, as a decode loop does after its prompt."""
+    one = _normal(2, 2, 8)
+    with torch.no_grad():
+        linear_attention_step_(state, one, one, one, -torch.rand(2, 2, device="cuda"))
+
+
+@pytest.mark.parametrize("decay_grad", [False, True])
+def test_a_step_in_place_on_the_state_leaves_the_backward(gpu_lib, decay_grad):
+    """The gradient from the output alone does not need the final state."""
+    announce(f"step in place before the backward, decay_grad={decay_grad}")
+    inputs = _prompt(decay_grad)
+    wanted = [t for t in inputs if t.requires_grad]
+    r = linear_attention(*inputs)
+    d = _normal(*r.output.shape)
+    want = torch.autograd.grad(r.output, wanted, d, retain_graph=True)
+    _advance(r.state)
+    got = torch.autograd.grad(r.output, wanted, d)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_a_modified_state_that_the_backward_needs_is_refused(gpu_lib):
+    """The decays' gradient from a cotangent of the state is of the state that the
+    forward gave; without the decays' it does not enter."""
+    announce("step in place on a state the backward needs")
+    for decay_grad in (True, False):
+        inputs = _prompt(decay_grad)
+        wanted = [t for t in inputs[1:] if t.requires_grad]
+        r = linear_attention(*inputs)
+        d = _normal(*r.state.shape)
+        want = torch.autograd.grad(r.state, wanted, d, retain_graph=True)
+        _advance(r.state.detach())
+        if decay_grad:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(r.state, wanted, d)
+        else:
+            for a, b in zip(torch.autograd.grad(r.state, wanted, d), want):
+                assert torch.equal(a, b)
