@@ -804,7 +804,7 @@ int m4rt_norm_backward(const void* x, const float* weight, const float* bias, co
     const std::string at = std::string(name) + ": ";
     std::string why;
     if (bad_norm(M, L, C, G, activation, &why)) return api_fail(M4MR_EINVAL, at + why);
-    if (!x || !d_output || !d_x || !stats || (gate && !d_gate))
+    if (!x || !d_output || !stats)
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x, gate, d_output, d_x, d_gate}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");

@@ -277,7 +277,8 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
             dz[k] = dv[i].get(k) * y[k];
             dg[k] = dv[i].get(k) * z[k] * slope[k];
           }
-          if (here && on[i]) Vec<In, V>::store(a.dgate, at + i * a.lanes * V, dg);
+          if (a.dgate && here && on[i])
+            Vec<In, V>::store(a.dgate, at + i * a.lanes * V, dg);
         } else {
 #pragma unroll
           for (int k = 0; k < V; ++k) dz[k] = dv[i].get(k) * slope[k];
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(ROW_THREADS) void norm_rows_kernel(Norm a) {
         float dx[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) dx[k] = inv * (dn[i][k] - s1 - n[i][k] * s2);
-        if (here && on[i]) Vec<In, V>::store(a.dx, at + i * a.lanes * V, dx);
+        if (a.dx && here && on[i]) Vec<In, V>::store(a.dx, at + i * a.lanes * V, dx);
       }
     }
   }
@@ -602,8 +603,8 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
                 dg[e] = dy * z[e] * slope[e];
                 dx[e] = inv * (dz * w[e] - s1 - n[e] * s2);
               }
-              Vec<In, V>::store(a.dx, p, dx);
-              if (a.gate) Vec<In, V>::store(a.dgate, p, dg);
+              if (a.dx) Vec<In, V>::store(a.dx, p, dx);
+              if (a.dgate) Vec<In, V>::store(a.dgate, p, dg);
             }
         }
     }

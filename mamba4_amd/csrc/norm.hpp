@@ -19,7 +19,7 @@ enum Phase { SUMS = 0, APPLY = 1, BOTH = 2 };
 struct Norm {
   const void *x, *gate, *dy;
   const float *weight, *bias;  // [C], or NULL
-  void *y, *dx, *dgate;
+  void *y, *dx, *dgate;        // dx, dgate: NULL if not wanted (dgate also without a gate)
   float* part;                 // column sums' partials [rows][2][C], or NULL
   long M;
   int L, C, G, D;

@@ -66,10 +66,10 @@ class _GroupNorm(torch.autograd.Function):
         samples, positions, channels = _sizes(x)
         bf16 = int(x.dtype == torch.bfloat16)
         d_y = d_y.to(x.dtype).contiguous()
-        d_x = torch.empty_like(x)
+        d_x = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         d_bias = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
-        d_gate = None if gate is None else torch.empty_like(gate)
+        d_gate = torch.empty_like(gate) if ctx.needs_input_grad[3] else None
         nbytes = lib.m4rt_norm_workspace_bytes(samples, positions, channels, groups, bf16, 1)
         workspace = _workspace(nbytes, x.device)
         _lib.check(

@@ -117,3 +117,54 @@ def test_a_modified_state_that_the_backward_needs_is_refused(gpu_lib):
         else:
             for a, b in zip(torch.autograd.grad(r.state, wanted, d), want):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("shape,groups", [((700, 96), 4), ((3, 200, 24), 3), ((2, 4000, 32), 2),
+                                          ((5, 4096), 1)])
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (3,), (0, 3), (1, 2)])
+def test_norm_gradients_one_by_one(gpu_lib, shape, groups, wanted):
+    """Any subset of the gradients has the bits of all of them."""
+    announce(f"norm gradients {shape} G{groups} {wanted}")
+    c = shape[-1]
+    tensors = [_normal(*shape), _normal(c), _normal(c), _normal(*shape)]
+    d = _normal(*shape)
+
+    def gradients(of):
+        x, w, b, gate = (t.clone().requires_grad_(i in of) for i, t in enumerate(tensors))
+        y = group_norm(x, groups, w, b, gate=gate, activation="silu")
+        return torch.autograd.grad(y, [(x, w, b, gate)[i] for i in of], d)
+
+    every = gradients((0, 1, 2, 3))
+    for i, got in zip(wanted, gradients(wanted)):
+        assert torch.equal(got, every[i])
+
+
+def test_norm_backward_takes_null_for_every_gradient(gpu_lib):
+    """The C entry point: what is not wanted is neither refused nor written."""
+    announce("norm backward with NULL gradients")
+    from mamba4_amd import _lib
+
+    m, c, groups = 70, 32, 2
+    x, gate, d = _normal(m, c), _normal(m, c), _normal(m, c)
+    stats = torch.empty(m, groups, 2, device="cuda")
+    y, stream = torch.empty_like(x), torch.cuda.current_stream().cuda_stream
+    lib = _lib.load()
+    size = max(lib.m4rt_norm_workspace_bytes(m, 1, c, groups, 0, b) for b in (0, 1))
+    work = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.m4rt_norm_forward(
+        x.data_ptr(), None, None, gate.data_ptr(), 0, m, 1, c, groups, 1, 1e-5, y.data_ptr(),
+        stats.data_ptr(), work.data_ptr(), size, stream))
+
+    def backward(d_x, d_weight, d_gate):
+        at = [None if t is None else t.data_ptr() for t in (d_x, d_weight, d_gate)]
+        _lib.check(lib.m4rt_norm_backward(
+            x.data_ptr(), None, None, gate.data_ptr(), d.data_ptr(), stats.data_ptr(), 0, m, 1, c,
+            groups, 1, 1e-5, at[0], at[1], None, at[2], work.data_ptr(), size, stream))
+
+    every = [torch.empty_like(x), torch.empty(c, device="cuda"), torch.empty_like(x)]
+    backward(*every)
+    for i in range(3):
+        got = [torch.empty_like(t) if i == j else None for j, t in enumerate(every)]
+        backward(*got)
+        assert torch.equal(got[i], every[i])
+    backward(None, None, None)
