@@ -149,6 +149,16 @@ bool attention_splits(const Shape& s, int blocks) {
   return split < walk;
 }
 
+// How a call runs its sequences.  Settled once a call: the workspace is carved for it.
+struct Route {
+  int segments;
+  bool split;
+};
+
+Route attention_route(const Shape& s, int blocks) {
+  return Route{segments(s, blocks), attention_splits(s, blocks)};
+}
+
 // The segments' states of one role (n keys wide, `tiles` blocks of values); no
 // segments: none are kept.
 void take_states(Carver& c, const Shape& s, int n, int tiles, int segments, la::Role* role) {
@@ -289,7 +299,7 @@ int start_attention(const la::Args& a, hipStream_t st) {
                     [&] { start_outputs<In>(a, dim3(x, a.split ? a.NS : 1), st); });
 }
 
-int run_attention(la::Args& a, const Shape& s, bool split, hipStream_t st) {
+int run_attention(la::Args& a, const Shape& s, const Route& route, hipStream_t st) {
   a.blocks = 0;
   for (int i = 0; i < a.roles; ++i) a.blocks += a.role[i].tiles;
   a.B = s.B;
@@ -297,8 +307,8 @@ int run_attention(la::Args& a, const Shape& s, bool split, hipStream_t st) {
   a.H = s.H;
   a.NC = s.chunks();
   a.seg = segment(s, a.blocks);
-  a.NS = segments(s, a.blocks);
-  a.split = split;
+  a.NS = route.segments;
+  a.split = route.split;
   return s.bf16 ? start_attention<la::bf16_t>(a, st) : start_attention<float>(a, st);
 }
 
@@ -332,11 +342,10 @@ struct Backward {
 int backward_tiles(const Shape& s) { return 2 * tiles_of(s.N) + tiles_of(s.P); }
 
 // The forward's workspace: the segments' states of a split, packed rows.
-size_t forward_workspace(const Shape& s, const m4rt_qkv& rows, void* base, la::Role* role,
-                         Operands* x) {
+size_t forward_workspace(const Shape& s, const m4rt_qkv& rows, const Route& route, void* base,
+                         la::Role* role, Operands* x) {
   Carver c{static_cast<char*>(base)};
-  const int tiles = tiles_of(s.P);
-  take_states(c, s, s.N, tiles, attention_splits(s, tiles) ? segments(s, tiles) : 0, role);
+  take_states(c, s, s.N, tiles_of(s.P), route.split ? route.segments : 0, role);
   x->q = rows_of(rows.q, s.H, s.bf16);
   x->k = rows_of(rows.k, s.H, s.bf16);
   x->v = rows_of(rows.v, s.H, s.bf16);
@@ -349,16 +358,16 @@ size_t forward_workspace(const Shape& s, const m4rt_qkv& rows, void* base, la::R
 // The backward's workspace: the segments' states (of dQ and dK for the decays'
 // gradient too), float32 gradients of shared heads before their sums, the dots, the
 // heads' sums, packed rows.
-size_t backward_workspace(const Shape& s, const m4rt_qkv& rows, const void* d_output, bool decays,
-                          void* base, Backward* out, Operands* x) {
+size_t backward_workspace(const Shape& s, const m4rt_qkv& rows, const Route& route,
+                          const void* d_output, bool decays, void* base, Backward* out,
+                          Operands* x) {
   Carver c{static_cast<char*>(base)};
   const int n[3] = {s.P, s.P, s.N}, p[3] = {s.N, s.N, s.P};
   const int heads[3] = {rows.q.heads, rows.k.heads, rows.v.heads};
   const size_t tokens = (size_t)s.B * s.T * s.H;
-  const int blocks = backward_tiles(s), count = segments(s, blocks);
-  const bool split = attention_splits(s, blocks);
+  const int count = route.segments;
   for (int i = 0; i < 3; ++i) {
-    take_states(c, s, n[i], tiles_of(p[i]), split || (decays && i < 2) ? count : 0,
+    take_states(c, s, n[i], tiles_of(p[i]), route.split || (decays && i < 2) ? count : 0,
                 &out->role[i]);
     out->part[i] = c.take<float>(heads[i] == s.H ? 0 : tokens * p[i]);
   }
@@ -404,7 +413,7 @@ size_t m4rt_attention_workspace_bytes(const m4rt_qkv* rows, int bf16, int B, int
   la::Role role{};
   Operands x{};
   if (bad_attention(rows, bf16, B, T, H, &s, &why)) return 0;
-  return forward_workspace(s, *rows, nullptr, &role, &x);
+  return forward_workspace(s, *rows, attention_route(s, tiles_of(s.P)), nullptr, &role, &x);
 }
 
 size_t m4rt_attention_backward_workspace_bytes(const m4rt_qkv* rows, const void* d_output,
@@ -414,7 +423,8 @@ size_t m4rt_attention_backward_workspace_bytes(const m4rt_qkv* rows, const void*
   Backward w{};
   Operands x{};
   if (bad_attention(rows, bf16, B, T, H, &s, &why)) return 0;
-  return backward_workspace(s, *rows, d_output, decays, nullptr, &w, &x);
+  return backward_workspace(s, *rows, attention_route(s, backward_tiles(s)), d_output, decays,
+                            nullptr, &w, &x);
 }
 
 int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
@@ -431,7 +441,8 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
     la::Args a{};
     la::Role& r = a.role[0];
     Operands x{};
-    const size_t need = forward_workspace(s, *rows, workspace, &r, &x);
+    const Route route = attention_route(s, tiles_of(s.P));
+    const size_t need = forward_workspace(s, *rows, route, workspace, &r, &x);
     if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
     r.q = x.q;
@@ -453,7 +464,7 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
     a.lengths = lengths;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int rc = run_packing(x.packing, s, st);
-    return rc ? rc : run_attention(a, s, attention_splits(s, r.tiles), st);
+    return rc ? rc : run_attention(a, s, route, st);
   });
 }
 
@@ -473,8 +484,9 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
     const int heads[3] = {rows->q.heads, rows->k.heads, rows->v.heads};
     Backward w{};
     Operands x{};
+    const Route route = attention_route(s, backward_tiles(s));
     const size_t need =
-        backward_workspace(s, *rows, d_output, d_log_decay != nullptr, workspace, &w, &x);
+        backward_workspace(s, *rows, route, d_output, d_log_decay != nullptr, workspace, &w, &x);
     if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -514,7 +526,7 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
     a.gb = per_token ? (long)T * H : 0;
     a.gt = per_token ? H : 0;
     a.lengths = lengths;
-    rc = run_attention(a, s, attention_splits(s, backward_tiles(s)), st);
+    rc = run_attention(a, s, route, st);
     if (rc) return rc;
     for (int i = 0; i < 3; ++i) {
       if (heads[i] == H) continue;
