@@ -84,6 +84,8 @@ bool bad_workspace(const void* base, size_t given, size_t need, std::string* why
 
 // ------------------------------------------------------ linear attention --
 
+constexpr int MAX_GRID_Y = 65535;
+
 struct Shape {
   int B, T, H, N, P, bf16;
   int chunks() const { return (T + la::C - 1) / la::C; }
@@ -95,10 +97,13 @@ int tiles_of(int width) { return (width + la::TILE - 1) / la::TILE; }
 // 4 while a segment is latency, up to 16 where the segments' states are traffic.
 // It does not depend on the batch (segments decide the bits).  Forward, 4 / 8 / 16,
 // whole calls of an earlier form of the kernels (24 and 275 now, as chosen):
-// T2000 H12 N64 P128 34 / 37 / 58 us, T32768 H16 N128 P128 342 / 299 / 292.
+// T2000 H12 N64 P128 34 / 37 / 58 us, T32768 H16 N128 P128 342 / 299 / 292.  Longer
+// ones only keep the segments within a launch's y blocks (past 67M tokens).
 int segment(const Shape& s, int blocks) {
   const long each = (long)s.chunks() * s.H * blocks / 768;
-  return each >= 16 ? 16 : each >= 8 ? 8 : 4;
+  int seg = each >= 16 ? 16 : each >= 8 ? 8 : 4;
+  while ((s.chunks() - 1) / seg >= MAX_GRID_Y) seg *= 2;
+  return seg;
 }
 
 int segments(const Shape& s, int blocks) {

@@ -7,7 +7,6 @@
 namespace la {
 
 constexpr int C = 64;        // tokens of a chunk
-constexpr int MAX_SEG = 16;  // most chunks of a segment
 constexpr int TILE = 64;     // value columns of a block
 constexpr int WAVES = 4;     // strips of 16 tokens in a chunk, each a wave's
 constexpr int MAX_WIDTH = 128;

@@ -46,3 +46,13 @@ def test_a_call_makes_its_choice_once():
                      "m4rt_attention_step": 0}
     assert len(re.findall(r"\battention_splits\(", text)) == 2  # its definition, the route's
     assert text.count("getenv") == 1
+
+
+def test_segments_of_the_longest_sequences_fit_a_launch(monkeypatch):
+    """65,535 blocks along y at most: 16-chunk segments reach that at 67M tokens."""
+    monkeypatch.setenv("M4RT_ATTENTION", "split")
+    slot = 64 * 64 * 4
+    for T, chunks in ((65535 * 1024, 16), (65535 * 1024 + 1, 32), (2**27 - 16, 64)):
+        count = -(-T // (64 * chunks))
+        assert count <= 65535
+        assert _sizes(T, H=1)[0] == count * slot + -(-4 * count // 256) * 256
