@@ -205,11 +205,17 @@ void pack_rows(Carver& c, const Shape& s, la::Rows* r, int heads, Packing* out) 
                 r->share, width, 1};
 }
 
+// Blocks of 256 threads that take an element each in turn: as many as the elements
+// need, within a launch's 2^32 threads (the kernels walk on from there).
+unsigned element_blocks(long count) {
+  return (unsigned)std::min<long>((count + 255) / 256, 1 << 16);
+}
+
 int run_packing(Packing& p, const Shape& s, hipStream_t st) {
   if (p.count == 0) return M4MR_OK;
   p.a.B = s.B;
   p.a.T = s.T;
-  const dim3 grid((unsigned)((p.most + 255) / 256), p.count), block(256);
+  const dim3 grid(element_blocks(p.most), p.count), block(256);
   return api_launch("attention_pack", st, [&] {
     if (s.bf16)
       hipLaunchKernelGGL(la::pack_kernel<la::bf16_t>, grid, block, 0, st, p.a);
@@ -537,7 +543,7 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
       if (heads[i] == H) continue;
       const long count = (long)B * T * heads[i] * a.role[i].p;
       rc = api_launch("attention_share", st, [&] {
-        const dim3 grid((unsigned)((count + 255) / 256));
+        const dim3 grid(element_blocks(count));
         const int share = H / heads[i];
         if (bf16)
           hipLaunchKernelGGL(la::share_sum_kernel<la::bf16_t>, grid, dim3(256), 0, st, w.part[i],

@@ -1055,20 +1055,21 @@ __global__ __launch_bounds__(64) void decay_heads_kernel(const double* head, int
 template <typename Out>
 __global__ void share_sum_kernel(const float* part, long tokens, int heads, int share, int width,
                                  Out* out) {
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
   const int own = heads / share;
-  if (i >= tokens * own * width) return;
-  const int x = (int)(i % width);
-  const long row = i / width;
-  const long t = row / own;
-  const int j = (int)(row - t * own);
-  const float* p = part + ((t * heads) + (long)j * share) * width + x;
-  float s = 0.f;
-  for (int k = 0; k < share; ++k) s += p[(long)k * width];
-  if constexpr (sizeof(Out) == 2)
-    out[i] = (bf16_t)pack(s, 0.f);
-  else
-    out[i] = s;
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < tokens * own * width;
+       i += (long)gridDim.x * blockDim.x) {
+    const int x = (int)(i % width);
+    const long row = i / width;
+    const long t = row / own;
+    const int j = (int)(row - t * own);
+    const float* p = part + ((t * heads) + (long)j * share) * width + x;
+    float s = 0.f;
+    for (int k = 0; k < share; ++k) s += p[(long)k * width];
+    if constexpr (sizeof(Out) == 2)
+      out[i] = (bf16_t)pack(s, 0.f);
+    else
+      out[i] = s;
+  }
 }
 
 // Rows that are no whole 16-byte pieces (by width, stride or address), copied to
@@ -1080,17 +1081,18 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack a) {
   constexpr int V = 16 / sizeof(In);
   const int which = blockIdx.y, pieces = a.padded[which] / V, heads = a.heads[which];
   const Rows& x = a.from[which];
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long)a.B * a.T * heads * pieces) return;
-  const int piece = (int)(i % pieces);
-  const long row = i / pieces, token = row / heads;
-  const int h = (int)(row - token * heads), b = (int)(token / a.T), t = (int)(token % a.T);
-  const In* from = static_cast<const In*>(x.base) + b * x.sb + t * x.st + h * x.sh + piece * V;
-  typedef In piece_t __attribute__((ext_vector_type(V)));
-  piece_t v;
+  const long count = (long)a.B * a.T * heads * pieces;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) {
+    const int piece = (int)(i % pieces);
+    const long row = i / pieces, token = row / heads;
+    const int h = (int)(row - token * heads), b = (int)(token / a.T), t = (int)(token % a.T);
+    const In* from = static_cast<const In*>(x.base) + b * x.sb + t * x.st + h * x.sh + piece * V;
+    typedef In piece_t __attribute__((ext_vector_type(V)));
+    piece_t v;
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = piece * V + e < x.width ? from[e] : (In)0;
-  *reinterpret_cast<piece_t*>(static_cast<In*>(a.to[which]) + i * V) = v;
+    for (int e = 0; e < V; ++e) v[e] = piece * V + e < x.width ? from[e] : (In)0;
+    *reinterpret_cast<piece_t*>(static_cast<In*>(a.to[which]) + i * V) = v;
+  }
 }
 
 // One token: S' = e^g S + k v^T, o = scale S'^T q.  The state is read and

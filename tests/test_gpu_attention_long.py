@@ -32,3 +32,43 @@ def test_more_segments_than_blocks_along_y(gpu_lib):
     for a, b in zip(whole, end):
         assert torch.isfinite(a).all()
         assert ((a.double() - b.double()).abs().max() <= 2.0 ** -8 * b.double().abs().max()).item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sums_of_shared_heads_over_many_elements(gpu_lib, dtype):
+    """33M elements of a shared head's gradient, twice the threads of the launch that
+    sums them: the sums of the heads' own gradients (float32: the same additions;
+    bfloat16: of parts rounded before their sum, 2^-8 of them)."""
+    time = 1 << 18
+    announce(f"shared heads T{time} {dtype}")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, v = (torch.randn(1, time, 2, 128, device="cuda", generator=gen).to(dtype) for _ in range(2))
+    k = torch.randn(1, time, 1, 128, device="cuda", generator=gen).to(dtype)
+    g = torch.full((2,), -0.1, device="cuda")
+    d = torch.randn(1, time, 2, 128, device="cuda", generator=gen).to(dtype)
+    k.requires_grad_()
+    (shared,) = torch.autograd.grad(linear_attention(q, k, v, g).output, k, d)
+    own = k.detach().expand(-1, -1, 2, -1).contiguous().requires_grad_()
+    (parts,) = torch.autograd.grad(linear_attention(q, own, v, g).output, own, d)
+    want = parts.float().sum(dim=2, keepdim=True)
+    if dtype == torch.float32:
+        assert torch.equal(shared, want)
+    else:
+        off = (shared.float() - want).abs().max()
+        assert (off <= 3 * 2.0 ** -9 * parts.float().abs().max()).item()
+
+
+def test_many_rows_of_odd_widths(gpu_lib):
+    """34M pieces of 16 bytes to be copied, twice the threads of the launch that
+    copies them: the results of the padded rows."""
+    time = 1 << 21
+    announce(f"odd widths T{time}")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(1, time, 2, w, device="cuda", generator=gen, dtype=torch.bfloat16)
+               for w in (63, 63, 61))
+    g = torch.full((2,), -0.1, device="cuda")
+    got = linear_attention(q, k, v, g)
+    pad = torch.nn.functional.pad
+    want = linear_attention(pad(q, (0, 1)), pad(k, (0, 1)), pad(v, (0, 3)), g)
+    assert torch.equal(got.output, want.output[..., :61])
+    assert torch.equal(got.state, want.state[..., :63, :61])
