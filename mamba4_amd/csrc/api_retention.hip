@@ -111,7 +111,8 @@ int segments(const Shape& s, int blocks) {
   return (s.chunks() + seg - 1) / seg;
 }
 
-bool bad_shape(const Shape& s, std::string* why) {
+// `blocks`, `threads`: blocks of the widest launch for each (b, h), and of a block.
+bool bad_shape(const Shape& s, int blocks, int threads, std::string* why) {
   if (s.B <= 0 || s.T <= 0 || s.H <= 0) {
     *why = "B, T and H must be positive";
     return true;
@@ -120,8 +121,8 @@ bool bad_shape(const Shape& s, std::string* why) {
     *why = "key and value widths must be in 1.." + std::to_string(M4RT_MAX_WIDTH);
     return true;
   }
-  // Grids: blocks of at most six tiles a (b, h), segments along y.
-  if ((double)s.B * s.H * 6 + 64 > INT_MAX / 2 || s.T > INT_MAX / 16) {
+  // A launch takes fewer than 2^32 threads along x; (b, h) are rounded up to eights.
+  if (((double)s.B * s.H + 8) * blocks * threads >= 4294967296.0 || s.T > INT_MAX / 16) {
     *why = "problem too large";
     return true;
   }
@@ -396,15 +397,17 @@ size_t backward_workspace(const Shape& s, const m4rt_qkv& rows, const Route& rou
   return c.used;
 }
 
-// The attention's shape from its rows, if they and it are sound.
-bool bad_attention(const m4rt_qkv* rows, int bf16, int B, int T, int H, Shape* s,
+// The attention's shape from its rows, if they and it are sound, for the forward or
+// the backward.
+bool bad_attention(const m4rt_qkv* rows, int bf16, int B, int T, int H, bool backward, Shape* s,
                    std::string* why) {
   if (!rows) {
     *why = "a required pointer is NULL";
     return true;
   }
   *s = Shape{B, T, H, rows->q.width, rows->v.width, bf16};
-  if (bad_shape(*s, why)) return true;
+  if (bad_shape(*s, backward ? backward_tiles(*s) : tiles_of(s->P), 128 * la::WAVES, why))
+    return true;
   for (const m4rt_rows* r : {&rows->q, &rows->k, &rows->v})
     if (bad_rows(r, H, bf16, true, why)) return true;
   if (rows->q.width != rows->k.width) {
@@ -423,7 +426,7 @@ size_t m4rt_attention_workspace_bytes(const m4rt_qkv* rows, int bf16, int B, int
   std::string why;
   la::Role role{};
   Operands x{};
-  if (bad_attention(rows, bf16, B, T, H, &s, &why)) return 0;
+  if (bad_attention(rows, bf16, B, T, H, false, &s, &why)) return 0;
   return forward_workspace(s, *rows, attention_route(s, tiles_of(s.P)), nullptr, &role, &x);
 }
 
@@ -433,7 +436,7 @@ size_t m4rt_attention_backward_workspace_bytes(const m4rt_qkv* rows, const void*
   std::string why;
   Backward w{};
   Operands x{};
-  if (bad_attention(rows, bf16, B, T, H, &s, &why)) return 0;
+  if (bad_attention(rows, bf16, B, T, H, true, &s, &why)) return 0;
   return backward_workspace(s, *rows, attention_route(s, backward_tiles(s)), d_output, decays,
                             nullptr, &w, &x);
 }
@@ -447,7 +450,7 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
     const std::string at = std::string(name) + ": ";
     Shape s;
     std::string why;
-    if (bad_attention(rows, bf16, B, T, H, &s, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (bad_attention(rows, bf16, B, T, H, false, &s, &why)) return api_fail(M4MR_EINVAL, at + why);
     if (!log_decay || !output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     la::Args a{};
     la::Role& r = a.role[0];
@@ -489,7 +492,7 @@ int m4rt_attention_backward(const m4rt_qkv* rows, int bf16, const float* log_dec
     const std::string at = std::string(name) + ": ";
     Shape s;
     std::string why;
-    if (bad_attention(rows, bf16, B, T, H, &s, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (bad_attention(rows, bf16, B, T, H, true, &s, &why)) return api_fail(M4MR_EINVAL, at + why);
     if (!log_decay || !d_output || !d_q || !d_k || !d_v || (d_state && d_log_decay && !state))
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     const int heads[3] = {rows->q.heads, rows->k.heads, rows->v.heads};
@@ -599,7 +602,7 @@ int m4rt_attention_step(const m4rt_qkv* rows, int bf16, const float* log_decay, 
     const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
     const Shape s{B, 1, H, q->width, v->width, bf16};
     std::string why;
-    if (bad_shape(s, &why) || bad_rows(q, H, bf16, false, &why) ||
+    if (bad_shape(s, 1, la::STEP_THREADS, &why) || bad_rows(q, H, bf16, false, &why) ||
         bad_rows(k, H, bf16, false, &why) || bad_rows(v, H, bf16, false, &why))
       return api_fail(M4MR_EINVAL, at + why);
     if (q->width != k->width) return api_fail(M4MR_EINVAL, at + "q and k disagree in width");

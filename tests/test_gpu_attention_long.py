@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mamba4_amd import linear_attention
+from mamba4_amd import linear_attention, linear_attention_step
 from tests.gpu_helpers import announce
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +72,25 @@ def test_many_rows_of_odd_widths(gpu_lib):
     want = linear_attention(pad(q, (0, 1)), pad(k, (0, 1)), pad(v, (0, 3)), g)
     assert torch.equal(got.output, want.output[..., :61])
     assert torch.equal(got.state, want.state[..., :63, :61])
+
+
+def test_the_largest_batches(gpu_lib):
+    """Just under the 2^32 threads of a launch, which the entry points allow."""
+    announce("largest batches")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+
+    def normal(*shape):
+        return torch.randn(*shape, device="cuda", generator=gen)
+
+    batch = 2**24 - 10
+    s, q, k, v = normal(batch, 1, 1, 1), *(normal(batch, 1, 1) for _ in range(3))
+    g = torch.tensor([-0.25], device="cuda")
+    r = linear_attention_step(s, q, k, v, g)
+    want = torch.exp(g) * s[..., 0] + k * v
+    assert torch.allclose(r.state[..., 0], want, rtol=1e-6, atol=1e-6)
+    assert torch.allclose(r.output, want * q, rtol=1e-6, atol=1e-6)
+    batch = 2**23 - 9
+    q, k, v = (normal(batch, 1, 1, 4) for _ in range(3))
+    r = linear_attention(q, k, v, g)
+    assert torch.allclose(r.state, k[:, 0, :, :, None] * v[:, 0, :, None, :], rtol=1e-5, atol=1e-5)
+    assert torch.allclose(r.output, (q * k).sum(-1, keepdim=True) * v, rtol=1e-4, atol=1e-4)

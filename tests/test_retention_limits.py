@@ -1,0 +1,67 @@
+"""Sizes that the retention entry points refuse, before any GPU work: M4MR_EINVAL with
+nothing launched, not a launch that fails after others.  What is refused has no
+workspace either."""
+
+import pytest
+
+from mamba4_amd import _lib
+
+DATA = 1 << 20  # stands for device memory: never read, every call here is refused
+HUGE = 1 << 60
+
+
+def _qkv(heads, widths, token=None):
+    """q, k, v of `heads` and `widths`, dense or with the token strides given."""
+    rows = []
+    for i, (h, w) in enumerate(zip(heads, widths)):
+        rows += [DATA, 0, h * w if token is None else token[i], w, h, w]
+    return _lib.pack_qkv(*rows)
+
+
+def _sizes(rows, bf16, B, T, H):
+    lib = _lib.load()
+    return (lib.m4rt_attention_workspace_bytes(rows, bf16, B, T, H),
+            lib.m4rt_attention_backward_workspace_bytes(rows, DATA, bf16, B, T, H, 1))
+
+
+def _forward(rows, bf16, B, T, H):
+    return _lib.load().m4rt_attention_forward(
+        rows, bf16, DATA, 0, None, None, 1.0, B, T, H, DATA, DATA, DATA, HUGE, None)
+
+
+def _backward(rows, bf16, B, T, H):
+    return _lib.load().m4rt_attention_backward(
+        rows, bf16, DATA, 0, None, None, 1.0, B, T, H, DATA, None, None, DATA, DATA, DATA, DATA,
+        None, DATA, HUGE, None)
+
+
+def _refused(rc, words):
+    assert rc == _lib.EINVAL
+    assert words in _lib.load().m4mr_last_error().decode()
+
+
+@pytest.mark.parametrize("p,blocks", [(64, 1), (128, 2)])
+def test_attention_forward_fits_a_launch(p, blocks):
+    """2^32 threads along x: 512 a block of 64 value columns of a (b, h)."""
+    most = 2**23 // blocks - 9
+    rows = _qkv((1, 1, 1), (64, 64, p))
+    _refused(_forward(rows, 1, most + 1, 5, 1), "too large")
+    assert _sizes(rows, 1, most + 1, 5, 1)[0] == 0
+    # (A call within the limits is not made here; it has a workspace where it needs one.)
+    odd = _qkv((1, 1, 1), (63, 63, p))
+    assert _sizes(odd, 1, most, 5, 1)[0] > 0 and _sizes(odd, 1, most + 1, 5, 1)[0] == 0
+
+
+@pytest.mark.parametrize("n,p,blocks", [(64, 64, 3), (128, 64, 5), (64, 128, 4), (128, 128, 6)])
+def test_attention_backward_fits_a_launch(n, p, blocks):
+    most = 2**23 // blocks - 9
+    rows = _qkv((1, 1, 1), (n, n, p))
+    _refused(_backward(rows, 1, most + 2, 5, 1), "too large")
+    assert _sizes(rows, 1, most, 5, 1)[1] > 0 and _sizes(rows, 1, most + 2, 5, 1)[1] == 0
+
+
+def test_attention_step_fits_a_launch():
+    """256 threads a (b, h)."""
+    rc = _lib.load().m4rt_attention_step(_qkv((1, 1, 1), (1, 1, 1)), 0, DATA, 0, None, 1.0, 2**24,
+                                         1, DATA, DATA, DATA, None)
+    _refused(rc, "too large")
