@@ -225,6 +225,20 @@ int run_packing(Packing& p, const Shape& s, hipStream_t st) {
   });
 }
 
+// A chunk's rows are addressed by 32-bit byte offsets.
+bool bad_stride(long token_stride, std::string* why) {
+  if (token_stride <= INT_MAX / (4 * la::C)) return false;
+  *why = "a token stride must be at least the width, and 64 of it below 2^31 bytes";
+  return true;
+}
+
+// The token stride of `r` as the kernels read it: of its copy, if it is copied.
+long read_stride(const m4rt_rows& r, int H, int bf16) {
+  const int piece = bf16 ? 8 : 4;
+  return rows_of(r, H, bf16).whole ? r.token_stride
+                                   : (long)r.heads * ((r.width + piece - 1) / piece * piece);
+}
+
 bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why) {
   if (!r->data) {
     *why = "a required pointer is NULL";
@@ -238,11 +252,9 @@ bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why
     *why = "rows must be aligned to their elements";
     return true;
   }
-  if (tokens && (r->token_stride < r->width || r->token_stride > INT_MAX / (4 * la::C))) {
-    *why = "a token stride must be at least the width, and 64 of it below 2^31 bytes";
-    return true;
-  }
-  return false;
+  if (!tokens) return false;
+  return bad_stride(r->token_stride < r->width ? LONG_MAX : r->token_stride, why) ||
+         bad_stride(read_stride(*r, H, bf16), why);
 }
 
 m4rt_rows dense(const void* data, int T, int H, int width) {
@@ -414,7 +426,9 @@ bool bad_attention(const m4rt_qkv* rows, int bf16, int B, int T, int H, bool bac
     *why = "q and k disagree in width";
     return true;
   }
-  return false;
+  // The backward reads d_output too, dense, or copied if its address asks for that.
+  const int piece = bf16 ? 8 : 4;
+  return backward && bad_stride((long)H * ((s->P + piece - 1) / piece * piece), why);
 }
 
 }  // namespace

@@ -65,3 +65,28 @@ def test_attention_step_fits_a_launch():
     rc = _lib.load().m4rt_attention_step(_qkv((1, 1, 1), (1, 1, 1)), 0, DATA, 0, None, 1.0, 2**24,
                                          1, DATA, DATA, DATA, None)
     _refused(rc, "too large")
+
+
+MOST = (2**31 - 1) // 256  # elements of a token stride: 64 of it in float32 below 2^31 bytes
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_rows_that_are_copied_keep_to_the_strides(bf16):
+    """Rows one element wide take a 16-byte piece in their copy."""
+    piece = 8 if bf16 else 4
+    most = MOST // piece
+    for width in (1, piece - 1):
+        ok, bad = (_qkv((1, 1, h), (8, 8, width), (8, 8, h * width)) for h in (most, most + 1))
+        assert _sizes(ok, bf16, 1, 2, most)[0] > 0
+        assert _sizes(bad, bf16, 1, 2, most + 1)[0] == 0
+        _refused(_forward(bad, bf16, 1, 2, most + 1), "token stride")
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_the_output_cotangent_keeps_to_the_strides(bf16):
+    """[B,T,H,P], dense, where the values have fewer heads."""
+    most = MOST // 128
+    rows = _qkv((1, 1, 1), (8, 8, 128))
+    assert _sizes(rows, bf16, 1, 2, most)[1] > 0
+    assert _sizes(rows, bf16, 1, 2, most + 1)[1] == 0
+    _refused(_backward(rows, bf16, 1, 2, most + 1), "token stride")
