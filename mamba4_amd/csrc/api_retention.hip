@@ -897,6 +897,13 @@ bool bad_embedding(long n, int rows, int width, std::string* why) {
   return false;
 }
 
+// Whether `blocks` of em::THREADS are more than a launch takes: under 2^32 threads.
+bool bad_blocks(long blocks, std::string* why) {
+  if (blocks < (1L << 32) / em::THREADS) return false;
+  *why = "problem too large";
+  return true;
+}
+
 int embedding_vec(int width, std::initializer_list<const void*> arrays) {
   uintptr_t at = 0;
   for (const void* p : arrays) at |= reinterpret_cast<uintptr_t>(p);
@@ -948,12 +955,15 @@ size_t embedding_plan(long n, int rows, int width, void* base, EmbeddingPlan* p)
   return c.used;
 }
 
+// Blocks whose threads take four pieces of `rows` rows each.
+long piece_blocks(long rows, int pieces) {
+  return (rows * pieces + 4 * em::THREADS - 1) / (4 * em::THREADS);
+}
+
 template <typename In, typename Out, int V>
 void start_lookup(const em::Lookup& a, hipStream_t st) {
-  const long items = a.n * (a.width / V);
   hipLaunchKernelGGL((em::lookup_kernel<In, Out, V>),
-                     dim3((unsigned)((items + 4 * em::THREADS - 1) / (4 * em::THREADS))),
-                     dim3(em::THREADS), 0, st, a);
+                     dim3((unsigned)piece_blocks(a.n, a.width / V)), dim3(em::THREADS), 0, st, a);
 }
 
 template <int V>
@@ -966,15 +976,14 @@ void launch_lookup(const em::Lookup& a, int table_bf16, int out_bf16, hipStream_
 }
 
 // Blocks of waves that take 64 pieces of a chunk's columns each.
-long chunk_blocks(const em::Sum& a, int V) {
+long chunk_blocks(long chunks, int pieces) {
   constexpr int waves = em::THREADS / 64;
-  return ((long)a.chunks * ((a.width / V + 63) / 64) + waves - 1) / waves;
+  return (chunks * ((pieces + 63) / 64) + waves - 1) / waves;
 }
 
 template <typename In, typename Out, int V>
 void start_sums(const em::Sum& a, hipStream_t st) {
-  const long vecs = a.width / V, sums = chunk_blocks(a, V);
-  const long zeros = (a.rows * vecs + 4 * em::THREADS - 1) / (4 * em::THREADS);
+  const long sums = chunk_blocks(a.chunks, a.width / V), zeros = piece_blocks(a.rows, a.width / V);
   hipLaunchKernelGGL((em::sum_kernel<In, Out, V>), dim3((unsigned)(sums + zeros)),
                      dim3(em::THREADS), 0, st, a, (unsigned)sums);
 }
@@ -990,7 +999,7 @@ void launch_sums(const em::Sum& a, int table_bf16, int out_bf16, hipStream_t st)
 
 template <int V>
 void launch_join(const em::Sum& a, int table_bf16, hipStream_t st) {
-  const dim3 grid((unsigned)chunk_blocks(a, V));
+  const dim3 grid((unsigned)chunk_blocks(a.chunks, a.width / V));
   if (table_bf16)
     hipLaunchKernelGGL((em::join_kernel<em::bf16_t, V>), grid, dim3(em::THREADS), 0, st, a);
   else
@@ -1024,6 +1033,7 @@ int m4rt_embedding_forward(const void* ids, int ids_int64, const void* table, in
     const em::Lookup a{ids, ids_int64, table, output, n, rows, width, scale};
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int vec = embedding_vec(width, {table, output});
+    if (bad_blocks(piece_blocks(n, width / vec), &why)) return api_fail(M4MR_EINVAL, at + why);
     return api_launch("embedding", st, [&] {
 #define EM_ARGS (a, table_bf16, output_bf16, st)
       EM_BY_VEC(vec, launch_lookup);
@@ -1055,6 +1065,9 @@ int m4rt_embedding_backward(const void* ids, int ids_int64, const void* d_output
     EmbeddingPlan p{};
     if (bad_workspace(workspace, workspace_bytes, embedding_plan(n, rows, width, workspace, &p),
                       &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    const int vec = embedding_vec(width, {d_output, d_table});
+    if (bad_blocks(chunk_blocks(p.chunks, width / vec) + piece_blocks(rows, width / vec), &why))
       return api_fail(M4MR_EINVAL, at + why);
     hipStream_t st = static_cast<hipStream_t>(stream);
     em::Sort sort{};
@@ -1094,7 +1107,6 @@ int m4rt_embedding_backward(const void* ids, int ids_int64, const void* d_output
     const int sorted = (p.passes - 1) & 1;
     const em::Sum sum{p.keys[sorted], p.tokens[sorted], p.present, d_output, d_table,
                       p.head, p.tail, n, rows, width, p.chunk, p.chunks, scale};
-    const int vec = embedding_vec(width, {d_output, d_table});
     rc = api_launch("embedding_sums", st, [&] {
 #define EM_ARGS (sum, table_bf16, output_bf16, st)
       EM_BY_VEC(vec, launch_sums);

@@ -90,3 +90,23 @@ def test_the_output_cotangent_keeps_to_the_strides(bf16):
     assert _sizes(rows, bf16, 1, 2, most)[1] > 0
     assert _sizes(rows, bf16, 1, 2, most + 1)[1] == 0
     _refused(_backward(rows, bf16, 1, 2, most + 1), "token stride")
+
+
+def _lookup(n, rows, width, out=DATA):
+    return _lib.load().m4rt_embedding_forward(DATA, 0, DATA, 1, n, rows, width, 1.0, out, 1, None)
+
+
+def _gradient(n, rows, width, table=DATA):
+    return _lib.load().m4rt_embedding_backward(DATA, 0, DATA, 1, n, rows, width, 1.0, table, 1,
+                                               DATA, HUGE, None)
+
+
+@pytest.mark.parametrize("width,shift,pieces", [(1024, 0, 128), (1024, 8, 256), (1001, 0, 1001)])
+def test_embedding_fits_a_launch(width, shift, pieces):
+    """2^32 threads, four pieces each: of 16 bytes, of 8 at such an address, of one
+    element in odd rows.  (The gradient's launch takes the table's rows so, beside the
+    chunks of the tokens.)"""
+    most = 4 * 2**32 // pieces
+    for call in (_lookup, _gradient):
+        n, rows = (most, 10) if call is _lookup else (10, most)
+        _refused(call(n, rows, width, DATA + shift), "too large")
