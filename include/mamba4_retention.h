@@ -59,8 +59,11 @@ typedef struct {
  * as three bfloat16 parts, all its bits, where the result is float32, and as two
  * where it is rounded to bfloat16.  A row's result does not depend on the batch
  * size.  A log decay of -infinity (or any that
- * underflows) drops what came before exactly.  An infinity or NaN in a row
- * that is present spreads to the outputs of its chunk of 64 tokens and after it.
+ * underflows) drops what came before exactly.  An infinity or NaN in a row that is
+ * present reaches what the recurrence carries it to, as NaN or an infinity: a value its
+ * column of the outputs from its token on, a key every column of them, a query its own
+ * output.  Others keep their bits.  (Float32 numbers beyond 3.39e38, which round to an
+ * infinite bfloat16, count as infinite.)
  */
 size_t m4rt_attention_workspace_bytes(const m4rt_qkv* rows, int bf16, int B, int T, int H);
 int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_decay, int per_token,
@@ -75,7 +78,9 @@ int m4rt_attention_forward(const m4rt_qkv* rows, int bf16, const float* log_deca
  * [B,T,heads,width] in the inputs' type, contiguous; d_log_decay float32,
  * [B,T,H] if per_token else [H], or NULL; d_initial [B,H,N,P], or NULL.
  * Gradients of shared heads are summed in float32 and rounded once.  `decays` of
- * the workspace's size: whether d_log_decay is wanted.
+ * the workspace's size: whether d_log_decay is wanted.  Infinities and NaN in q, k, v
+ * and d_output reach d_q, d_k and d_v as the recurrences of these carry them, and any
+ * of d_log_decay of their batch row and head.
  */
 size_t m4rt_attention_backward_workspace_bytes(const m4rt_qkv* rows, const void* d_output,
                                                int bf16, int B, int T, int H, int decays);

@@ -214,7 +214,8 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
     log_decay [B,T,H], or [H] for one constant a head (log of the factor that the
     state keeps; -inf drops it).  initial [B,H,N,P] is the state before the first token
     (zeros by default).  lengths [B] (integers): tokens from lengths[b] on are
-    absent, whatever their rows hold; their outputs and gradients are zero.
+    absent, whatever their rows hold; their outputs and gradients are zero.  An infinity or
+    NaN in a row that is present reaches its own and later outputs alone (possibly as NaN).
 
     Returns LinearAttentionResult(output [B,T,H,P] in the values' dtype, state
     [B,H,N,P] float32 after the last token).  A row's result does not depend on

@@ -253,6 +253,22 @@ __device__ __forceinline__ Frag<PLANES> rows(const bf16_t (&tile)[PLANES][NT][C 
   return f;
 }
 
+// A fragment with zeros in place of what is not finite.
+template <int PLANES>
+__device__ __forceinline__ Frag<PLANES> finite(Frag<PLANES> f) {
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i) {
+    u4 u = __builtin_bit_cast(u4, f.p[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
+      if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
+    }
+    f.p[i] = __builtin_bit_cast(b8, u);
+  }
+  return f;
+}
+
 // The eight values of a fragment, times eight weights, as computed planes.
 template <int MADE>
 __device__ __forceinline__ Frag<MADE> weighted(const Frag<1>& f, const float (&w)[8]) {
@@ -680,6 +696,132 @@ struct Block {
     }
   }
 
+  // The scores of the blocks ja and jb (the s-th pair from the strip) with their decays,
+  // zeros where the queries do not look.  With dots, a token's score with itself is kept
+  // out of them.
+  template <bool DOTS, typename Sh>
+  __device__ __forceinline__ void decayed(const Sh& sh, int s, int ja, int jb, int reached,
+                                          float near, int g, int r, f4 (&acc)[2],
+                                          float* diagonal) const {
+    if (s == 0) {
+      const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
+      const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * w + 4 * g]);
+      const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * w + 4 * g]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float gap = (ph - kh[q]) + (pl - kl[q]);
+        const int ahead = REV ? 4 * g + q - r : r - 4 * g - q;  // query - key
+        const float x = acc[0][q] * (__builtin_amdgcn_exp2f(REV ? -gap : gap) * R.intra);
+        acc[0][q] = ahead > (DOTS ? 0 : -1) ? x : 0.f;
+        if (DOTS && ahead == 0) *diagonal = x;
+      }
+    } else {
+      acc[0] *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * ja + 4 * g]);
+    }
+    // A block past the last one seen gives no scores.
+    const f4 far = near * *reinterpret_cast<const f4*>(&sh.far[w][16 * jb + 4 * g]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[1][q] = 2 * s + 1 < reached ? acc[1][q] * far[q] : 0.f;
+  }
+
+  // Whether any output of the wave is not finite.
+  __device__ __forceinline__ static bool unsound(const f4 (&out)[4]) {
+    f4 x = out[0] * 0.f;
+#pragma unroll
+    for (int pb = 1; pb < 4; ++pb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = fmaf(out[pb][q], 0.f, x[q]);
+    const float y = (x[0] + x[1]) + (x[2] + x[3]);
+    return __any(y != y);
+  }
+  // Whether any of the chunk's values is (each lane looks at a token's).
+  template <typename Sh>
+  __device__ __forceinline__ static bool spoiled(const Sh& sh, int lane) {
+    bool bad = false;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const u4 u = *reinterpret_cast<const u4*>(&sh.v[0][0][64 * lane + 8 * i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        bad |= (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
+    }
+    return __any(bad);
+  }
+
+  // The outputs of the wave's strip once more, the same products in the same order, where
+  // one of the chunk's values is not finite: it counts as zero, which keeps it from the
+  // tokens that do not look back on it (a score of zero times NaN is NaN), and then
+  // makes its column of the others' outputs NaN.  Few registers rather than fast: it
+  // costs other calls up to 2% (T32768 H16 N128 P128 271 -> 278 us, B16 T1024 H12
+  // forward and backward 233 -> 234).
+  template <int SP, bool DOTS>
+  __device__ __forceinline__ float attend_finite(const Shared<In, NT, SP>& sh, const Source& qs,
+                                                 int c, const Reach& d, int g, int r,
+                                                 f4 (&out)[4]) const {
+    const int strip = opaque_strip(), reached = seen(strip), t = 16 * w + r;
+    const Rsrc qr = chunk_rows(qs, c, have(c));
+    auto query = [&](int kk) {
+      return planes(load_piece(qr, t * qs.stride, 32 * kk + 8 * g, R.n, (const In*)nullptr));
+    };
+    auto apart = [] { asm volatile("" ::: "memory"); };
+#pragma unroll
+    for (int pb = 0; pb < 4; ++pb) out[pb] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int kk = 0; kk < 2 * NT; ++kk) {
+      const Frag<IN> qf = query(kk);
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb) {
+        const Frag<SP> sf[1] = {rows<SP, NT>(sh.s, 16 * pb, kk, g, r)};
+        mma(sf, qf, &out[pb]);
+        apart();
+      }
+    }
+    const float inter = R.inter * __shfl(d.inter, t);
+    const float near = R.intra * __shfl(d.near, t);
+#pragma unroll
+    for (int pb = 0; pb < 4; ++pb) out[pb] *= inter;
+    float diagonal = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (2 * s >= reached) continue;
+      const int ja = block(strip, 2 * s), jb = block(strip, 2 * s + 1);
+      f4 acc[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 1
+      for (int kk = 0; kk < 2 * NT; ++kk) {
+        const Frag<IN> qf = query(kk);
+        const Frag<IN> kf[2] = {rows<IN, NT>(sh.k, 16 * ja, kk, g, r),
+                                rows<IN, NT>(sh.k, 16 * jb, kk, g, r)};
+        mma(kf, qf, acc);
+      }
+      decayed<DOTS>(sh, s, ja, jb, reached, near, g, r, acc, &diagonal);
+      const float x[8] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3],
+                          acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
+      const Frag<SP> score = split8<SP>(x);
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb) {
+        const Frag<IN> vf[1] = {finite(columns<IN, 1>(sh.v, 0, ja, jb, pb, g, r))};
+        mma(vf, score, &out[pb]);
+        apart();
+      }
+    }
+#pragma unroll 1
+    for (int j = 0; j < C; ++j) {
+      const int ahead = REV ? j - t : t - j;
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb) {
+        const u2 u = *reinterpret_cast<const u2*>(
+            &sh.v[0][0][unit(j, 2 * pb + (g >> 1)) + 4 * (g & 1)]);
+        const f4 v{low(u[0]), high(u[0]), low(u[1]), high(u[1])};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float x = v[q] * 0.f;
+          if (ahead > (DOTS ? 0 : -1) && x != x) out[pb][q] = x;
+        }
+      }
+    }
+    return diagonal;
+  }
+
   template <int SP, bool DOTS>
   __device__ __forceinline__ void write_outputs(int c0, int c1, Shared<In, NT, SP>& sh) {
     const Source vs = source<In>(R.v, b, h), qs = source<In>(R.q, b, h);
@@ -695,6 +837,14 @@ struct Block {
                                      32 * kk + 8 * (lane >> 4), R.n, (const In*)nullptr);
       graw = decay(c, lane);
     };
+    auto fetch_e = [&](Quad<In> (&e)[4], int c, int g, int r) {
+      const Source es = source<In>(R.e, b, h);
+      const Rsrc er = chunk_rows(es, c, have(c));
+#pragma unroll
+      for (int pb = 0; pb < 4; ++pb)
+        e[pb] = load_quad(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p,
+                          (const In*)nullptr);
+    };
     fetch(REV ? c1 - 1 : c0);
     Reach d{};
     int known = -1;
@@ -708,15 +858,8 @@ struct Block {
 #pragma unroll
         for (int kk = 0; kk < 2 * NT; ++kk) qf[kk] = planes(qraw[kk]);
         if (unknown(c, &known)) d = reach<REV>(sh.ph[w], sh.pl[w], sh.far[w], graw, lane, w);
-        if constexpr (DOTS) {
-          // Before the next chunk's loads, so that their wait does not include those.
-          const Source es = source<In>(R.e, b, h);
-          const Rsrc er = chunk_rows(es, c, have(c));
-#pragma unroll
-          for (int pb = 0; pb < 4; ++pb)
-            e[pb] = load_quad(er, (16 * w + r) * es.stride, col0 + 16 * pb + 4 * g, R.p,
-                                     (const In*)nullptr);
-        }
+        // Before the next chunk's loads, so that their wait does not include those.
+        if constexpr (DOTS) fetch_e(e, c, g, r);
       }
       __syncthreads();
       if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
@@ -753,25 +896,7 @@ struct Block {
                                     rows<IN, NT>(sh.k, 16 * jb, kk, g, r)};
             mma(kf, qf[kk], acc);
           }
-          if (s == 0) {
-            const float ph = sh.ph[w][16 * w + r], pl = sh.pl[w][16 * w + r];
-            const f4 kh = *reinterpret_cast<const f4*>(&sh.ph[w][16 * w + 4 * g]);
-            const f4 kl = *reinterpret_cast<const f4*>(&sh.pl[w][16 * w + 4 * g]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float gap = (ph - kh[q]) + (pl - kl[q]);
-              const int ahead = REV ? 4 * g + q - r : r - 4 * g - q;  // query - key
-              const float x = acc[0][q] * (__builtin_amdgcn_exp2f(REV ? -gap : gap) * R.intra);
-              acc[0][q] = ahead > (DOTS ? 0 : -1) ? x : 0.f;
-              if (DOTS && ahead == 0) diagonal = x;
-            }
-          } else {
-            acc[0] *= near * *reinterpret_cast<const f4*>(&sh.far[w][16 * ja + 4 * g]);
-          }
-          // A block past the last one seen gives no scores.
-          const f4 far = near * *reinterpret_cast<const f4*>(&sh.far[w][16 * jb + 4 * g]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[1][q] = 2 * s + 1 < reached ? acc[1][q] * far[q] : 0.f;
+          decayed<DOTS>(sh, s, ja, jb, reached, near, g, r, acc, &diagonal);
           const float x[8] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3],
                               acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
           const Frag<SP> score = split8<SP>(x);
@@ -783,6 +908,12 @@ struct Block {
               vf[pb] = columns<IN, 1>(sh.v, 0, ja, jb, p0 + pb, g, r);
             mma(vf, score, &out[p0]);
           }
+        }
+        if (__builtin_expect(unsound(out), 0) && spoiled(sh, lane)) {
+          // (What is on its way is fetched again afterwards, so that it takes no registers.)
+          diagonal = attend_finite<SP, DOTS>(sh, qs, c, d, g, r, out);
+          if constexpr (DOTS) fetch_e(e, c, g, r);
+          if (it + 1 < c1 - c0) fetch(REV ? c - 1 : c + 1);
         }
         const int t = 16 * w + r;
         if constexpr (DOTS) {
