@@ -113,7 +113,7 @@ int m4rt_attention_step(const m4rt_qkv* rows, int bf16, const float* log_decay, 
  * output [M,L,C] in x's type: act(z), or z act(gate) with a gate [M,L,C] in x's
  * type (NULL: none).  stats: [M][G][2] float32, mean and 1 / sqrt(variance +
  * eps), for the gradient (NULL: not wanted).  Statistics and sums are float32, the
- * variance about the mean.
+ * variance about the mean.  A sample's bits do not depend on M.
  */
 size_t m4rt_norm_workspace_bytes(long M, int L, int C, int G, int bf16, int backward);
 int m4rt_norm_forward(const void* x, const float* weight, const float* bias, const void* gate,

@@ -677,7 +677,8 @@ struct NormPlan {
   int vec, pieces;  // pieces a lane holds; 0: position kernels
   dim3 grid;
   int threads, part_rows;
-  size_t sums;      // floats of the position kernels' partial statistics
+  bool whole;       // position kernels: in one launch
+  size_t sums;      // floats of their partial statistics
 };
 
 NormPlan norm_plan(long M, int L, int C, int G, int vec, gn::Norm* a) {
@@ -718,17 +719,23 @@ NormPlan norm_plan(long M, int L, int C, int G, int vec, gn::Norm* a) {
   a->span = a->subs > 1 ? 1 : std::min(G, gn::POS_THREADS / vecs);
   a->rows = a->subs > 1 ? 1 : std::max(1, std::min(L, gn::POS_THREADS / (vecs * a->span)));
   const int slots = (G * a->subs + a->span - 1) / a->span;
-  // Enough blocks for the card, each with some rows for each thread.
-  const long want = (2L * cus + M * slots - 1) / (M * slots);
-  a->blocks = (int)std::max<long>(1, std::min<long>(want, L / (8L * a->rows)));
-  if (a->subs > 1 && a->blocks == 1) a->blocks = std::min(L, 2);
-  const bool whole = a->blocks == 1 && a->subs == 1;
+  // Parts of the positions, of 8 rows a thread up to 8 parts and of 16 beyond: they
+  // depend on the sample alone, since the order of its sums does.  16 / 8 rows, forward
+  // us: M1 L4000 C64 bfloat16 (3 / 7 parts) 24 / 17, M512 L196 C512 float32 (3 / 6, one
+  // launch) 108 / 111, M8 L4000 C512 float32 (62 / 125) 39 / 51.
+  const long rows = L / a->rows;
+  a->parts = (int)std::max<long>(
+      1, std::min<long>((2L * cus + slots - 1) / slots, std::max(std::min(8L, rows / 8), rows / 16)));
+  if (a->subs > 1 && a->parts == 1) a->parts = std::min(L, 2);
+  // A block takes a part, or whole samples where those are blocks enough for the card.
+  p.whole = a->subs == 1 && (a->parts == 1 || M * slots >= 2L * cus);
+  const int blocks = p.whole ? 1 : a->parts;
   // Blocks walk over samples past these (the column sums have a part for each).
-  const long samples = std::min<long>(M, std::max(1L, 4L * cus / ((long)slots * a->blocks)));
-  p.grid = dim3(a->blocks, (unsigned)samples, slots);
+  const long samples = std::min<long>(M, std::max(1L, 4L * cus / ((long)slots * blocks)));
+  p.grid = dim3(blocks, (unsigned)samples, slots);
   p.threads = gn::POS_THREADS;
-  p.part_rows = (int)samples * a->blocks;
-  p.sums = whole ? 0 : (size_t)M * a->blocks * a->subs * G * 4;
+  p.part_rows = (int)samples * blocks;
+  p.sums = a->parts == 1 && a->subs == 1 ? 0 : (size_t)M * a->parts * a->subs * G * 4;
   return p;
 }
 
@@ -768,7 +775,7 @@ void launch_norm(const gn::Norm& a, const NormPlan& p, int bf16, int phase, hipS
 template <bool BWD>
 int run_norm(const gn::Norm& a, const NormPlan& p, int bf16, hipStream_t st) {
   const char* name = BWD ? "norm_backward" : "norm";
-  if (p.pieces || p.sums == 0)
+  if (p.pieces || p.whole)
     return api_launch(name, st, [&] { launch_norm<BWD>(a, p, bf16, gn::BOTH, st); });
   int rc = api_launch(BWD ? "norm_backward_sums" : "norm_sums", st,
                       [&] { launch_norm<BWD>(a, p, bf16, gn::SUMS, st); });

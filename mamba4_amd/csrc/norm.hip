@@ -396,8 +396,11 @@ __device__ __forceinline__ T team_join(T mine, T* fold, int first, int k, int te
 
 // A block: positions of one sample, the channels of `span` groups (or a part
 // of one).  Thread: one vector of channels and every rows-th position.  A group's
-// threads are consecutive: thread = (group, row, vector).  Blocks that hold whole
-// samples walk them, blockIdx.y and every gridDim.y-th after it.  Bound by memory: 8 x
+// threads are consecutive: thread = (group, row, vector).  Statistics are of `parts`
+// ranges of the positions, joined in the same order whether a block takes one part
+// (SUMS, then APPLY) or a whole sample (BOTH): a sample's bits do not depend on how
+// many there are.  Blocks walk over the samples, blockIdx.y and every gridDim.y-th
+// after it.  Bound by memory: 8 x
 // 4000 x 512 float32 16 + 27 us forward, 25 + 33 backward (65 MB an array).
 template <typename In, int V, bool BWD, int PHASE>
 __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
@@ -412,8 +415,10 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
   const int v = sub * POS_THREADS + j;
   const bool member = local < a.span && group < a.G;
   const bool on = member && v < a.vecs;
-  const int per = (a.L + a.blocks - 1) / a.blocks;
-  const int l0 = blockIdx.x * per, l1 = min(a.L, l0 + per);
+  const int per = (a.L + a.parts - 1) / a.parts;
+  const int part0 = PHASE == BOTH ? 0 : blockIdx.x, part1 = PHASE == BOTH ? a.parts : part0 + 1;
+  auto begin = [&](int part) { return (int)min((long)a.L, (long)part * per); };
+  const int l0 = begin(part0), l1 = begin(part1);
   const long column = (long)group * a.D + v * V;
   const float count = (float)a.L * a.D;
   float w[V], bias[V], dw[V], db[V];
@@ -426,53 +431,58 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
   constexpr int AHEAD = 4;
   for (long m = blockIdx.y; m < a.M; m += gridDim.y) {
     const long at = m * a.L * a.C + column;
-    // Partial sums of unit u from block b: [m][b][sub][group][4].
-    auto slot = [&](int b, int s) {
-      return a.sums + (((m * a.blocks + b) * a.subs + s) * a.G + group) * 4;
+    // Partial sums: [m][part][sub][group][4].
+    auto slot = [&](int part, int s) {
+      return a.sums + (((m * a.parts + part) * a.subs + s) * a.G + group) * 4;
     };
     float mean = 0.f, inv = 0.f;
 
     if constexpr (!BWD) {
       Moments mine{0.f, 0.f, 0.f};
       if constexpr (PHASE != APPLY) {
-        if (on)
-          for (int l = l0 + rr; l < l1; l += AHEAD * a.rows) {
-            Vec<In, V> x[AHEAD];
-            int have = 0;
+        for (int part = part0; part < part1; ++part) {
+          const int end = begin(part + 1);
+          mine = Moments{0.f, 0.f, 0.f};
+          if (on)
+            for (int l = begin(part) + rr; l < end; l += AHEAD * a.rows) {
+              Vec<In, V> x[AHEAD];
+              int have = 0;
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-              x[i].zero();
-              if (l + i * a.rows < l1) {
-                x[i].load(a.x, at + (long)(l + i * a.rows) * a.C);
-                have = i + 1;
+              for (int i = 0; i < AHEAD; ++i) {
+                x[i].zero();
+                if (l + i * a.rows < end) {
+                  x[i].load(a.x, at + (long)(l + i * a.rows) * a.C);
+                  have = i + 1;
+                }
               }
+              float s = 0.f, q = 0.f;
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += x[i].get(e);
+              const float c = s / (float)(have * V);
+#pragma unroll
+              for (int i = 0; i < AHEAD; ++i)
+                if (i < have)
+#pragma unroll
+                  for (int e = 0; e < V; ++e) q = fmaf(x[i].get(e) - c, x[i].get(e) - c, q);
+              mine = join(mine, Moments{(float)(have * V), c, q});
             }
-            float s = 0.f, q = 0.f;
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-              for (int e = 0; e < V; ++e) s += x[i].get(e);
-            const float c = s / (float)(have * V);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-              if (i < have)
-#pragma unroll
-                for (int e = 0; e < V; ++e) q = fmaf(x[i].get(e) - c, x[i].get(e) - c, q);
-            mine = join(mine, Moments{(float)(have * V), c, q});
-          }
-        mine = team_join(mine, folded, first, k, team, member);
-        if constexpr (PHASE == SUMS) {
-          if (member && k == 0) {
-            float* s = slot(blockIdx.x, sub);
+          mine = team_join(mine, folded, first, k, team, member);
+          if ((PHASE == SUMS || a.parts > 1) && member && k == 0) {
+            float* s = slot(part, sub);
             s[0] = mine.n;
             s[1] = mine.mean;
             s[2] = mine.m2;
           }
-          continue;
         }
-      } else {
+        if constexpr (PHASE == SUMS) continue;
+      }
+      if (PHASE == APPLY || a.parts > 1) {
+        if (PHASE == BOTH) __syncthreads();  // the slots are written
+        mine = Moments{0.f, 0.f, 0.f};
         if (member)
-          for (int b = k; b < a.blocks * a.subs; b += team) {
+          for (int b = k; b < a.parts * a.subs; b += team) {
             const float* s = slot(b / a.subs, b % a.subs);
             mine = join(mine, Moments{s[0], s[1], s[2]});
           }
@@ -517,57 +527,62 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
       }
       Pair mine{0.f, 0.f};
       if constexpr (PHASE != APPLY) {
-        float dws[V], dbs[V];  // of this sample
+        for (int part = part0; part < part1; ++part) {
+          const int end = begin(part + 1);
+          mine = Pair{0.f, 0.f};
+          float dws[V], dbs[V];  // of this part
 #pragma unroll
-        for (int e = 0; e < V; ++e) dws[e] = dbs[e] = 0.f;
-        if (on)
-          for (int l = l0 + rr; l < l1; l += AHEAD * a.rows) {
-            Vec<In, V> x[AHEAD], g[AHEAD], d[AHEAD];
+          for (int e = 0; e < V; ++e) dws[e] = dbs[e] = 0.f;
+          if (on)
+            for (int l = begin(part) + rr; l < end; l += AHEAD * a.rows) {
+              Vec<In, V> x[AHEAD], g[AHEAD], d[AHEAD];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-              if (l + i * a.rows < l1) {
-                const long p = at + (long)(l + i * a.rows) * a.C;
-                x[i].load(a.x, p);
-                d[i].load(a.dy, p);
-                if (a.gate) g[i].load(a.gate, p);
-              }
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-              if (l + i * a.rows < l1) {
-                float n[V], u[V], y[V], slope[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                  n[e] = (x[i].get(e) - mean) * inv;
-                  u[e] = a.gate ? g[i].get(e) : fmaf(n[e], w[e], bias[e]);
+              for (int i = 0; i < AHEAD; ++i)
+                if (l + i * a.rows < end) {
+                  const long p = at + (long)(l + i * a.rows) * a.C;
+                  x[i].load(a.x, p);
+                  d[i].load(a.dy, p);
+                  if (a.gate) g[i].load(a.gate, p);
                 }
-                activate<V>(u, a.act, y, slope);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                  const float dz = d[i].get(e) * (a.gate ? y[e] : slope[e]);
-                  dws[e] = fmaf(dz, n[e], dws[e]);
-                  dbs[e] += dz;
+              for (int i = 0; i < AHEAD; ++i)
+                if (l + i * a.rows < end) {
+                  float n[V], u[V], y[V], slope[V];
+#pragma unroll
+                  for (int e = 0; e < V; ++e) {
+                    n[e] = (x[i].get(e) - mean) * inv;
+                    u[e] = a.gate ? g[i].get(e) : fmaf(n[e], w[e], bias[e]);
+                  }
+                  activate<V>(u, a.act, y, slope);
+#pragma unroll
+                  for (int e = 0; e < V; ++e) {
+                    const float dz = d[i].get(e) * (a.gate ? y[e] : slope[e]);
+                    dws[e] = fmaf(dz, n[e], dws[e]);
+                    dbs[e] += dz;
+                  }
                 }
-              }
+            }
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            mine.a = fmaf(w[e], dbs[e], mine.a);
+            mine.b = fmaf(w[e], dws[e], mine.b);
+            dw[e] += dws[e];
+            db[e] += dbs[e];
           }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          mine.a = fmaf(w[e], dbs[e], mine.a);
-          mine.b = fmaf(w[e], dws[e], mine.b);
-          dw[e] += dws[e];
-          db[e] += dbs[e];
-        }
-        mine = team_join(mine, pairs, first, k, team, member);
-        if constexpr (PHASE == SUMS) {
-          if (member && k == 0) {
-            float* s = slot(blockIdx.x, sub);
+          mine = team_join(mine, pairs, first, k, team, member);
+          if ((PHASE == SUMS || a.parts > 1) && member && k == 0) {
+            float* s = slot(part, sub);
             s[0] = mine.a;
             s[1] = mine.b;
           }
-          continue;
         }
-      } else {
+        if constexpr (PHASE == SUMS) continue;
+      }
+      if (PHASE == APPLY || a.parts > 1) {
+        if (PHASE == BOTH) __syncthreads();  // the slots are written
+        mine = Pair{0.f, 0.f};
         if (member)
-          for (int b = k; b < a.blocks * a.subs; b += team) {
+          for (int b = k; b < a.parts * a.subs; b += team) {
             const float* s = slot(b / a.subs, b % a.subs);
             mine = join(mine, Pair{s[0], s[1]});
           }
@@ -620,7 +635,7 @@ __global__ __launch_bounds__(POS_THREADS) void norm_positions_kernel(Norm a) {
       if (on && rr == 0) {
         Pair s = pairs[tid];
         for (int i = 1; i < a.rows; ++i) s = join(s, pairs[tid + i * vecs]);
-        float* p = a.part + ((long)blockIdx.y * a.blocks + blockIdx.x) * 2 * a.C + column + e;
+        float* p = a.part + ((long)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.C + column + e;
         p[0] = s.a;
         p[a.C] = s.b;
       }

@@ -90,7 +90,7 @@ def group_norm(x, groups, weight=None, bias=None, *, gate=None, activation="none
 
     bfloat16 x (with a bfloat16 gate) is read and written as bfloat16; any other
     dtype is computed in float32 and returned in x's dtype.  Statistics are
-    float32 either way.
+    float32 either way.  A sample's result does not depend on how many there are.
     """
     _same_device(x, weight, bias, gate)
     if activation not in ACTIVATIONS:
