@@ -58,7 +58,7 @@ typedef struct {
  * and multiplied again (the scores, the state, the weighted keys) enters the products
  * as three bfloat16 parts, all its bits, where the result is float32, and as two
  * where it is rounded to bfloat16.  A row's result does not depend on the batch
- * size.  A log decay of -infinity (or any that
+ * size (at the same T).  A log decay of -infinity (or any that
  * underflows) drops what came before exactly.  An infinity or NaN in a row that is
  * present reaches what the recurrence carries it to, as NaN or an infinity: a value its
  * column of the outputs from its token on, a key every column of them, a query its own

@@ -218,8 +218,8 @@ def linear_attention(queries, keys, values, log_decay, *, initial=None, lengths=
     NaN in a row that is present reaches its own and later outputs alone (possibly as NaN).
 
     Returns LinearAttentionResult(output [B,T,H,P] in the values' dtype, state
-    [B,H,N,P] float32 after the last token).  A row's result does not depend on
-    the batch it is in.
+    [B,H,N,P] float32 after the last token).  A row's result does not depend on the
+    batch size (nor, beyond rounding, on a longer T of the rows beside it).
     """
     device = _same_device(queries, keys, values, log_decay, initial, lengths)
     heads, q, k, v = _model_rows("linear_attention", queries, keys, values, 4)

@@ -95,10 +95,11 @@ int tiles_of(int width) { return (width + la::TILE - 1) / la::TILE; }
 
 // Chunks of a segment, by the chunk-tiles of one row (`blocks` tiles a head):
 // 4 while a segment is latency, up to 16 where the segments' states are traffic.
-// It does not depend on the batch (segments decide the bits).  Forward, 4 / 8 / 16,
-// whole calls of an earlier form of the kernels (24 and 275 now, as chosen):
-// T2000 H12 N64 P128 34 / 37 / 58 us, T32768 H16 N128 P128 342 / 299 / 292.  Longer
-// ones only keep the segments within a launch's y blocks (past 67M tokens).
+// It does not depend on the batch size (segments decide the bits).  Forward calls,
+// bfloat16, 4 / 8 / 16: B1 T2000 H12 N64 P128 29 / 37 / 62 us, B1 T4200 H32 N128 P128
+// 101 / 96 / 105, B1 T32768 H16 N128 P128 390 / 334 / 319; forward and backward, B1
+// T2100 and T4200 H32 N128 P128 206 / 193 / 252 and 412 / 351 / 343.  Longer ones only
+// keep the segments within a launch's y blocks (past 67M tokens).
 int segment(const Shape& s, int blocks) {
   const long each = (long)s.chunks() * s.H * blocks / 768;
   int seg = each >= 16 ? 16 : each >= 8 ? 8 : 4;
@@ -133,10 +134,10 @@ bool bad_shape(const Shape& s, int blocks, int threads, std::string* why) {
 // then carried, then all walked at once) instead of walked from end to end.  A walk
 // takes a chunk's latency a chunk while the card has a block a compute unit, and the
 // chunks' throughput beyond; a split run three launches, a segment's latency twice,
-// and 1.7 times the throughput.  Walk / split in us: forward bfloat16 N64 P128
-// H12 B4 T2000 68 / 46, B8 T1024 37 / 46, B16 T1024 53 / 78; float32 B4 T1024 69 / 51,
-// B8 T1024 72 / 81; backward float32 N64 P64 H8 B8 T1000 104 / 79.  M4RT_ATTENTION =
-// "walk" or "split" overrides the choice; the bits are the same.
+// and 1.7 times the throughput.  Walk / split in us, calls: forward bfloat16 N64 P128
+// H12 B4 T2000 73 / 49, B8 T1024 40 / 47, B16 T1024 57 / 79; float32 B4 T1024 78 / 56,
+// B8 T1024 80 / 83; forward and backward float32 N64 P64 H8 B8 T1000 191 / 153.
+// M4RT_ATTENTION = "walk" or "split" overrides the choice; the bits are the same.
 bool attention_splits(const Shape& s, int blocks) {
   if (segments(s, blocks) < 2) return false;
   if (const char* mode = std::getenv("M4RT_ATTENTION")) {
@@ -939,9 +940,10 @@ size_t embedding_plan(long n, int rows, int width, void* base, EmbeddingPlan* p)
   p->tile = 1024;
   while ((n + p->tile - 1) / p->tile > 128) p->tile *= 2;
   p->tiles = (int)((n + p->tile - 1) / p->tile);
-  // Short chunks fill the card, long ones leave fewer parts to join: sums and
-  // joins of 16,384 tokens of 768 23 + 11 us in chunks of 16, 53 + 4 in 64s; of
-  // 131,071 tokens of 1,024 120 + 66 and 118 + 17 us.
+  // Short chunks fill the card, long ones leave fewer parts to join: sums + joins in
+  // us in chunks of 16 and 64, of tokens of 768 into a float32 table: 4,096 22 + 8 and
+  // 30 + 7, 16,384 24 + 12 and 29 + 8, 32,768 27 + 19 and 28 + 9; of 1,024 bfloat16:
+  // 65,536 39 + 32 and 38 + 12, 131,071 84 + 64 and 82 + 20.
   p->chunk = n >= 65536 ? 64 : 16;
   p->chunks = (int)((n + p->chunk - 1) / p->chunk);
   Carver c{static_cast<char*>(base)};

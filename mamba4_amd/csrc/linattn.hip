@@ -993,8 +993,10 @@ __device__ __forceinline__ int chunks_of(const Args& a, int* c0, int* c1) {
 }
 
 // Eight waves a block: two blocks a compute unit need no more than 128 registers
-// (float32 with wide keys: one block, by its LDS).  Bound by the issue of vector and
-// matrix instructions: B16 T1024 H12 N64 P128 bfloat16 61 us, its 151 MB 30 us.
+// (float32 with wide keys: one block, by its LDS).  That costs spills: 8 registers a lane
+// of bfloat16 with wide keys, 14 of float32 with narrow ones.  Bound by the issue of
+// vector and matrix instructions, 64 and 20% of a busy unit's cycles: B16 T1024 H12 N64
+// P128 bfloat16 62 us, its 151 MB 30 us.
 constexpr int waves_per_simd(int bytes, int nt) { return bytes == 4 && nt == 2 ? 2 : 4; }
 
 template <typename In, int NT>
@@ -1011,7 +1013,9 @@ __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NT)) void a
 
 // The gradients: dQ forward in time, dK and dV in reverse; NP and NN 64s of the
 // value and key widths, DOTS with what the decays' gradient needs.  Bound as the
-// forward: B16 T1024 H12 N64 P128 bfloat16 178 us.
+// forward (69 and 25%): B16 T1024 H12 N64 P128 bfloat16 175 us.  Float32 with narrow
+// widths spills most, 113 registers a lane and 135 with DOTS, and its waves wait 61% of
+// their cycles: B8 T1000 H8 N64 P64 53 us.
 template <typename In, int NP, int NN, bool DOTS>
 __global__ __launch_bounds__(128 * WAVES, waves_per_simd(sizeof(In), NP > NN ? NP : NN)) void
 attention_backward_kernel(Args a) {
@@ -1034,8 +1038,9 @@ attention_backward_kernel(Args a) {
       .template outputs<SV, false>(seg, c0, c1, sh.n);
 }
 
-// Split runs: the segments' own states, of all roles.  T32768 H16 N128 P128 bfloat16
-// with keys shared by four heads 78 us, 402 MB of loads, 168 MB of them from memory.
+// Split runs: the segments' own states, of all roles.  Bound by issue (VALU 74, MFMA 34%
+// of the busy cycles): T32768 H16 N128 P128 bfloat16 with keys shared by four heads 76
+// us, 402 MB of loads of 168 MB of rows.
 template <typename In, int NT>
 __global__ __launch_bounds__(64 * WAVES) void attention_states_kernel(Args a) {
   __shared__ Shared<In, NT, 0> sh;
@@ -1204,8 +1209,8 @@ __global__ void share_sum_kernel(const float* part, long tokens, int heads, int 
 }
 
 // Rows that are no whole 16-byte pieces (by width, stride or address), copied to
-// padded ones; a thread writes one piece.  Bound by memory: 500 MB in 134 us at B16
-// T1024 H12 N63 P127, forward and backward, whose attention then takes 302 us.  (Read
+// padded ones; a thread writes one piece.  Bound by memory: 500 MB in 132 us at B16
+// T1024 H12 N63 P127, forward and backward, whose attention then takes 310 us.  (Read
 // an element at a time where they are used, such rows took 587 us.)
 template <typename In>
 __global__ __launch_bounds__(256) void pack_kernel(Pack a) {
