@@ -193,6 +193,9 @@ struct Packing {
   long most = 0;  // pieces of the largest copy
 };
 
+// The token stride of dense rows; of one token, whose stride is no stride, the width.
+long token_stride(int T, int heads, int width) { return T > 1 ? (long)heads * width : width; }
+
 void pack_rows(Carver& c, const Shape& s, la::Rows* r, int heads, Packing* out) {
   if (r->whole) return;
   const int piece = s.bf16 ? 8 : 4, i = out->count++;
@@ -203,7 +206,7 @@ void pack_rows(Carver& c, const Shape& s, la::Rows* r, int heads, Packing* out) 
   out->a.heads[i] = heads;
   out->a.padded[i] = width;
   out->most = std::max(out->most, (long)(rows * (width / piece)));
-  *r = la::Rows{out->a.to[i], (long)s.T * heads * width, (long)heads * width, width,
+  *r = la::Rows{out->a.to[i], (long)s.T * heads * width, token_stride(s.T, heads, width), width,
                 r->share, width, 1};
 }
 
@@ -234,13 +237,15 @@ bool bad_stride(long token_stride, std::string* why) {
 }
 
 // The token stride of `r` as the kernels read it: of its copy, if it is copied.
-long read_stride(const m4rt_rows& r, int H, int bf16) {
+long read_stride(const m4rt_rows& r, int T, int H, int bf16) {
   const int piece = bf16 ? 8 : 4;
-  return rows_of(r, H, bf16).whole ? r.token_stride
-                                   : (long)r.heads * ((r.width + piece - 1) / piece * piece);
+  return rows_of(r, H, bf16).whole
+             ? r.token_stride
+             : token_stride(T, r.heads, (r.width + piece - 1) / piece * piece);
 }
 
-bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why) {
+// T: tokens, or zero for rows without that axis.
+bool bad_rows(const m4rt_rows* r, int H, int bf16, int T, std::string* why) {
   if (!r->data) {
     *why = "a required pointer is NULL";
     return true;
@@ -253,13 +258,13 @@ bool bad_rows(const m4rt_rows* r, int H, int bf16, bool tokens, std::string* why
     *why = "rows must be aligned to their elements";
     return true;
   }
-  if (!tokens) return false;
+  if (T == 0) return false;
   return bad_stride(r->token_stride < r->width ? LONG_MAX : r->token_stride, why) ||
-         bad_stride(read_stride(*r, H, bf16), why);
+         bad_stride(read_stride(*r, T, H, bf16), why);
 }
 
 m4rt_rows dense(const void* data, int T, int H, int width) {
-  return m4rt_rows{data, (long)T * H * width, (long)H * width, width, H, width};
+  return m4rt_rows{data, (long)T * H * width, token_stride(T, H, width), width, H, width};
 }
 
 int wide_keys(const la::Args& a) {
@@ -422,14 +427,14 @@ bool bad_attention(const m4rt_qkv* rows, int bf16, int B, int T, int H, bool bac
   if (bad_shape(*s, backward ? backward_tiles(*s) : tiles_of(s->P), 128 * la::WAVES, why))
     return true;
   for (const m4rt_rows* r : {&rows->q, &rows->k, &rows->v})
-    if (bad_rows(r, H, bf16, true, why)) return true;
+    if (bad_rows(r, H, bf16, T, why)) return true;
   if (rows->q.width != rows->k.width) {
     *why = "q and k disagree in width";
     return true;
   }
   // The backward reads d_output too, dense, or copied if its address asks for that.
   const int piece = bf16 ? 8 : 4;
-  return backward && bad_stride((long)H * ((s->P + piece - 1) / piece * piece), why);
+  return backward && bad_stride(token_stride(T, H, (s->P + piece - 1) / piece * piece), why);
 }
 
 }  // namespace
@@ -617,8 +622,8 @@ int m4rt_attention_step(const m4rt_qkv* rows, int bf16, const float* log_decay, 
     const m4rt_rows *q = &rows->q, *k = &rows->k, *v = &rows->v;
     const Shape s{B, 1, H, q->width, v->width, bf16};
     std::string why;
-    if (bad_shape(s, 1, la::STEP_THREADS, &why) || bad_rows(q, H, bf16, false, &why) ||
-        bad_rows(k, H, bf16, false, &why) || bad_rows(v, H, bf16, false, &why))
+    if (bad_shape(s, 1, la::STEP_THREADS, &why) || bad_rows(q, H, bf16, 0, &why) ||
+        bad_rows(k, H, bf16, 0, &why) || bad_rows(v, H, bf16, 0, &why))
       return api_fail(M4MR_EINVAL, at + why);
     if (q->width != k->width) return api_fail(M4MR_EINVAL, at + "q and k disagree in width");
     if (!log_decay || !state || !new_state || !output)

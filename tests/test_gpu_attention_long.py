@@ -202,3 +202,23 @@ def test_strided_rows_of_a_long_sequence(gpu_lib):
     out, state = oracle.attention(rows[:, :, 0], rows[:, :, 1], rows[:, :, 2], g)
     assert normwise(host(r.output), out) <= 2e-5
     assert normwise(host(r.state), state) <= 2e-5
+
+
+@pytest.mark.parametrize("p", [128, 127])
+def test_one_token_of_many_heads(gpu_lib, p):
+    """More heads than a token stride could hold: o = (q . k) v for each, the gradients
+    of the shared rows sums over the heads (70,000 terms, sqrt(n) 2^-24 = 2e-5)."""
+    announce(f"linear attention one token P{p}")
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    heads = 70_000
+    q, k = (torch.randn(1, 1, h, 8, device="cuda", generator=gen).requires_grad_()
+            for h in (1, heads))
+    v = torch.randn(1, 1, 1, p, device="cuda", generator=gen).requires_grad_()
+    d = torch.randn(1, 1, heads, p, device="cuda", generator=gen)
+    r = linear_attention(q, k, v, torch.zeros(heads, device="cuda"))
+    want = (q.double() * k.double()).sum(-1, keepdim=True) * v.double()
+    assert (r.output.double() - want).abs().max() <= 1e-5 * want.abs().max()
+    grads = torch.autograd.grad(r.output, (q, k, v), d)
+    expected = torch.autograd.grad(want, (q, k, v), d.double())
+    for a, e in zip(grads, expected):
+        assert (a.double() - e.double()).abs().max() <= 5e-5 * e.double().abs().max()

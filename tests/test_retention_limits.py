@@ -110,3 +110,14 @@ def test_embedding_fits_a_launch(width, shift, pieces):
     for call in (_lookup, _gradient):
         n, rows = (most, 10) if call is _lookup else (10, most)
         _refused(call(n, rows, width, DATA + shift), "too large")
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_one_token_has_no_stride(bf16):
+    """However many heads: rows, copies and the cotangent of one token are within reach."""
+    heads = MOST // 8 + 1
+    for widths in ((8, 8, 128), (7, 7, 127)):
+        rows = _qkv((1, 1, heads), widths, token=widths)
+        assert _sizes(rows, bf16, 1, 1, heads)[1] > 0
+        wide = _qkv((1, 1, heads), widths)
+        assert _sizes(wide, bf16, 1, 2, heads)[1] == 0
