@@ -1,0 +1,100 @@
+/*
+ * mamba4_selective.h -- C ABI of the MI355X (gfx950) selective state space
+ * layer's operators: the selective scan over prompts and training batches, its
+ * gradient, and its step for single tokens (the library that also holds
+ * mamba4_memread.h).
+ *
+ * Plain pointers and sizes only; every buffer is on the device and owned by
+ * the caller.  `stream` is a hipStream_t passed as void* (NULL = the null
+ * stream).  No function allocates, frees or synchronises.  Return values are
+ * those of mamba4_memread.h (M4MR_OK, M4MR_EINVAL with nothing launched,
+ * M4MR_EHIP); m4mr_last_error() gives the message.
+ */
+#ifndef MAMBA4_SELECTIVE_H
+#define MAMBA4_SELECTIVE_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Most states of a channel. */
+#define M4SL_MAX_STATES 64
+/* Tokens between the states that a forward call keeps for the backward. */
+#define M4SL_TILE 16
+
+/*
+ * Rows [B,T,...] with unit stride along the channels (or states) and strides in
+ * elements along the others (the token stride is not read by the steps).
+ */
+typedef struct {
+  const void* data;
+  long batch_stride, token_stride;
+} m4sl_rows;
+
+/*
+ * The selective scan: every channel d of D has N states,
+ *   s_t = softplus(delta_t + delta_bias) if `softplus` is not zero, else
+ *         delta_t + delta_bias
+ *   h_t[n] = exp(s_t a[d,n]) h_{t-1}[n] + s_t b_t[g,n] x_t
+ *   y_t = sum over n of c_t[g,n] h_t[n] + skip x_t,    out_t = y_t silu(gate_t)
+ * x, delta, gate [B,T,D] and b, c [B,T,G,N] in float32, or bfloat16 if `bf16` is
+ * not zero; G divides D and channel d reads group g = d / (D / G).  a [D,N],
+ * skip [D], delta_bias [D] float32.  gate.data, skip, delta_bias: NULL for none.
+ */
+typedef struct {
+  m4sl_rows x, delta, gate, b, c;
+  long b_group_stride, c_group_stride;
+  const float *a, *skip, *delta_bias;
+  int B, T, D, G, N, bf16, softplus;
+} m4sl_scan;
+
+/* Floats of the states that the forward keeps for the backward. */
+long m4sl_scan_kept_floats(const m4sl_scan* scan);
+
+/*
+ * initial [B,D,N] float32, or NULL for zeros.  lengths [B] int32, or NULL: tokens at
+ * lengths[b] and after are absent (their rows are not read into any result, their
+ * output is zero; lengths outside 0..T are clamped).  output [B,T,D] in x's type;
+ * state [B,D,N] float32, after the last token.  kept: for the backward, or NULL.
+ *
+ * Steps, decays, states and sums are float32; each result is rounded once.  A long
+ * sequence of a small batch is cut into segments whose states are formed first, so
+ * that a row's result may depend on the batch size, by rounding.
+ */
+size_t m4sl_scan_workspace_bytes(const m4sl_scan* scan);
+int m4sl_scan_forward(const m4sl_scan* scan, const float* initial, const int* lengths,
+                      void* output, float* state, float* kept, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * Its gradient, from the cotangents d_output [B,T,D] in x's type and d_state
+ * [B,D,N] (NULL: zero) and what the forward kept.  Gradients: x, delta, gate
+ * [B,T,D] and b, c [B,T,G,N] in the inputs' type, contiguous; a, skip, delta_bias
+ * and initial float32.  gate, skip, delta_bias, initial and a: NULL if not wanted.
+ * Sums over tokens, channels and states are float32 in a fixed order.
+ */
+typedef struct {
+  void *x, *delta, *gate, *b, *c;
+  float *a, *skip, *delta_bias, *initial;
+} m4sl_scan_grads;
+size_t m4sl_scan_backward_workspace_bytes(const m4sl_scan* scan);
+int m4sl_scan_backward(const m4sl_scan* scan, const int* lengths, const void* d_output,
+                       const float* d_state, const float* kept, const m4sl_scan_grads* grads,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One token (T is not read): state [B,D,N] float32 to new_state (which may be state
+ * itself: in place) and output [B,D] in x's type.  active [B] bytes, or NULL: a row
+ * whose byte is zero keeps its state and its output is zero.
+ */
+int m4sl_scan_step(const m4sl_scan* scan, const uint8_t* active, const float* state,
+                   float* new_state, void* output, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif

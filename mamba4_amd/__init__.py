@@ -10,7 +10,8 @@ implemented by hand-written HIP kernels behind the C ABI in
 and the order head's gated scan (``order_memory_chunked``, ``order_memory``;
 lm/models/mamba4.py:46-95).  Beside them, the retention layer's operators
 (``linear_attention``, ``linear_attention_step``, ``group_norm``,
-``embedding``).
+``embedding``) and the selective layer's (``selective_scan``,
+``selective_scan_step``).
 """
 
 from mamba4_amd.attention import (  # noqa: F401
@@ -42,6 +43,12 @@ from mamba4_amd.embedding import embedding  # noqa: F401
 from mamba4_amd.flashmamba import mamba3_fused  # noqa: F401
 from mamba4_amd.norm import group_norm  # noqa: F401
 from mamba4_amd.order import order_memory, order_memory_chunked  # noqa: F401
+from mamba4_amd.selective import (  # noqa: F401
+    SelectiveScanResult,
+    selective_scan,
+    selective_scan_step,
+    selective_scan_step_,
+)
 
 __all__ = [
     "LinearAttentionResult",
@@ -50,6 +57,7 @@ __all__ = [
     "MixerRead",
     "SOLVERS",
     "SelectiveResult",
+    "SelectiveScanResult",
     "SelectiveState",
     "embedding",
     "linear_attention",
@@ -67,5 +75,8 @@ __all__ = [
     "selective_diagnostics",
     "selective_gaussian_memory",
     "selective_initial_state",
+    "selective_scan",
+    "selective_scan_step",
+    "selective_scan_step_",
     "spd_solve",
 ]

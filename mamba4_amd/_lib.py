@@ -13,7 +13,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = os.path.join(HERE, "libmamba4_memread.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "mamba4_memread.h")
 HEADERS = [HEADER] + [os.path.join(os.path.dirname(HERE), "include", name)
-                      for name in ("mamba3_scan.h", "mamba4_retention.h")]
+                      for name in ("mamba3_scan.h", "mamba4_retention.h",
+                                   "mamba4_selective.h")]
 
 EINVAL = 1
 EHIP = 2
@@ -66,6 +67,10 @@ class ResizeArray(ctypes.Structure):
 # m4rt_rows (include/mamba4_retention.h) three times: an m4rt_qkv, packed into
 # bytes (a fraction of the time of filling a ctypes.Structure).
 pack_qkv = struct.Struct("@" + 3 * "Plllii").pack
+# An m4sl_scan (include/mamba4_selective.h): five m4sl_rows, two group strides, three
+# arrays, seven sizes; and an m4sl_scan_grads.
+pack_scan = struct.Struct("@" + 5 * "Pll" + "llPPP" + 7 * "i" + "0P").pack
+pack_scan_grads = struct.Struct("@" + 9 * "P").pack
 
 _F = ctypes.c_float
 
@@ -145,6 +150,12 @@ SIGNATURES = {
     "m4rt_embedding_workspace_bytes": (_S, [_L, _I, _I]),
     "m4rt_embedding_backward": (
         _I, [_P, _I, _P, _I, _L, _I, _I, _F, _P, _I, _P, _S, _P]),
+    "m4sl_scan_kept_floats": (_L, [_P]),
+    "m4sl_scan_workspace_bytes": (_S, [_P]),
+    "m4sl_scan_forward": (_I, [_P] * 7 + [_S, _P]),
+    "m4sl_scan_backward_workspace_bytes": (_S, [_P]),
+    "m4sl_scan_backward": (_I, [_P] * 7 + [_S, _P]),
+    "m4sl_scan_step": (_I, [_P] * 6),
     "m4mr_profile_enable": (None, [_I]),
     "m4mr_profile_select": (None, [ctypes.c_char_p]),
     "m4mr_profile_reset": (None, []),
@@ -164,9 +175,9 @@ class MemreadError(RuntimeError):
 
 def header_functions():
     """Names of the functions declared in include/mamba4_memread.h,
-    include/mamba3_scan.h and include/mamba4_retention.h."""
+    include/mamba3_scan.h, include/mamba4_retention.h and include/mamba4_selective.h."""
     text = "".join(open(h).read() for h in HEADERS)
-    pattern = r"^\s*(?:const\s+)?\w+\**\s+\**((?:m4mr|m3s|m4rt)_\w+)\s*\("
+    pattern = r"^\s*(?:const\s+)?\w+\**\s+\**((?:m4mr|m3s|m4rt|m4sl)_\w+)\s*\("
     return sorted(set(re.findall(pattern, text, re.M)))
 
 

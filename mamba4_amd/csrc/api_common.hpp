@@ -1,7 +1,9 @@
 // What the C entry points of every source share: the thread's error message,
-// launches with the profiling log, and the device's compute units.
+// launches with the profiling log, the device's compute units, and workspaces.
 #pragma once
 
+#include <cstddef>
+#include <cstdint>
 #include <exception>
 #include <string>
 
@@ -37,6 +39,33 @@ int api_entry(const char* name, F&& body) noexcept {
   } catch (...) {
     return M4MR_EHIP;
   }
+}
+
+inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Consecutive pieces of one workspace (sizes only, if base is NULL).
+struct Carver {
+  char* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t count) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += align256(count * sizeof(T));
+    return p;
+  }
+};
+
+inline bool bad_workspace(const void* base, size_t given, size_t need, std::string* why) {
+  if (need == 0) return false;
+  if (!base || given < need) {
+    *why = "workspace too small";
+    return true;
+  }
+  if (reinterpret_cast<uintptr_t>(base) & 255) {
+    *why = "workspace must be 256-byte aligned";
+    return true;
+  }
+  return false;
 }
 
 }  // namespace m4

@@ -52,35 +52,11 @@ __global__ void join_kernel(Sum);
 
 namespace {
 
+using m4::align256;
 using m4::api_fail;
 using m4::api_launch;
-
-size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-// Consecutive pieces of one workspace (sizes only, if base is NULL).
-struct Carver {
-  char* base;
-  size_t used = 0;
-  template <typename T>
-  T* take(size_t count) {
-    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
-    used += align256(count * sizeof(T));
-    return p;
-  }
-};
-
-bool bad_workspace(const void* base, size_t given, size_t need, std::string* why) {
-  if (need == 0) return false;
-  if (!base || given < need) {
-    *why = "workspace too small";
-    return true;
-  }
-  if (reinterpret_cast<uintptr_t>(base) & 255) {
-    *why = "workspace must be 256-byte aligned";
-    return true;
-  }
-  return false;
-}
+using m4::bad_workspace;
+using m4::Carver;
 
 // ------------------------------------------------------ linear attention --
 
