@@ -11,7 +11,8 @@ and the order head's gated scan (``order_memory_chunked``, ``order_memory``;
 lm/models/mamba4.py:46-95).  Beside them, the retention layer's operators
 (``linear_attention``, ``linear_attention_step``, ``group_norm``,
 ``embedding``) and the selective layer's (``selective_scan``,
-``selective_scan_step``).
+``selective_scan_step``, ``causal_conv``, ``causal_conv_step``, ``rms_norm``,
+``rms_norm_e4m3``).
 """
 
 from mamba4_amd.attention import (  # noqa: F401
@@ -19,6 +20,12 @@ from mamba4_amd.attention import (  # noqa: F401
     linear_attention,
     linear_attention_step,
     linear_attention_step_,
+)
+from mamba4_amd.conv import (  # noqa: F401
+    CausalConvResult,
+    causal_conv,
+    causal_conv_step,
+    causal_conv_step_,
 )
 from mamba4_amd.memory import (  # noqa: F401
     MEMORY_SOLVE,
@@ -41,7 +48,13 @@ from mamba4_amd.mixer import (  # noqa: F401
 )
 from mamba4_amd.embedding import embedding  # noqa: F401
 from mamba4_amd.flashmamba import mamba3_fused  # noqa: F401
-from mamba4_amd.norm import group_norm  # noqa: F401
+from mamba4_amd.norm import (  # noqa: F401
+    RmsNormE4M3Result,
+    RmsNormResult,
+    group_norm,
+    rms_norm,
+    rms_norm_e4m3,
+)
 from mamba4_amd.order import order_memory, order_memory_chunked  # noqa: F401
 from mamba4_amd.selective import (  # noqa: F401
     SelectiveScanResult,
@@ -51,14 +64,20 @@ from mamba4_amd.selective import (  # noqa: F401
 )
 
 __all__ = [
+    "CausalConvResult",
     "LinearAttentionResult",
     "MEMORY_SOLVE",
     "MemoryInputs",
     "MixerRead",
+    "RmsNormE4M3Result",
+    "RmsNormResult",
     "SOLVERS",
     "SelectiveResult",
     "SelectiveScanResult",
     "SelectiveState",
+    "causal_conv",
+    "causal_conv_step",
+    "causal_conv_step_",
     "embedding",
     "linear_attention",
     "linear_attention_step",
@@ -70,6 +89,8 @@ __all__ = [
     "mixer_read",
     "order_memory",
     "order_memory_chunked",
+    "rms_norm",
+    "rms_norm_e4m3",
     "selective_decode",
     "selective_decode_",
     "selective_diagnostics",

@@ -67,8 +67,9 @@ class ResizeArray(ctypes.Structure):
 # m4rt_rows (include/mamba4_retention.h) three times: an m4rt_qkv, packed into
 # bytes (a fraction of the time of filling a ctypes.Structure).
 pack_qkv = struct.Struct("@" + 3 * "Plllii").pack
-# An m4sl_scan (include/mamba4_selective.h): five m4sl_rows, two group strides, three
+# An m4sl_rows (include/mamba4_selective.h); an m4sl_scan: five m4sl_rows, two group strides, three
 # arrays, seven sizes; and an m4sl_scan_grads.
+pack_rows = struct.Struct("@Pll").pack
 pack_scan = struct.Struct("@" + 5 * "Pll" + "llPPP" + 7 * "i" + "0P").pack
 pack_scan_grads = struct.Struct("@" + 9 * "P").pack
 
@@ -156,6 +157,15 @@ SIGNATURES = {
     "m4sl_scan_backward_workspace_bytes": (_S, [_P]),
     "m4sl_scan_backward": (_I, [_P] * 7 + [_S, _P]),
     "m4sl_scan_step": (_I, [_P] * 6),
+    "m4sl_conv_forward": (_I, [_P] * 5 + [_I] * 6 + [_P] * 3),
+    "m4sl_conv_backward_workspace_bytes": (_S, [_I] * 5),
+    "m4sl_conv_backward": (_I, [_P] * 7 + [_I] * 6 + [_P] * 5 + [_S, _P]),
+    "m4sl_rms_forward": (_I, [_P, _I] * 2 + [_P, _L, _I, _F] + [_P] * 4),
+    "m4sl_rms_e4m3": (_I, [_P, _I] * 2 + [_P, _L, _I, _F, _I] + [_P] * 4),
+    "m4sl_rms_backward_workspace_bytes": (_S, [_L, _I]),
+    "m4sl_rms_backward": (
+        _I, [_P, _I] + [_P] * 3 + [_I, _P, _L, _I] + [_P] * 4 + [_S, _P]),
+    "m4sl_conv_step": (_I, [_P] * 4 + [_I] * 5 + [_P] * 4),
     "m4mr_profile_enable": (None, [_I]),
     "m4mr_profile_select": (None, [ctypes.c_char_p]),
     "m4mr_profile_reset": (None, []),

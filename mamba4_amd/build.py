@@ -20,7 +20,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIBRARY = os.path.join(HERE, "libmamba4_memread.so")
 SOURCES = ["api.hip", "states.hip", "factor.hip", "chunk.hip", "mixer.hip", "order.hip",
            "scan3.hip", "diag.hip", "spd_wide.hip", "resize.hip", "api_retention.hip",
-           "linattn.hip", "norm.hip", "embed.hip", "api_selective.hip", "selscan.hip"]
+           "linattn.hip", "norm.hip", "embed.hip", "api_selective.hip", "selscan.hip",
+           "conv.hip", "rms.hip"]
 ARCH = "gfx950"
 
 FLAGS = [

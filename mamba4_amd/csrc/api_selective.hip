@@ -8,6 +8,8 @@
 
 #include "../../include/mamba4_selective.h"
 #include "api_common.hpp"
+#include "conv.hpp"
+#include "rms.hpp"
 #include "selscan.hpp"
 
 namespace ss {
@@ -23,6 +25,24 @@ __global__ void join_rows_kernel(const float*, long, long, long, float, float*);
 template <typename In>
 __global__ void step_kernel(Step);
 }  // namespace ss
+
+namespace cv {
+template <typename In, int V, int W>
+__global__ void conv_kernel(Conv);
+template <typename In, int V, int W>
+__global__ void conv_backward_kernel(Conv);
+template <typename In, int V, int W>
+__global__ void conv_step_kernel(Step);
+__global__ void conv_join_kernel(const float*, int, int, int, float*, float*);
+}  // namespace cv
+
+namespace rn {
+template <typename X, typename R, int V, int IT, bool E4M3>
+__global__ void rms_kernel(Rms);
+template <typename X, typename R, int V, int IT>
+__global__ void rms_backward_kernel(Rms);
+__global__ void rms_join_kernel(const float*, int, int, float*);
+}  // namespace rn
 
 namespace {
 
@@ -365,6 +385,482 @@ int m4sl_scan_step(const m4sl_scan* s, const uint8_t* active, const float* state
         hipLaunchKernelGGL(ss::step_kernel<ss::bf16_t>, grid, block, 0, st, a);
       else
         hipLaunchKernelGGL(ss::step_kernel<float>, grid, block, 0, st, a);
+    });
+  });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------ causal convolution --
+
+namespace {
+
+bool bad_conv(const m4sl_rows* x, const float* weight, int B, int T, int D, int W, int activation,
+              std::string* why) {
+  if (B <= 0 || T <= 0 || D <= 0) {
+    *why = "B, T and D must be positive";
+    return true;
+  }
+  if (W <= 0 || W > M4SL_MAX_TAPS) {
+    *why = "the taps must be in 1.." + std::to_string(M4SL_MAX_TAPS);
+    return true;
+  }
+  if (activation != M4SL_NONE && activation != M4SL_SILU) {
+    *why = "unknown activation";
+    return true;
+  }
+  if (T > INT_MAX - (1 << 16) || D > INT_MAX - (1 << 16) || (double)B * T * D > 1e15) {
+    *why = "problem too large";
+    return true;
+  }
+  if (!x || !x->data || !weight) {
+    *why = "a required pointer is NULL";
+    return true;
+  }
+  return false;
+}
+
+// Channels of a thread's piece: 16 bytes, where all rows consist of such pieces.
+int conv_vec(const m4sl_rows& x, int T, int D, int bf16,
+             std::initializer_list<const void*> arrays) {
+  const int vec = bf16 ? 8 : 4;
+  bool whole = D % vec == 0 && x.batch_stride % vec == 0 && (T == 1 || x.token_stride % vec == 0) &&
+               reinterpret_cast<uintptr_t>(x.data) % 16 == 0;
+  for (const void* p : arrays) whole = whole && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  return whole ? vec : 1;
+}
+
+// Threads that keep the card busy.
+long busy_threads() { return 768L * m4::api_compute_units(); }
+
+// The backward's lines (runs of rows) and blocks.
+struct ConvPlan {
+  int run, runs, cols, wide, lines;
+  unsigned rows, columns;  // blocks
+};
+
+// Runs are as short as a busy card needs: the W - 1 rows at an edge are read twice.
+ConvPlan conv_plan(int B, int T, int D, int W, int vec) {
+  ConvPlan p{};
+  p.cols = D / vec;
+  p.wide = 1;
+  while (p.wide < 64 && p.wide < p.cols) p.wide *= 2;
+  p.lines = cv::THREADS / p.wide;
+  p.columns = (unsigned)((p.cols + p.wide - 1) / p.wide);
+  const long each = (long)B * T * p.cols / busy_threads();
+  const int fours = (int)std::min(16L, std::max(W > 4 ? 3L : 2L, (each + W + 2) / 4));
+  p.run = 4 * fours - (W - 1);
+  p.runs = (T + p.run - 1) / p.run;
+  const long blocks = ((long)B * p.runs + p.lines - 1) / p.lines;
+  const long most = std::max(1L, 4L * m4::api_compute_units() / p.columns);
+  p.rows = (unsigned)std::min(blocks, most);
+  return p;
+}
+
+template <typename In, int V, int W>
+void start_conv(const cv::Conv& a, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((cv::conv_kernel<In, V, W>), grid, dim3(cv::THREADS), 0, st, a);
+}
+template <typename In, int V, int W>
+void start_conv_backward(const cv::Conv& a, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((cv::conv_backward_kernel<In, V, W>), grid, dim3(cv::THREADS), 0, st, a);
+}
+template <typename In, int V, int W>
+void start_conv_step(const cv::Step& a, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((cv::conv_step_kernel<In, V, W>), grid, dim3(cv::THREADS), 0, st, a);
+}
+
+enum class Conv { FORWARD, BACKWARD, STEP };
+
+template <Conv WHAT, typename In, int V, int W, typename Args>
+void start_one(const Args& a, dim3 grid, hipStream_t st) {
+  if constexpr (WHAT == Conv::FORWARD) start_conv<In, V, W>(a, grid, st);
+  else if constexpr (WHAT == Conv::BACKWARD) start_conv_backward<In, V, W>(a, grid, st);
+  else start_conv_step<In, V, W>(a, grid, st);
+}
+
+template <Conv WHAT, typename In, int V, typename Args>
+void start_taps(const Args& a, int W, dim3 grid, hipStream_t st) {
+  switch (W) {
+    case 1: return start_one<WHAT, In, V, 1>(a, grid, st);
+    case 2: return start_one<WHAT, In, V, 2>(a, grid, st);
+    case 3: return start_one<WHAT, In, V, 3>(a, grid, st);
+    case 4: return start_one<WHAT, In, V, 4>(a, grid, st);
+    case 5: return start_one<WHAT, In, V, 5>(a, grid, st);
+    case 6: return start_one<WHAT, In, V, 6>(a, grid, st);
+    case 7: return start_one<WHAT, In, V, 7>(a, grid, st);
+    default: return start_one<WHAT, In, V, 8>(a, grid, st);
+  }
+}
+
+template <Conv WHAT, typename Args>
+void start_width(const Args& a, int bf16, int vec, int W, dim3 grid, hipStream_t st) {
+  if (bf16) {
+    if (vec == 8) return start_taps<WHAT, cv::bf16_t, 8>(a, W, grid, st);
+    return start_taps<WHAT, cv::bf16_t, 1>(a, W, grid, st);
+  }
+  if (vec == 4) return start_taps<WHAT, float, 4>(a, W, grid, st);
+  return start_taps<WHAT, float, 1>(a, W, grid, st);
+}
+
+cv::Conv conv_of(const m4sl_rows& x, const float* weight, const float* bias, const void* initial,
+                 const int* lengths, int B, int T, int D, int activation) {
+  cv::Conv a{};
+  a.x = x.data;
+  a.xb = x.batch_stride;
+  a.xt = x.token_stride;
+  a.weight = weight;
+  a.bias = bias;
+  a.initial = initial;
+  a.lengths = lengths;
+  a.B = B;
+  a.T = T;
+  a.D = D;
+  a.act = activation;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int m4sl_conv_forward(const m4sl_rows* x, const float* weight, const float* bias,
+                      const void* initial, const int* lengths, int bf16, int B, int T, int D,
+                      int W, int activation, void* output, void* state, void* stream) {
+  const char* name = "m4sl_conv_forward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_conv(x, weight, B, T, D, W, activation, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(bf16, {x->data, initial, output, state}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    const int vec = conv_vec(*x, T, D, bf16, {initial, output, state});
+    cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
+    a.y = output;
+    a.state = state;
+    a.cols = D / vec;
+    // Runs of eight tokens, longer ones where those are more than a busy card needs.
+    const long eights = (long)B * T * a.cols / busy_threads() / 8;
+    a.run = 8 * (int)std::min(8L, std::max(1L, eights));
+    a.runs = (T + a.run - 1) / a.run;
+    const double blocks = ((double)B * a.runs * a.cols + cv::THREADS - 1) / cv::THREADS;
+    if (too_many(blocks, cv::THREADS)) return api_fail(M4MR_EINVAL, at + "problem too large");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return api_launch("conv", st, [&] {
+      start_width<Conv::FORWARD>(a, bf16, vec, W, dim3((unsigned)blocks), st);
+    });
+  });
+}
+
+size_t m4sl_conv_backward_workspace_bytes(int B, int T, int D, int W, int bf16) {
+  std::string why;
+  const m4sl_rows any{&why, 0, 0};
+  if (bad_conv(&any, reinterpret_cast<const float*>(&why), B, T, D, W, M4SL_NONE, &why)) return 0;
+  // (The pieces depend on addresses.)
+  size_t rows = conv_plan(B, T, D, W, 1).rows;
+  const int vec = bf16 ? 8 : 4;
+  if (D % vec == 0) rows = std::max<size_t>(rows, conv_plan(B, T, D, W, vec).rows);
+  return align256(rows * (W + 1) * D * sizeof(float));
+}
+
+int m4sl_conv_backward(const m4sl_rows* x, const float* weight, const float* bias,
+                       const void* initial, const int* lengths, const void* d_output,
+                       const void* d_state, int bf16, int B, int T, int D, int W,
+                       int activation, void* d_x, void* d_initial, float* d_weight,
+                       float* d_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "m4sl_conv_backward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_conv(x, weight, B, T, D, W, activation, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!d_output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(bf16, {x->data, initial, d_output, d_state, d_x, d_initial}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    const size_t need = m4sl_conv_backward_workspace_bytes(B, T, D, W, bf16);
+    if (bad_workspace(workspace, workspace_bytes, need, &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    const int vec = conv_vec(*x, T, D, bf16, {initial, d_output, d_state, d_x, d_initial});
+    const ConvPlan p = conv_plan(B, T, D, W, vec);
+    cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
+    const bool sums = d_weight || d_bias;
+    a.run = p.run;
+    a.runs = p.runs;
+    a.cols = p.cols;
+    a.lines = p.lines;
+    a.dy = d_output;
+    a.dstate = d_state;
+    a.dx = d_x;
+    a.dinitial = d_initial;
+    a.part = sums ? static_cast<float*>(workspace) : nullptr;
+    if (p.columns > 65535) return api_fail(M4MR_EINVAL, at + "problem too large");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int rc = api_launch("conv_backward", st, [&] {
+      start_width<Conv::BACKWARD>(a, bf16, vec, W, dim3(p.rows, p.columns), st);
+    });
+    if (rc || !sums) return rc;
+    return api_launch("conv_join", st, [&] {
+      hipLaunchKernelGGL(cv::conv_join_kernel, dim3((D + 63) / 64, W + 1), dim3(1024), 0, st,
+                         a.part, (int)p.rows, W, D, d_weight, d_bias);
+    });
+  });
+}
+
+int m4sl_conv_step(const m4sl_rows* x, const float* weight, const float* bias,
+                   const uint8_t* active, int bf16, int B, int D, int W, int activation,
+                   const void* state, void* new_state, void* output, void* stream) {
+  const char* name = "m4sl_conv_step";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_conv(x, weight, B, 1, D, W, activation, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!output || (W > 1 && (!state || !new_state)))
+      return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(bf16, {x->data, state, new_state, output}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    const int vec = conv_vec(*x, 1, D, bf16, {state, new_state, output});
+    cv::Step a{};
+    a.x = x->data;
+    a.xb = x->batch_stride;
+    a.weight = weight;
+    a.bias = bias;
+    a.active = active;
+    a.state = state;
+    a.new_state = new_state;
+    a.y = output;
+    a.B = B;
+    a.D = D;
+    a.act = activation;
+    a.cols = D / vec;
+    const double blocks = ((double)B * a.cols + cv::THREADS - 1) / cv::THREADS;
+    if (too_many(blocks, cv::THREADS)) return api_fail(M4MR_EINVAL, at + "problem too large");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return api_launch("conv_step", st, [&] {
+      start_width<Conv::STEP>(a, bf16, vec, W, dim3((unsigned)blocks), st);
+    });
+  });
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------- root-mean-square norm --
+
+namespace {
+
+bool bad_rms(long M, int C, std::string* why) {
+  if (M <= 0 || C <= 0) {
+    *why = "M and C must be positive";
+    return true;
+  }
+  if (C > M4SL_MAX_NORM) {
+    *why = "the channels must be at most " + std::to_string(M4SL_MAX_NORM);
+    return true;
+  }
+  if ((double)M * C > 1e15) {
+    *why = "problem too large";
+    return true;
+  }
+  return false;
+}
+
+// Channels of a piece: eight, where all rows consist of such pieces.
+int rms_vec(int C, std::initializer_list<const void*> arrays) {
+  bool whole = C % 8 == 0;
+  for (const void* p : arrays) whole = whole && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  return whole ? 8 : 1;
+}
+
+// How a row is spread: `pieces` of a lane, lanes of a wave up to 128 pieces of eight, more
+// waves beyond.
+struct RmsPlan {
+  int pieces, threads;
+  unsigned blocks;
+};
+
+RmsPlan rms_plan(long M, int C, int vec, rn::Rms* a) {
+  const int count = (C + vec - 1) / vec;
+  RmsPlan p{};
+  if (count <= 64) {
+    p.pieces = 1;
+    a->lanes = 1;
+    while (a->lanes < count) a->lanes *= 2;
+  } else {
+    const int few = vec == 8 ? 2 : count <= 256 ? 4 : 8;
+    p.pieces = count <= few * 1024 ? few : vec == 8 ? 4 : 32;
+    a->lanes = ((count + p.pieces - 1) / p.pieces + 63) / 64 * 64;
+  }
+  a->rows = a->lanes <= 64 ? rn::THREADS / a->lanes : 1;
+  p.threads = a->lanes * a->rows;
+  const long most = 2048L * m4::api_compute_units() / p.threads;
+  p.blocks = (unsigned)std::min((M + a->rows - 1) / a->rows, std::max(1L, most));
+  a->M = M;
+  a->C = C;
+  return p;
+}
+
+// What the launches do: the result in x's type, in 8 bits, or the gradient.
+enum class Norm { FORWARD, E4M3, BACKWARD };
+
+template <Norm WHAT, typename X, typename R, int V, int IT>
+void start_rms_pieces(const rn::Rms& a, const RmsPlan& p, hipStream_t st) {
+  const dim3 grid(p.blocks), block(p.threads);
+  if constexpr (WHAT == Norm::BACKWARD)
+    hipLaunchKernelGGL((rn::rms_backward_kernel<X, R, V, IT>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((rn::rms_kernel<X, R, V, IT, WHAT == Norm::E4M3>), grid, block, 0, st, a);
+}
+
+template <Norm WHAT, typename X, typename R>
+void start_rms(const rn::Rms& a, const RmsPlan& p, int vec, hipStream_t st) {
+  if (vec == 8) {
+    if (p.pieces == 1) return start_rms_pieces<WHAT, X, R, 8, 1>(a, p, st);
+    if (p.pieces == 2) return start_rms_pieces<WHAT, X, R, 8, 2>(a, p, st);
+    return start_rms_pieces<WHAT, X, R, 8, 4>(a, p, st);
+  }
+  if (p.pieces == 1) return start_rms_pieces<WHAT, X, R, 1, 1>(a, p, st);
+  if (p.pieces == 4) return start_rms_pieces<WHAT, X, R, 1, 4>(a, p, st);
+  if (p.pieces == 8) return start_rms_pieces<WHAT, X, R, 1, 8>(a, p, st);
+  return start_rms_pieces<WHAT, X, R, 1, 32>(a, p, st);
+}
+
+template <Norm WHAT>
+int run_rms(const char* name, const rn::Rms& a, const RmsPlan& p, int vec, int x_bf16, int r_bf16,
+            hipStream_t st) {
+  return api_launch(name, st, [&] {
+    if (x_bf16)
+      r_bf16 ? start_rms<WHAT, rn::bf16_t, rn::bf16_t>(a, p, vec, st)
+             : start_rms<WHAT, rn::bf16_t, float>(a, p, vec, st);
+    else
+      r_bf16 ? start_rms<WHAT, float, rn::bf16_t>(a, p, vec, st)
+             : start_rms<WHAT, float, float>(a, p, vec, st);
+  });
+}
+
+// The forward's checks, shared by both forms of the result.
+bool bad_rms_forward(const void* x, int x_bf16, const void* residual, int residual_bf16, long M,
+                     int C, const void* output, int output_bytes, const void* sum,
+                     std::string* why) {
+  if (bad_rms(M, C, why)) return true;
+  if (!x || !output) {
+    *why = "a required pointer is NULL";
+    return true;
+  }
+  if (!residual && sum) {
+    *why = "without a residual there is no sum";
+    return true;
+  }
+  if (misaligned(x_bf16, {x}) || misaligned(residual_bf16, {residual, sum}) ||
+      reinterpret_cast<uintptr_t>(output) % output_bytes) {
+    *why = "arrays must be aligned to their elements";
+    return true;
+  }
+  return false;
+}
+
+}  // namespace
+
+extern "C" {
+
+int m4sl_rms_forward(const void* x, int x_bf16, const void* residual, int residual_bf16,
+                     const float* weight, long M, int C, float eps, void* output, void* sum,
+                     float* inverse, void* stream) {
+  const char* name = "m4sl_rms_forward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_rms_forward(x, x_bf16, residual, residual_bf16, M, C, output, x_bf16 ? 2 : 4, sum,
+                        &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    const int vec = rms_vec(C, {x, residual, weight, output, sum});
+    rn::Rms a{};
+    const RmsPlan p = rms_plan(M, C, vec, &a);
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.eps = eps;
+    a.y = output;
+    a.sum = sum;
+    a.inverse = inverse;
+    return run_rms<Norm::FORWARD>("rms", a, p, vec, x_bf16, residual ? residual_bf16 : x_bf16,
+                                  static_cast<hipStream_t>(stream));
+  });
+}
+
+int m4sl_rms_e4m3(const void* x, int x_bf16, const void* residual, int residual_bf16,
+                  const float* weight, long M, int C, float eps, int block, void* output,
+                  float* scale, void* sum, void* stream) {
+  const char* name = "m4sl_rms_e4m3";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_rms_forward(x, x_bf16, residual, residual_bf16, M, C, output, 1, sum, &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    if (!scale) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    const bool power = block >= 32 && block <= 512 && (block & (block - 1)) == 0;
+    if (block <= 0 || (block < C && !power))
+      return api_fail(M4MR_EINVAL,
+                      at + "a scale's block must be a power of two in 32..512, or at least C");
+    const int vec = rms_vec(C, {x, residual, weight, output, sum});
+    rn::Rms a{};
+    const RmsPlan p = rms_plan(M, C, vec, &a);
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.eps = eps;
+    a.y = output;
+    a.sum = sum;
+    a.scale = scale;
+    a.block = std::min(block, M4SL_MAX_NORM);
+    a.blocks = (C + a.block - 1) / a.block;
+    a.group = std::min(64, a.lanes);
+    if (block < C) a.group = std::min(a.group, block / vec);
+    return run_rms<Norm::E4M3>("rms_e4m3", a, p, vec, x_bf16, residual ? residual_bf16 : x_bf16,
+                               static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t m4sl_rms_backward_workspace_bytes(long M, int C) {
+  std::string why;
+  if (bad_rms(M, C, &why)) return 0;
+  // (The pieces depend on addresses.)
+  rn::Rms a{};
+  unsigned blocks = rms_plan(M, C, 1, &a).blocks;
+  if (C % 8 == 0) blocks = std::max(blocks, rms_plan(M, C, 8, &a).blocks);
+  return align256((size_t)blocks * C * sizeof(float));
+}
+
+int m4sl_rms_backward(const void* sum, int sum_bf16, const float* weight, const float* inverse,
+                      const void* d_output, int x_bf16, const void* d_sum, long M, int C,
+                      void* d_x, void* d_residual, float* d_weight, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const char* name = "m4sl_rms_backward";
+  return m4::api_entry(name, [&] {
+    const std::string at = std::string(name) + ": ";
+    std::string why;
+    if (bad_rms(M, C, &why)) return api_fail(M4MR_EINVAL, at + why);
+    if (!sum || !inverse || !d_output)
+      return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
+    if (misaligned(x_bf16, {d_output, d_x}) || misaligned(sum_bf16, {sum, d_sum, d_residual}))
+      return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
+    if (bad_workspace(workspace, workspace_bytes, m4sl_rms_backward_workspace_bytes(M, C), &why))
+      return api_fail(M4MR_EINVAL, at + why);
+    const int vec = rms_vec(C, {sum, weight, d_output, d_sum, d_x, d_residual});
+    rn::Rms a{};
+    const RmsPlan p = rms_plan(M, C, vec, &a);
+    a.x = sum;
+    a.weight = weight;
+    a.inverse = const_cast<float*>(inverse);
+    a.dy = d_output;
+    a.dsum = d_sum;
+    a.dx = d_x;
+    a.dresidual = d_residual;
+    a.part = d_weight ? static_cast<float*>(workspace) : nullptr;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int rc = run_rms<Norm::BACKWARD>("rms_backward", a, p, vec, x_bf16, sum_bf16, st);
+    if (rc || !d_weight) return rc;
+    return api_launch("rms_join", st, [&] {
+      hipLaunchKernelGGL(rn::rms_join_kernel, dim3((C + 63) / 64), dim3(1024), 0, st, a.part,
+                         (int)p.blocks, C, d_weight);
     });
   });
 }

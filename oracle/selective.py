@@ -113,3 +113,67 @@ def scan_backward(x, delta, a, b, c, d_output, d_state=None, skip=None, gate=Non
                 skip=(dy * s.x).sum((0, 1)),
                 gate=None if s.gate is None else d_out * y * silu_slope(s.gate),
                 bias=d_delta.sum((0, 1)), initial=g)
+
+
+def conv(x, weight, bias=None, activation="none", initial=None, lengths=None):
+    """output [B,T,D] and the last W - 1 rows that are present [B,W-1,D]."""
+    x, weight = _f64(x), _f64(weight)
+    batch, time, d = x.shape
+    taps = weight.shape[1]
+    here = _here(lengths, batch, time)
+    rows, z = _conv(x, weight, bias, initial, here)
+    y = silu(z) if activation == "silu" else z
+    ends = here.sum(1)
+    state = np.stack([rows[i, e:e + taps - 1] for i, e in enumerate(ends)])
+    return np.where(here[..., None], y, 0.0), state
+
+
+def _conv(x, weight, bias, initial, here):
+    batch, time, d = x.shape
+    taps = weight.shape[1]
+    start = np.zeros((batch, taps - 1, d)) if initial is None else _f64(initial)
+    rows = np.concatenate([start, np.where(here[..., None], x, 0.0)], axis=1)
+    z = np.zeros(x.shape) + (0.0 if bias is None else _f64(bias))
+    for j in range(taps):
+        z = z + rows[:, j:j + time] * weight[:, j]
+    return rows, z
+
+
+def conv_backward(x, weight, d_output, d_state=None, bias=None, activation="none", initial=None,
+                  lengths=None):
+    """Gradients by name: x, weight, bias, initial."""
+    x, weight = _f64(x), _f64(weight)
+    batch, time, d = x.shape
+    taps = weight.shape[1]
+    here = _here(lengths, batch, time)
+    rows, z = _conv(x, weight, bias, initial, here)
+    dz = np.where(here[..., None], _f64(d_output), 0.0)
+    if activation == "silu":
+        dz = np.where(here[..., None], dz * silu_slope(z), 0.0)
+    d_rows = np.zeros(rows.shape)
+    d_weight = np.zeros(weight.shape)
+    for j in range(taps):
+        d_rows[:, j:j + time] += dz * weight[:, j]
+        d_weight[:, j] = (dz * rows[:, j:j + time]).sum((0, 1))
+    if d_state is not None:
+        for i, e in enumerate(here.sum(1)):
+            d_rows[i, e:e + taps - 1] += _f64(d_state)[i]
+    return dict(x=d_rows[:, taps - 1:], weight=d_weight, bias=dz.sum((0, 1)),
+                initial=d_rows[:, :taps - 1])
+
+
+def rms(x, weight=None, residual=None, eps=1e-5, rounded=lambda s: s):
+    """The norm and the sum; ``rounded``: what the sum's type makes of it."""
+    s = _f64(x) if residual is None else rounded(_f64(x) + _f64(residual))
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + eps)
+    return (y if weight is None else y * _f64(weight)), s
+
+
+def rms_backward(s, d_output, d_sum=None, weight=None, eps=1e-5):
+    """Gradients of the sum s [M,C] (those of x and the residual) and of the weight."""
+    s, d_output = _f64(s), _f64(d_output)
+    inverse = 1.0 / np.sqrt((s * s).mean(-1, keepdims=True) + eps)
+    n = s * inverse
+    dn = d_output if weight is None else d_output * _f64(weight)
+    d_s = inverse * (dn - n * (dn * n).mean(-1, keepdims=True))
+    return (d_s if d_sum is None else d_s + _f64(d_sum)), (d_output * n).sum(0)

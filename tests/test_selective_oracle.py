@@ -87,3 +87,50 @@ def test_absent_tokens_do_nothing():
     np.testing.assert_array_equal(out, again)
     np.testing.assert_array_equal(state, end)
     assert (out[1] == 0).all() and (state[1] == x["initial"][1]).all()
+
+
+@pytest.mark.parametrize("taps,activation,lengths", [(4, "silu", None), (1, "none", [5, 0, 3]),
+                                                     (3, "silu", [0, 1, 5])])
+def test_conv_gradients(taps, activation, lengths):
+    rng = np.random.default_rng(5)
+    arrays = dict(x=rng.normal(size=(3, 5, 4)), weight=rng.normal(size=(4, taps)),
+                  bias=rng.normal(size=4), initial=rng.normal(size=(3, taps - 1, 4)))
+    d_out, d_state = rng.normal(size=(3, 5, 4)), rng.normal(size=(3, taps - 1, 4))
+
+    def loss(**a):
+        out, state = oracle.conv(**a, activation=activation, lengths=lengths)
+        return (out * d_out).sum() + (state * d_state).sum()
+
+    grads = oracle.conv_backward(**arrays, d_output=d_out, d_state=d_state,
+                                 activation=activation, lengths=lengths)
+    _against_differences(loss, arrays, grads, rng)
+
+
+def test_conv_in_two_parts_and_its_state():
+    rng = np.random.default_rng(6)
+    x, w = rng.normal(size=(2, 9, 3)), rng.normal(size=(3, 4))
+    out, state = oracle.conv(x, w)
+    np.testing.assert_array_equal(state, x[:, -3:])
+    first, middle = oracle.conv(x[:, :2], w)
+    np.testing.assert_array_equal(middle, np.concatenate([np.zeros((2, 1, 3)), x[:, :2]], 1))
+    second, _ = oracle.conv(x[:, 2:], w, initial=middle)
+    np.testing.assert_allclose(np.concatenate([first, second], 1), out, rtol=1e-12, atol=1e-12)
+    one, _ = oracle.conv(x, np.array([[0.0, 0.0, 1.0, 0.0]] * 3))
+    np.testing.assert_array_equal(one[:, 1:], x[:, :-1])
+
+
+def test_rms_gradients_and_norm():
+    rng = np.random.default_rng(7)
+    x, r, w = rng.normal(size=(4, 6)), rng.normal(size=(4, 6)), rng.normal(size=6)
+    d_y, d_sum = rng.normal(size=(4, 6)), rng.normal(size=(4, 6))
+    y, s = oracle.rms(x, None, r, eps=0.0)
+    np.testing.assert_allclose((y * y).mean(-1), 1.0, rtol=1e-12)
+    np.testing.assert_array_equal(s, x + r)
+
+    def loss(**a):
+        y, s = oracle.rms(**a, eps=1e-3)
+        return (y * d_y).sum() + (s * d_sum).sum()
+
+    d_s, d_w = oracle.rms_backward(s, d_y, d_sum, w, eps=1e-3)
+    _against_differences(loss, dict(x=x, residual=r, weight=w),
+                         dict(x=d_s, residual=d_s, weight=d_w), rng)

@@ -152,3 +152,144 @@ def test_lengths_and_active():
     for bad in (torch.ones(2), torch.ones(3, dtype=torch.bool)):
         with pytest.raises(ValueError, match="boolean active"):
             _active("f", bad, 2)
+
+
+def _conv_forward(x=DATA, weight=DATA, initial=None, bf16=0, B=2, T=10, D=8, W=4, activation=1,
+                  output=DATA, state=DATA):
+    rows = _lib.pack_rows(x, T * D, D)
+    return _lib.load().m4sl_conv_forward(rows, weight, None, initial, None, bf16, B, T, D, W,
+                                         activation, output, state, None)
+
+
+def _conv_backward(x=DATA, weight=DATA, bf16=0, B=2, T=10, D=8, W=4, activation=1, d_output=DATA,
+                   d_x=DATA, workspace=DATA, nbytes=HUGE):
+    rows = _lib.pack_rows(x, T * D, D)
+    return _lib.load().m4sl_conv_backward(rows, weight, None, None, None, d_output, None, bf16, B,
+                                          T, D, W, activation, d_x, None, DATA, DATA, workspace,
+                                          nbytes, None)
+
+
+def _conv_step(x=DATA, weight=DATA, bf16=0, B=2, D=8, W=4, activation=1, state=DATA,
+               new_state=DATA, output=DATA):
+    return _lib.load().m4sl_conv_step(_lib.pack_rows(x, D, 0), weight, None, None, bf16, B, D, W,
+                                      activation, state, new_state, output, None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(B=0), "positive"), (dict(D=-1), "positive"), (dict(W=0), "taps must be in"),
+    (dict(W=9), "taps must be in"), (dict(activation=2), "activation"),
+    (dict(activation=-1), "activation"), (dict(x=0), "NULL"), (dict(weight=None), "NULL"),
+    (dict(x=DATA + 2), "aligned"), (dict(x=DATA + 1, bf16=1), "aligned"),
+    (dict(D=2**31 - 10), "too large"),
+])
+def test_conv_refuses(change, words):
+    for call in (_conv_forward, _conv_backward, _conv_step):
+        _refused(call(**change), words)
+
+
+def test_conv_refuses_buffers():
+    _refused(_conv_forward(T=0), "positive")
+    _refused(_conv_forward(output=None), "NULL")
+    _refused(_conv_forward(initial=DATA + 2), "aligned")
+    _refused(_conv_forward(state=DATA + 2), "aligned")
+    _refused(_conv_backward(d_output=None), "NULL")
+    _refused(_conv_backward(d_x=DATA + 2), "aligned")
+    _refused(_conv_backward(workspace=None), "workspace too small")
+    _refused(_conv_backward(nbytes=64), "workspace too small")
+    _refused(_conv_backward(workspace=DATA + 4), "256-byte aligned")
+    for change in (dict(state=None), dict(new_state=None), dict(output=None)):
+        _refused(_conv_step(**change), "NULL")
+    # 2^32 threads of a piece each.
+    _refused(_conv_step(B=2**30, D=2**6, x=DATA + 4), "too large")
+    _refused(_conv_forward(B=2**20, T=2**17, D=2**6, x=DATA + 4), "too large")
+    size = _lib.load().m4sl_conv_backward_workspace_bytes
+    assert size(2, 0, 8, 4, 0) == 0 and size(2, 10, 8, 9, 0) == 0
+    assert size(2, 10, 8, 4, 1) >= 5 * 8 * 4
+    assert size(16, 1024, 1536, 4, 1) % 256 == 0
+
+
+def test_conv_arguments():
+    from mamba4_amd import causal_conv
+    from mamba4_amd.conv import _inputs, _state
+
+    x, w = torch.zeros(2, 5, 8), torch.zeros(8, 4)
+    for args, words in (
+            ((x[0], w, None, "none"), "floating-point x"), ((x.int(), w, None, "none"), "floating"),
+            ((x[..., :0], w, None, "none"), "channels"), ((x, w[:7], None, "none"), "weight"),
+            ((x, torch.zeros(8, 9), None, "none"), "weight"),
+            ((x, w[:, :0], None, "none"), "weight"), ((x, w, w, "none"), "bias"),
+            ((x, w, None, "gelu"), "activation"), ((x, w + 0j, None, "none"), "complex")):
+        with pytest.raises(ValueError, match=words):
+            _inputs("causal_conv", 2, *args)
+    with pytest.raises(ValueError, match="initial"):
+        _state("causal_conv", "initial", torch.zeros(2, 4, 8), x, w)
+    with pytest.raises(ValueError, match="complex"):
+        _state("causal_conv", "initial", torch.zeros(2, 3, 8) + 0j, x, w)
+    with pytest.raises(ValueError, match="ROCm device"):
+        causal_conv(x, w)
+
+
+def _rms_forward(x=DATA, x_bf16=0, residual=DATA, residual_bf16=0, M=4, C=64, output=DATA,
+                 sum=DATA):
+    return _lib.load().m4sl_rms_forward(x, x_bf16, residual, residual_bf16, None, M, C, 1e-5,
+                                        output, sum, None, None)
+
+
+def _rms_e4m3(x=DATA, x_bf16=0, residual=DATA, residual_bf16=0, M=4, C=64, output=DATA, sum=DATA,
+              block=32, scale=DATA):
+    return _lib.load().m4sl_rms_e4m3(x, x_bf16, residual, residual_bf16, None, M, C, 1e-5, block,
+                                     output, scale, sum, None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(M=0), "positive"), (dict(C=0), "positive"), (dict(C=32769), "at most"),
+    (dict(M=2**50), "too large"), (dict(x=None), "NULL"), (dict(output=None), "NULL"),
+    (dict(residual=None), "no sum"), (dict(x=DATA + 2), "aligned"),
+    (dict(x=DATA + 1, x_bf16=1), "aligned"), (dict(residual=DATA + 2), "aligned"),
+    (dict(sum=DATA + 1, residual_bf16=1), "aligned"),
+])
+def test_rms_refuses(change, words):
+    _refused(_rms_forward(**change), words)
+    _refused(_rms_e4m3(**change), words)
+
+
+def test_rms_refuses_buffers():
+    _refused(_rms_forward(output=DATA + 2), "aligned")
+    _refused(_rms_e4m3(scale=None), "NULL")
+    for block in (0, -32, 16, 48, 63):
+        _refused(_rms_e4m3(block=block), "block")
+    _refused(_rms_e4m3(C=2000, block=1024), "block")
+    lib = _lib.load()
+
+    def backward(sum=DATA, inverse=DATA, d_output=DATA, M=4, C=64, d_x=DATA, workspace=DATA,
+                 nbytes=HUGE):
+        return lib.m4sl_rms_backward(sum, 0, None, inverse, d_output, 0, None, M, C, d_x, None,
+                                     DATA, workspace, nbytes, None)
+
+    for change, words in ((dict(sum=None), "NULL"), (dict(inverse=None), "NULL"),
+                          (dict(d_output=None), "NULL"), (dict(M=0), "positive"),
+                          (dict(C=40000), "at most"), (dict(d_x=DATA + 2), "aligned"),
+                          (dict(workspace=None), "workspace too small"),
+                          (dict(nbytes=16), "workspace too small"),
+                          (dict(workspace=DATA + 8), "256-byte aligned")):
+        _refused(backward(**change), words)
+    assert lib.m4sl_rms_backward_workspace_bytes(0, 64) == 0
+    assert lib.m4sl_rms_backward_workspace_bytes(100, 64) >= 64 * 4
+
+
+def test_rms_arguments():
+    from mamba4_amd import rms_norm, rms_norm_e4m3
+    from mamba4_amd.norm import _rms_inputs
+
+    x = torch.zeros(3, 8)
+    for args, words in (((x[0, 0], None, None), "floating-point x"),
+                        ((x.int(), None, None), "floating-point x"),
+                        ((x[:, :0], None, None), "channels"), ((x, x[0, :7], None), "weight"),
+                        ((x, x, None), "weight"), ((x, None, x[:2]), "residual"),
+                        ((x, None, x.int()), "residual"), ((x, x[0] + 0j, None), "complex"),
+                        ((torch.zeros(1, 32769), None, None), "channels")):
+        with pytest.raises(ValueError, match=words):
+            _rms_inputs("rms_norm", *args)
+    for call in (rms_norm, rms_norm_e4m3):
+        with pytest.raises(ValueError, match="ROCm device"):
+            call(x)
