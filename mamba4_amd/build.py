@@ -37,7 +37,7 @@ FLAGS = [
 ]
 
 # Sources whose inline-asm DPP multiply-adds are re-checked on the compiled code.
-HAZARD_CHECKED = ["factor.hip"]
+HAZARD_CHECKED = ["factor.hip", "selscan.hip"]
 
 # Per-source extra flags.  The factorization accumulates its trailing blocks
 # in place with MFMA; keeping MFMA operands and results in VGPRs avoids a

@@ -13,9 +13,9 @@
 #include "selscan.hpp"
 
 namespace ss {
-template <typename In, int NG, bool OUT>
+template <typename In, int NG, bool OUT, bool WHOLE>
 __global__ void scan_kernel(Scan);
-template <typename In, int NG, bool ALL>
+template <typename In, int NG, bool ALL, bool WHOLE>
 __global__ void scan_backward_kernel(Scan);
 template <bool BWD>
 __global__ void carry_kernel(Scan);
@@ -73,10 +73,6 @@ bool whole_at(int bf16, std::initializer_list<const void*> arrays) {
   return true;
 }
 
-bool whole_rows(const m4sl_rows& r) {
-  return r.batch_stride % 4 == 0 && r.token_stride % 4 == 0;
-}
-
 // ---------------------------------------------------------- selective scan --
 
 int tiles_of(int T) { return (T + ss::TILE - 1) / ss::TILE; }
@@ -124,6 +120,7 @@ bool bad_scan(const m4sl_scan* s, bool tokens, std::string* why) {
 // so that sequences are cut only where their waves leave the card idle, and into no
 // more than fill it.
 int segments(const m4sl_scan& s) {
+  if (const char* e = std::getenv("M4SL_SEGMENTS")) { int v = std::atoi(e); if (v) return std::min(v, std::max(1, tiles_of(s.T))); }
   const long waves = (long)s.B * s.G * ((s.D / s.G + 15) / 16);
   const long full = 4L * m4::api_compute_units();
   if (waves >= full) return 1;
@@ -134,15 +131,36 @@ int segments(const m4sl_scan& s) {
 
 ss::Rows rows_of(const m4sl_rows& r) { return ss::Rows{r.data, r.batch_stride, r.token_stride}; }
 
+// Whether rows of `width` can be read through a tile's descriptor: aligned pieces of four,
+// tokens at least a row apart, and a tile's bytes below 2^31.
+bool tile_rows(const ss::Rows& r, int width, int bf16) {
+  return width % 4 == 0 && r.batch % 4 == 0 && r.token % 4 == 0 && whole_at(bf16, {r.p}) &&
+         r.token >= width && r.token <= INT_MAX / (4 * ss::TILE);
+}
+
+// Whether all rows are such (the kernels read others an element at a time).
+bool whole_scan(const ss::Scan& a, int bf16, std::initializer_list<const void*> results) {
+  const ss::Rows dense{nullptr, 0, a.D};
+  return a.Dg % 4 == 0 && a.bg % 4 == 0 && a.cg % 4 == 0 && whole_at(bf16, results) &&
+         tile_rows(dense, a.D, bf16) && tile_rows(a.x, a.D, bf16) &&
+         tile_rows(a.delta, a.D, bf16) && tile_rows(a.gate, a.D, bf16) &&
+         tile_rows(a.b, a.N, bf16) && tile_rows(a.c, a.N, bf16);
+}
+
 ss::Scan scan_of(const m4sl_scan& s, const int* lengths) {
   ss::Scan a{};
   a.x = rows_of(s.x);
   a.delta = rows_of(s.delta);
-  a.gate = rows_of(s.gate);
+  a.gate = rows_of(s.gate.data ? s.gate : s.x);
+  a.gated = s.gate.data != nullptr;
   a.b = rows_of(s.b);
   a.c = rows_of(s.c);
   a.bg = s.b_group_stride;
   a.cg = s.c_group_stride;
+  if (s.T == 1) {  // (Strides of one token are no strides.)
+    a.x.token = a.delta.token = a.gate.token = s.D;
+    a.b.token = a.c.token = s.N;
+  }
   a.a = s.a;
   a.skip = s.skip;
   a.bias = s.delta_bias;
@@ -154,10 +172,6 @@ ss::Scan scan_of(const m4sl_scan& s, const int* lengths) {
   a.Dg = s.D / s.G;
   a.N = s.N;
   a.softplus = s.softplus;
-  a.whole = a.Dg % 4 == 0 && whole_rows(s.x) && whole_rows(s.delta) && whole_rows(s.gate) &&
-            whole_at(s.bf16, {s.x.data, s.delta.data, s.gate.data});
-  a.whole_bc = s.N % 4 == 0 && whole_rows(s.b) && whole_rows(s.c) && a.bg % 4 == 0 &&
-               a.cg % 4 == 0 && whole_at(s.bf16, {s.b.data, s.c.data});
   a.blocks = blocks_of(s);
   const int cut = segments(s), tiles = tiles_of(s.T);
   a.seg = (tiles + cut - 1) / cut * ss::TILE;
@@ -181,26 +195,40 @@ size_t take_backward(Carver& c, ss::Scan* a) {
   return c.used;
 }
 
-template <typename In, bool OUT>
-void start_scan(const ss::Scan& a, hipStream_t st) {
+template <typename In, int NG, bool WHOLE>
+void start_groups(const ss::Scan& a, bool backward, bool all, hipStream_t st) {
   const dim3 grid(a.B * a.G * a.blocks, a.NS), block(64 * ss::WAVES);
-  if (a.N <= 16)
-    hipLaunchKernelGGL((ss::scan_kernel<In, 1, OUT>), grid, block, 0, st, a);
-  else if (a.N <= 32)
-    hipLaunchKernelGGL((ss::scan_kernel<In, 2, OUT>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((ss::scan_kernel<In, 4, OUT>), grid, block, 0, st, a);
+  if (backward) {
+    if (all)
+      hipLaunchKernelGGL((ss::scan_backward_kernel<In, NG, true, WHOLE>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((ss::scan_backward_kernel<In, NG, false, WHOLE>), grid, block, 0, st, a);
+  } else {
+    if (all)
+      hipLaunchKernelGGL((ss::scan_kernel<In, NG, true, WHOLE>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((ss::scan_kernel<In, NG, false, WHOLE>), grid, block, 0, st, a);
+  }
 }
 
-template <typename In, bool ALL>
-void start_scan_backward(const ss::Scan& a, hipStream_t st) {
-  const dim3 grid(a.B * a.G * a.blocks, a.NS), block(64 * ss::WAVES);
-  if (a.N <= 16)
-    hipLaunchKernelGGL((ss::scan_backward_kernel<In, 1, ALL>), grid, block, 0, st, a);
-  else if (a.N <= 32)
-    hipLaunchKernelGGL((ss::scan_backward_kernel<In, 2, ALL>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((ss::scan_backward_kernel<In, 4, ALL>), grid, block, 0, st, a);
+template <typename In, bool WHOLE>
+void start_states(const ss::Scan& a, bool backward, bool all, hipStream_t st) {
+  if (a.N <= 16) return start_groups<In, 1, WHOLE>(a, backward, all, st);
+  if (a.N <= 32) return start_groups<In, 2, WHOLE>(a, backward, all, st);
+  return start_groups<In, 4, WHOLE>(a, backward, all, st);
+}
+
+// `all`: the results; else what the segments add.
+int run_scan(const char* name, const ss::Scan& a, int bf16, bool whole, bool backward, bool all,
+             hipStream_t st) {
+  return api_launch(name, st, [&] {
+    if (bf16)
+      whole ? start_states<ss::bf16_t, true>(a, backward, all, st)
+            : start_states<ss::bf16_t, false>(a, backward, all, st);
+    else
+      whole ? start_states<float, true>(a, backward, all, st)
+            : start_states<float, false>(a, backward, all, st);
+  });
 }
 
 template <bool BWD>
@@ -252,7 +280,7 @@ int m4sl_scan_forward(const m4sl_scan* s, const float* initial, const int* lengt
     Carver c{static_cast<char*>(workspace)};
     if (bad_workspace(workspace, workspace_bytes, take_segments(c, &a), &why))
       return api_fail(M4MR_EINVAL, at + why);
-    a.whole = a.whole && whole_at(s->bf16, {output});
+    const bool whole = whole_scan(a, s->bf16, {output});
     a.initial = initial;
     a.out = output;
     a.state = state;
@@ -260,16 +288,11 @@ int m4sl_scan_forward(const m4sl_scan* s, const float* initial, const int* lengt
     a.whole_n = a.N % 4 == 0 && whole_at(0, {a.a, initial, state, kept});
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a.NS > 1) {
-      int rc = api_launch("scan_states", st, [&] {
-        s->bf16 ? start_scan<ss::bf16_t, false>(a, st) : start_scan<float, false>(a, st);
-      });
-      if (rc) return rc;
-      rc = run_carry<false>(a, st);
+      int rc = run_scan("scan_states", a, s->bf16, whole, false, false, st);
+      if (!rc) rc = run_carry<false>(a, st);
       if (rc) return rc;
     }
-    return api_launch("scan", st, [&] {
-      s->bf16 ? start_scan<ss::bf16_t, true>(a, st) : start_scan<float, true>(a, st);
-    });
+    return run_scan("scan", a, s->bf16, whole, false, true, st);
   });
 }
 
@@ -297,7 +320,8 @@ int m4sl_scan_backward(const m4sl_scan* s, const int* lengths, const void* d_out
     Carver c{static_cast<char*>(workspace)};
     if (bad_workspace(workspace, workspace_bytes, take_backward(c, &a), &why))
       return api_fail(M4MR_EINVAL, at + why);
-    a.whole = a.whole && whole_at(s->bf16, {d_output, grads->x, grads->delta, grads->gate});
+    const bool whole =
+        whole_scan(a, s->bf16, {d_output, grads->x, grads->delta, grads->gate});
     a.dout = d_output;
     a.dstate = d_state;
     a.kept = const_cast<float*>(kept);
@@ -309,18 +333,11 @@ int m4sl_scan_backward(const m4sl_scan* s, const int* lengths, const void* d_out
     hipStream_t st = static_cast<hipStream_t>(stream);
     int rc;
     if (a.NS > 1) {
-      rc = api_launch("scan_backward_states", st, [&] {
-        s->bf16 ? start_scan_backward<ss::bf16_t, false>(a, st)
-                : start_scan_backward<float, false>(a, st);
-      });
-      if (rc) return rc;
-      rc = run_carry<true>(a, st);
+      rc = run_scan("scan_backward_states", a, s->bf16, whole, true, false, st);
+      if (!rc) rc = run_carry<true>(a, st);
       if (rc) return rc;
     }
-    rc = api_launch("scan_backward", st, [&] {
-      s->bf16 ? start_scan_backward<ss::bf16_t, true>(a, st)
-              : start_scan_backward<float, true>(a, st);
-    });
+    rc = run_scan("scan_backward", a, s->bf16, whole, true, true, st);
     if (rc) return rc;
     ss::Join j{a.part_bc, a.blocks, a.B, a.T, a.G, a.N, lengths, grads->b, grads->c};
     rc = api_launch("scan_join_bc", st, [&] {

@@ -25,6 +25,7 @@ namespace ss {
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
@@ -104,6 +105,32 @@ __device__ __forceinline__ float exp_minus(float v) {
   return p < -200.f ? 0.f : fmaf(e, low * LN2, e);
 }
 
+// Rows through a buffer's descriptor: reads past its bytes are zero and writes dropped, so
+// that a tile's absent tokens, and lanes without a channel (whose offset is ABSENT), need
+// no branch and no clearing.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr unsigned ABSENT = 0x80000000u;
+
+__device__ __forceinline__ Rsrc rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
+}
+// `rows` (or fewer than one: none) of `stride` bytes, the last one `width` >= 0.
+__device__ __forceinline__ Rsrc rows_rsrc(const char* base, int stride, int rows, int width) {
+  return rsrc(base, rows > 0 ? (rows - 1) * stride + width : 0);
+}
+__device__ __forceinline__ void read4(Rsrc r, unsigned at, Four<float>& v) {
+  v.r = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+}
+__device__ __forceinline__ void read4(Rsrc r, unsigned at, Four<bf16_t>& v) {
+  v.r = __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+}
+__device__ __forceinline__ void write4(Rsrc r, unsigned at, const Four<float>& v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v.r), r, at, 0, 0);
+}
+__device__ __forceinline__ void write4(Rsrc r, unsigned at, const Four<bf16_t>& v) {
+  __builtin_amdgcn_raw_buffer_store_b64(v.r, r, at, 0, 0);
+}
+
 // log(1 + exp(v)): u = 1 + e is rounded, and log(u) e / (u - 1) takes the rounding back
 // (Kahan's form of log1p).
 __device__ __forceinline__ float softplus(float v) {
@@ -112,27 +139,41 @@ __device__ __forceinline__ float softplus(float v) {
   return fmaxf(v, 0.f) + (d == 0.f ? e : l);
 }
 
-// 1 / (1 + exp(-v)), small values to their own precision.
+// 1 / (1 + exp(-v)), to 2^-24 of itself and of v.
 __device__ __forceinline__ float sigmoid(float v) {
-  const float e = exp_minus(v), r = __builtin_amdgcn_rcpf(1.f + e);
-  return v < 0.f ? e * r : r;
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * v));
 }
 
-// Lane K's value of each row of 16 lanes.
+// acc + K's lane of src in each row of 16 lanes, times mul, as one instruction (the
+// compiler takes two).  `settled` has to come between what writes src and this.
 template <int K>
-__device__ __forceinline__ float lane_of_row(float v) {
-  return __int_as_float(
-      __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + K, 0xf, 0xf, true));
+__device__ __forceinline__ void fmac_row(float& acc, float src, float mul) {
+  asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf"
+      : "+v"(acc)
+      : "v"(src), "v"(mul), "n"(K));
+}
+template <int K>
+__device__ __forceinline__ float mul_row(float src, float mul) {
+  float r;
+  asm("v_mul_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf"
+      : "=v"(r)
+      : "v"(src), "v"(mul), "n"(K));
+  return r;
 }
 
-template <int CTRL, int BANKS = 0xf>
-__device__ __forceinline__ float dpp(float old, float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL,
-                                                    0xf, BANKS, BANKS == 0xf));
+// The two wait states between an instruction that writes a register and one that reads it
+// from other lanes, which the compiler does not see to inside inline assembly.  (The
+// build checks the compiled code for them.)
+__device__ __forceinline__ void settled(float (&v)[4], float (&w)[4]) {
+  asm volatile("s_nop 1"
+               : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(w[0]), "+v"(w[1]),
+                 "+v"(w[2]), "+v"(w[3]));
 }
 
-// Sums over the four rows of a wave: row q has that of v[q].
-__device__ __forceinline__ float join_rows(const float (&v)[4]) {
+// Sums over the four rows of a wave: row q has that of v[q].  (v comes of inline
+// assembly, to whose writes a swap needs the same two wait states.)
+__device__ __forceinline__ float join_rows(float (&v)[4]) {
+  asm volatile("s_nop 1" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0]), __float_as_uint(v[2]),
                                                   false, false);
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[1]), __float_as_uint(v[3]),
@@ -144,20 +185,35 @@ __device__ __forceinline__ float join_rows(const float (&v)[4]) {
   return __uint_as_float(c[0]) + __uint_as_float(c[1]);
 }
 
-// x in banks KEEP (of four lanes each) of a row, y in the others.
-template <int KEEP>
-__device__ __forceinline__ float banks(float x, float y) {
-  return dpp<0xE4, KEEP>(y, x);
-}
-
-// Sums over the 16 lanes of a row: bank b has that of v[b with its two bits swapped].
-__device__ __forceinline__ float join_lanes(const float (&v)[4]) {
-  const float s = banks<0x3>(v[0], v[1]) + dpp<0x128>(0.f, banks<0x3>(v[1], v[0]));
-  const float t = banks<0x3>(v[2], v[3]) + dpp<0x128>(0.f, banks<0x3>(v[3], v[2]));
-  float u = banks<0x5>(s, t) + dpp<0x141>(0.f, banks<0x5>(t, s));
-  u += dpp<0xB1>(0.f, u);
-  u += dpp<0x4E>(0.f, u);
-  return u;
+// Sums of v and of w over the 16 lanes of a row: bank b (of four lanes) has that of v[b
+// with its two bits swapped].  Each level adds the lanes 8, then 4 apart of one value in
+// half of the banks and of another in the rest, so that four values take eight
+// instructions; those of v and w alternate to keep two wait states between an
+// instruction and the next that reads its result from other lanes.
+__device__ __forceinline__ void join_lanes(const float (&v)[4], const float (&w)[4], float& sv,
+                                           float& sw) {
+  float a, b, c, d;
+  asm("s_nop 1\n"
+      "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+      "v_add_f32_dpp %2, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %3, %8, %8 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+      "v_add_f32_dpp %3, %9, %9 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %4, %10, %10 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+      "v_add_f32_dpp %4, %11, %11 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %5, %12, %12 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+      "v_add_f32_dpp %5, %13, %13 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0x5\n"
+      "v_add_f32_dpp %0, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+      "v_add_f32_dpp %1, %4, %4 row_half_mirror row_mask:0xf bank_mask:0x5\n"
+      "v_add_f32_dpp %1, %5, %5 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+      "v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
+      "s_nop 0\n"
+      "v_add_f32_dpp %1, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
+      "s_nop 0\n"
+      "v_add_f32_dpp %1, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf"
+      : "=&v"(sv), "=&v"(sw), "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+      : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(w[0]), "v"(w[1]), "v"(w[2]), "v"(w[3]));
 }
 
 // Orders a wave's own LDS accesses (which the hardware keeps in order).
@@ -196,7 +252,7 @@ struct Place {
 __device__ __forceinline__ Place place(const Scan& a) {
   Place p;
   p.lane = threadIdx.x & 63;
-  p.wave = threadIdx.x >> 6;
+  p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   p.q = p.lane >> 4;
   p.ch = p.lane & 15;
   p.token = p.lane >> 2;
@@ -218,37 +274,120 @@ __device__ __forceinline__ Place place(const Scan& a) {
   return p;
 }
 
-// A tile's rows as they are in memory.
-template <typename In, int NG, bool GATE, bool DOUT>
+// An array's rows of a wave's channels (or of its group's states), from the batch row's
+// first token: the stride of a token in bytes, and where in a tile the lane reads.
+struct Lines {
+  const char* base;
+  int stride;
+  unsigned at;
+};
+
+template <typename In>
+__device__ __forceinline__ Lines channel_lines(const Place& p, const void* data, long batch,
+                                               long token) {
+  const In* base = static_cast<const In*>(data) + batch + (p.d - p.ch);
+  const int stride = (int)token * (int)sizeof(In);
+  const unsigned at = p.token * stride + p.piece * sizeof(In);
+  return Lines{reinterpret_cast<const char*>(base), stride, p.count > 0 ? at : ABSENT};
+}
+
+// The arrays that a kernel reads by tiles.
+template <typename In, int NG>
+struct Sources {
+  Lines x, delta, gate, dout, b, c;
+  int width;  // bytes of the wave's channels
+
+  __device__ __forceinline__ Sources(const Scan& a, const Place& p) {
+    const auto lines = [&](const Rows& r) {
+      return channel_lines<In>(p, r.p, p.b * r.batch, r.token);
+    };
+    x = lines(a.x);
+    delta = lines(a.delta);
+    gate = lines(a.gate);
+    dout = channel_lines<In>(p, a.dout, (long)p.b * a.T * a.D, a.D);
+    const auto states = [&](const Rows& r, long group) {
+      const In* base = static_cast<const In*>(r.p) + p.b * r.batch + p.g * group;
+      const int stride = (int)r.token * (int)sizeof(In);
+      return Lines{reinterpret_cast<const char*>(base), stride,
+                   (unsigned)(p.ch * stride + 4 * p.q * (int)sizeof(In))};
+    };
+    b = states(a.b, a.bg);
+    c = states(a.c, a.cg);
+    width = min(16, max(0, a.Dg - p.first)) * (int)sizeof(In);
+  }
+};
+
+// A tile's rows as they are in memory; absent tokens and channels are zero.  WHOLE: all
+// rows consist of aligned pieces of four.
+template <typename In, int NG, bool GATE, bool DOUT, bool WHOLE>
 struct TileRows {
   Four<In> x, delta, gate, dout, b[NG], c[NG];
 
-  __device__ __forceinline__ void fetch(const Scan& a, const Place& p, int t0) {
-    const int last = min(p.end, p.len);
-    const int t = t0 + p.token;
-    const int count = t < last ? p.count : 0;
-    const auto row = [&](const Rows& r) {
-      return load4(static_cast<const In*>(r.p) + p.b * r.batch + t * r.token + p.d4, count,
-                   a.whole);
-    };
-    x = row(a.x);
-    delta = row(a.delta);
-    if (GATE) {
-      if (a.gate.p) gate = row(a.gate);
-      else gate.r = 0;
-    }
-    if (DOUT)
-      dout = load4(static_cast<const In*>(a.dout) + ((long)p.b * a.T + t) * a.D + p.d4, count,
-                   a.whole);
-    const int k = t0 + p.ch;
+  // Tokens t0 .. t0 + 15 of those before `last`.
+  __device__ __forceinline__ void fetch(const Scan& a, const Place& p, const Sources<In, NG>& from,
+                                        int t0, int last) {
+    if constexpr (WHOLE) {
+      const int rows = min(TILE, last - t0);
+      const auto read = [&](const Lines& l, Four<In>& v) {
+        read4(rows_rsrc(l.base + (long)t0 * l.stride, l.stride, rows, from.width), l.at, v);
+      };
+      read(from.x, x);
+      read(from.delta, delta);
+      if (GATE) read(from.gate, gate);
+      if (DOUT) read(from.dout, dout);
+      const int wide = a.N * (int)sizeof(In);
+      const Rsrc rb = rows_rsrc(from.b.base + (long)t0 * from.b.stride, from.b.stride, rows, wide);
+      const Rsrc rc = rows_rsrc(from.c.base + (long)t0 * from.c.stride, from.c.stride, rows, wide);
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const int n = 16 * i + 4 * p.q;
-      const int have = k < last ? min(4, max(0, a.N - n)) : 0;
-      b[i] = load4(static_cast<const In*>(a.b.p) + p.b * a.b.batch + k * a.b.token +
-                       p.g * a.bg + n, have, a.whole_bc);
-      c[i] = load4(static_cast<const In*>(a.c.p) + p.b * a.c.batch + k * a.c.token +
-                       p.g * a.cg + n, have, a.whole_bc);
+      for (int i = 0; i < NG; ++i) {
+        const unsigned n = 16 * i + 4 * p.q, more = 16 * i * sizeof(In);
+        read4(rb, n < (unsigned)a.N ? from.b.at + more : ABSENT, b[i]);
+        read4(rc, n < (unsigned)a.N ? from.c.at + more : ABSENT, c[i]);
+      }
+    } else {
+      const int t = t0 + p.token, count = t < last ? p.count : 0;
+      const auto row = [&](const Rows& r) {
+        return load4(static_cast<const In*>(r.p) + p.b * r.batch + t * r.token + p.d4, count,
+                     false);
+      };
+      x = row(a.x);
+      delta = row(a.delta);
+      if (GATE) gate = row(a.gate);
+      if (DOUT)
+        dout = load4(static_cast<const In*>(a.dout) + ((long)p.b * a.T + t) * a.D + p.d4, count,
+                     false);
+      const int k = t0 + p.ch;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int n = 16 * i + 4 * p.q, have = k < last ? min(4, max(0, a.N - n)) : 0;
+        b[i] = load4(static_cast<const In*>(a.b.p) + p.b * a.b.batch + k * a.b.token + p.g * a.bg +
+                         n, have, false);
+        c[i] = load4(static_cast<const In*>(a.c.p) + p.b * a.c.batch + k * a.c.token + p.g * a.cg +
+                         n, have, false);
+      }
+    }
+  }
+};
+
+// Rows [B,T,D] that a kernel writes by tiles, of the wave's channels.
+template <typename In, bool WHOLE>
+struct Result {
+  Lines l;
+  int width;
+  __device__ __forceinline__ Result(const Scan& a, const Place& p, void* to) {
+    l = channel_lines<In>(p, to, (long)p.b * a.T * a.D, a.D);
+    width = min(16, max(0, a.Dg - p.first)) * (int)sizeof(In);
+  }
+  // Tokens t0 .. t0 + 15 of those before `end`.
+  __device__ __forceinline__ void put(const Place& p, int t0, int end, const float (&v)[4]) const {
+    Four<In> f;
+    f.set(v);
+    const char* to = l.base + (long)t0 * l.stride;
+    if constexpr (WHOLE) {
+      write4(rows_rsrc(to, l.stride, min(TILE, end - t0), width), l.at, f);
+    } else if (t0 + p.token < end) {
+      store4(reinterpret_cast<In*>(const_cast<char*>(to) + (long)p.token * l.stride) + p.piece, v,
+             p.count, false);
     }
   }
 };
@@ -301,9 +440,15 @@ __device__ __forceinline__ void steps(const Scan& a, const Four<In>& delta, cons
                                       bool here, float (&s)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float v = delta.get(e) + bias[e];
-    s[e] = here ? (a.softplus ? softplus(v) : v) : 0.f;
+    const float v = delta.get(e) + bias[e], soft = softplus(v);
+    s[e] = here ? (a.softplus ? soft : v) : 0.f;
   }
+}
+
+template <typename In>
+__device__ __forceinline__ void widen(const Four<In>& f, float (&v)[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = f.get(r);
 }
 
 __device__ __forceinline__ void load_bias(const float* from, const Place& p, float (&v)[4]) {
@@ -324,94 +469,112 @@ __device__ __forceinline__ void store_token_sums(const Place& p, float (&v)[4], 
 // ------------------------------------------------------------ forward
 
 // OUT: a segment's outputs from its start state (and the last one's end state); else
-// what the segment adds to the state, and the sum of its steps.
-template <typename In, int NG, bool OUT>
-__global__ __launch_bounds__(64 * WAVES) void scan_kernel(Scan a) {
-  __shared__ f4 shared[WAVES][OUT ? 192 : 128];
+// what the segment adds to the state, and the sum of its steps.  A tile's steps are
+// formed while the one before is computed, and its outputs written while the next is.
+template <typename In, int NG, bool OUT, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel(Scan a) {
+  __shared__ f2 shared_su[WAVES][2][256];              // [16 tokens][16 channels]
+  __shared__ float shared_y[OUT ? WAVES : 1][2][256];  // the same
   const Place p = place(a);
   if (p.first >= a.Dg) return;
-  f2* su = reinterpret_cast<f2*>(shared[p.wave]);               // [16 tokens][16 channels]
-  float* yl = reinterpret_cast<float*>(shared[p.wave] + 128);   // the same
+  auto& su = shared_su[p.wave];
+  auto& yl = shared_y[OUT ? p.wave : 0];
   float rate[NG][4], h[NG][4], bias[4], skip[4], total[4] = {0.f, 0.f, 0.f, 0.f};
   load_decays(a, p, rate);
   load_bias(a.bias, p, bias);
   load_bias(a.skip, p, skip);
-  const float* from = nullptr;
+  const float* begin = nullptr;
   if (OUT)
-    from = a.NS > 1 ? a.ends + (p.row * a.D + p.d) * a.N
+    begin = a.NS > 1 ? a.ends + (p.row * a.D + p.d) * a.N
            : a.initial ? a.initial + ((long)p.b * a.D + p.d) * a.N : nullptr;
-  load_states(a, p, from, h);
+  load_states(a, p, begin, h);
   const int tiles = (a.T + TILE - 1) / TILE;
-  TileRows<In, NG, OUT, false> next;
-  next.fetch(a, p, p.begin);
-  for (int t0 = p.begin; t0 < p.end; t0 += TILE) {
-    const bool here = t0 + p.token < min(p.end, p.len);
-    const long at = ((long)p.b * a.T + t0 + p.token) * a.D + p.d4;
-    if (t0 >= p.len) {
-      if (!OUT) break;
-      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      if (t0 + p.token < p.end) store4(static_cast<In*>(a.out) + at, zero, p.count, a.whole);
-      continue;
-    }
-    const TileRows<In, NG, OUT, false> now = next;
-    next.fetch(a, p, t0 + TILE);
-    if (OUT && a.kept)
-      store_states(a, p, a.kept + (((long)p.b * tiles + t0 / TILE) * a.D + p.d) * a.N, h);
+  const int last = min(p.end, p.len);
+  const Sources<In, NG> from(a, p);
+  const Result<In, WHOLE> out(a, p, a.out);
+  using RowsOf = TileRows<In, NG, OUT, false, WHOLE>;
+
+  const auto stage = [&](const RowsOf& rows, int t0, f2* to) {
     float s[4];
-    steps(a, now.delta, bias, here, s);
+    steps(a, rows.delta, bias, t0 + p.token < last, s);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      su[p.token * 16 + p.piece + e] = f2{s[e], s[e] * now.x.get(e)};
+      to[p.token * 16 + p.piece + e] = f2{s[e], s[e] * rows.x.get(e)};
       if (!OUT) total[e] += s[e];
     }
+  };
+  const auto finish = [&](const Four<In>& x, const Four<In>& gate, int t0, const float* sums) {
+    const f4 v = *reinterpret_cast<const f4*>(sums + p.token * 16 + p.piece);
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float z = gate.get(e), open = z * sigmoid(z);
+      o[e] = a.skip ? fmaf(skip[e], x.get(e), v[e]) : v[e];
+      o[e] *= a.gated ? open : 1.f;
+      o[e] = t0 + p.token < last ? o[e] : 0.f;
+    }
+    out.put(p, t0, p.end, o);
+  };
+
+  if (p.begin < last) {
+    RowsOf now, next;
+    Four<In> x, gate;  // of the tile before
+    now.fetch(a, p, from, p.begin, last);
+    stage(now, p.begin, su[0]);
+    next.fetch(a, p, from, p.begin + TILE, last);
     wave_sync();
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    int turn = 0;
+    for (int t0 = p.begin; t0 < last; t0 += TILE) {
+      if (OUT && a.kept)
+        store_states(a, p, a.kept + (((long)p.b * tiles + t0 / TILE) * a.D + p.d) * a.N, h);
+      stage(next, t0 + TILE, su[turn ^ 1]);
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      float bv[4], cv[4], part[4];
+      for (int i = 0; i < NG; ++i) {
+        float bv[4], cv[4], part[4];
+        widen(now.b[i], bv);
+        widen(now.c[i], cv);
+        settled(bv, cv);
+        unroll<0, TILE>([&](auto k) {
+          constexpr int t = k.value;
+          const f2 v = su[turn][t * 16 + p.ch];
+          if (OUT) part[t & 3] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        bv[r] = now.b[i].get(r);
-        cv[r] = now.c[i].get(r);
+          for (int r = 0; r < 4; ++r) {
+            const float keep = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
+            h[i][r] = fmaf(keep, h[i][r], mul_row<t>(bv[r], v.y));
+            if (OUT) fmac_row<t>(part[t & 3], cv[r], h[i][r]);
+          }
+          if (OUT && (t & 3) == 3) y[t / 4] += join_rows(part);
+        });
       }
-      unroll<0, TILE>([&](auto k) {
-        constexpr int t = k.value;
-        const f2 v = su[t * 16 + p.ch];
-        if (OUT) part[t & 3] = 0.f;
+      if (OUT) {
+        if (t0 > p.begin) finish(x, gate, t0 - TILE, yl[turn ^ 1]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float keep = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
-          h[i][r] = fmaf(keep, h[i][r], v.y * lane_of_row<t>(bv[r]));
-          if (OUT) part[t & 3] = fmaf(lane_of_row<t>(cv[r]), h[i][r], part[t & 3]);
-        }
-        if (OUT && (t & 3) == 3) y[t / 4] += join_rows(part);
-      });
+        for (int j = 0; j < 4; ++j) yl[turn][(4 * j + p.q) * 16 + p.ch] = y[j];
+        x = now.x;
+        gate = now.gate;
+      }
+      now = next;
+      next.fetch(a, p, from, t0 + 2 * TILE, last);
+      wave_sync();
+      turn ^= 1;
     }
     if (OUT) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) yl[(4 * j + p.q) * 16 + p.ch] = y[j];
-      wave_sync();
-      const f4 v = *reinterpret_cast<const f4*>(yl + p.token * 16 + p.piece);
-      float o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[e] = fmaf(skip[e], now.x.get(e), v[e]);
-        if (a.gate.p) {
-          const float z = now.gate.get(e);
-          o[e] *= z * sigmoid(z);
-        }
-        o[e] = here ? o[e] : 0.f;
-      }
-      if (t0 + p.token < p.end) store4(static_cast<In*>(a.out) + at, o, p.count, a.whole);
-      wave_sync();
+      const int t0 = p.begin + (last - 1 - p.begin) / TILE * TILE;
+      finish(x, gate, t0, yl[turn ^ 1]);
     }
   }
   if (!OUT) {
     store_states(a, p, a.ends + (p.row * a.D + p.d) * a.N, h);
     store_token_sums(p, total, a.sums + p.row * a.D);
-  } else if (p.s == a.NS - 1) {
-    store_states(a, p, a.state + ((long)p.b * a.D + p.d) * a.N, h);
+    return;
   }
+  if (p.s == a.NS - 1) store_states(a, p, a.state + ((long)p.b * a.D + p.d) * a.N, h);
+  // Tiles without a token that is present.
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int t = p.begin + (max(0, last - p.begin) + TILE - 1) / TILE * TILE; t < p.end; t += TILE)
+    out.put(p, t, p.end, zero);
 }
 
 // What each segment starts from, in the place of what it adds: h <- exp(a sum s) h + end.
@@ -439,19 +602,22 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
 // ------------------------------------------------------------ backward
 
 // ALL: a segment's gradients from the cotangent of the state after it; else what the
-// segment adds to the cotangent of the state before it, and the sum of its steps.
-template <typename In, int NG, bool ALL>
-__global__ __launch_bounds__(64 * WAVES) void scan_backward_kernel(Scan a) {
-  // A wave's steps, inflows and cotangents [16 tokens][16 channels], then sums over the
-  // states of the same shape; and every wave's sums over channels [16 tokens][16 states].
-  __shared__ f4 shared[WAVES][ALL ? 256 : 128];
-  __shared__ f4 sums[ALL ? 2 : 1][WAVES][ALL ? 128 : 1];
+// segment adds to the cotangent of the state before it, and the sum of its steps.  A
+// tile is walked forwards from the state that the forward call kept, its states and
+// decays staying in registers, then backwards.
+template <typename In, int NG, bool ALL, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backward_kernel(Scan a) {
+  // A wave's steps, inflows and cotangents [16 tokens][16 channels], its sums over the
+  // states of the same shape, and every wave's sums over channels [16 tokens][16 states].
+  __shared__ f4 shared_in[WAVES][2][256];
+  __shared__ float shared_out[ALL ? WAVES : 1][3][256];
+  __shared__ float sums[ALL ? 2 : 1][WAVES][2][ALL ? 256 : 1];
   const Place p = place(a);
   const bool idle = p.first >= a.Dg;
   if (!ALL && idle) return;
   const int active = min(WAVES, (a.Dg - p.block * BLOCK_CHANNELS + 15) / 16);
-  f4* sud = shared[p.wave];
-  float* joined = reinterpret_cast<float*>(shared[p.wave]);
+  auto& in = shared_in[p.wave];
+  auto& out = shared_out[ALL ? p.wave : 0];
   float rate[NG][4], g[NG][4], da[NG][4], bias[4], skip[4];
   float dskip[4] = {0.f, 0.f, 0.f, 0.f}, dbias[4] = {0.f, 0.f, 0.f, 0.f};
   load_decays(a, p, rate);
@@ -461,173 +627,177 @@ __global__ __launch_bounds__(64 * WAVES) void scan_backward_kernel(Scan a) {
   for (int i = 0; i < NG; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) da[i][r] = 0.f;
-  const float* from = nullptr;
+  const float* begin = nullptr;
   if (ALL)
-    from = a.NS > 1 ? a.ends + (p.row * a.D + p.d) * a.N
+    begin = a.NS > 1 ? a.ends + (p.row * a.D + p.d) * a.N
            : a.dstate ? a.dstate + ((long)p.b * a.D + p.d) * a.N : nullptr;
-  load_states(a, p, from, g);
+  load_states(a, p, begin, g);
   const int tiles = (a.T + TILE - 1) / TILE;
-  const int first = p.begin / TILE, last = (p.end + TILE - 1) / TILE;
-  // The tile to begin with: the last one with a token that is present.
-  int tile = last - 1;
-  for (; tile >= first && tile * TILE >= p.len; --tile) {
-    const int t = tile * TILE + p.token;
-    if (ALL && !idle && t < p.end) {
-      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      const long at = ((long)p.b * a.T + t) * a.D + p.d4;
-      store4(static_cast<In*>(a.dx) + at, zero, p.count, a.whole);
-      store4(static_cast<In*>(a.ddelta) + at, zero, p.count, a.whole);
-      if (a.dgate) store4(static_cast<In*>(a.dgate) + at, zero, p.count, a.whole);
-    }
-  }
-  TileRows<In, NG, true, true> next;
-  if (tile >= first) next.fetch(a, p, tile * TILE);
-  int turn = 0;
-  for (; tile >= first; --tile) {
-    const int t0 = tile * TILE;
-    const bool here = t0 + p.token < min(p.end, p.len);
-    const TileRows<In, NG, true, true> now = next;
-    if (tile > first) next.fetch(a, p, t0 - TILE);
-    float s[4], dy[4];
-    steps(a, now.delta, bias, here, s);
+  const int first = p.begin / TILE, last = min(p.end, p.len);
+  const Sources<In, NG> from(a, p);
+  const Result<In, WHOLE> dxs(a, p, a.dx), dds(a, p, a.ddelta), dzs(a, p, a.dgate);
+  using RowsOf = TileRows<In, NG, true, true, WHOLE>;
+
+  float s[4], dy[4];  // of the tile that is staged
+  const auto stage = [&](const RowsOf& rows, int t0, f4* to) {
+    steps(a, rows.delta, bias, t0 + p.token < last, s);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float z = now.gate.get(e);
-      dy[e] = now.dout.get(e) * (a.gate.p ? z * sigmoid(z) : 1.f);
-      const f4 v = {s[e], s[e] * now.x.get(e), dy[e], 0.f};
-      if (ALL) {
-        sud[p.token * 16 + p.piece + e] = v;
-      } else {
-        reinterpret_cast<f2*>(sud)[p.token * 16 + p.piece + e] = f2{s[e], dy[e]};
-        dbias[e] += s[e];
-      }
+      const float z = rows.gate.get(e), open = z * sigmoid(z);
+      dy[e] = rows.dout.get(e) * (a.gated ? open : 1.f);
+      to[p.token * 16 + p.piece + e] = f4{s[e], s[e] * rows.x.get(e), dy[e], 0.f};
+      if (!ALL) dbias[e] += s[e];
     }
+  };
+
+  // From the last tile with a token that is present.
+  int tile = (last + TILE - 1) / TILE - 1;
+  if (tile >= first) {
+    RowsOf now, next;
+    now.fetch(a, p, from, tile * TILE, last);
+    stage(now, tile * TILE, in[0]);
+    if (tile > first) next.fetch(a, p, from, (tile - 1) * TILE, last);
+    float start[NG][4];
+    if (ALL) load_states(a, p, a.kept + (((long)p.b * tiles + tile) * a.D + p.d) * a.N, start);
     wave_sync();
-    if constexpr (!ALL) {
+    int turn = 0;
+    for (; tile >= first; --tile) {
+      const int t0 = tile * TILE;
+      const f4* sud = in[turn];
+      if constexpr (!ALL) {
+        if (tile > first) stage(next, t0 - TILE, in[turn ^ 1]);
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        float cv[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) cv[r] = now.c[i].get(r);
-        unroll<0, TILE>([&](auto k) {
-          constexpr int t = TILE - 1 - k.value;
-          const f2 v = reinterpret_cast<f2*>(sud)[t * 16 + p.ch];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            g[i][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]) *
-                      fmaf(lane_of_row<t>(cv[r]), v.y, g[i][r]);
-        });
-      }
-      wave_sync();
-    } else {
-      float y[4] = {0.f, 0.f, 0.f, 0.f}, flow[4] = {0.f, 0.f, 0.f, 0.f},
-            slope[4] = {0.f, 0.f, 0.f, 0.f};
-      float start[NG][4];
-      load_states(a, p, a.kept + (((long)p.b * tiles + tile) * a.D + p.d) * a.N, start);
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        float* mine = reinterpret_cast<float*>(sums[turn][p.wave]);
-        if (!idle) {
-          float bv[4], cv[4], h[TILE][4], keep[TILE][4], part[4], part2[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            bv[r] = now.b[i].get(r);
-            cv[r] = now.c[i].get(r);
-          }
-          unroll<0, TILE>([&](auto k) {
-            constexpr int t = k.value;
-            const f4 v = sud[t * 16 + p.ch];
-            part[t & 3] = 0.f;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
-              keep[t][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
-              h[t][r] = fmaf(keep[t][r], before, v.y * lane_of_row<t>(bv[r]));
-              part[t & 3] = fmaf(lane_of_row<t>(cv[r]), h[t][r], part[t & 3]);
-            }
-            if ((t & 3) == 3) y[t / 4] += join_rows(part);
-          });
+        for (int i = 0; i < NG; ++i) {
+          float cv[4], none[4] = {0.f, 0.f, 0.f, 0.f};
+          widen(now.c[i], cv);
+          settled(cv, none);
           unroll<0, TILE>([&](auto k) {
             constexpr int t = TILE - 1 - k.value;
             const f4 v = sud[t * 16 + p.ch];
-            float pb[4], pc[4];
-            part[t & 3] = 0.f;
-            part2[t & 3] = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
-              g[i][r] = fmaf(lane_of_row<t>(cv[r]), v.z, g[i][r]);
-              pc[r] = h[t][r] * v.z;
-              pb[r] = g[i][r] * v.y;
-              part[t & 3] = fmaf(lane_of_row<t>(bv[r]), g[i][r], part[t & 3]);
-              g[i][r] *= keep[t][r];
-              const float m = g[i][r] * before;
-              part2[t & 3] = fmaf(m, rate[i][r], part2[t & 3]);
-              da[i][r] = fmaf(m, v.x, da[i][r]);
-            }
-            // Bank j of row q: state 4 q + (j with its bits swapped).
-            const int n = 4 * p.q + ((p.ch >> 3) | (p.ch >> 1 & 2));
-            mine[t * 16 + n] = join_lanes(pb);
-            mine[256 + t * 16 + n] = join_lanes(pc);
-            if ((t & 3) == 0) {
-              flow[t / 4] += join_rows(part);
-              slope[t / 4] += join_rows(part2);
+              fmac_row<t>(g[i][r], cv[r], v.z);
+              g[i][r] *= __builtin_amdgcn_exp2f(v.x * rate[i][r]);
             }
           });
         }
-        __syncthreads();
-        // The block's channels, in their order.
-        const float* all = reinterpret_cast<const float*>(sums[turn]);
-        const int t = threadIdx.x >> 4, n = 16 * i + (threadIdx.x & 15);
-        float db = 0.f, dc = 0.f;
-        for (int w = 0; w < active; ++w) {
-          db += all[w * 512 + threadIdx.x];
-          dc += all[w * 512 + 256 + threadIdx.x];
-        }
-        if (n < a.N && t0 + t < min(p.end, p.len)) {
-          const long tokens = (long)a.B * a.T;
-          float* to = a.part_bc +
-                      ((p.block * tokens + (long)p.b * a.T + t0 + t) * a.G + p.g) * 2 * a.N + n;
-          to[0] = db;
-          to[a.N] = dc;
-        }
-        turn ^= 1;
-      }
-      if (!idle) {
+        now = next;
+        if (tile > first + 1) next.fetch(a, p, from, t0 - 2 * TILE, last);
         wave_sync();
+      } else {
+        float y[4] = {0.f, 0.f, 0.f, 0.f}, flow[4] = {0.f, 0.f, 0.f, 0.f},
+              slope[4] = {0.f, 0.f, 0.f, 0.f};
+        int side = NG == 1 ? turn : 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = (4 * j + p.q) * 16 + p.ch;
-          joined[at] = y[j];
-          joined[256 + at] = flow[j];
-          joined[512 + at] = slope[j];
-        }
-        wave_sync();
-        const int from4 = p.token * 16 + p.piece;
-        const f4 yv = *reinterpret_cast<const f4*>(joined + from4);
-        const f4 fv = *reinterpret_cast<const f4*>(joined + 256 + from4);
-        const f4 sv = *reinterpret_cast<const f4*>(joined + 512 + from4);
-        wave_sync();
-        float dx[4], dd[4], dz[4];
+        for (int i = 0; i < NG; ++i) {
+          auto& mine = sums[side][p.wave];
+          if (!idle) {
+            float bv[4], cv[4], h[TILE][4], keep[TILE][4], part[4], part2[4];
+            widen(now.b[i], bv);
+            widen(now.c[i], cv);
+            settled(bv, cv);
+            unroll<0, TILE>([&](auto k) {
+              constexpr int t = k.value;
+              const f4 v = sud[t * 16 + p.ch];
+              part[t & 3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = now.x.get(e), z = now.gate.get(e), sg = sigmoid(z);
-          const float whole = fmaf(skip[e], x, yv[e]);
-          dz[e] = here ? now.dout.get(e) * whole * (sg * fmaf(z, 1.f - sg, 1.f)) : 0.f;
-          dx[e] = here ? fmaf(s[e], fv[e], skip[e] * dy[e]) : 0.f;
-          float v = fmaf(x, fv[e], sv[e] * LN2);
-          if (a.softplus) v *= sigmoid(now.delta.get(e) + bias[e]);
-          dd[e] = here ? v : 0.f;
-          dskip[e] += here ? dy[e] * x : 0.f;
-          dbias[e] += dd[e];
+              for (int r = 0; r < 4; ++r) {
+                const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
+                keep[t][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
+                h[t][r] = fmaf(keep[t][r], before, mul_row<t>(bv[r], v.y));
+                fmac_row<t>(part[t & 3], cv[r], h[t][r]);
+              }
+              if ((t & 3) == 3) y[t / 4] += join_rows(part);
+            });
+            // Bank j of row q: state 4 q + (j with its bits swapped).
+            const int n = 4 * p.q + ((p.ch >> 3) | (p.ch >> 1 & 2));
+            unroll<0, TILE>([&](auto k) {
+              constexpr int t = TILE - 1 - k.value;
+              const f4 v = sud[t * 16 + p.ch];
+              float pb[4], pc[4], sb, sc;
+              part[t & 3] = 0.f;
+              part2[t & 3] = 0.f;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
+                fmac_row<t>(g[i][r], cv[r], v.z);
+                pc[r] = h[t][r] * v.z;
+                pb[r] = g[i][r] * v.y;
+                fmac_row<t>(part[t & 3], bv[r], g[i][r]);
+                g[i][r] *= keep[t][r];
+                const float m = g[i][r] * before;
+                part2[t & 3] = fmaf(m, rate[i][r], part2[t & 3]);
+                da[i][r] = fmaf(m, v.x, da[i][r]);
+              }
+              join_lanes(pb, pc, sb, sc);
+              mine[0][t * 16 + n] = sb;
+              mine[1][t * 16 + n] = sc;
+              if ((t & 3) == 0) {
+                flow[t / 4] += join_rows(part);
+                slope[t / 4] += join_rows(part2);
+              }
+            });
+          }
+          if (i == NG - 1 && !idle) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int at = (4 * j + p.q) * 16 + p.ch;
+              out[0][at] = y[j];
+              out[1][at] = flow[j];
+              out[2][at] = slope[j];
+            }
+          }
+          __syncthreads();
+          // The block's channels, in their order.
+          const int t = threadIdx.x >> 4, n = 16 * i + (threadIdx.x & 15);
+          float db = 0.f, dc = 0.f;
+          for (int w = 0; w < active; ++w) {
+            db += sums[side][w][0][threadIdx.x];
+            dc += sums[side][w][1][threadIdx.x];
+          }
+          if (n < a.N && t0 + t < last) {
+            const long tokens = (long)a.B * a.T;
+            float* to = a.part_bc +
+                        ((p.block * tokens + (long)p.b * a.T + t0 + t) * a.G + p.g) * 2 * a.N + n;
+            to[0] = db;
+            to[a.N] = dc;
+          }
+          side ^= 1;
         }
-        if (t0 + p.token < p.end) {
-          const long at = ((long)p.b * a.T + t0 + p.token) * a.D + p.d4;
-          store4(static_cast<In*>(a.dx) + at, dx, p.count, a.whole);
-          store4(static_cast<In*>(a.ddelta) + at, dd, p.count, a.whole);
-          if (a.dgate) store4(static_cast<In*>(a.dgate) + at, dz, p.count, a.whole);
+        const RowsOf was = now;
+        const float s0[4] = {s[0], s[1], s[2], s[3]}, dy0[4] = {dy[0], dy[1], dy[2], dy[3]};
+        now = next;
+        if (tile > first) {
+          stage(now, t0 - TILE, in[turn ^ 1]);
+          load_states(a, p, a.kept + (((long)p.b * tiles + tile - 1) * a.D + p.d) * a.N, start);
         }
+        if (tile > first + 1) next.fetch(a, p, from, t0 - 2 * TILE, last);
+        if (!idle) {
+          const bool here = t0 + p.token < last;
+          const int from4 = p.token * 16 + p.piece;
+          const f4 yv = *reinterpret_cast<const f4*>(&out[0][from4]);
+          const f4 fv = *reinterpret_cast<const f4*>(&out[1][from4]);
+          const f4 sv = *reinterpret_cast<const f4*>(&out[2][from4]);
+          float dx[4], dd[4], dz[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = was.x.get(e), z = was.gate.get(e), sg = sigmoid(z);
+            const float whole = a.skip ? fmaf(skip[e], x, yv[e]) : yv[e];
+            dz[e] = here ? was.dout.get(e) * whole * (sg * fmaf(z, 1.f - sg, 1.f)) : 0.f;
+            dx[e] = here ? fmaf(s0[e], fv[e], a.skip ? skip[e] * dy0[e] : 0.f) : 0.f;
+            const float v = fmaf(x, fv[e], sv[e] * LN2);
+            const float soft = v * sigmoid(was.delta.get(e) + bias[e]);
+            dd[e] = here ? (a.softplus ? soft : v) : 0.f;
+            dskip[e] += here ? dy0[e] * x : 0.f;
+            dbias[e] += dd[e];
+          }
+          dxs.put(p, t0, p.end, dx);
+          dds.put(p, t0, p.end, dd);
+          if (a.dgate) dzs.put(p, t0, p.end, dz);
+        }
+        wave_sync();
       }
+      turn ^= 1;
     }
   }
   if (idle) return;
@@ -641,6 +811,13 @@ __global__ __launch_bounds__(64 * WAVES) void scan_backward_kernel(Scan a) {
   store_token_sums(p, dbias, a.part_d + (p.row * 2 + 1) * a.D);
   if (a.NS == 1 && a.dinitial)
     store_states(a, p, a.dinitial + ((long)p.b * a.D + p.d) * a.N, g);
+  // Tiles without a token that is present.
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int t = p.begin + (max(0, last - p.begin) + TILE - 1) / TILE * TILE; t < p.end; t += TILE) {
+    dxs.put(p, t, p.end, zero);
+    dds.put(p, t, p.end, zero);
+    if (a.dgate) dzs.put(p, t, p.end, zero);
+  }
 }
 
 // The gradients of b and c: the sums over the channel blocks.
@@ -737,20 +914,20 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   else static_cast<bf16_t*>(a.out)[row] = (bf16_t)pack(y, 0.f);
 }
 
-#define M4SL_SCAN(In)                                               \
-  template __global__ void scan_kernel<In, 1, true>(Scan);          \
-  template __global__ void scan_kernel<In, 2, true>(Scan);          \
-  template __global__ void scan_kernel<In, 4, true>(Scan);          \
-  template __global__ void scan_kernel<In, 1, false>(Scan);         \
-  template __global__ void scan_kernel<In, 2, false>(Scan);         \
-  template __global__ void scan_kernel<In, 4, false>(Scan);         \
-  template __global__ void scan_backward_kernel<In, 1, true>(Scan); \
-  template __global__ void scan_backward_kernel<In, 2, true>(Scan); \
-  template __global__ void scan_backward_kernel<In, 4, true>(Scan); \
-  template __global__ void scan_backward_kernel<In, 1, false>(Scan);\
-  template __global__ void scan_backward_kernel<In, 2, false>(Scan);\
-  template __global__ void scan_backward_kernel<In, 4, false>(Scan);\
-  template __global__ void join_bc_kernel<In>(Join);                \
+#define M4SL_SCAN_GROUPS(In, NG)                                            \
+  template __global__ void scan_kernel<In, NG, true, true>(Scan);           \
+  template __global__ void scan_kernel<In, NG, true, false>(Scan);          \
+  template __global__ void scan_kernel<In, NG, false, true>(Scan);          \
+  template __global__ void scan_kernel<In, NG, false, false>(Scan);         \
+  template __global__ void scan_backward_kernel<In, NG, true, true>(Scan);  \
+  template __global__ void scan_backward_kernel<In, NG, true, false>(Scan); \
+  template __global__ void scan_backward_kernel<In, NG, false, true>(Scan); \
+  template __global__ void scan_backward_kernel<In, NG, false, false>(Scan);
+#define M4SL_SCAN(In)                                \
+  M4SL_SCAN_GROUPS(In, 1)                            \
+  M4SL_SCAN_GROUPS(In, 2)                            \
+  M4SL_SCAN_GROUPS(In, 4)                            \
+  template __global__ void join_bc_kernel<In>(Join); \
   template __global__ void step_kernel<In>(Step);
 M4SL_SCAN(float)
 M4SL_SCAN(bf16_t)

@@ -24,10 +24,8 @@ struct Scan {
   const float *a, *skip, *bias;   // [D,N], [D], [D] (skip, bias: or NULL)
   const int* lengths;             // [B], or NULL
   int B, T, D, G, Dg, N;          // Dg = D / G
-  int softplus;
-  int whole;                      // rows of channels are read in pieces of four
-  int whole_bc;                   // b and c too
-  int whole_n;                    // float32 states and a too
+  int softplus, gated;            // (gate: x's rows, where there is none)
+  int whole_n;                    // float32 states are read in pieces of four
   int blocks;                     // blocks of a group's channels
   int seg, NS;                    // tokens of a segment, segments
   const float* initial;           // [B,D,N], or NULL (NS == 1: the start state)
