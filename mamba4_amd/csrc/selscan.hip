@@ -96,13 +96,10 @@ __device__ __forceinline__ void store4(In* p, const float (&v)[4], int count, bo
     }
 }
 
-// exp(-|v|), to float32's own precision: the product's rounding is put back.
-__device__ __forceinline__ float exp_minus(float v) {
-  const float a = -fabsf(v), p = a * LOG2E;
-  const float low = fmaf(a, LOG2E, -p) + a * 1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(p);
-  // (Far below the range the low part is no number any more.)
-  return p < -200.f ? 0.f : fmaf(e, low * LN2, e);
+// v where `mask` is all ones, zero where it is zero.  (A select costs 4.6 cycles a wave,
+// and 23 where its condition is in VCC and was not just formed; this costs 3.)
+__device__ __forceinline__ float masked(float v, unsigned mask) {
+  return __uint_as_float(__float_as_uint(v) & mask);
 }
 
 // Rows through a buffer's descriptor: reads past its bytes are zero and writes dropped, so
@@ -131,12 +128,11 @@ __device__ __forceinline__ void write4(Rsrc r, unsigned at, const Four<bf16_t>& 
   __builtin_amdgcn_raw_buffer_store_b64(v.r, r, at, 0, 0);
 }
 
-// log(1 + exp(v)): u = 1 + e is rounded, and log(u) e / (u - 1) takes the rounding back
-// (Kahan's form of log1p).
+// log(1 + exp(v)): of u = 1 + e, rounded, and of what the rounding lost, (e - (u - 1)) / u.
 __device__ __forceinline__ float softplus(float v) {
-  const float e = exp_minus(v), u = 1.f + e, d = u - 1.f;
-  const float l = __builtin_amdgcn_logf(u) * LN2 * (e * __builtin_amdgcn_rcpf(d));
-  return fmaxf(v, 0.f) + (d == 0.f ? e : l);
+  const float e = __builtin_amdgcn_exp2f(-LOG2E * fabsf(v)), u = 1.f + e;
+  const float lost = (e - (u - 1.f)) * __builtin_amdgcn_rcpf(u);
+  return fmaxf(v, 0.f) + fmaf(__builtin_amdgcn_logf(u), LN2, lost);
 }
 
 // 1 / (1 + exp(-v)), to 2^-24 of itself and of v.
@@ -278,7 +274,7 @@ __device__ __forceinline__ Place place(const Scan& a) {
 // first token: the stride of a token in bytes, and where in a tile the lane reads.
 struct Lines {
   const char* base;
-  int stride;
+  long stride;  // (WHOLE: sixteen of them are below 2^31)
   unsigned at;
 };
 
@@ -286,8 +282,8 @@ template <typename In>
 __device__ __forceinline__ Lines channel_lines(const Place& p, const void* data, long batch,
                                                long token) {
   const In* base = static_cast<const In*>(data) + batch + (p.d - p.ch);
-  const int stride = (int)token * (int)sizeof(In);
-  const unsigned at = p.token * stride + p.piece * sizeof(In);
+  const long stride = token * (long)sizeof(In);
+  const unsigned at = p.token * (int)stride + p.piece * sizeof(In);
   return Lines{reinterpret_cast<const char*>(base), stride, p.count > 0 ? at : ABSENT};
 }
 
@@ -307,9 +303,9 @@ struct Sources {
     dout = channel_lines<In>(p, a.dout, (long)p.b * a.T * a.D, a.D);
     const auto states = [&](const Rows& r, long group) {
       const In* base = static_cast<const In*>(r.p) + p.b * r.batch + p.g * group;
-      const int stride = (int)r.token * (int)sizeof(In);
+      const long stride = r.token * (long)sizeof(In);
       return Lines{reinterpret_cast<const char*>(base), stride,
-                   (unsigned)(p.ch * stride + 4 * p.q * (int)sizeof(In))};
+                   (unsigned)(p.ch * (int)stride + 4 * p.q * (int)sizeof(In))};
     };
     b = states(a.b, a.bg);
     c = states(a.c, a.cg);
@@ -329,15 +325,17 @@ struct TileRows {
     if constexpr (WHOLE) {
       const int rows = min(TILE, last - t0);
       const auto read = [&](const Lines& l, Four<In>& v) {
-        read4(rows_rsrc(l.base + (long)t0 * l.stride, l.stride, rows, from.width), l.at, v);
+        read4(rows_rsrc(l.base + t0 * l.stride, (int)l.stride, rows, from.width), l.at, v);
       };
       read(from.x, x);
       read(from.delta, delta);
       if (GATE) read(from.gate, gate);
       if (DOUT) read(from.dout, dout);
       const int wide = a.N * (int)sizeof(In);
-      const Rsrc rb = rows_rsrc(from.b.base + (long)t0 * from.b.stride, from.b.stride, rows, wide);
-      const Rsrc rc = rows_rsrc(from.c.base + (long)t0 * from.c.stride, from.c.stride, rows, wide);
+      const Rsrc rb =
+          rows_rsrc(from.b.base + t0 * from.b.stride, (int)from.b.stride, rows, wide);
+      const Rsrc rc =
+          rows_rsrc(from.c.base + t0 * from.c.stride, (int)from.c.stride, rows, wide);
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         const unsigned n = 16 * i + 4 * p.q, more = 16 * i * sizeof(In);
@@ -382,11 +380,11 @@ struct Result {
   __device__ __forceinline__ void put(const Place& p, int t0, int end, const float (&v)[4]) const {
     Four<In> f;
     f.set(v);
-    const char* to = l.base + (long)t0 * l.stride;
+    const char* to = l.base + t0 * l.stride;
     if constexpr (WHOLE) {
-      write4(rows_rsrc(to, l.stride, min(TILE, end - t0), width), l.at, f);
+      write4(rows_rsrc(to, (int)l.stride, min(TILE, end - t0), width), l.at, f);
     } else if (t0 + p.token < end) {
-      store4(reinterpret_cast<In*>(const_cast<char*>(to) + (long)p.token * l.stride) + p.piece, v,
+      store4(reinterpret_cast<In*>(const_cast<char*>(to) + p.token * l.stride) + p.piece, v,
              p.count, false);
     }
   }
@@ -434,14 +432,19 @@ __device__ __forceinline__ void store_states(const Scan& a, const Place& p, floa
   }
 }
 
+// All ones where token t is before `last`, else zero.
+__device__ __forceinline__ unsigned present(int t, int last) {
+  return (unsigned)((t - last) >> 31);
+}
+
 // The steps of a lane's piece.
 template <typename In>
 __device__ __forceinline__ void steps(const Scan& a, const Four<In>& delta, const float (&bias)[4],
-                                      bool here, float (&s)[4]) {
+                                      unsigned here, float (&s)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float v = delta.get(e) + bias[e], soft = softplus(v);
-    s[e] = here ? (a.softplus ? soft : v) : 0.f;
+    s[e] = masked(a.softplus ? soft : v, here);
   }
 }
 
@@ -496,7 +499,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
 
   const auto stage = [&](const RowsOf& rows, int t0, f2* to) {
     float s[4];
-    steps(a, rows.delta, bias, t0 + p.token < last, s);
+    steps(a, rows.delta, bias, present(t0 + p.token, last), s);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       to[p.token * 16 + p.piece + e] = f2{s[e], s[e] * rows.x.get(e)};
@@ -505,13 +508,14 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
   };
   const auto finish = [&](const Four<In>& x, const Four<In>& gate, int t0, const float* sums) {
     const f4 v = *reinterpret_cast<const f4*>(sums + p.token * 16 + p.piece);
+    const unsigned here = present(t0 + p.token, last);
     float o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float z = gate.get(e), open = z * sigmoid(z);
       o[e] = a.skip ? fmaf(skip[e], x.get(e), v[e]) : v[e];
       o[e] *= a.gated ? open : 1.f;
-      o[e] = t0 + p.token < last ? o[e] : 0.f;
+      o[e] = masked(o[e], here);
     }
     out.put(p, t0, p.end, o);
   };
@@ -640,7 +644,7 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
 
   float s[4], dy[4];  // of the tile that is staged
   const auto stage = [&](const RowsOf& rows, int t0, f4* to) {
-    steps(a, rows.delta, bias, t0 + p.token < last, s);
+    steps(a, rows.delta, bias, present(t0 + p.token, last), s);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float z = rows.gate.get(e), open = z * sigmoid(z);
@@ -773,7 +777,7 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
         }
         if (tile > first + 1) next.fetch(a, p, from, t0 - 2 * TILE, last);
         if (!idle) {
-          const bool here = t0 + p.token < last;
+          const unsigned here = present(t0 + p.token, last);
           const int from4 = p.token * 16 + p.piece;
           const f4 yv = *reinterpret_cast<const f4*>(&out[0][from4]);
           const f4 fv = *reinterpret_cast<const f4*>(&out[1][from4]);
@@ -783,12 +787,12 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
           for (int e = 0; e < 4; ++e) {
             const float x = was.x.get(e), z = was.gate.get(e), sg = sigmoid(z);
             const float whole = a.skip ? fmaf(skip[e], x, yv[e]) : yv[e];
-            dz[e] = here ? was.dout.get(e) * whole * (sg * fmaf(z, 1.f - sg, 1.f)) : 0.f;
-            dx[e] = here ? fmaf(s0[e], fv[e], a.skip ? skip[e] * dy0[e] : 0.f) : 0.f;
+            dz[e] = masked(was.dout.get(e) * whole * (sg * fmaf(z, 1.f - sg, 1.f)), here);
+            dx[e] = masked(fmaf(s0[e], fv[e], a.skip ? skip[e] * dy0[e] : 0.f), here);
             const float v = fmaf(x, fv[e], sv[e] * LN2);
             const float soft = v * sigmoid(was.delta.get(e) + bias[e]);
-            dd[e] = here ? (a.softplus ? soft : v) : 0.f;
-            dskip[e] += here ? dy0[e] * x : 0.f;
+            dd[e] = masked(a.softplus ? soft : v, here);
+            dskip[e] = fmaf(dy0[e], x, dskip[e]);
             dbias[e] += dd[e];
           }
           dxs.put(p, t0, p.end, dx);
