@@ -20,9 +20,8 @@ __global__ void scan_backward_kernel(Scan);
 template <bool BWD>
 __global__ void carry_kernel(Scan);
 template <typename In>
-__global__ void join_bc_kernel(Join);
-__global__ void join_rows_kernel(const float*, long, long, long, float, float*);
-template <typename In>
+__global__ void join_kernel(Join);
+template <typename In, int ROWS>
 __global__ void step_kernel(Step);
 }  // namespace ss
 
@@ -72,6 +71,9 @@ bool whole_at(int bf16, std::initializer_list<const void*> arrays) {
     if (reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16)) return false;
   return true;
 }
+
+// Threads that keep the card busy.
+long busy_threads() { return 768L * m4::api_compute_units(); }
 
 // ---------------------------------------------------------- selective scan --
 
@@ -239,12 +241,13 @@ int run_carry(const ss::Scan& a, hipStream_t st) {
   });
 }
 
-int run_join(const char* name, const float* part, long rows, long stride, long count, float* out,
-             hipStream_t st) {
-  return api_launch(name, st, [&] {
-    hipLaunchKernelGGL(ss::join_rows_kernel, dim3(element_blocks(count)), dim3(256), 0, st, part,
-                       rows, stride, count, 1.f, out);
-  });
+template <typename In>
+void start_step(const ss::Step& a, int rows, unsigned blocks, hipStream_t st) {
+  const dim3 grid(blocks), block(ss::STEP_THREADS);
+  if (rows == 4)
+    hipLaunchKernelGGL((ss::step_kernel<In, 4>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((ss::step_kernel<In, 1>), grid, block, 0, st, a);
 }
 
 }  // namespace
@@ -339,22 +342,33 @@ int m4sl_scan_backward(const m4sl_scan* s, const int* lengths, const void* d_out
     }
     rc = run_scan("scan_backward", a, s->bf16, whole, true, true, st);
     if (rc) return rc;
-    ss::Join j{a.part_bc, a.blocks, a.B, a.T, a.G, a.N, lengths, grads->b, grads->c};
-    rc = api_launch("scan_join_bc", st, [&] {
-      const dim3 grid(element_blocks((long)a.B * a.T * a.G * a.N)), block(256);
+    ss::Join j{};
+    j.part_bc = a.part_bc;
+    j.part_a = a.part_a;
+    j.part_d = a.part_d;
+    j.bc_blocks = element_blocks((long)a.B * a.T * a.G * a.N);
+    j.blocks = a.blocks;
+    j.rows = a.B * a.NS;
+    j.B = a.B;
+    j.T = a.T;
+    j.D = a.D;
+    j.G = a.G;
+    j.N = a.N;
+    j.lengths = lengths;
+    j.db = grads->b;
+    j.dc = grads->c;
+    j.da = grads->a;
+    j.dskip = s->skip ? grads->skip : nullptr;
+    j.dbias = s->delta_bias ? grads->delta_bias : nullptr;
+    const bool sums = j.da || j.dskip || j.dbias;
+    const long columns = sums ? (long)a.D * (a.N + 2) : 0;
+    return api_launch("scan_join", st, [&] {
+      const dim3 grid(j.bc_blocks + (unsigned)((columns + 63) / 64)), block(256);
       if (s->bf16)
-        hipLaunchKernelGGL(ss::join_bc_kernel<ss::bf16_t>, grid, block, 0, st, j);
+        hipLaunchKernelGGL(ss::join_kernel<ss::bf16_t>, grid, block, 0, st, j);
       else
-        hipLaunchKernelGGL(ss::join_bc_kernel<float>, grid, block, 0, st, j);
+        hipLaunchKernelGGL(ss::join_kernel<float>, grid, block, 0, st, j);
     });
-    if (rc) return rc;
-    const long rows = (long)a.B * a.NS, states = (long)a.D * a.N;
-    if (grads->a) rc = run_join("scan_join_a", a.part_a, rows, states, states, grads->a, st);
-    if (!rc && grads->skip && s->skip)
-      rc = run_join("scan_join_skip", a.part_d, rows, 2L * a.D, a.D, grads->skip, st);
-    if (!rc && grads->delta_bias && s->delta_bias)
-      rc = run_join("scan_join_bias", a.part_d + a.D, rows, 2L * a.D, a.D, grads->delta_bias, st);
-    return rc;
   });
 }
 
@@ -390,18 +404,22 @@ int m4sl_scan_step(const m4sl_scan* s, const uint8_t* active, const float* state
     a.N = s->N;
     a.softplus = s->softplus;
     a.whole_n = a.N % 4 == 0 && whole_at(0, {a.a, state, new_state});
-    while (a.span < 2 && 4 << a.span < s->N) ++a.span;
-    const double blocks =
-        ((double)s->B * s->D * (1 << a.span) + ss::STEP_THREADS - 1) / ss::STEP_THREADS;
+    a.whole_bc = s->N % 4 == 0 && a.b.batch % 4 == 0 && a.c.batch % 4 == 0 && a.bg % 4 == 0 &&
+                 a.cg % 4 == 0 && whole_at(s->bf16, {a.b.p, a.c.p});
+    while (4 << a.span < s->N) ++a.span;
+    const long lanes = (long)s->D << a.span;
+    // Four rows a thread, where that leaves the card busy.
+    const int rows = lanes * s->B >= 4 * busy_threads() ? 4 : 1;
+    a.blocks = (int)((lanes + ss::STEP_THREADS - 1) / ss::STEP_THREADS);
+    const double blocks = (double)a.blocks * ((s->B + rows - 1) / rows);
     if (too_many(blocks, ss::STEP_THREADS))
       return api_fail(M4MR_EINVAL, at + "problem too large");
     hipStream_t st = static_cast<hipStream_t>(stream);
     return api_launch("scan_step", st, [&] {
-      const dim3 grid((unsigned)blocks), block(ss::STEP_THREADS);
       if (s->bf16)
-        hipLaunchKernelGGL(ss::step_kernel<ss::bf16_t>, grid, block, 0, st, a);
+        start_step<ss::bf16_t>(a, rows, (unsigned)blocks, st);
       else
-        hipLaunchKernelGGL(ss::step_kernel<float>, grid, block, 0, st, a);
+        start_step<float>(a, rows, (unsigned)blocks, st);
     });
   });
 }
@@ -446,9 +464,6 @@ int conv_vec(const m4sl_rows& x, int T, int D, int bf16,
   for (const void* p : arrays) whole = whole && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   return whole ? vec : 1;
 }
-
-// Threads that keep the card busy.
-long busy_threads() { return 768L * m4::api_compute_units(); }
 
 // The backward's lines (runs of rows) and blocks.
 struct ConvPlan {
@@ -552,7 +567,7 @@ int m4sl_conv_forward(const m4sl_rows* x, const float* weight, const float* bias
     if (!output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x->data, initial, output, state}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
-    const int vec = conv_vec(*x, T, D, bf16, {initial, output, state});
+    const int vec = conv_vec(*x, T, D, bf16, {weight, bias, initial, output, state});
     cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
     a.y = output;
     a.state = state;
@@ -597,7 +612,8 @@ int m4sl_conv_backward(const m4sl_rows* x, const float* weight, const float* bia
     const size_t need = m4sl_conv_backward_workspace_bytes(B, T, D, W, bf16);
     if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
-    const int vec = conv_vec(*x, T, D, bf16, {initial, d_output, d_state, d_x, d_initial});
+    const int vec =
+        conv_vec(*x, T, D, bf16, {weight, bias, initial, d_output, d_state, d_x, d_initial});
     const ConvPlan p = conv_plan(B, T, D, W, vec);
     cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
     const bool sums = d_weight || d_bias;
@@ -635,7 +651,7 @@ int m4sl_conv_step(const m4sl_rows* x, const float* weight, const float* bias,
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x->data, state, new_state, output}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
-    const int vec = conv_vec(*x, 1, D, bf16, {state, new_state, output});
+    const int vec = conv_vec(*x, 1, D, bf16, {weight, bias, state, new_state, output});
     cv::Step a{};
     a.x = x->data;
     a.xb = x->batch_stride;
@@ -694,7 +710,7 @@ struct RmsPlan {
   unsigned blocks;
 };
 
-RmsPlan rms_plan(long M, int C, int vec, rn::Rms* a) {
+RmsPlan rms_plan(long M, int C, int vec, bool backward, rn::Rms* a) {
   const int count = (C + vec - 1) / vec;
   RmsPlan p{};
   if (count <= 64) {
@@ -706,9 +722,10 @@ RmsPlan rms_plan(long M, int C, int vec, rn::Rms* a) {
     p.pieces = count <= few * 1024 ? few : vec == 8 ? 4 : 32;
     a->lanes = ((count + p.pieces - 1) / p.pieces + 63) / 64 * 64;
   }
-  a->rows = a->lanes <= 64 ? rn::THREADS / a->lanes : 1;
+  a->rows = a->lanes <= 64 ? (backward ? 1024 : rn::THREADS) / a->lanes : 1;
   p.threads = a->lanes * a->rows;
-  const long most = 2048L * m4::api_compute_units() / p.threads;
+  // (The backward's blocks leave partial sums: as few as keep the card busy.)
+  const long most = (backward ? 1024L : 2048L) * m4::api_compute_units() / p.threads;
   p.blocks = (unsigned)std::min((M + a->rows - 1) / a->rows, std::max(1L, most));
   a->M = M;
   a->C = C;
@@ -790,7 +807,7 @@ int m4sl_rms_forward(const void* x, int x_bf16, const void* residual, int residu
       return api_fail(M4MR_EINVAL, at + why);
     const int vec = rms_vec(C, {x, residual, weight, output, sum});
     rn::Rms a{};
-    const RmsPlan p = rms_plan(M, C, vec, &a);
+    const RmsPlan p = rms_plan(M, C, vec, false, &a);
     a.x = x;
     a.residual = residual;
     a.weight = weight;
@@ -819,7 +836,7 @@ int m4sl_rms_e4m3(const void* x, int x_bf16, const void* residual, int residual_
                       at + "a scale's block must be a power of two in 32..512, or at least C");
     const int vec = rms_vec(C, {x, residual, weight, output, sum});
     rn::Rms a{};
-    const RmsPlan p = rms_plan(M, C, vec, &a);
+    const RmsPlan p = rms_plan(M, C, vec, false, &a);
     a.x = x;
     a.residual = residual;
     a.weight = weight;
@@ -841,8 +858,8 @@ size_t m4sl_rms_backward_workspace_bytes(long M, int C) {
   if (bad_rms(M, C, &why)) return 0;
   // (The pieces depend on addresses.)
   rn::Rms a{};
-  unsigned blocks = rms_plan(M, C, 1, &a).blocks;
-  if (C % 8 == 0) blocks = std::max(blocks, rms_plan(M, C, 8, &a).blocks);
+  unsigned blocks = rms_plan(M, C, 1, true, &a).blocks;
+  if (C % 8 == 0) blocks = std::max(blocks, rms_plan(M, C, 8, true, &a).blocks);
   return align256((size_t)blocks * C * sizeof(float));
 }
 
@@ -863,7 +880,7 @@ int m4sl_rms_backward(const void* sum, int sum_bf16, const float* weight, const 
       return api_fail(M4MR_EINVAL, at + why);
     const int vec = rms_vec(C, {sum, weight, d_output, d_sum, d_x, d_residual});
     rn::Rms a{};
-    const RmsPlan p = rms_plan(M, C, vec, &a);
+    const RmsPlan p = rms_plan(M, C, vec, true, &a);
     a.x = sum;
     a.weight = weight;
     a.inverse = const_cast<float*>(inverse);

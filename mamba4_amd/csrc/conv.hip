@@ -83,14 +83,30 @@ __device__ __forceinline__ Piece<In, V> row(const Conv& a, long b, int c, int t,
   return r;
 }
 
+// The taps of a piece's channels, V * W consecutive floats, and the biases.
 template <int V, int W>
 __device__ __forceinline__ void load_taps(const float* weight, const float* bias, int c,
                                           float (&w)[W][V], float (&bv)[V]) {
+  const float* from = weight + (long)c * W;
+  if constexpr (V >= 4) {
+    f4 r[V * W / 4], b[V / 4];
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    bv[k] = bias ? bias[c + k] : 0.f;
+    for (int i = 0; i < V * W / 4; ++i) r[i] = reinterpret_cast<const f4*>(from)[i];
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j][k] = weight[(long)(c + k) * W + j];
+    for (int i = 0; i < V / 4; ++i) {
+      b[i] = f4{0.f, 0.f, 0.f, 0.f};
+      if (bias) b[i] = reinterpret_cast<const f4*>(bias + c)[i];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      bv[k] = b[k / 4][k % 4];
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j][k] = r[(k * W + j) / 4][(k * W + j) % 4];
+    }
+  } else {
+    bv[0] = bias ? bias[c] : 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][0] = from[j];
   }
 }
 

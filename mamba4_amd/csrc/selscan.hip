@@ -593,11 +593,24 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
     v = v < -3.4e38f ? -3.4e38f : v > 3.4e38f ? 3.4e38f : v;
     const float* from = BWD ? a.dstate : a.initial;
     float h = from ? from[i] : 0.f;
-    for (int j = 0; j < a.NS; ++j) {
-      const long row = b * a.NS + (BWD ? a.NS - 1 - j : j);
-      const float end = a.ends[row * each + rest];
-      a.ends[row * each + rest] = h;
-      h = fmaf(__builtin_amdgcn_exp2f(a.sums[row * a.D + d] * v), h, end);
+    // A batch of segments is loaded at a time: one after the other, each would wait for
+    // memory (B1 T2000 D1536 N16, 42 segments: 12 us).
+    constexpr int U = 8;
+    for (int j = 0; j < a.NS; j += U) {
+      float end[U], keep[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long row = b * a.NS + (BWD ? max(0, a.NS - 1 - j - u) : min(a.NS - 1, j + u));
+        end[u] = a.ends[row * each + rest];
+        keep[u] = __builtin_amdgcn_exp2f(a.sums[row * a.D + d] * v);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j + u >= a.NS) continue;
+        const long row = b * a.NS + (BWD ? a.NS - 1 - j - u : j + u);
+        a.ends[row * each + rest] = h;
+        h = fmaf(keep[u], h, end[u]);
+      }
     }
     if (BWD && a.dinitial) a.dinitial[i] = h;
   }
@@ -824,98 +837,138 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   }
 }
 
-// The gradients of b and c: the sums over the channel blocks.
+// The gradients of b and c: the sums over the channel blocks, in their order; by the
+// first `bc_blocks` blocks.  By the rest those of a, skip and the bias: the sums over the
+// batch rows and segments, in four parts, joined in their order.
 template <typename In>
-__global__ __launch_bounds__(256) void join_bc_kernel(Join a) {
-  const long each = (long)a.G * a.N, tokens = (long)a.B * a.T, count = tokens * each;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) {
-    const long token = i / each, rest = i - token * each;
-    const long g = rest / a.N, n = rest - g * a.N;
-    const long b = token / a.T;
-    const bool here = !a.lengths || token - b * a.T < a.lengths[b];
-    const float* from = a.part_bc + (token * a.G + g) * 2 * a.N + n;
-    float db = 0.f, dc = 0.f;
-    if (here)
-      for (int j = 0; j < a.blocks; ++j) {
-        db += from[j * tokens * each * 2];
-        dc += from[j * tokens * each * 2 + a.N];
+__global__ __launch_bounds__(256) void join_kernel(Join a) {
+  constexpr int U = 8;
+  if (blockIdx.x < a.bc_blocks) {
+    const long each = (long)a.G * a.N, tokens = (long)a.B * a.T, count = tokens * each;
+    const long stride = 2 * tokens * each;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += a.bc_blocks * 256L) {
+      const long token = i / each, rest = i - token * each;
+      const long g = rest / a.N, n = rest - g * a.N;
+      const long b = token / a.T;
+      const bool here = !a.lengths || token - b * a.T < a.lengths[b];
+      const float* from = a.part_bc + (token * a.G + g) * 2 * a.N + n;
+      float db = 0.f, dc = 0.f;
+      if (here)
+        for (int j = 0; j < a.blocks; j += U) {
+          float vb[U], vc[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const long at = min(j + u, a.blocks - 1) * stride;
+            vb[u] = from[at];
+            vc[u] = from[at + a.N];
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (j + u < a.blocks) {
+              db += vb[u];
+              dc += vc[u];
+            }
+        }
+      if constexpr (sizeof(In) == 4) {
+        static_cast<float*>(a.db)[i] = db;
+        static_cast<float*>(a.dc)[i] = dc;
+      } else {
+        static_cast<bf16_t*>(a.db)[i] = (bf16_t)pack(db, 0.f);
+        static_cast<bf16_t*>(a.dc)[i] = (bf16_t)pack(dc, 0.f);
       }
-    if constexpr (sizeof(In) == 4) {
-      static_cast<float*>(a.db)[i] = db;
-      static_cast<float*>(a.dc)[i] = dc;
-    } else {
-      static_cast<bf16_t*>(a.db)[i] = (bf16_t)pack(db, 0.f);
-      static_cast<bf16_t*>(a.dc)[i] = (bf16_t)pack(dc, 0.f);
     }
+    return;
   }
-}
-
-// Sums over rows ([rows][stride], `count` of each from `part` on): of the batch rows and
-// segments.
-__global__ __launch_bounds__(256) void join_rows_kernel(const float* part, long rows, long stride,
-                                                        long count, float scale, float* out) {
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long)gridDim.x * 256) {
-    float s = 0.f;
-    for (long j = 0; j < rows; ++j) s += part[j * stride + i];
-    out[i] = s * scale;
+  __shared__ float fold[256];
+  const int slice = threadIdx.x >> 6;
+  const long states = (long)a.D * a.N;
+  const long i = (long)(blockIdx.x - a.bc_blocks) * 64 + (threadIdx.x & 63);
+  const bool on = i < states + 2L * a.D, of_a = i < states;
+  const float* from = of_a ? a.part_a + i : a.part_d + (i - states);
+  const long stride = of_a ? states : 2L * a.D;
+  const int quarter = (a.rows + 3) / 4, end = min(a.rows, (slice + 1) * quarter);
+  float s = 0.f;
+  for (int j = slice * quarter; on && j < end; j += U) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = from[min(j + u, end - 1) * stride];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j + u < end) s += v[u];
   }
+  fold[threadIdx.x] = s;
+  __syncthreads();
+  if (slice || !on) return;
+  for (int k = 1; k < 4; ++k) s += fold[threadIdx.x + 64 * k];
+  const long d = i - states;
+  float* to = of_a ? a.da : d < a.D ? a.dskip : a.dbias;
+  if (to) to[of_a ? i : d < a.D ? d : d - a.D] = s;
 }
 
 // ------------------------------------------------------------ one token
 
-// Bound by memory: the states are read and written once.  2^span lanes hold a
-// channel, four states each at a time.
-template <typename In>
+// Bound by memory: the states are read and written once.  2^span lanes hold a channel,
+// four states each, and take ROWS batch rows, whose loads are in flight together; what
+// belongs to the channel stays in registers.
+template <typename In, int ROWS>
 __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
-  const long i = (long)blockIdx.x * STEP_THREADS + threadIdx.x;
-  const long row = i >> a.span;
-  const int part = (int)(i & ((1 << a.span) - 1));
-  if (row >= a.B * a.D) return;
-  const long b = row / a.D;
-  const int d = (int)(row - b * a.D), g = d / a.Dg;
-  const bool on = !a.active || a.active[b];
+  const int rows = blockIdx.x / a.blocks;
+  const long i = (long)(blockIdx.x - rows * a.blocks) * STEP_THREADS + threadIdx.x;
+  const int d = (int)(i >> a.span), n = 4 * ((int)i & ((1 << a.span) - 1));
+  if (d >= a.D) return;
+  const int g = d / a.Dg, have = min(4, max(0, a.N - n));
   const auto one = [](const void* p, long at) {
     const In v = static_cast<const In*>(p)[at];
     if constexpr (sizeof(In) == 4) return (float)v;
     else return __uint_as_float((unsigned)v << 16);
   };
-  const float* from = a.state + row * a.N;
-  float* to = a.new_state + row * a.N;
-  float x = 0.f, s = 0.f, y = 0.f;
-  if (on) {
-    x = one(a.x.p, b * a.x.batch + d);
-    s = one(a.delta.p, b * a.delta.batch + d) + (a.bias ? a.bias[d] : 0.f);
-    if (a.softplus) s = softplus(s);
-  }
-  const float u = s * x;
-  const bool whole = a.whole_n;
-  for (int n = 4 * part; n < a.N; n += 4 << a.span) {
-    const int have = min(4, a.N - n);
-    const Four<float> h = load4(from + n, have, whole);
-    const Four<float> rate = load4(a.a + (long)d * a.N + n, have, whole);
-    float v[4];
+  Four<float> rate = load4(a.a + (long)d * a.N + n, have, a.whole_n);
+  const float bias = a.bias ? a.bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+  const long first = (long)rows * ROWS;
+  Four<float> h[ROWS];
+  Four<In> b[ROWS], c[ROWS];
+  float x[ROWS], delta[ROWS], z[ROWS];
+  bool on[ROWS];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      v[r] = h.get(r);
-      if (on && r < have) {
-        v[r] = fmaf(__builtin_amdgcn_exp2f(s * (rate.get(r) * LOG2E)), v[r],
-                    u * one(a.b.p, b * a.b.batch + g * a.bg + n + r));
-        y = fmaf(one(a.c.p, b * a.c.batch + g * a.cg + n + r), v[r], y);
+  for (int j = 0; j < ROWS; ++j) {
+    const long row = first + j;
+    on[j] = row < a.B && (!a.active || a.active[row]);
+    if (row < a.B) h[j] = load4(a.state + (row * a.D + d) * a.N + n, have, a.whole_n);
+    if (!on[j]) continue;
+    b[j] = load4(static_cast<const In*>(a.b.p) + row * a.b.batch + g * a.bg + n, have, a.whole_bc);
+    c[j] = load4(static_cast<const In*>(a.c.p) + row * a.c.batch + g * a.cg + n, have, a.whole_bc);
+    x[j] = one(a.x.p, row * a.x.batch + d);
+    delta[j] = one(a.delta.p, row * a.delta.batch + d);
+    if (a.gate.p) z[j] = one(a.gate.p, row * a.gate.batch + d);
+  }
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const long row = first + j;
+    if (row >= a.B) return;
+    float v[4], y = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = h[j].get(r);
+    if (on[j]) {
+      float s = delta[j] + bias;
+      if (a.softplus) s = softplus(s);
+      const float u = s * x[j];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[r] = fmaf(__builtin_amdgcn_exp2f(s * (rate.get(r) * LOG2E)), v[r], u * b[j].get(r));
+        y = fmaf(c[j].get(r), v[r], y);
       }
     }
-    if (on || to != from) store4(to + n, v, have, whole);
-  }
-  for (int m = 1; m < 1 << a.span; m *= 2) y += __shfl_xor(y, m);
-  if (part) return;
-  if (on) {
-    if (a.skip) y = fmaf(a.skip[d], x, y);
-    if (a.gate.p) {
-      const float z = one(a.gate.p, b * a.gate.batch + d);
-      y *= z * sigmoid(z);
+    if (on[j] || a.new_state != a.state)
+      store4(a.new_state + (row * a.D + d) * a.N + n, v, have, a.whole_n);
+    for (int m = 1; m < 1 << a.span; m *= 2) y += __shfl_xor(y, m);
+    if (n) continue;
+    if (on[j]) {
+      if (a.skip) y = fmaf(skip, x[j], y);
+      if (a.gate.p) y *= z[j] * sigmoid(z[j]);
     }
+    if constexpr (sizeof(In) == 4) static_cast<float*>(a.out)[row * a.D + d] = y;
+    else static_cast<bf16_t*>(a.out)[row * a.D + d] = (bf16_t)pack(y, 0.f);
   }
-  if constexpr (sizeof(In) == 4) static_cast<float*>(a.out)[row] = y;
-  else static_cast<bf16_t*>(a.out)[row] = (bf16_t)pack(y, 0.f);
 }
 
 #define M4SL_SCAN_GROUPS(In, NG)                                            \
@@ -931,8 +984,9 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   M4SL_SCAN_GROUPS(In, 1)                            \
   M4SL_SCAN_GROUPS(In, 2)                            \
   M4SL_SCAN_GROUPS(In, 4)                            \
-  template __global__ void join_bc_kernel<In>(Join); \
-  template __global__ void step_kernel<In>(Step);
+  template __global__ void join_kernel<In>(Join);    \
+  template __global__ void step_kernel<In, 1>(Step); \
+  template __global__ void step_kernel<In, 4>(Step);
 M4SL_SCAN(float)
 M4SL_SCAN(bf16_t)
 template __global__ void carry_kernel<false>(Scan);

@@ -46,11 +46,15 @@ struct Scan {
   float* part_d;                  // [B,NS][2][D]: of skip and bias
 };
 
+// The sums of the backward's parts.
 struct Join {
-  const float* part_bc;
-  int blocks, B, T, G, N;
+  const float *part_bc, *part_a, *part_d;
+  unsigned bc_blocks;             // blocks of the launch that join b's and c's
+  int blocks, rows;               // channel blocks; batch rows and segments
+  int B, T, D, G, N;
   const int* lengths;
   void *db, *dc;
+  float *da, *dskip, *dbias;      // or NULL
 };
 
 struct Step {
@@ -63,8 +67,9 @@ struct Step {
   void* out;
   long B;
   int D, Dg, N, softplus;
-  int whole_n;                    // states and a are read in pieces of four
+  int whole_n, whole_bc;          // states and a, b and c are read in pieces of four
   int span;                       // 2^span threads hold a channel's states
+  int blocks;                     // of all channels
 };
 
 }  // namespace ss
