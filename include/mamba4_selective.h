@@ -116,7 +116,7 @@ int m4sl_conv_forward(const m4sl_rows* x, const float* weight, const float* bias
  * type: d_x [B,T,D] and d_initial [B,W-1,D] in x's type, d_weight [D,W] and
  * d_bias [D] float32, each NULL if not wanted.  Sums are float32 in a fixed order.
  */
-size_t m4sl_conv_backward_workspace_bytes(int B, int T, int D, int W, int bf16);
+size_t m4sl_conv_backward_workspace_bytes(int B, int T, int D, int W);
 int m4sl_conv_backward(const m4sl_rows* x, const float* weight, const float* bias,
                        const void* initial, const int* lengths, const void* d_output,
                        const void* d_state, int bf16, int B, int T, int D, int W,

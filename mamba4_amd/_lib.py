@@ -158,7 +158,7 @@ SIGNATURES = {
     "m4sl_scan_backward": (_I, [_P] * 7 + [_S, _P]),
     "m4sl_scan_step": (_I, [_P] * 6),
     "m4sl_conv_forward": (_I, [_P] * 5 + [_I] * 6 + [_P] * 3),
-    "m4sl_conv_backward_workspace_bytes": (_S, [_I] * 5),
+    "m4sl_conv_backward_workspace_bytes": (_S, [_I] * 4),
     "m4sl_conv_backward": (_I, [_P] * 7 + [_I] * 6 + [_P] * 5 + [_S, _P]),
     "m4sl_rms_forward": (_I, [_P, _I] * 2 + [_P, _L, _I, _F] + [_P] * 4),
     "m4sl_rms_e4m3": (_I, [_P, _I] * 2 + [_P, _L, _I, _F, _I] + [_P] * 4),

@@ -79,7 +79,7 @@ class _CausalConv(torch.autograd.Function):
         lib = _lib.load()
         sizes = (batch, time, channels, taps)
         bf16 = x.dtype == _BF16
-        nbytes = lib.m4sl_conv_backward_workspace_bytes(*sizes, bf16)
+        nbytes = lib.m4sl_conv_backward_workspace_bytes(*sizes)
         workspace = _workspace(nbytes, device)
         d_x, d_weight, d_bias, d_initial = grads
         rc = lib.m4sl_conv_backward(

@@ -30,7 +30,7 @@ template <typename In, int V, int W>
 __global__ void conv_kernel(Conv);
 template <typename In, int V, int W>
 __global__ void conv_backward_kernel(Conv);
-template <typename In, int V, int W>
+template <typename In, int V, int W, int ROWS>
 __global__ void conv_step_kernel(Step);
 __global__ void conv_join_kernel(const float*, int, int, int, float*, float*);
 }  // namespace cv
@@ -455,14 +455,15 @@ bool bad_conv(const m4sl_rows* x, const float* weight, int B, int T, int D, int 
   return false;
 }
 
-// Channels of a thread's piece: 16 bytes, where all rows consist of such pieces.
-int conv_vec(const m4sl_rows& x, int T, int D, int bf16,
+// Channels of a thread's piece: four, where all rows consist of such pieces and the
+// parameters (float32) are aligned to theirs.
+int conv_vec(const m4sl_rows& x, int T, int D, int bf16, const float* weight, const float* bias,
              std::initializer_list<const void*> arrays) {
-  const int vec = bf16 ? 8 : 4;
-  bool whole = D % vec == 0 && x.batch_stride % vec == 0 && (T == 1 || x.token_stride % vec == 0) &&
-               reinterpret_cast<uintptr_t>(x.data) % 16 == 0;
-  for (const void* p : arrays) whole = whole && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  return whole ? vec : 1;
+  return D % 4 == 0 && x.batch_stride % 4 == 0 && (T == 1 || x.token_stride % 4 == 0) &&
+                 whole_at(bf16, {x.data}) && whole_at(bf16, arrays) &&
+                 whole_at(0, {weight, bias})
+             ? 4
+             : 1;
 }
 
 // The backward's lines (runs of rows) and blocks.
@@ -497,18 +498,19 @@ template <typename In, int V, int W>
 void start_conv_backward(const cv::Conv& a, dim3 grid, hipStream_t st) {
   hipLaunchKernelGGL((cv::conv_backward_kernel<In, V, W>), grid, dim3(cv::THREADS), 0, st, a);
 }
-template <typename In, int V, int W>
+template <typename In, int V, int W, int ROWS>
 void start_conv_step(const cv::Step& a, dim3 grid, hipStream_t st) {
-  hipLaunchKernelGGL((cv::conv_step_kernel<In, V, W>), grid, dim3(cv::THREADS), 0, st, a);
+  hipLaunchKernelGGL((cv::conv_step_kernel<In, V, W, ROWS>), grid, dim3(cv::THREADS), 0, st, a);
 }
 
-enum class Conv { FORWARD, BACKWARD, STEP };
+enum class Conv { FORWARD, BACKWARD, STEP, STEP_ROWS };
+constexpr int STEP_ROWS = 4;
 
 template <Conv WHAT, typename In, int V, int W, typename Args>
 void start_one(const Args& a, dim3 grid, hipStream_t st) {
   if constexpr (WHAT == Conv::FORWARD) start_conv<In, V, W>(a, grid, st);
   else if constexpr (WHAT == Conv::BACKWARD) start_conv_backward<In, V, W>(a, grid, st);
-  else start_conv_step<In, V, W>(a, grid, st);
+  else start_conv_step<In, V, W, WHAT == Conv::STEP ? 1 : STEP_ROWS>(a, grid, st);
 }
 
 template <Conv WHAT, typename In, int V, typename Args>
@@ -528,7 +530,7 @@ void start_taps(const Args& a, int W, dim3 grid, hipStream_t st) {
 template <Conv WHAT, typename Args>
 void start_width(const Args& a, int bf16, int vec, int W, dim3 grid, hipStream_t st) {
   if (bf16) {
-    if (vec == 8) return start_taps<WHAT, cv::bf16_t, 8>(a, W, grid, st);
+    if (vec == 4) return start_taps<WHAT, cv::bf16_t, 4>(a, W, grid, st);
     return start_taps<WHAT, cv::bf16_t, 1>(a, W, grid, st);
   }
   if (vec == 4) return start_taps<WHAT, float, 4>(a, W, grid, st);
@@ -567,7 +569,7 @@ int m4sl_conv_forward(const m4sl_rows* x, const float* weight, const float* bias
     if (!output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x->data, initial, output, state}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
-    const int vec = conv_vec(*x, T, D, bf16, {weight, bias, initial, output, state});
+    const int vec = conv_vec(*x, T, D, bf16, weight, bias, {initial, output, state});
     cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
     a.y = output;
     a.state = state;
@@ -585,14 +587,13 @@ int m4sl_conv_forward(const m4sl_rows* x, const float* weight, const float* bias
   });
 }
 
-size_t m4sl_conv_backward_workspace_bytes(int B, int T, int D, int W, int bf16) {
+size_t m4sl_conv_backward_workspace_bytes(int B, int T, int D, int W) {
   std::string why;
   const m4sl_rows any{&why, 0, 0};
   if (bad_conv(&any, reinterpret_cast<const float*>(&why), B, T, D, W, M4SL_NONE, &why)) return 0;
   // (The pieces depend on addresses.)
   size_t rows = conv_plan(B, T, D, W, 1).rows;
-  const int vec = bf16 ? 8 : 4;
-  if (D % vec == 0) rows = std::max<size_t>(rows, conv_plan(B, T, D, W, vec).rows);
+  if (D % 4 == 0) rows = std::max<size_t>(rows, conv_plan(B, T, D, W, 4).rows);
   return align256(rows * (W + 1) * D * sizeof(float));
 }
 
@@ -609,11 +610,11 @@ int m4sl_conv_backward(const m4sl_rows* x, const float* weight, const float* bia
     if (!d_output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x->data, initial, d_output, d_state, d_x, d_initial}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
-    const size_t need = m4sl_conv_backward_workspace_bytes(B, T, D, W, bf16);
+    const size_t need = m4sl_conv_backward_workspace_bytes(B, T, D, W);
     if (bad_workspace(workspace, workspace_bytes, need, &why))
       return api_fail(M4MR_EINVAL, at + why);
-    const int vec =
-        conv_vec(*x, T, D, bf16, {weight, bias, initial, d_output, d_state, d_x, d_initial});
+    const int vec = conv_vec(*x, T, D, bf16, weight, bias,
+                             {initial, d_output, d_state, d_x, d_initial});
     const ConvPlan p = conv_plan(B, T, D, W, vec);
     cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
     const bool sums = d_weight || d_bias;
@@ -651,7 +652,7 @@ int m4sl_conv_step(const m4sl_rows* x, const float* weight, const float* bias,
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x->data, state, new_state, output}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
-    const int vec = conv_vec(*x, 1, D, bf16, {weight, bias, state, new_state, output});
+    const int vec = conv_vec(*x, 1, D, bf16, weight, bias, {state, new_state, output});
     cv::Step a{};
     a.x = x->data;
     a.xb = x->batch_stride;
@@ -665,11 +666,17 @@ int m4sl_conv_step(const m4sl_rows* x, const float* weight, const float* bias,
     a.D = D;
     a.act = activation;
     a.cols = D / vec;
-    const double blocks = ((double)B * a.cols + cv::THREADS - 1) / cv::THREADS;
+    a.blocks = (a.cols + cv::THREADS - 1) / cv::THREADS;
+    const bool rows = (long)B * a.cols >= STEP_ROWS * busy_threads() / 2;
+    const double blocks = (double)a.blocks * (rows ? (B + STEP_ROWS - 1) / STEP_ROWS : B);
     if (too_many(blocks, cv::THREADS)) return api_fail(M4MR_EINVAL, at + "problem too large");
     hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid((unsigned)blocks);
     return api_launch("conv_step", st, [&] {
-      start_width<Conv::STEP>(a, bf16, vec, W, dim3((unsigned)blocks), st);
+      if (rows)
+        start_width<Conv::STEP_ROWS>(a, bf16, vec, W, grid, st);
+      else
+        start_width<Conv::STEP>(a, bf16, vec, W, grid, st);
     });
   });
 }

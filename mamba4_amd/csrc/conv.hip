@@ -2,10 +2,12 @@
 //   z_t = bias + sum over j < W of w[j] x_{t-W+1+j},   y_t = act(z_t).
 // Gradient, with dz = dy act'(z):
 //   dx_s = sum over j of w[j] dz_{s+W-1-j},   dw[j] = sum over t of dz_t x_{t-W+1+j}.
-// It moves data and computes little: a thread holds a 16-byte piece of channels and
-// walks a run of tokens, several rows in flight at a time, with the last W - 1 rows
-// (backward: and the last W - 1 dz) in registers, so that rows are read once but for
-// the W - 1 at a run's edge.  The backward forms z again instead of keeping it.
+// It moves data and computes little: a thread holds a piece of four channels and walks a
+// run of tokens, several rows in flight at a time, with the last W - 1 rows (backward:
+// and the last W - 1 dz) in registers, so that rows are read once but for the W - 1 at a
+// run's edge.  The backward forms z again instead of keeping it.  (Pieces of eight
+// bfloat16 channels, 16 bytes, leave two waves a SIMD in the backward: B16 T1024 D1536
+// W4 60 us for 47 here, and 28 for 24 in the forward.)
 #include <hip/hip_runtime.h>
 
 #include "conv.hpp"
@@ -13,7 +15,7 @@
 namespace cv {
 
 typedef float f2 __attribute__((ext_vector_type(2)));
-typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
@@ -21,7 +23,7 @@ __device__ __forceinline__ unsigned pack(float a, float b) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
 }
 
-// V channels as they are in memory: 16 bytes, or a single element.
+// V channels as they are in memory: four, or a single one.
 template <typename In, int V>
 struct Piece;
 template <>
@@ -37,13 +39,13 @@ struct Piece<float, 1> {
   __device__ __forceinline__ void set(const float (&v)[1]) { r = v[0]; }
 };
 template <>
-struct Piece<bf16_t, 8> {
-  u4 r = {0, 0, 0, 0};
+struct Piece<bf16_t, 4> {
+  u2 r = {0, 0};
   __device__ __forceinline__ float get(int i) const {
     return __uint_as_float(i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
   }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-    r = u4{pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])};
+  __device__ __forceinline__ void set(const float (&v)[4]) {
+    r = u2{pack(v[0], v[1]), pack(v[2], v[3])};
   }
 };
 template <>
@@ -88,18 +90,14 @@ template <int V, int W>
 __device__ __forceinline__ void load_taps(const float* weight, const float* bias, int c,
                                           float (&w)[W][V], float (&bv)[V]) {
   const float* from = weight + (long)c * W;
-  if constexpr (V >= 4) {
-    f4 r[V * W / 4], b[V / 4];
+  if constexpr (V == 4) {
+    f4 r[W], b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < V * W / 4; ++i) r[i] = reinterpret_cast<const f4*>(from)[i];
+    for (int i = 0; i < W; ++i) r[i] = reinterpret_cast<const f4*>(from)[i];
+    if (bias) b = *reinterpret_cast<const f4*>(bias + c);
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-      b[i] = f4{0.f, 0.f, 0.f, 0.f};
-      if (bias) b[i] = reinterpret_cast<const f4*>(bias + c)[i];
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      bv[k] = b[k / 4][k % 4];
+    for (int k = 0; k < 4; ++k) {
+      bv[k] = b[k];
 #pragma unroll
       for (int j = 0; j < W; ++j) w[j][k] = r[(k * W + j) / 4][(k * W + j) % 4];
     }
@@ -307,40 +305,56 @@ __global__ __launch_bounds__(1024) void conv_join_kernel(const float* part, int 
 
 // ------------------------------------------------------------ one token
 
-template <typename In, int V, int W>
+// Bound by memory; a thread takes ROWS batch rows, whose loads are in flight together, with
+// the taps of its channels in registers (2,048 rows of 1536 bfloat16: one row 25 us).
+template <typename In, int V, int W, int ROWS>
 __global__ __launch_bounds__(THREADS) void conv_step_kernel(Step a) {
-  const long i = (long)blockIdx.x * THREADS + threadIdx.x;
-  const long b = i / a.cols;
-  const int c = (int)(i - b * a.cols) * V;
-  if (b >= a.B) return;
-  const bool on = !a.active || a.active[b];
-  Piece<In, V> x[W];
+  const int rows = blockIdx.x / a.blocks;
+  const int i = (blockIdx.x - rows * a.blocks) * THREADS + threadIdx.x;
+  if (i >= a.cols) return;
+  const int c = i * V;
+  const long first = (long)rows * ROWS;
+  Piece<In, V> x[ROWS][W];
+  bool on[ROWS];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) x[j] = load<In, V>(a.state, (b * (W - 1) + j) * a.D + c);
-  if (on) x[W - 1] = load<In, V>(a.x, b * a.xb + c);
-  float w[W][V], y[V];
-  load_taps<V, W>(a.weight, a.bias, c, w, y);
+  for (int m = 0; m < ROWS; ++m) {
+    const long b = first + m;
+    on[m] = b < a.B && (!a.active || a.active[b]);
+    if (b >= a.B) continue;
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    float z = y[k];
-#pragma unroll
-    for (int j = 0; j < W; ++j) z = fmaf(w[j][k], x[j].get(k), z);
-    if (a.act == SILU) z *= sigmoid(z);
-    y[k] = on ? z : 0.f;
+    for (int j = 0; j < W - 1; ++j) x[m][j] = load<In, V>(a.state, (b * (W - 1) + j) * a.D + c);
+    if (on[m]) x[m][W - 1] = load<In, V>(a.x, b * a.xb + c);
   }
-  Piece<In, V> p;
-  p.set(y);
-  store<In, V>(a.y, b * a.D + c, p);
-  if (on || a.new_state != a.state)
+  float w[W][V], bias[V];
+  load_taps<V, W>(a.weight, a.bias, c, w, bias);
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j)
-      store<In, V>(a.new_state, (b * (W - 1) + j) * a.D + c, on ? x[j + 1] : x[j]);
+  for (int m = 0; m < ROWS; ++m) {
+    const long b = first + m;
+    if (b >= a.B) return;
+    float y[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float z = bias[k];
+#pragma unroll
+      for (int j = 0; j < W; ++j) z = fmaf(w[j][k], x[m][j].get(k), z);
+      if (a.act == SILU) z *= sigmoid(z);
+      y[k] = on[m] ? z : 0.f;
+    }
+    Piece<In, V> p;
+    p.set(y);
+    store<In, V>(a.y, b * a.D + c, p);
+    if (on[m] || a.new_state != a.state)
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+        store<In, V>(a.new_state, (b * (W - 1) + j) * a.D + c, on[m] ? x[m][j + 1] : x[m][j]);
+  }
 }
 
 #define M4SL_CONV_TAPS(In, V, W)                             \
   template __global__ void conv_kernel<In, V, W>(Conv);      \
   template __global__ void conv_backward_kernel<In, V, W>(Conv); \
-  template __global__ void conv_step_kernel<In, V, W>(Step);
+  template __global__ void conv_step_kernel<In, V, W, 1>(Step);  \
+  template __global__ void conv_step_kernel<In, V, W, 4>(Step);
 #define M4SL_CONV(In, V)   \
   M4SL_CONV_TAPS(In, V, 1) \
   M4SL_CONV_TAPS(In, V, 2) \
@@ -352,7 +366,7 @@ __global__ __launch_bounds__(THREADS) void conv_step_kernel(Step a) {
   M4SL_CONV_TAPS(In, V, 8)
 M4SL_CONV(float, 4)
 M4SL_CONV(float, 1)
-M4SL_CONV(bf16_t, 8)
+M4SL_CONV(bf16_t, 4)
 M4SL_CONV(bf16_t, 1)
 
 }  // namespace cv

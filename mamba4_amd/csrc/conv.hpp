@@ -41,6 +41,7 @@ struct Step {
   void *new_state, *y;
   long B;
   int D, act, cols;
+  int blocks;                    // of a row
 };
 
 }  // namespace cv
