@@ -455,15 +455,21 @@ bool bad_conv(const m4sl_rows* x, const float* weight, int B, int T, int D, int 
   return false;
 }
 
-// Channels of a thread's piece: four, where all rows consist of such pieces and the
-// parameters (float32) are aligned to theirs.
+// Whether all rows consist of aligned pieces of `vec` channels, and the parameters
+// (float32) are aligned to pieces of four.
+bool conv_pieces(int vec, const m4sl_rows& x, int T, int D, int bf16, const float* weight,
+                 const float* bias, std::initializer_list<const void*> arrays) {
+  const int bytes = vec * (bf16 ? 2 : 4);
+  bool whole = D % vec == 0 && x.batch_stride % vec == 0 && (T == 1 || x.token_stride % vec == 0) &&
+               reinterpret_cast<uintptr_t>(x.data) % bytes == 0 && whole_at(0, {weight, bias});
+  for (const void* p : arrays) whole = whole && reinterpret_cast<uintptr_t>(p) % bytes == 0;
+  return whole;
+}
+
+// Channels of a thread's piece: four if they can be.
 int conv_vec(const m4sl_rows& x, int T, int D, int bf16, const float* weight, const float* bias,
              std::initializer_list<const void*> arrays) {
-  return D % 4 == 0 && x.batch_stride % 4 == 0 && (T == 1 || x.token_stride % 4 == 0) &&
-                 whole_at(bf16, {x.data}) && whole_at(bf16, arrays) &&
-                 whole_at(0, {weight, bias})
-             ? 4
-             : 1;
+  return conv_pieces(4, x, T, D, bf16, weight, bias, arrays) ? 4 : 1;
 }
 
 // The backward's lines (runs of rows) and blocks.
@@ -530,6 +536,8 @@ void start_taps(const Args& a, int W, dim3 grid, hipStream_t st) {
 template <Conv WHAT, typename Args>
 void start_width(const Args& a, int bf16, int vec, int W, dim3 grid, hipStream_t st) {
   if (bf16) {
+    if constexpr (WHAT == Conv::FORWARD)
+      if (vec == 8) return start_taps<WHAT, cv::bf16_t, 8>(a, W, grid, st);
     if (vec == 4) return start_taps<WHAT, cv::bf16_t, 4>(a, W, grid, st);
     return start_taps<WHAT, cv::bf16_t, 1>(a, W, grid, st);
   }
@@ -569,7 +577,9 @@ int m4sl_conv_forward(const m4sl_rows* x, const float* weight, const float* bias
     if (!output) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(bf16, {x->data, initial, output, state}))
       return api_fail(M4MR_EINVAL, at + "arrays must be aligned to their elements");
-    const int vec = conv_vec(*x, T, D, bf16, weight, bias, {initial, output, state});
+    const bool wide =
+        bf16 && conv_pieces(8, *x, T, D, bf16, weight, bias, {initial, output, state});
+    const int vec = wide ? 8 : conv_vec(*x, T, D, bf16, weight, bias, {initial, output, state});
     cv::Conv a = conv_of(*x, weight, bias, initial, lengths, B, T, D, activation);
     a.y = output;
     a.state = state;

@@ -2,12 +2,12 @@
 //   z_t = bias + sum over j < W of w[j] x_{t-W+1+j},   y_t = act(z_t).
 // Gradient, with dz = dy act'(z):
 //   dx_s = sum over j of w[j] dz_{s+W-1-j},   dw[j] = sum over t of dz_t x_{t-W+1+j}.
-// It moves data and computes little: a thread holds a piece of four channels and walks a
-// run of tokens, several rows in flight at a time, with the last W - 1 rows (backward:
-// and the last W - 1 dz) in registers, so that rows are read once but for the W - 1 at a
-// run's edge.  The backward forms z again instead of keeping it.  (Pieces of eight
-// bfloat16 channels, 16 bytes, leave two waves a SIMD in the backward: B16 T1024 D1536
-// W4 60 us for 47 here, and 28 for 24 in the forward.)
+// It moves data and computes little: a thread holds a piece of four channels (forward:
+// eight, where they are bfloat16) and walks a run of tokens, several rows in flight at a
+// time, with the last W - 1 rows (backward: and the last W - 1 dz) in registers, so that
+// rows are read once but for the W - 1 at a run's edge.  The backward forms z again
+// instead of keeping it.  (Pieces of eight bfloat16 channels leave it two waves a SIMD:
+// B16 T1024 D1536 W4 77 us for 54; the forward takes 30 us with them and 35 with four.)
 #include <hip/hip_runtime.h>
 
 #include "conv.hpp"
@@ -16,6 +16,7 @@ namespace cv {
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
@@ -23,7 +24,7 @@ __device__ __forceinline__ unsigned pack(float a, float b) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, b2));
 }
 
-// V channels as they are in memory: four, or a single one.
+// V channels as they are in memory.
 template <typename In, int V>
 struct Piece;
 template <>
@@ -37,6 +38,16 @@ struct Piece<float, 1> {
   float r = 0.f;
   __device__ __forceinline__ float get(int) const { return r; }
   __device__ __forceinline__ void set(const float (&v)[1]) { r = v[0]; }
+};
+template <>
+struct Piece<bf16_t, 8> {
+  u4 r = {0, 0, 0, 0};
+  __device__ __forceinline__ float get(int i) const {
+    return __uint_as_float(i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    r = u4{pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])};
+  }
 };
 template <>
 struct Piece<bf16_t, 4> {
@@ -90,14 +101,18 @@ template <int V, int W>
 __device__ __forceinline__ void load_taps(const float* weight, const float* bias, int c,
                                           float (&w)[W][V], float (&bv)[V]) {
   const float* from = weight + (long)c * W;
-  if constexpr (V == 4) {
-    f4 r[W], b = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (V >= 4) {
+    f4 r[V / 4 * W], b[V / 4];
 #pragma unroll
-    for (int i = 0; i < W; ++i) r[i] = reinterpret_cast<const f4*>(from)[i];
-    if (bias) b = *reinterpret_cast<const f4*>(bias + c);
+    for (int i = 0; i < V / 4 * W; ++i) r[i] = reinterpret_cast<const f4*>(from)[i];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      bv[k] = b[k];
+    for (int i = 0; i < V / 4; ++i) {
+      b[i] = f4{0.f, 0.f, 0.f, 0.f};
+      if (bias) b[i] = reinterpret_cast<const f4*>(bias + c)[i];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      bv[k] = b[k / 4][k % 4];
 #pragma unroll
       for (int j = 0; j < W; ++j) w[j][k] = r[(k * W + j) / 4][(k * W + j) % 4];
     }
@@ -350,23 +365,25 @@ __global__ __launch_bounds__(THREADS) void conv_step_kernel(Step a) {
   }
 }
 
-#define M4SL_CONV_TAPS(In, V, W)                             \
-  template __global__ void conv_kernel<In, V, W>(Conv);      \
+#define M4SL_CONV_TAPS(In, V, W)                                 \
+  template __global__ void conv_kernel<In, V, W>(Conv);          \
   template __global__ void conv_backward_kernel<In, V, W>(Conv); \
   template __global__ void conv_step_kernel<In, V, W, 1>(Step);  \
   template __global__ void conv_step_kernel<In, V, W, 4>(Step);
-#define M4SL_CONV(In, V)   \
-  M4SL_CONV_TAPS(In, V, 1) \
-  M4SL_CONV_TAPS(In, V, 2) \
-  M4SL_CONV_TAPS(In, V, 3) \
-  M4SL_CONV_TAPS(In, V, 4) \
-  M4SL_CONV_TAPS(In, V, 5) \
-  M4SL_CONV_TAPS(In, V, 6) \
-  M4SL_CONV_TAPS(In, V, 7) \
-  M4SL_CONV_TAPS(In, V, 8)
-M4SL_CONV(float, 4)
-M4SL_CONV(float, 1)
-M4SL_CONV(bf16_t, 4)
-M4SL_CONV(bf16_t, 1)
+#define M4SL_CONV_FORWARD(In, V, W) template __global__ void conv_kernel<In, V, W>(Conv);
+#define M4SL_CONV(TAPS, In, V) \
+  TAPS(In, V, 1)               \
+  TAPS(In, V, 2)               \
+  TAPS(In, V, 3)               \
+  TAPS(In, V, 4)               \
+  TAPS(In, V, 5)               \
+  TAPS(In, V, 6)               \
+  TAPS(In, V, 7)               \
+  TAPS(In, V, 8)
+M4SL_CONV(M4SL_CONV_TAPS, float, 4)
+M4SL_CONV(M4SL_CONV_TAPS, float, 1)
+M4SL_CONV(M4SL_CONV_TAPS, bf16_t, 4)
+M4SL_CONV(M4SL_CONV_TAPS, bf16_t, 1)
+M4SL_CONV(M4SL_CONV_FORWARD, bf16_t, 8)
 
 }  // namespace cv
