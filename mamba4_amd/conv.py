@@ -14,9 +14,9 @@ from typing import NamedTuple
 import torch
 
 from mamba4_amd import _lib
-from mamba4_amd.attention import _f32, _on, _same_device, _stream, _workspace
+from mamba4_amd.attention import _on, _same_device, _stream, _workspace
 from mamba4_amd.memory import _differentiated, _ptr
-from mamba4_amd.selective import _active, _lengths, _rows, _unit
+from mamba4_amd.selective import _active, _as, _dense, _lengths, _parameter, _rows, _unit
 
 ACTIVATIONS = {"none": 0, "silu": 1}
 MAX_TAPS = 8
@@ -65,7 +65,7 @@ class _CausalConv(torch.autograd.Function):
         taps, device = weight.shape[1], x.device
         inputs = (x, weight, bias, initial)
         if d_state is not None:
-            d_state = d_state.to(x.dtype).contiguous()
+            d_state = _dense(d_state, x.dtype)
         if batch == 0 or time == 0:
             grads = [None if t is None else torch.zeros_like(t) for t in inputs]
             if initial is not None and d_state is not None:
@@ -73,7 +73,7 @@ class _CausalConv(torch.autograd.Function):
             return (*grads, None, None)
         if d_output is None:
             d_output = torch.zeros(x.shape, dtype=x.dtype, device=device)
-        d_output = d_output.to(x.dtype).contiguous()
+        d_output = _dense(d_output, x.dtype)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=device) if wanted else None
                  for t, wanted in zip(inputs, ctx.needs_input_grad)]
         lib = _lib.load()
@@ -106,8 +106,8 @@ def _inputs(name, lead, x, weight, bias, activation):
         raise ValueError(f"{name} needs a weight [D,W] with W in 1..{MAX_TAPS}")
     if bias is not None and tuple(bias.shape) != (channels,):
         raise ValueError(f"{name} needs a bias [D]")
-    rows = x if x.dtype == _BF16 else x.to(torch.float32)
-    return _unit(rows), _f32(weight), None if bias is None else _f32(bias)
+    rows = x if x.dtype == _BF16 else _as(x, torch.float32)
+    return _unit(rows), _parameter(weight), _parameter(bias)
 
 
 def _state(name, label, state, x, weight):
@@ -116,7 +116,7 @@ def _state(name, label, state, x, weight):
         raise ValueError(f"{name} needs {label} [B,W-1,D]")
     if state.dtype.is_complex:
         raise ValueError(f"{label} is complex; take its real part first")
-    return state.to(x.dtype).contiguous()
+    return _dense(state, x.dtype)
 
 
 def causal_conv(x, weight, bias=None, *, activation="none", initial=None, lengths=None):
@@ -145,7 +145,7 @@ def causal_conv(x, weight, bias=None, *, activation="none", initial=None, length
             output, state = _CausalConv.apply(*args)
         else:
             output, state = _forward(*args)
-    return CausalConvResult(output.to(dtype), state.to(dtype))
+    return CausalConvResult(_as(output, dtype), _as(state, dtype))
 
 
 def _step(state, new_state, x, weight, bias, activation, active):
@@ -182,7 +182,7 @@ def causal_conv_step(state, x, weight, bias=None, *, activation="none", active=N
         return CausalConvResult(one.output[:, 0].to(dtype), one.state.to(dtype))
     new = torch.empty_like(old)
     output = _step(old, new, x, weight, bias, activation, active)
-    return CausalConvResult(output.to(dtype), new.to(dtype))
+    return CausalConvResult(_as(output, dtype), _as(new, dtype))
 
 
 def causal_conv_step_(state, x, weight, bias=None, *, activation="none", active=None):
@@ -202,4 +202,4 @@ def causal_conv_step_(state, x, weight, bias=None, *, activation="none", active=
     # The state may be saved for a backward: the write counts as one of torch's.
     torch.autograd.graph.increment_version(state)
     output = _step(state, state, x, weight, bias, activation, active)
-    return CausalConvResult(output.to(dtype), state)
+    return CausalConvResult(_as(output, dtype), state)

@@ -2,6 +2,7 @@
 // of the arguments and the launches.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <initializer_list>
@@ -117,18 +118,43 @@ bool bad_scan(const m4sl_scan* s, bool tokens, std::string* why) {
   return false;
 }
 
-// Segments that a sequence is cut into.  A walk from end to end takes a tile's latency
-// a tile; segments cost their states first (0.75 of the outputs' instructions, again),
-// so that sequences are cut only where their waves leave the card idle, and into no
-// more than fill it.
-int segments(const m4sl_scan& s) {
-  if (const char* e = std::getenv("M4SL_SEGMENTS")) { int v = std::atoi(e); if (v) return std::min(v, std::max(1, tiles_of(s.T))); }
+// Microseconds a tile of a SIMD with `waves` waves: of the results, or of what a segment
+// adds.  A wave alone takes the latency of its instructions, several the throughput
+// (bfloat16, N16: T32768 D2048, 3 waves a SIMD 4.1 and 2.7, 8 waves 10.4 and 7.0; B16
+// T1024 D1536, 2 waves, 3.1).  The backward keeps two waves a SIMD and takes more in turn.
+double tile_pace(double waves, bool backward, bool results) {
+  if (!backward || !results) return (results ? 1.25 : 0.81) * (std::max(2.0, waves) + 0.4);
+  const double pairs = std::floor(waves / 2), rest = waves - 2 * pairs;
+  return 8.1 * pairs + (rest <= 0 ? 0.0 : rest <= 1 ? 6.0 : 8.1);
+}
+
+// Tiles of the segments that a sequence is cut into.  A walk from end to end leaves SIMDs
+// idle where there are few sequences; segments cost their states first, a carry and two
+// launches.  The best by the paces above (B16 T1024 D1536: the forward walks, the backward
+// takes four segments, 520 -> 484 us; B1 T2000: 32 segments).  M4SL_SEGMENTS = a number
+// overrides the choice; results differ by rounding.
+int segment_tiles(const m4sl_scan& s, bool backward) {
+  const int tiles = tiles_of(s.T);
   const long waves = (long)s.B * s.G * ((s.D / s.G + 15) / 16);
-  const long full = 4L * m4::api_compute_units();
-  if (waves >= full) return 1;
-  const long want = (3 * full + waves - 1) / waves, most = tiles_of(s.T) / 2;
-  const long cut = std::min(want, most);
-  return cut < 3 ? 1 : (int)std::min(cut, 4096L);
+  const int least = (tiles + 59999) / 60000;  // (segments are a launch's y blocks)
+  if (const char* e = std::getenv("M4SL_SEGMENTS"))
+    if (const int cut = std::atoi(e); cut > 0) return std::max(least, (tiles + cut - 1) / cut);
+  const double units = 4.0 * m4::api_compute_units();
+  int best = tiles;
+  double time = 0;
+  for (int each = tiles;;) {
+    const int cut = (tiles + each - 1) / each;
+    const double all = std::ceil(waves * (double)cut / units),
+                 some = std::ceil(waves * (cut - 1.0) / units);
+    double t = each * tile_pace(all, backward, true);
+    if (cut > 1) t += 14.0 + 0.15 * cut + each * tile_pace(some, backward, false);
+    if (each == tiles || t < 0.97 * time) {
+      best = each;
+      time = t;
+    }
+    if (each <= least) return best;
+    each = std::max(least, std::min(each - 1, each * 4 / 5));
+  }
 }
 
 ss::Rows rows_of(const m4sl_rows& r) { return ss::Rows{r.data, r.batch_stride, r.token_stride}; }
@@ -149,7 +175,7 @@ bool whole_scan(const ss::Scan& a, int bf16, std::initializer_list<const void*> 
          tile_rows(a.b, a.N, bf16) && tile_rows(a.c, a.N, bf16);
 }
 
-ss::Scan scan_of(const m4sl_scan& s, const int* lengths) {
+ss::Scan scan_of(const m4sl_scan& s, const int* lengths, bool backward) {
   ss::Scan a{};
   a.x = rows_of(s.x);
   a.delta = rows_of(s.delta);
@@ -175,8 +201,7 @@ ss::Scan scan_of(const m4sl_scan& s, const int* lengths) {
   a.N = s.N;
   a.softplus = s.softplus;
   a.blocks = blocks_of(s);
-  const int cut = segments(s), tiles = tiles_of(s.T);
-  a.seg = (tiles + cut - 1) / cut * ss::TILE;
+  a.seg = segment_tiles(s, backward) * ss::TILE;
   a.NS = (s.T + a.seg - 1) / a.seg;
   return a;
 }
@@ -199,7 +224,8 @@ size_t take_backward(Carver& c, ss::Scan* a) {
 
 template <typename In, int NG, bool WHOLE>
 void start_groups(const ss::Scan& a, bool backward, bool all, hipStream_t st) {
-  const dim3 grid(a.B * a.G * a.blocks, a.NS), block(64 * ss::WAVES);
+  // (What a sequence's last segment adds, backward the first one's, nobody starts from.)
+  const dim3 grid(a.B * a.G * a.blocks, all ? a.NS : a.NS - 1), block(64 * ss::WAVES);
   if (backward) {
     if (all)
       hipLaunchKernelGGL((ss::scan_backward_kernel<In, NG, true, WHOLE>), grid, block, 0, st, a);
@@ -263,7 +289,7 @@ long m4sl_scan_kept_floats(const m4sl_scan* s) {
 size_t m4sl_scan_workspace_bytes(const m4sl_scan* s) {
   std::string why;
   if (bad_scan(s, true, &why)) return 0;
-  ss::Scan a = scan_of(*s, nullptr);
+  ss::Scan a = scan_of(*s, nullptr, false);
   Carver c{nullptr};
   return take_segments(c, &a);
 }
@@ -279,7 +305,7 @@ int m4sl_scan_forward(const m4sl_scan* s, const float* initial, const int* lengt
     if (!output || !state) return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(s->bf16, {output}))
       return api_fail(M4MR_EINVAL, at + "rows must be aligned to their elements");
-    ss::Scan a = scan_of(*s, lengths);
+    ss::Scan a = scan_of(*s, lengths, false);
     Carver c{static_cast<char*>(workspace)};
     if (bad_workspace(workspace, workspace_bytes, take_segments(c, &a), &why))
       return api_fail(M4MR_EINVAL, at + why);
@@ -302,7 +328,7 @@ int m4sl_scan_forward(const m4sl_scan* s, const float* initial, const int* lengt
 size_t m4sl_scan_backward_workspace_bytes(const m4sl_scan* s) {
   std::string why;
   if (bad_scan(s, true, &why)) return 0;
-  ss::Scan a = scan_of(*s, nullptr);
+  ss::Scan a = scan_of(*s, nullptr, true);
   Carver c{nullptr};
   return take_backward(c, &a);
 }
@@ -319,7 +345,7 @@ int m4sl_scan_backward(const m4sl_scan* s, const int* lengths, const void* d_out
       return api_fail(M4MR_EINVAL, at + "a required pointer is NULL");
     if (misaligned(s->bf16, {d_output, grads->x, grads->delta, grads->gate, grads->b, grads->c}))
       return api_fail(M4MR_EINVAL, at + "rows must be aligned to their elements");
-    ss::Scan a = scan_of(*s, lengths);
+    ss::Scan a = scan_of(*s, lengths, true);
     Carver c{static_cast<char*>(workspace)};
     if (bad_workspace(workspace, workspace_bytes, take_backward(c, &a), &why))
       return api_fail(M4MR_EINVAL, at + why);
@@ -336,7 +362,9 @@ int m4sl_scan_backward(const m4sl_scan* s, const int* lengths, const void* d_out
     hipStream_t st = static_cast<hipStream_t>(stream);
     int rc;
     if (a.NS > 1) {
+      a.skipped = 1;
       rc = run_scan("scan_backward_states", a, s->bf16, whole, true, false, st);
+      a.skipped = 0;
       if (!rc) rc = run_carry<true>(a, st);
       if (rc) return rc;
     }

@@ -258,7 +258,7 @@ __device__ __forceinline__ Place place(const Scan& a) {
   p.b = rest / a.G;
   p.g = rest - p.b * a.G;
   p.first = p.block * BLOCK_CHANNELS + p.wave * 16;
-  p.s = blockIdx.y;
+  p.s = blockIdx.y + a.skipped;
   p.begin = p.s * a.seg;
   p.end = min(a.T, p.begin + a.seg);
   p.len = a.lengths ? min(max(a.lengths[p.b], 0), a.T) : a.T;
@@ -582,7 +582,8 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
 }
 
 // What each segment starts from, in the place of what it adds: h <- exp(a sum s) h + end.
-// Backward: from the last to the first, from the state's cotangent, to d_initial.
+// Backward: from the last to the first, from the state's cotangent.  (What the last one of
+// these adds is not needed, nor formed.)
 template <bool BWD>
 __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
   const long each = (long)a.D * a.N, count = a.B * each;
@@ -612,7 +613,6 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
         h = fmaf(keep[u], h, end[u]);
       }
     }
-    if (BWD && a.dinitial) a.dinitial[i] = h;
   }
 }
 
@@ -826,7 +826,7 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   if (a.part_a) store_states(a, p, a.part_a + (p.row * a.D + p.d) * a.N, da);
   store_token_sums(p, dskip, a.part_d + p.row * 2 * a.D);
   store_token_sums(p, dbias, a.part_d + (p.row * 2 + 1) * a.D);
-  if (a.NS == 1 && a.dinitial)
+  if (p.s == 0 && a.dinitial)
     store_states(a, p, a.dinitial + ((long)p.b * a.D + p.d) * a.N, g);
   // Tiles without a token that is present.
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};

@@ -28,6 +28,7 @@ struct Scan {
   int whole_n;                    // float32 states are read in pieces of four
   int blocks;                     // blocks of a group's channels
   int seg, NS;                    // tokens of a segment, segments
+  int skipped;                    // first segments that a launch leaves out
   const float* initial;           // [B,D,N], or NULL (NS == 1: the start state)
   // Of the segments ([B,NS,D,N] and [B,NS,D]): what each adds to the state (forward)
   // or its cotangent (backward) from zero, then, carried, what each starts from; and

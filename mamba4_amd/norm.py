@@ -27,6 +27,7 @@ import torch
 from mamba4_amd import _lib
 from mamba4_amd.attention import _f32, _on, _same_device, _stream, _workspace
 from mamba4_amd.memory import _differentiated, _ptr
+from mamba4_amd.selective import _as, _dense, _parameter
 
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2}
 
@@ -187,8 +188,8 @@ class _RmsNorm(torch.autograd.Function):
         rows, channels = total.shape
         if d_y is None:
             d_y = torch.zeros((rows, channels), dtype=ctx.dtype, device=device)
-        d_y = d_y.to(ctx.dtype).contiguous()
-        d_sum = None if d_sum is None else d_sum.to(total.dtype).contiguous()
+        d_y = _dense(d_y, ctx.dtype)
+        d_sum = None if d_sum is None else _dense(d_sum, total.dtype)
         # (One array for both, where they have one type: they are the same numbers.)
         same = ctx.dtype == total.dtype
         d_x = d_residual = None
@@ -214,8 +215,8 @@ class _RmsNorm(torch.autograd.Function):
 
 def _rms_rows(t):
     """[M,C] in a dtype of the kernels."""
-    t = t if t.dtype == torch.bfloat16 else t.to(torch.float32)
-    return t.contiguous().view(-1, t.shape[-1])
+    t = _dense(t, torch.bfloat16 if t.dtype == torch.bfloat16 else torch.float32)
+    return t if t.dim() == 2 else t.view(-1, t.shape[-1])
 
 
 def _rms_inputs(name, x, weight, residual):
@@ -230,7 +231,7 @@ def _rms_inputs(name, x, weight, residual):
     if weight is not None and tuple(weight.shape) != (channels,):
         raise ValueError(f"{name} needs a weight [C]")
     return (_rms_rows(x), None if residual is None else _rms_rows(residual),
-            None if weight is None else _f32(weight))
+            _parameter(weight))
 
 
 def rms_norm(x, weight=None, *, residual=None, eps=1e-5):
@@ -253,8 +254,10 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-5):
             y, total = _RmsNorm.apply(rows, other, scale, float(eps))
         else:
             y, total, _ = _rms_forward(rows, other, scale, float(eps), False)
-    y = y.view(x.shape).to(x.dtype)
-    return RmsNormResult(y, x if residual is None else total.view(x.shape).to(residual.dtype))
+    if x.dim() != 2:
+        y, total = y.view(x.shape), None if residual is None else total.view(x.shape)
+    return RmsNormResult(_as(y, x.dtype),
+                         x if residual is None else _as(total, residual.dtype))
 
 
 def rms_norm_e4m3(x, weight=None, *, residual=None, eps=1e-5, block=None):

@@ -33,9 +33,30 @@ class SelectiveScanResult(NamedTuple):
     state: torch.Tensor
 
 
+# (The checks before each conversion save its microsecond in the usual call.)
+
+
 def _unit(t):
     """t, or a contiguous copy where its last axis is not dense."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _as(t, dtype):
+    return t if t.dtype == dtype else t.to(dtype)
+
+
+def _dense(t, dtype):
+    """t in dtype, contiguous."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _parameter(t):
+    """t in float32, contiguous (None stays None)."""
+    if t is None or (t.dtype == _F32 and t.is_contiguous()):
+        return t
+    return _f32(t)
 
 
 def _rows(t, axes):
@@ -104,7 +125,7 @@ class _SelectiveScan(torch.autograd.Function):
         x, delta, a, b, c, skip, gate, bias, initial, lengths, kept = ctx.saved_tensors
         wanted = ctx.needs_input_grad
         inputs = (x, delta, a, b, c, skip, gate, bias, initial)
-        d_state = None if d_state is None else _f32(d_state)
+        d_state = _parameter(d_state)
         if kept is None:
             grads = [None if t is None else torch.zeros_like(t) for t in inputs]
             if initial is not None and d_state is not None:
@@ -114,7 +135,7 @@ class _SelectiveScan(torch.autograd.Function):
         device = x.device
         if d_output is None:
             d_output = torch.zeros(x.shape, dtype=x.dtype, device=device)
-        d_output = d_output.to(x.dtype).contiguous()
+        d_output = _dense(d_output, x.dtype)
         # (The kernels form those of x, delta, b and c in any case.)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=device)
                  if t is not None and (wanted[i] or i in (0, 1, 3, 4)) else None
@@ -168,12 +189,13 @@ def _scan_inputs(name, lead, x, delta, a, b, c, skip, gate, delta_bias):
     for label, t in (("skip", skip), ("delta_bias", delta_bias)):
         if t is not None and tuple(t.shape) != (channels,):
             raise ValueError(f"{name} needs {label} [D]")
-    rows = (x, delta, b, c, gate)
-    if any(t is not None and t.dtype != _BF16 for t in rows):
-        rows = tuple(None if t is None else t.to(_F32) for t in rows)
-    x, delta, b, c, gate = (None if t is None else _unit(t) for t in rows)
-    skip, delta_bias = (None if t is None else _f32(t) for t in (skip, delta_bias))
-    return x, delta, _f32(a), b, c, skip, gate, delta_bias
+    dtype = _F32
+    if x.dtype == delta.dtype == b.dtype == c.dtype == _BF16 \
+            and (gate is None or gate.dtype == _BF16):
+        dtype = _BF16
+    gate = None if gate is None else _unit(_as(gate, dtype))
+    return (_unit(_as(x, dtype)), _unit(_as(delta, dtype)), _parameter(a), _unit(_as(b, dtype)),
+            _unit(_as(c, dtype)), _parameter(skip), gate, _parameter(delta_bias))
 
 
 def _lengths(name, lengths, batch, time):
@@ -219,14 +241,14 @@ def selective_scan(x, delta, a, b, c, *, skip=None, gate=None, delta_bias=None, 
     if initial is not None:
         if tuple(initial.shape) != (batch, channels, a.shape[1]):
             raise ValueError("selective_scan needs initial [B,D,N]")
-        initial = _f32(initial)
+        initial = _parameter(initial)
     lengths = _lengths("selective_scan", lengths, batch, time)
     with _on(device):
         if _differentiated(*inputs, initial):
             output, state = _SelectiveScan.apply(*inputs, initial, bool(softplus), lengths)
         else:
             output, state, _ = _forward(*inputs, initial, bool(softplus), lengths, False)
-    return SelectiveScanResult(output.to(dtype), state)
+    return SelectiveScanResult(_as(output, dtype), state)
 
 
 def _scan_step(state, new_state, inputs, softplus, active, dtype):
@@ -239,7 +261,7 @@ def _scan_step(state, new_state, inputs, softplus, active, dtype):
                 output.data_ptr(), _stream(x.device))
         if rc:
             _lib.check(rc)
-    return SelectiveScanResult(output.to(dtype), new_state)
+    return SelectiveScanResult(_as(output, dtype), new_state)
 
 
 def _step_checks(state, x, delta, a, b, c, skip, gate, delta_bias, active):
@@ -267,7 +289,7 @@ def selective_scan_step(state, x, delta, a, b, c, *, skip=None, gate=None, delta
             gate=None if gate1 is None else gate1[:, None], delta_bias=bias1, softplus=softplus,
             initial=state, lengths=None if active is None else active.to(torch.int32))
         return SelectiveScanResult(one.output[:, 0].to(x.dtype), one.state)
-    old = _f32(state)
+    old = _parameter(state)
     return _scan_step(old, torch.empty_like(old), inputs, bool(softplus), active, x.dtype)
 
 
