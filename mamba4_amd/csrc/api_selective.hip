@@ -103,7 +103,7 @@ bool bad_scan(const m4sl_scan* s, bool tokens, std::string* why) {
     return true;
   }
   if (too_many((double)s->B * s->G * blocks_of(*s), 64 * ss::WAVES) ||
-      (tokens && s->T > INT_MAX - (1 << 16)) || (double)s->D * s->N > 1e9) {
+      (tokens && s->T > INT_MAX - (1 << 16)) || (double)s->D * (s->N + 2) > 1e9) {
     *why = "problem too large";
     return true;
   }
@@ -376,7 +376,7 @@ int m4sl_scan_backward(const m4sl_scan* s, const int* lengths, const void* d_out
     j.part_d = a.part_d;
     j.bc_blocks = element_blocks((long)a.B * a.T * a.G * a.N);
     j.blocks = a.blocks;
-    j.rows = a.B * a.NS;
+    j.rows = (long)a.B * a.NS;
     j.B = a.B;
     j.T = a.T;
     j.D = a.D;

@@ -886,9 +886,9 @@ __global__ __launch_bounds__(256) void join_kernel(Join a) {
   const bool on = i < states + 2L * a.D, of_a = i < states;
   const float* from = of_a ? a.part_a + i : a.part_d + (i - states);
   const long stride = of_a ? states : 2L * a.D;
-  const int quarter = (a.rows + 3) / 4, end = min(a.rows, (slice + 1) * quarter);
+  const long quarter = (a.rows + 3) / 4, end = min(a.rows, (slice + 1) * quarter);
   float s = 0.f;
-  for (int j = slice * quarter; on && j < end; j += U) {
+  for (long j = slice * quarter; on && j < end; j += U) {
     float v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = from[min(j + u, end - 1) * stride];

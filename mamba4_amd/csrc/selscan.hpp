@@ -51,7 +51,8 @@ struct Scan {
 struct Join {
   const float *part_bc, *part_a, *part_d;
   unsigned bc_blocks;             // blocks of the launch that join b's and c's
-  int blocks, rows;               // channel blocks; batch rows and segments
+  int blocks;                     // of channels
+  long rows;                      // batch rows and segments
   int B, T, D, G, N;
   const int* lengths;
   void *db, *dc;

@@ -46,7 +46,7 @@ def _scan_step(scan, state=DATA, new_state=DATA, output=DATA):
     (dict(a=0), "NULL"),
     (dict(x=DATA + 2), "aligned"), (dict(b=DATA + 1, bf16=1), "aligned"),
     (dict(gate=DATA + 2), "aligned"),
-    (dict(B=2**24, D=1), "too large"), (dict(B=2**14, D=2**10, G=2**10), "too large"),
+    (dict(B=2**24, D=1), "too large"), (dict(B=1, T=16, D=2**29, N=1), "too large"), (dict(B=2**14, D=2**10, G=2**10), "too large"),
 ])
 def test_scan_refuses_a_shape(change, words):
     scan = _scan(**change)
