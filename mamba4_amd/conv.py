@@ -16,7 +16,7 @@ import torch
 from mamba4_amd import _lib
 from mamba4_amd.attention import _on, _same_device, _stream, _workspace
 from mamba4_amd.memory import _differentiated, _ptr
-from mamba4_amd.selective import _active, _as, _dense, _lengths, _parameter, _rows, _unit
+from mamba4_amd.selective import _active, _as, _dense, _lengths, _new, _parameter, _rows, _unit
 
 ACTIVATIONS = {"none": 0, "silu": 1}
 MAX_TAPS = 8
@@ -31,7 +31,7 @@ class CausalConvResult(NamedTuple):
 def _forward(x, weight, bias, initial, activation, lengths):
     batch, time, channels = x.shape
     taps, device = weight.shape[1], x.device
-    output = torch.empty((batch, time, channels), dtype=x.dtype, device=device)
+    output = _new(x)
     if batch == 0 or time == 0:
         state = output.new_zeros((batch, taps - 1, channels)) if initial is None \
             else initial.clone()
@@ -74,8 +74,7 @@ class _CausalConv(torch.autograd.Function):
         if d_output is None:
             d_output = torch.zeros(x.shape, dtype=x.dtype, device=device)
         d_output = _dense(d_output, x.dtype)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=device) if wanted else None
-                 for t, wanted in zip(inputs, ctx.needs_input_grad)]
+        grads = [_new(t) if wanted else None for t, wanted in zip(inputs, ctx.needs_input_grad)]
         lib = _lib.load()
         sizes = (batch, time, channels, taps)
         bf16 = x.dtype == _BF16
@@ -150,7 +149,7 @@ def causal_conv(x, weight, bias=None, *, activation="none", initial=None, length
 
 def _step(state, new_state, x, weight, bias, activation, active):
     batch, channels = x.shape
-    output = torch.empty((batch, channels), dtype=x.dtype, device=x.device)
+    output = _new(x)
     if batch:
         with _on(x.device):
             rc = _lib.load().m4sl_conv_step(

@@ -128,6 +128,15 @@ double tile_pace(double waves, bool backward, bool results) {
   return 8.1 * pairs + (rest <= 0 ? 0.0 : rest <= 1 ? 6.0 : 8.1);
 }
 
+// Most tiles of a segment whose rows stay, with two tiles more, below 2^31 bytes (as they
+// have to where they are read through descriptors).
+int most_tiles(const m4sl_scan& s) {
+  long widest = s.D;
+  for (const m4sl_rows* r : {&s.x, &s.delta, &s.gate, &s.b, &s.c})
+    if (r->data) widest = std::max(widest, r->token_stride);
+  return (int)(INT_MAX / 4 / ss::TILE / widest) - 2;
+}
+
 // Tiles of the segments that a sequence is cut into.  A walk from end to end leaves SIMDs
 // idle where there are few sequences; segments cost their states first, a carry and two
 // launches.  The best by the paces above (B16 T1024 D1536: the forward walks, the backward
@@ -137,18 +146,20 @@ int segment_tiles(const m4sl_scan& s, bool backward) {
   const int tiles = tiles_of(s.T);
   const long waves = (long)s.B * s.G * ((s.D / s.G + 15) / 16);
   const int least = (tiles + 59999) / 60000;  // (segments are a launch's y blocks)
+  const int most = std::max(least, std::min(tiles, most_tiles(s)));
   if (const char* e = std::getenv("M4SL_SEGMENTS"))
-    if (const int cut = std::atoi(e); cut > 0) return std::max(least, (tiles + cut - 1) / cut);
+    if (const int cut = std::atoi(e); cut > 0)
+      return std::max(least, std::min(most, (tiles + cut - 1) / cut));
   const double units = 4.0 * m4::api_compute_units();
-  int best = tiles;
+  int best = most;
   double time = 0;
-  for (int each = tiles;;) {
+  for (int each = most;;) {
     const int cut = (tiles + each - 1) / each;
     const double all = std::ceil(waves * (double)cut / units),
                  some = std::ceil(waves * (cut - 1.0) / units);
     double t = each * tile_pace(all, backward, true);
     if (cut > 1) t += 14.0 + 0.15 * cut + each * tile_pace(some, backward, false);
-    if (each == tiles || t < 0.97 * time) {
+    if (each == most || t < 0.97 * time) {
       best = each;
       time = t;
     }
@@ -159,20 +170,20 @@ int segment_tiles(const m4sl_scan& s, bool backward) {
 
 ss::Rows rows_of(const m4sl_rows& r) { return ss::Rows{r.data, r.batch_stride, r.token_stride}; }
 
-// Whether rows of `width` can be read through a tile's descriptor: aligned pieces of four,
-// tokens at least a row apart, and a tile's bytes below 2^31.
-bool tile_rows(const ss::Rows& r, int width, int bf16) {
+// Whether rows of `width` can be read through a segment's descriptor: aligned pieces of
+// four, tokens at least a row apart, and a segment and two tiles more below 2^31 bytes.
+bool tile_rows(const ss::Rows& r, int width, int seg, int bf16) {
   return width % 4 == 0 && r.batch % 4 == 0 && r.token % 4 == 0 && whole_at(bf16, {r.p}) &&
-         r.token >= width && r.token <= INT_MAX / (4 * ss::TILE);
+         r.token >= width && r.token <= INT_MAX / 4 / (seg + 2L * ss::TILE);
 }
 
 // Whether all rows are such (the kernels read others an element at a time).
 bool whole_scan(const ss::Scan& a, int bf16, std::initializer_list<const void*> results) {
   const ss::Rows dense{nullptr, 0, a.D};
   return a.Dg % 4 == 0 && a.bg % 4 == 0 && a.cg % 4 == 0 && whole_at(bf16, results) &&
-         tile_rows(dense, a.D, bf16) && tile_rows(a.x, a.D, bf16) &&
-         tile_rows(a.delta, a.D, bf16) && tile_rows(a.gate, a.D, bf16) &&
-         tile_rows(a.b, a.N, bf16) && tile_rows(a.c, a.N, bf16);
+         tile_rows(dense, a.D, a.seg, bf16) && tile_rows(a.x, a.D, a.seg, bf16) &&
+         tile_rows(a.delta, a.D, a.seg, bf16) && tile_rows(a.gate, a.D, a.seg, bf16) &&
+         tile_rows(a.b, a.N, a.seg, bf16) && tile_rows(a.c, a.N, a.seg, bf16);
 }
 
 ss::Scan scan_of(const m4sl_scan& s, const int* lengths, bool backward) {

@@ -103,17 +103,13 @@ __device__ __forceinline__ float masked(float v, unsigned mask) {
 }
 
 // Rows through a buffer's descriptor: reads past its bytes are zero and writes dropped, so
-// that a tile's absent tokens, and lanes without a channel (whose offset is ABSENT), need
+// that absent tokens, and lanes without a channel (whose offset is ABSENT or more), need
 // no branch and no clearing.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr unsigned ABSENT = 0x80000000u;
 
 __device__ __forceinline__ Rsrc rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
-}
-// `rows` (or fewer than one: none) of `stride` bytes, the last one `width` >= 0.
-__device__ __forceinline__ Rsrc rows_rsrc(const char* base, int stride, int rows, int width) {
-  return rsrc(base, rows > 0 ? (rows - 1) * stride + width : 0);
 }
 __device__ __forceinline__ void read4(Rsrc r, unsigned at, Four<float>& v) {
   v.r = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
@@ -155,6 +151,13 @@ __device__ __forceinline__ float mul_row(float src, float mul) {
       : "=v"(r)
       : "v"(src), "v"(mul), "n"(K));
   return r;
+}
+
+// The same as the first of a sum.
+template <int K>
+__device__ __forceinline__ void add_row(float& acc, float src, float mul, bool first) {
+  if (first) acc = mul_row<K>(src, mul);
+  else fmac_row<K>(acc, src, mul);
 }
 
 // The two wait states between an instruction that writes a register and one that reads it
@@ -260,7 +263,7 @@ __device__ __forceinline__ Place place(const Scan& a) {
   p.first = p.block * BLOCK_CHANNELS + p.wave * 16;
   p.s = blockIdx.y + a.skipped;
   p.begin = p.s * a.seg;
-  p.end = min(a.T, p.begin + a.seg);
+  p.end = p.begin + min(a.T - p.begin, a.seg);
   p.len = a.lengths ? min(max(a.lengths[p.b], 0), a.T) : a.T;
   p.row = (long)p.b * a.NS + p.s;
   p.on = p.first + p.ch < a.Dg;
@@ -270,46 +273,52 @@ __device__ __forceinline__ Place place(const Scan& a) {
   return p;
 }
 
-// An array's rows of a wave's channels (or of its group's states), from the batch row's
-// first token: the stride of a token in bytes, and where in a tile the lane reads.
+// An array's rows of a wave's channels (or of its group's states), from the segment's first
+// token up to some last one: their bytes, that of a token, and where in a tile the lane
+// reads.  (WHOLE: a segment and two tiles more are below 2^31 bytes.)
 struct Lines {
   const char* base;
-  long stride;  // (WHOLE: sixteen of them are below 2^31)
+  int bytes, stride;
   unsigned at;
+  __device__ __forceinline__ Rsrc rows() const { return rsrc(base, bytes); }
+  __device__ __forceinline__ unsigned tile(int t) const { return at + (unsigned)(t * stride); }
 };
 
+// `last` - p.begin rows (or fewer than one: none) of a.D channels.
 template <typename In>
-__device__ __forceinline__ Lines channel_lines(const Place& p, const void* data, long batch,
-                                               long token) {
-  const In* base = static_cast<const In*>(data) + batch + (p.d - p.ch);
-  const long stride = token * (long)sizeof(In);
-  const unsigned at = p.token * (int)stride + p.piece * sizeof(In);
-  return Lines{reinterpret_cast<const char*>(base), stride, p.count > 0 ? at : ABSENT};
+__device__ __forceinline__ Lines channel_lines(const Scan& a, const Place& p, const void* data,
+                                               long batch, long token, int last) {
+  const In* base = static_cast<const In*>(data) + batch + p.begin * token + (p.d - p.ch);
+  const int stride = (int)token * (int)sizeof(In), rows = last - p.begin,
+            width = min(16, max(0, a.Dg - p.first)) * (int)sizeof(In);
+  return Lines{reinterpret_cast<const char*>(base), rows > 0 ? (rows - 1) * stride + width : 0,
+               stride,
+               p.count > 0 ? (unsigned)(p.token * stride + p.piece * (int)sizeof(In)) : ABSENT};
 }
 
 // The arrays that a kernel reads by tiles.
 template <typename In, int NG>
 struct Sources {
   Lines x, delta, gate, dout, b, c;
-  int width;  // bytes of the wave's channels
 
-  __device__ __forceinline__ Sources(const Scan& a, const Place& p) {
+  __device__ __forceinline__ Sources(const Scan& a, const Place& p, int last) {
     const auto lines = [&](const Rows& r) {
-      return channel_lines<In>(p, r.p, p.b * r.batch, r.token);
+      return channel_lines<In>(a, p, r.p, p.b * r.batch, r.token, last);
     };
     x = lines(a.x);
     delta = lines(a.delta);
     gate = lines(a.gate);
-    dout = channel_lines<In>(p, a.dout, (long)p.b * a.T * a.D, a.D);
+    dout = channel_lines<In>(a, p, a.dout, (long)p.b * a.T * a.D, a.D, last);
     const auto states = [&](const Rows& r, long group) {
-      const In* base = static_cast<const In*>(r.p) + p.b * r.batch + p.g * group;
-      const long stride = r.token * (long)sizeof(In);
-      return Lines{reinterpret_cast<const char*>(base), stride,
-                   (unsigned)(p.ch * (int)stride + 4 * p.q * (int)sizeof(In))};
+      const In* base =
+          static_cast<const In*>(r.p) + p.b * r.batch + p.begin * r.token + p.g * group;
+      const int stride = (int)r.token * (int)sizeof(In), rows = last - p.begin;
+      return Lines{reinterpret_cast<const char*>(base),
+                   rows > 0 ? (rows - 1) * stride + a.N * (int)sizeof(In) : 0, stride,
+                   (unsigned)(p.ch * stride + 4 * p.q * (int)sizeof(In))};
     };
     b = states(a.b, a.bg);
     c = states(a.c, a.cg);
-    width = min(16, max(0, a.Dg - p.first)) * (int)sizeof(In);
   }
 };
 
@@ -323,24 +332,18 @@ struct TileRows {
   __device__ __forceinline__ void fetch(const Scan& a, const Place& p, const Sources<In, NG>& from,
                                         int t0, int last) {
     if constexpr (WHOLE) {
-      const int rows = min(TILE, last - t0);
-      const auto read = [&](const Lines& l, Four<In>& v) {
-        read4(rows_rsrc(l.base + t0 * l.stride, (int)l.stride, rows, from.width), l.at, v);
-      };
+      const int rel = t0 - p.begin;
+      const auto read = [&](const Lines& l, Four<In>& v) { read4(l.rows(), l.tile(rel), v); };
       read(from.x, x);
       read(from.delta, delta);
       if (GATE) read(from.gate, gate);
       if (DOUT) read(from.dout, dout);
-      const int wide = a.N * (int)sizeof(In);
-      const Rsrc rb =
-          rows_rsrc(from.b.base + t0 * from.b.stride, (int)from.b.stride, rows, wide);
-      const Rsrc rc =
-          rows_rsrc(from.c.base + t0 * from.c.stride, (int)from.c.stride, rows, wide);
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         const unsigned n = 16 * i + 4 * p.q, more = 16 * i * sizeof(In);
-        read4(rb, n < (unsigned)a.N ? from.b.at + more : ABSENT, b[i]);
-        read4(rc, n < (unsigned)a.N ? from.c.at + more : ABSENT, c[i]);
+        const bool on = n < (unsigned)a.N;
+        read4(from.b.rows(), on ? from.b.tile(rel) + more : ABSENT, b[i]);
+        read4(from.c.rows(), on ? from.c.tile(rel) + more : ABSENT, c[i]);
       }
     } else {
       const int t = t0 + p.token, count = t < last ? p.count : 0;
@@ -367,25 +370,24 @@ struct TileRows {
   }
 };
 
-// Rows [B,T,D] that a kernel writes by tiles, of the wave's channels.
+// Rows [B,T,D] that a kernel writes by tiles, of the wave's channels, up to the segment's
+// end.
 template <typename In, bool WHOLE>
 struct Result {
   Lines l;
-  int width;
-  __device__ __forceinline__ Result(const Scan& a, const Place& p, void* to) {
-    l = channel_lines<In>(p, to, (long)p.b * a.T * a.D, a.D);
-    width = min(16, max(0, a.Dg - p.first)) * (int)sizeof(In);
+  In* to;
+  __device__ __forceinline__ Result(const Scan& a, const Place& p, void* data) {
+    l = channel_lines<In>(a, p, data, (long)p.b * a.T * a.D, a.D, p.end);
+    to = static_cast<In*>(data) + (long)p.b * a.T * a.D + p.d4;
   }
-  // Tokens t0 .. t0 + 15 of those before `end`.
-  __device__ __forceinline__ void put(const Place& p, int t0, int end, const float (&v)[4]) const {
-    Four<In> f;
-    f.set(v);
-    const char* to = l.base + t0 * l.stride;
+  __device__ __forceinline__ void put(const Scan& a, const Place& p, int t0,
+                                      const float (&v)[4]) const {
     if constexpr (WHOLE) {
-      write4(rows_rsrc(to, (int)l.stride, min(TILE, end - t0), width), l.at, f);
-    } else if (t0 + p.token < end) {
-      store4(reinterpret_cast<In*>(const_cast<char*>(to) + p.token * l.stride) + p.piece, v,
-             p.count, false);
+      Four<In> f;
+      f.set(v);
+      write4(l.rows(), l.tile(t0 - p.begin), f);
+    } else if (t0 + p.token < p.end) {
+      store4(to + (long)(t0 + p.token) * a.D, v, p.count, false);
     }
   }
 };
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
   load_states(a, p, begin, h);
   const int tiles = (a.T + TILE - 1) / TILE;
   const int last = min(p.end, p.len);
-  const Sources<In, NG> from(a, p);
+  const Sources<In, NG> from(a, p, last);
   const Result<In, WHOLE> out(a, p, a.out);
   using RowsOf = TileRows<In, NG, OUT, false, WHOLE>;
 
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
       o[e] *= a.gated ? open : 1.f;
       o[e] = masked(o[e], here);
     }
-    out.put(p, t0, p.end, o);
+    out.put(a, p, t0, o);
   };
 
   if (p.begin < last) {
@@ -542,12 +544,11 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
         unroll<0, TILE>([&](auto k) {
           constexpr int t = k.value;
           const f2 v = su[turn][t * 16 + p.ch];
-          if (OUT) part[t & 3] = 0.f;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float keep = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
             h[i][r] = fmaf(keep, h[i][r], mul_row<t>(bv[r], v.y));
-            if (OUT) fmac_row<t>(part[t & 3], cv[r], h[i][r]);
+            if (OUT) add_row<t>(part[t & 3], cv[r], h[i][r], r == 0);
           }
           if (OUT && (t & 3) == 3) y[t / 4] += join_rows(part);
         });
@@ -578,7 +579,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
   // Tiles without a token that is present.
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   for (int t = p.begin + (max(0, last - p.begin) + TILE - 1) / TILE * TILE; t < p.end; t += TILE)
-    out.put(p, t, p.end, zero);
+    out.put(a, p, t, zero);
 }
 
 // What each segment starts from, in the place of what it adds: h <- exp(a sum s) h + end.
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   load_states(a, p, begin, g);
   const int tiles = (a.T + TILE - 1) / TILE;
   const int first = p.begin / TILE, last = min(p.end, p.len);
-  const Sources<In, NG> from(a, p);
+  const Sources<In, NG> from(a, p, last);
   const Result<In, WHOLE> dxs(a, p, a.dx), dds(a, p, a.ddelta), dzs(a, p, a.dgate);
   using RowsOf = TileRows<In, NG, true, true, WHOLE>;
 
@@ -716,13 +717,12 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
             unroll<0, TILE>([&](auto k) {
               constexpr int t = k.value;
               const f4 v = sud[t * 16 + p.ch];
-              part[t & 3] = 0.f;
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
                 keep[t][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
                 h[t][r] = fmaf(keep[t][r], before, mul_row<t>(bv[r], v.y));
-                fmac_row<t>(part[t & 3], cv[r], h[t][r]);
+                add_row<t>(part[t & 3], cv[r], h[t][r], r == 0);
               }
               if ((t & 3) == 3) y[t / 4] += join_rows(part);
             });
@@ -732,18 +732,16 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
               constexpr int t = TILE - 1 - k.value;
               const f4 v = sud[t * 16 + p.ch];
               float pb[4], pc[4], sb, sc;
-              part[t & 3] = 0.f;
-              part2[t & 3] = 0.f;
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
                 fmac_row<t>(g[i][r], cv[r], v.z);
                 pc[r] = h[t][r] * v.z;
                 pb[r] = g[i][r] * v.y;
-                fmac_row<t>(part[t & 3], bv[r], g[i][r]);
+                add_row<t>(part[t & 3], bv[r], g[i][r], r == 0);
                 g[i][r] *= keep[t][r];
                 const float m = g[i][r] * before;
-                part2[t & 3] = fmaf(m, rate[i][r], part2[t & 3]);
+                part2[t & 3] = r ? fmaf(m, rate[i][r], part2[t & 3]) : m * rate[i][r];
                 da[i][r] = fmaf(m, v.x, da[i][r]);
               }
               join_lanes(pb, pc, sb, sc);
@@ -808,9 +806,9 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
             dskip[e] = fmaf(dy0[e], x, dskip[e]);
             dbias[e] += dd[e];
           }
-          dxs.put(p, t0, p.end, dx);
-          dds.put(p, t0, p.end, dd);
-          if (a.dgate) dzs.put(p, t0, p.end, dz);
+          dxs.put(a, p, t0, dx);
+          dds.put(a, p, t0, dd);
+          if (a.dgate) dzs.put(a, p, t0, dz);
         }
         wave_sync();
       }
@@ -831,9 +829,9 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   // Tiles without a token that is present.
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   for (int t = p.begin + (max(0, last - p.begin) + TILE - 1) / TILE * TILE; t < p.end; t += TILE) {
-    dxs.put(p, t, p.end, zero);
-    dds.put(p, t, p.end, zero);
-    if (a.dgate) dzs.put(p, t, p.end, zero);
+    dxs.put(a, p, t, zero);
+    dds.put(a, p, t, zero);
+    if (a.dgate) dzs.put(a, p, t, zero);
   }
 }
 
