@@ -124,11 +124,12 @@ __device__ __forceinline__ void write4(Rsrc r, unsigned at, const Four<bf16_t>& 
   __builtin_amdgcn_raw_buffer_store_b64(v.r, r, at, 0, 0);
 }
 
-// log(1 + exp(v)): of u = 1 + e, rounded, and of what the rounding lost, (e - (u - 1)) / u.
+// log(1 + exp(v)): of u = 1 + e, rounded, and of what the rounding lost, l = e - (u - 1).
+// (That is l / u to first order; l itself is off by at most l e / u <= 2^-24 e / u, less than
+// 2^-24 of log(1 + e) >= e / u, and spares a reciprocal of 8 cycles.)
 __device__ __forceinline__ float softplus(float v) {
   const float e = __builtin_amdgcn_exp2f(-LOG2E * fabsf(v)), u = 1.f + e;
-  const float lost = (e - (u - 1.f)) * __builtin_amdgcn_rcpf(u);
-  return fmaxf(v, 0.f) + fmaf(__builtin_amdgcn_logf(u), LN2, lost);
+  return fmaxf(v, 0.f) + fmaf(__builtin_amdgcn_logf(u), LN2, e - (u - 1.f));
 }
 
 // 1 / (1 + exp(-v)), to 2^-24 of itself and of v.
@@ -434,20 +435,27 @@ __device__ __forceinline__ void store_states(const Scan& a, const Place& p, floa
   }
 }
 
-// All ones where token t is before `last`, else zero.
+// All ones where token t is before `last`, else zero.  (Were its origin known, the compiler
+// would make selects of what it masks.)
 __device__ __forceinline__ unsigned present(int t, int last) {
-  return (unsigned)((t - last) >> 31);
+  unsigned mask = (unsigned)((t - last) >> 31);
+  asm("" : "+v"(mask));
+  return mask;
 }
 
 // The steps of a lane's piece.
 template <typename In>
 __device__ __forceinline__ void steps(const Scan& a, const Four<In>& delta, const float (&bias)[4],
                                       unsigned here, float (&s)[4]) {
+  if (a.softplus) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float v = delta.get(e) + bias[e], soft = softplus(v);
-    s[e] = masked(a.softplus ? soft : v, here);
+    for (int e = 0; e < 4; ++e) s[e] = softplus(delta.get(e) + bias[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = delta.get(e) + bias[e];
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = masked(s[e], here);
 }
 
 template <typename In>
@@ -513,12 +521,18 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
     const unsigned here = present(t0 + p.token, last);
     float o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float z = gate.get(e), open = z * sigmoid(z);
-      o[e] = a.skip ? fmaf(skip[e], x.get(e), v[e]) : v[e];
-      o[e] *= a.gated ? open : 1.f;
-      o[e] = masked(o[e], here);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = v[e];
+    if (a.skip)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(skip[e], x.get(e), o[e]);
+    if (a.gated)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = gate.get(e);
+        o[e] *= z * sigmoid(z);
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = masked(o[e], here);
     out.put(a, p, t0, o);
   };
 
@@ -660,9 +674,15 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   const auto stage = [&](const RowsOf& rows, int t0, f4* to) {
     steps(a, rows.delta, bias, present(t0 + p.token, last), s);
 #pragma unroll
+    for (int e = 0; e < 4; ++e) dy[e] = rows.dout.get(e);
+    if (a.gated)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = rows.gate.get(e);
+        dy[e] *= z * sigmoid(z);
+      }
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float z = rows.gate.get(e), open = z * sigmoid(z);
-      dy[e] = rows.dout.get(e) * (a.gated ? open : 1.f);
       to[p.token * 16 + p.piece + e] = f4{s[e], s[e] * rows.x.get(e), dy[e], 0.f};
       if (!ALL) dbias[e] += s[e];
     }
@@ -793,22 +813,41 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
           const f4 yv = *reinterpret_cast<const f4*>(&out[0][from4]);
           const f4 fv = *reinterpret_cast<const f4*>(&out[1][from4]);
           const f4 sv = *reinterpret_cast<const f4*>(&out[2][from4]);
-          float dx[4], dd[4], dz[4];
+          float dx[4], dd[4], whole[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = was.x.get(e), z = was.gate.get(e), sg = sigmoid(z);
-            const float whole = a.skip ? fmaf(skip[e], x, yv[e]) : yv[e];
-            dz[e] = masked(was.dout.get(e) * whole * (sg * fmaf(z, 1.f - sg, 1.f)), here);
-            dx[e] = masked(fmaf(s0[e], fv[e], a.skip ? skip[e] * dy0[e] : 0.f), here);
-            const float v = fmaf(x, fv[e], sv[e] * LN2);
-            const float soft = v * sigmoid(was.delta.get(e) + bias[e]);
-            dd[e] = masked(a.softplus ? soft : v, here);
+            const float x = was.x.get(e);
+            whole[e] = yv[e];
+            dx[e] = s0[e] * fv[e];
+            dd[e] = fmaf(x, fv[e], sv[e] * LN2);
             dskip[e] = fmaf(dy0[e], x, dskip[e]);
+          }
+          if (a.skip)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              whole[e] = fmaf(skip[e], was.x.get(e), whole[e]);
+              dx[e] = fmaf(skip[e], dy0[e], dx[e]);
+            }
+          if (a.softplus)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dd[e] *= sigmoid(was.delta.get(e) + bias[e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            dx[e] = masked(dx[e], here);
+            dd[e] = masked(dd[e], here);
             dbias[e] += dd[e];
           }
           dxs.put(a, p, t0, dx);
           dds.put(a, p, t0, dd);
-          if (a.dgate) dzs.put(a, p, t0, dz);
+          if (a.dgate) {
+            float dz[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float z = was.gate.get(e), sg = sigmoid(z);
+              dz[e] = masked(was.dout.get(e) * whole[e] * (sg * fmaf(z, 1.f - sg, 1.f)), here);
+            }
+            dzs.put(a, p, t0, dz);
+          }
         }
         wave_sync();
       }
