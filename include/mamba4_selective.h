@@ -24,8 +24,6 @@ extern "C" {
 /* Most states of a channel, and most taps of the convolution. */
 #define M4SL_MAX_STATES 64
 #define M4SL_MAX_TAPS 8
-/* Tokens between the states that a forward call keeps for the backward. */
-#define M4SL_TILE 16
 
 /*
  * Rows [B,T,...] with unit stride along the channels (or states) and strides in
@@ -53,7 +51,8 @@ typedef struct {
   int B, T, D, G, N, bf16, softplus;
 } m4sl_scan;
 
-/* Floats of the states that the forward keeps for the backward. */
+/* Floats of the states that the forward keeps for the backward: every 16 tokens, with more
+ * than 16 states every 8. */
 long m4sl_scan_kept_floats(const m4sl_scan* scan);
 
 /*

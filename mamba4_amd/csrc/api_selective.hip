@@ -80,6 +80,9 @@ long busy_threads() { return 768L * m4::api_compute_units(); }
 
 int tiles_of(int T) { return (T + ss::TILE - 1) / ss::TILE; }
 
+// Groups of 16 states that a lane holds four of.
+int groups_of(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
+
 int blocks_of(const m4sl_scan& s) {
   return (s.D / s.G + ss::BLOCK_CHANNELS - 1) / ss::BLOCK_CHANNELS;
 }
@@ -252,8 +255,8 @@ void start_groups(const ss::Scan& a, bool backward, bool all, hipStream_t st) {
 
 template <typename In, bool WHOLE>
 void start_states(const ss::Scan& a, bool backward, bool all, hipStream_t st) {
-  if (a.N <= 16) return start_groups<In, 1, WHOLE>(a, backward, all, st);
-  if (a.N <= 32) return start_groups<In, 2, WHOLE>(a, backward, all, st);
+  if (groups_of(a.N) == 1) return start_groups<In, 1, WHOLE>(a, backward, all, st);
+  if (groups_of(a.N) == 2) return start_groups<In, 2, WHOLE>(a, backward, all, st);
   return start_groups<In, 4, WHOLE>(a, backward, all, st);
 }
 
@@ -294,7 +297,7 @@ extern "C" {
 long m4sl_scan_kept_floats(const m4sl_scan* s) {
   std::string why;
   if (bad_scan(s, true, &why)) return 0;
-  return (long)s->B * tiles_of(s->T) * s->D * s->N;
+  return (long)s->B * tiles_of(s->T) * (ss::TILE / ss::kept_tokens(groups_of(s->N))) * s->D * s->N;
 }
 
 size_t m4sl_scan_workspace_bytes(const m4sl_scan* s) {

@@ -425,14 +425,22 @@ __device__ __forceinline__ void load_states(const Scan& a, const Place& p, const
   }
 }
 
+__device__ __forceinline__ void store_some(const Scan& a, const Place& p, int i, float* to,
+                                           const float (&h)[4]) {
+  const int n = 16 * i + 4 * p.q;
+  if (p.on) store4(to + n, h, min(4, max(0, a.N - n)), a.whole_n);
+}
 template <int NG>
 __device__ __forceinline__ void store_states(const Scan& a, const Place& p, float* to,
                                              const float (&h)[NG][4]) {
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    const int n = 16 * i + 4 * p.q;
-    if (p.on) store4(to + n, h[i], min(4, max(0, a.N - n)), a.whole_n);
-  }
+  for (int i = 0; i < NG; ++i) store_some(a, p, i, to, h[i]);
+}
+
+// The states of a channel that are kept of a tile, before its tokens 0, KEPT, ...
+template <int KEPT>
+__device__ __forceinline__ float* kept_at(const Scan& a, const Place& p, int tiles, int tile) {
+  return a.kept + (((long)p.b * tiles + tile) * (TILE / KEPT) * a.D + p.d) * a.N;
 }
 
 // All ones where token t is before `last`, else zero.  (Were its origin known, the compiler
@@ -490,6 +498,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
   __shared__ float shared_y[OUT ? WAVES : 1][2][256];  // the same
   const Place p = place(a);
   if (p.first >= a.Dg) return;
+  constexpr int KEPT = kept_tokens(NG);
   auto& su = shared_su[p.wave];
   auto& yl = shared_y[OUT ? p.wave : 0];
   float rate[NG][4], h[NG][4], bias[4], skip[4], total[4] = {0.f, 0.f, 0.f, 0.f};
@@ -545,8 +554,8 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
     wave_sync();
     int turn = 0;
     for (int t0 = p.begin; t0 < last; t0 += TILE) {
-      if (OUT && a.kept)
-        store_states(a, p, a.kept + (((long)p.b * tiles + t0 / TILE) * a.D + p.d) * a.N, h);
+      float* kept = nullptr;
+      if (OUT && a.kept) kept = kept_at<KEPT>(a, p, tiles, t0 / TILE);
       stage(next, t0 + TILE, su[turn ^ 1]);
       float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -557,6 +566,8 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
         settled(bv, cv);
         unroll<0, TILE>([&](auto k) {
           constexpr int t = k.value;
+          if (OUT && t % KEPT == 0 && kept)
+            store_some(a, p, i, kept + t / KEPT * (long)a.D * a.N, h[i]);
           const f2 v = su[turn][t * 16 + p.ch];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -639,17 +650,17 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
 // decays staying in registers, then backwards.
 template <typename In, int NG, bool ALL, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backward_kernel(Scan a) {
-  // A wave's steps, inflows and cotangents [16 tokens][16 channels], its sums over the
-  // states of the same shape, and every wave's sums over channels [16 tokens][16 states].
+  // A wave's steps, inflows and cotangents [16 tokens][16 channels] (in whose place are
+  // then its sums over the states), and every wave's sums over channels [16 tokens][16
+  // states].
   __shared__ f4 shared_in[WAVES][2][256];
-  __shared__ float shared_out[ALL ? WAVES : 1][3][256];
   __shared__ float sums[ALL ? 2 : 1][WAVES][2][ALL ? 256 : 1];
   const Place p = place(a);
   const bool idle = p.first >= a.Dg;
   if (!ALL && idle) return;
   const int active = min(WAVES, (a.Dg - p.block * BLOCK_CHANNELS + 15) / 16);
+  constexpr int KEPT = kept_tokens(NG);
   auto& in = shared_in[p.wave];
-  auto& out = shared_out[ALL ? p.wave : 0];
   float rate[NG][4], g[NG][4], da[NG][4], bias[4], skip[4];
   float dskip[4] = {0.f, 0.f, 0.f, 0.f}, dbias[4] = {0.f, 0.f, 0.f, 0.f};
   load_decays(a, p, rate);
@@ -695,13 +706,21 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
     now.fetch(a, p, from, tile * TILE, last);
     stage(now, tile * TILE, in[0]);
     if (tile > first) next.fetch(a, p, from, (tile - 1) * TILE, last);
-    float start[NG][4];
-    if (ALL) load_states(a, p, a.kept + (((long)p.b * tiles + tile) * a.D + p.d) * a.N, start);
+    constexpr int PARTS = TILE / KEPT;
+    const long part_stride = (long)a.D * a.N;
+    float start[PARTS][NG][4];
+    const auto load_starts = [&](int of) {
+#pragma unroll
+      for (int j = 0; j < PARTS; ++j)
+        load_states(a, p, kept_at<KEPT>(a, p, tiles, of) + j * part_stride, start[j]);
+    };
+    if (ALL) load_starts(tile);
     wave_sync();
     int turn = 0;
     for (; tile >= first; --tile) {
       const int t0 = tile * TILE;
       const f4* sud = in[turn];
+      float* out = reinterpret_cast<float*>(in[turn]);
       if constexpr (!ALL) {
         if (tile > first) stage(next, t0 - TILE, in[turn ^ 1]);
 #pragma unroll
@@ -730,56 +749,61 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
         for (int i = 0; i < NG; ++i) {
           auto& mine = sums[side][p.wave];
           if (!idle) {
-            float bv[4], cv[4], h[TILE][4], keep[TILE][4], part[4], part2[4];
+            float bv[4], cv[4];
             widen(now.b[i], bv);
             widen(now.c[i], cv);
             settled(bv, cv);
-            unroll<0, TILE>([&](auto k) {
-              constexpr int t = k.value;
-              const f4 v = sud[t * 16 + p.ch];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
-                keep[t][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
-                h[t][r] = fmaf(keep[t][r], before, mul_row<t>(bv[r], v.y));
-                add_row<t>(part[t & 3], cv[r], h[t][r], r == 0);
-              }
-              if ((t & 3) == 3) y[t / 4] += join_rows(part);
-            });
             // Bank j of row q: state 4 q + (j with its bits swapped).
             const int n = 4 * p.q + ((p.ch >> 3) | (p.ch >> 1 & 2));
-            unroll<0, TILE>([&](auto k) {
-              constexpr int t = TILE - 1 - k.value;
-              const f4 v = sud[t * 16 + p.ch];
-              float pb[4], pc[4], sb, sc;
+            unroll<0, PARTS>([&](auto of) {
+              constexpr int o = PARTS - 1 - of.value, t0 = o * KEPT;
+              float h[KEPT][4], keep[KEPT][4], part[4], part2[4];
+              unroll<0, KEPT>([&](auto k) {
+                constexpr int t = t0 + k.value;
+                const f4 v = sud[t * 16 + p.ch];
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float before = t ? h[t ? t - 1 : 0][r] : start[i][r];
-                fmac_row<t>(g[i][r], cv[r], v.z);
-                pc[r] = h[t][r] * v.z;
-                pb[r] = g[i][r] * v.y;
-                add_row<t>(part[t & 3], bv[r], g[i][r], r == 0);
-                g[i][r] *= keep[t][r];
-                const float m = g[i][r] * before;
-                part2[t & 3] = r ? fmaf(m, rate[i][r], part2[t & 3]) : m * rate[i][r];
-                da[i][r] = fmaf(m, v.x, da[i][r]);
-              }
-              join_lanes(pb, pc, sb, sc);
-              mine[0][t * 16 + n] = sb;
-              mine[1][t * 16 + n] = sc;
-              if ((t & 3) == 0) {
-                flow[t / 4] += join_rows(part);
-                slope[t / 4] += join_rows(part2);
-              }
+                for (int r = 0; r < 4; ++r) {
+                  const float before = k.value ? h[k.value ? k.value - 1 : 0][r] : start[o][i][r];
+                  keep[k.value][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
+                  h[k.value][r] = fmaf(keep[k.value][r], before, mul_row<t>(bv[r], v.y));
+                  add_row<t>(part[t & 3], cv[r], h[k.value][r], r == 0);
+                }
+                if ((t & 3) == 3) y[t / 4] += join_rows(part);
+              });
+              unroll<0, KEPT>([&](auto back) {
+                constexpr int k = KEPT - 1 - back.value, t = t0 + k;
+                const f4 v = sud[t * 16 + p.ch];
+                float pb[4], pc[4], sb, sc;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float before = k ? h[k ? k - 1 : 0][r] : start[o][i][r];
+                  fmac_row<t>(g[i][r], cv[r], v.z);
+                  pc[r] = h[k][r] * v.z;
+                  pb[r] = g[i][r] * v.y;
+                  add_row<t>(part[t & 3], bv[r], g[i][r], r == 0);
+                  g[i][r] *= keep[k][r];
+                  const float m = g[i][r] * before;
+                  part2[t & 3] = r ? fmaf(m, rate[i][r], part2[t & 3]) : m * rate[i][r];
+                  da[i][r] = fmaf(m, v.x, da[i][r]);
+                }
+                join_lanes(pb, pc, sb, sc);
+                mine[0][t * 16 + n] = sb;
+                mine[1][t * 16 + n] = sc;
+                if ((t & 3) == 0) {
+                  flow[t / 4] += join_rows(part);
+                  slope[t / 4] += join_rows(part2);
+                }
+              });
             });
           }
           if (i == NG - 1 && !idle) {
+            wave_sync();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int at = (4 * j + p.q) * 16 + p.ch;
-              out[0][at] = y[j];
-              out[1][at] = flow[j];
-              out[2][at] = slope[j];
+              out[at] = y[j];
+              out[256 + at] = flow[j];
+              out[512 + at] = slope[j];
             }
           }
           __syncthreads();
@@ -804,15 +828,15 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
         now = next;
         if (tile > first) {
           stage(now, t0 - TILE, in[turn ^ 1]);
-          load_states(a, p, a.kept + (((long)p.b * tiles + tile - 1) * a.D + p.d) * a.N, start);
+          load_starts(tile - 1);
         }
         if (tile > first + 1) next.fetch(a, p, from, t0 - 2 * TILE, last);
         if (!idle) {
           const unsigned here = present(t0 + p.token, last);
           const int from4 = p.token * 16 + p.piece;
-          const f4 yv = *reinterpret_cast<const f4*>(&out[0][from4]);
-          const f4 fv = *reinterpret_cast<const f4*>(&out[1][from4]);
-          const f4 sv = *reinterpret_cast<const f4*>(&out[2][from4]);
+          const f4 yv = *reinterpret_cast<const f4*>(&out[from4]);
+          const f4 fv = *reinterpret_cast<const f4*>(&out[256 + from4]);
+          const f4 sv = *reinterpret_cast<const f4*>(&out[512 + from4]);
           float dx[4], dd[4], whole[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {

@@ -9,6 +9,9 @@ namespace ss {
 typedef unsigned short bf16_t;
 
 constexpr int TILE = 16;    // tokens of a tile: the lanes of a row hold a tile's b and c
+// Tokens between the states that the forward keeps (of NG groups of 16 states): a tile, or
+// half of one where the backward could not hold a tile's states in registers.
+constexpr int kept_tokens(int NG) { return NG == 1 ? TILE : TILE / 2; }
 constexpr int WAVES = 4;    // waves of a block, of 16 channels each
 constexpr int BLOCK_CHANNELS = 16 * WAVES;
 constexpr int STEP_THREADS = 256;
