@@ -495,12 +495,13 @@ __device__ __forceinline__ void store_token_sums(const Place& p, float (&v)[4], 
 template <typename In, int NG, bool OUT, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel(Scan a) {
   __shared__ f2 shared_su[WAVES][2][256];              // [16 tokens][16 channels]
-  __shared__ float shared_y[OUT ? WAVES : 1][2][256];  // the same
+  __shared__ f4 shared_y[OUT ? WAVES : 1][256];        // the same, of the four rows' states
   const Place p = place(a);
   if (p.first >= a.Dg) return;
   constexpr int KEPT = kept_tokens(NG);
   auto& su = shared_su[p.wave];
-  auto& yl = shared_y[OUT ? p.wave : 0];
+  f4* yl = shared_y[OUT ? p.wave : 0];
+  float* yr = reinterpret_cast<float*>(yl);
   float rate[NG][4], h[NG][4], bias[4], skip[4], total[4] = {0.f, 0.f, 0.f, 0.f};
   load_decays(a, p, rate);
   load_bias(a.bias, p, bias);
@@ -525,12 +526,14 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
       if (!OUT) total[e] += s[e];
     }
   };
-  const auto finish = [&](const Four<In>& x, const Four<In>& gate, int t0, const float* sums) {
-    const f4 v = *reinterpret_cast<const f4*>(sums + p.token * 16 + p.piece);
+  const auto finish = [&](const Four<In>& x, const Four<In>& gate, int t0) {
     const unsigned here = present(t0 + p.token, last);
     float o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = v[e];
+    for (int e = 0; e < 4; ++e) {
+      const f4 v = yl[p.token * 16 + p.piece + e];
+      o[e] = (v[0] + v[2]) + (v[1] + v[3]);
+    }
     if (a.skip)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(skip[e], x.get(e), o[e]);
@@ -557,10 +560,12 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
       float* kept = nullptr;
       if (OUT && a.kept) kept = kept_at<KEPT>(a, p, tiles, t0 / TILE);
       stage(next, t0 + TILE, su[turn ^ 1]);
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (OUT && t0 > p.begin) finish(x, gate, t0 - TILE);
+      wave_sync();
+      float y[TILE];
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        float bv[4], cv[4], part[4];
+        float bv[4], cv[4];
         widen(now.b[i], bv);
         widen(now.c[i], cv);
         settled(bv, cv);
@@ -573,15 +578,12 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
           for (int r = 0; r < 4; ++r) {
             const float keep = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
             h[i][r] = fmaf(keep, h[i][r], mul_row<t>(bv[r], v.y));
-            if (OUT) add_row<t>(part[t & 3], cv[r], h[i][r], r == 0);
+            if (OUT) add_row<t>(y[t], cv[r], h[i][r], i == 0 && r == 0);
           }
-          if (OUT && (t & 3) == 3) y[t / 4] += join_rows(part);
+          if (OUT && i == NG - 1) yr[(t * 16 + p.ch) * 4 + p.q] = y[t];
         });
       }
       if (OUT) {
-        if (t0 > p.begin) finish(x, gate, t0 - TILE, yl[turn ^ 1]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) yl[turn][(4 * j + p.q) * 16 + p.ch] = y[j];
         x = now.x;
         gate = now.gate;
       }
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
     }
     if (OUT) {
       const int t0 = p.begin + (last - 1 - p.begin) / TILE * TILE;
-      finish(x, gate, t0, yl[turn ^ 1]);
+      finish(x, gate, t0);
     }
   }
   if (!OUT) {
