@@ -170,21 +170,6 @@ __device__ __forceinline__ void settled(float (&v)[4], float (&w)[4]) {
                  "+v"(w[2]), "+v"(w[3]));
 }
 
-// Sums over the four rows of a wave: row q has that of v[q].  (v comes of inline
-// assembly, to whose writes a swap needs the same two wait states.)
-__device__ __forceinline__ float join_rows(float (&v)[4]) {
-  asm volatile("s_nop 1" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0]), __float_as_uint(v[2]),
-                                                  false, false);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[1]), __float_as_uint(v[3]),
-                                                  false, false);
-  const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const float t = __uint_as_float(b[0]) + __uint_as_float(b[1]);
-  const auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(t), false,
-                                                  false);
-  return __uint_as_float(c[0]) + __uint_as_float(c[1]);
-}
-
 // Sums of v and of w over the 16 lanes of a row: bank b (of four lanes) has that of v[b
 // with its two bits swapped].  Each level adds the lanes 8, then 4 apart of one value in
 // half of the banks and of another in the rest, so that four values take eight
@@ -652,10 +637,11 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
 // decays staying in registers, then backwards.
 template <typename In, int NG, bool ALL, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backward_kernel(Scan a) {
-  // A wave's steps, inflows and cotangents [16 tokens][16 channels] (in whose place are
-  // then its sums over the states), and every wave's sums over channels [16 tokens][16
-  // states].
+  // A wave's steps, inflows, cotangents and x [16 tokens][16 channels], two sums over the
+  // states of each row of lanes of the same shape, and every wave's sums over channels [16
+  // tokens][16 states].
   __shared__ f4 shared_in[WAVES][2][256];
+  __shared__ f4 shared_rows[ALL ? WAVES : 1][2][256];
   __shared__ float sums[ALL ? 2 : 1][WAVES][2][ALL ? 256 : 1];
   const Place p = place(a);
   const bool idle = p.first >= a.Dg;
@@ -663,6 +649,9 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   const int active = min(WAVES, (a.Dg - p.block * BLOCK_CHANNELS + 15) / 16);
   constexpr int KEPT = kept_tokens(NG);
   auto& in = shared_in[p.wave];
+  auto& row_sums = shared_rows[ALL ? p.wave : 0];
+  float* const rows0 = reinterpret_cast<float*>(row_sums[0]);
+  float* const rows1 = reinterpret_cast<float*>(row_sums[1]);
   float rate[NG][4], g[NG][4], da[NG][4], bias[4], skip[4];
   float dskip[4] = {0.f, 0.f, 0.f, 0.f}, dbias[4] = {0.f, 0.f, 0.f, 0.f};
   load_decays(a, p, rate);
@@ -683,6 +672,10 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   const Result<In, WHOLE> dxs(a, p, a.dx), dds(a, p, a.ddelta), dzs(a, p, a.dgate);
   using RowsOf = TileRows<In, NG, true, true, WHOLE>;
 
+  // Whether there are registers for the steps and cotangents of a lane's piece until its
+  // results are formed (B16 T1024 D1536 N16 bfloat16 training 626 us from LDS, 607 so);
+  // float32 and more states would spill others (648 us from LDS, 711 so).
+  constexpr bool HELD = NG == 1 && sizeof(In) == 2;
   float s[4], dy[4];  // of the tile that is staged
   const auto stage = [&](const RowsOf& rows, int t0, f4* to) {
     steps(a, rows.delta, bias, present(t0 + p.token, last), s);
@@ -696,7 +689,8 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
       }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      to[p.token * 16 + p.piece + e] = f4{s[e], s[e] * rows.x.get(e), dy[e], 0.f};
+      const float x = rows.x.get(e);
+      to[p.token * 16 + p.piece + e] = f4{s[e], s[e] * x, dy[e], x};
       if (!ALL) dbias[e] += s[e];
     }
   };
@@ -722,7 +716,6 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
     for (; tile >= first; --tile) {
       const int t0 = tile * TILE;
       const f4* sud = in[turn];
-      float* out = reinterpret_cast<float*>(in[turn]);
       if constexpr (!ALL) {
         if (tile > first) stage(next, t0 - TILE, in[turn ^ 1]);
 #pragma unroll
@@ -744,8 +737,15 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
         if (tile > first + 1) next.fetch(a, p, from, t0 - 2 * TILE, last);
         wave_sync();
       } else {
-        float y[4] = {0.f, 0.f, 0.f, 0.f}, flow[4] = {0.f, 0.f, 0.f, 0.f},
-              slope[4] = {0.f, 0.f, 0.f, 0.f};
+        float yv[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f},
+              sv[4] = {0.f, 0.f, 0.f, 0.f};
+        const auto join = [&](const f4* from, unsigned mask, float (&sum)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f4 v = from[p.token * 16 + p.piece + e];
+            sum[e] += masked((v[0] + v[2]) + (v[1] + v[3]), mask);
+          }
+        };
         int side = NG == 1 ? turn : 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -759,54 +759,50 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
             const int n = 4 * p.q + ((p.ch >> 3) | (p.ch >> 1 & 2));
             unroll<0, PARTS>([&](auto of) {
               constexpr int o = PARTS - 1 - of.value, t0 = o * KEPT;
-              float h[KEPT][4], keep[KEPT][4], part[4], part2[4];
+              float h[KEPT][4], keep[KEPT][4];
               unroll<0, KEPT>([&](auto k) {
                 constexpr int t = t0 + k.value;
                 const f4 v = sud[t * 16 + p.ch];
+                float y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   const float before = k.value ? h[k.value ? k.value - 1 : 0][r] : start[o][i][r];
                   keep[k.value][r] = __builtin_amdgcn_exp2f(v.x * rate[i][r]);
                   h[k.value][r] = fmaf(keep[k.value][r], before, mul_row<t>(bv[r], v.y));
-                  add_row<t>(part[t & 3], cv[r], h[k.value][r], r == 0);
+                  add_row<t>(y, cv[r], h[k.value][r], r == 0);
                 }
-                if ((t & 3) == 3) y[t / 4] += join_rows(part);
+                rows0[(t * 16 + p.ch) * 4 + p.q] = y;
               });
+              wave_sync();
+              join(row_sums[0], PARTS == 1 || p.token / KEPT == o ? ~0u : 0u, yv);
+              wave_sync();
               unroll<0, KEPT>([&](auto back) {
                 constexpr int k = KEPT - 1 - back.value, t = t0 + k;
                 const f4 v = sud[t * 16 + p.ch];
-                float pb[4], pc[4], sb, sc;
+                float pb[4], pc[4], sb, sc, flow, slope;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   const float before = k ? h[k ? k - 1 : 0][r] : start[o][i][r];
                   fmac_row<t>(g[i][r], cv[r], v.z);
                   pc[r] = h[k][r] * v.z;
                   pb[r] = g[i][r] * v.y;
-                  add_row<t>(part[t & 3], bv[r], g[i][r], r == 0);
+                  add_row<t>(flow, bv[r], g[i][r], r == 0);
                   g[i][r] *= keep[k][r];
                   const float m = g[i][r] * before;
-                  part2[t & 3] = r ? fmaf(m, rate[i][r], part2[t & 3]) : m * rate[i][r];
+                  slope = r ? fmaf(m, rate[i][r], slope) : m * rate[i][r];
                   da[i][r] = fmaf(m, v.x, da[i][r]);
                 }
                 join_lanes(pb, pc, sb, sc);
                 mine[0][t * 16 + n] = sb;
                 mine[1][t * 16 + n] = sc;
-                if ((t & 3) == 0) {
-                  flow[t / 4] += join_rows(part);
-                  slope[t / 4] += join_rows(part2);
-                }
+                rows0[(t * 16 + p.ch) * 4 + p.q] = slope;
+                rows1[(t * 16 + p.ch) * 4 + p.q] = flow;
               });
             });
-          }
-          if (i == NG - 1 && !idle) {
             wave_sync();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int at = (4 * j + p.q) * 16 + p.ch;
-              out[at] = y[j];
-              out[256 + at] = flow[j];
-              out[512 + at] = slope[j];
-            }
+            join(row_sums[0], ~0u, sv);
+            join(row_sums[1], ~0u, fv);
+            wave_sync();
           }
           __syncthreads();
           // The block's channels, in their order.
@@ -826,7 +822,10 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
           side ^= 1;
         }
         const RowsOf was = now;
-        const float s0[4] = {s[0], s[1], s[2], s[3]}, dy0[4] = {dy[0], dy[1], dy[2], dy[3]};
+        f4 piece[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          piece[e] = HELD ? f4{s[e], 0.f, dy[e], was.x.get(e)} : sud[p.token * 16 + p.piece + e];
         now = next;
         if (tile > first) {
           stage(now, t0 - TILE, in[turn ^ 1]);
@@ -835,24 +834,19 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
         if (tile > first + 1) next.fetch(a, p, from, t0 - 2 * TILE, last);
         if (!idle) {
           const unsigned here = present(t0 + p.token, last);
-          const int from4 = p.token * 16 + p.piece;
-          const f4 yv = *reinterpret_cast<const f4*>(&out[from4]);
-          const f4 fv = *reinterpret_cast<const f4*>(&out[256 + from4]);
-          const f4 sv = *reinterpret_cast<const f4*>(&out[512 + from4]);
           float dx[4], dd[4], whole[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = was.x.get(e);
             whole[e] = yv[e];
-            dx[e] = s0[e] * fv[e];
-            dd[e] = fmaf(x, fv[e], sv[e] * LN2);
-            dskip[e] = fmaf(dy0[e], x, dskip[e]);
+            dx[e] = piece[e].x * fv[e];
+            dd[e] = fmaf(piece[e].w, fv[e], sv[e] * LN2);
+            dskip[e] = fmaf(piece[e].z, piece[e].w, dskip[e]);
           }
           if (a.skip)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              whole[e] = fmaf(skip[e], was.x.get(e), whole[e]);
-              dx[e] = fmaf(skip[e], dy0[e], dx[e]);
+              whole[e] = fmaf(skip[e], piece[e].w, whole[e]);
+              dx[e] = fmaf(skip[e], piece[e].z, dx[e]);
             }
           if (a.softplus)
 #pragma unroll
