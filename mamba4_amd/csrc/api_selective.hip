@@ -123,12 +123,14 @@ bool bad_scan(const m4sl_scan* s, bool tokens, std::string* why) {
 
 // Microseconds a tile of a SIMD with `waves` waves: of the results, or of what a segment
 // adds.  A wave alone takes the latency of its instructions, several the throughput
-// (bfloat16, N16: T32768 D2048, 3 waves a SIMD 4.1 and 2.7, 8 waves 10.4 and 7.0; B16
-// T1024 D1536, 2 waves, 3.1).  The backward keeps two waves a SIMD and takes more in turn.
+// (bfloat16, N16: T32768 D2048, 3 waves a SIMD 3.9 and 2.8, 8 waves 9.6 and 7.1; B16 T1024
+// D1536, 2 waves, 2.7).  The backward keeps two waves a SIMD and takes more in turn (two
+// 7.4; what a segment adds, 5 waves, 5.4).
 double tile_pace(double waves, bool backward, bool results) {
-  if (!backward || !results) return (results ? 1.25 : 0.81) * (std::max(2.0, waves) + 0.4);
+  if (!results) return (backward ? 1.0 : 0.86) * (std::max(2.0, waves) + 0.3);
+  if (!backward) return 1.16 * (std::max(2.0, waves) + 0.35);
   const double pairs = std::floor(waves / 2), rest = waves - 2 * pairs;
-  return 8.1 * pairs + (rest <= 0 ? 0.0 : rest <= 1 ? 6.0 : 8.1);
+  return 7.4 * pairs + (rest <= 0 ? 0.0 : rest <= 1 ? 5.5 : 7.4);
 }
 
 // Most tiles of a segment whose rows stay, with two tiles more, below 2^31 bytes (as they
@@ -142,9 +144,10 @@ int most_tiles(const m4sl_scan& s) {
 
 // Tiles of the segments that a sequence is cut into.  A walk from end to end leaves SIMDs
 // idle where there are few sequences; segments cost their states first, a carry and two
-// launches.  The best by the paces above (B16 T1024 D1536: the forward walks, the backward
-// takes four segments, 520 -> 484 us; B1 T2000: 32 segments).  M4SL_SEGMENTS = a number
-// overrides the choice; results differ by rounding.
+// launches.  Of the cuts that fill every SIMD with 1, 2, ... waves the best by the paces
+// above (B16 T1024 D1536: the forward walks, the backward takes four segments, 636 -> 606 us
+// together; B1 T2000: 21 segments, 41 us for 46 with 63; T32768 D2048: 64, 446 us for 490
+// with 24).  M4SL_SEGMENTS = a number overrides the choice; results differ by rounding.
 int segment_tiles(const m4sl_scan& s, bool backward) {
   const int tiles = tiles_of(s.T);
   const long waves = (long)s.B * s.G * ((s.D / s.G + 15) / 16);
@@ -152,23 +155,26 @@ int segment_tiles(const m4sl_scan& s, bool backward) {
   const int most = std::max(least, std::min(tiles, most_tiles(s)));
   if (const char* e = std::getenv("M4SL_SEGMENTS"))
     if (const int cut = std::atoi(e); cut > 0)
-      return std::max(least, std::min(most, (tiles + cut - 1) / cut));
-  const double units = 4.0 * m4::api_compute_units();
-  int best = most;
+      return std::max(least, std::min(most, (int)((tiles + cut - 1L) / cut)));
+  const long units = 4L * m4::api_compute_units();
+  int best = most, each = 0;
   double time = 0;
-  for (int each = most;;) {
+  for (int fill = 0; fill <= 16; ++fill) {
+    const long want = std::max(1L, fill * units / waves);
+    const int size = (int)std::max<long>(least, std::min<long>(most, (tiles + want - 1) / want));
+    if (size == each) continue;
+    each = size;
     const int cut = (tiles + each - 1) / each;
     const double all = std::ceil(waves * (double)cut / units),
                  some = std::ceil(waves * (cut - 1.0) / units);
     double t = each * tile_pace(all, backward, true);
     if (cut > 1) t += 14.0 + 0.15 * cut + each * tile_pace(some, backward, false);
-    if (each == most || t < 0.97 * time) {
+    if (fill == 0 || t < 0.99 * time) {
       best = each;
       time = t;
     }
-    if (each <= least) return best;
-    each = std::max(least, std::min(each - 1, each * 4 / 5));
   }
+  return best;
 }
 
 ss::Rows rows_of(const m4sl_rows& r) { return ss::Rows{r.data, r.batch_stride, r.token_stride}; }
