@@ -7,7 +7,10 @@
 // time, with the last W - 1 rows (backward: and the last W - 1 dz) in registers, so that
 // rows are read once but for the W - 1 at a run's edge.  The backward forms z again
 // instead of keeping it.  (Pieces of eight bfloat16 channels leave it two waves a SIMD:
-// B16 T1024 D1536 W4 77 us for 54; the forward takes 30 us with them and 35 with four.)
+// B16 T1024 D1536 W4 77 us for 55; the forward takes 30 us with them and 35 with four.)
+// Those 30 and 55 us are 3.4 and 2.8 TB/s of the rows read and written once, float32 B8 T1000
+// D768 12 and 23 us 4.1 and 3.2: it waits for memory, with vector instructions in half of
+// the cycles.
 #include <hip/hip_runtime.h>
 
 #include "conv.hpp"
@@ -296,7 +299,7 @@ __global__ __launch_bounds__(THREADS) void conv_backward_kernel(Conv a) {
 }
 
 // Sums of the blocks' parts [rows][W + 1][D], in 16 slices of the rows joined in their
-// order, to dweight [D,W] and dbias [D].
+// order, to dweight [D,W] and dbias [D].  Latency: 4 us.
 __global__ __launch_bounds__(1024) void conv_join_kernel(const float* part, int rows, int W,
                                                          int D, float* dweight, float* dbias) {
   __shared__ float fold[1024];
@@ -321,7 +324,8 @@ __global__ __launch_bounds__(1024) void conv_join_kernel(const float* part, int 
 // ------------------------------------------------------------ one token
 
 // Bound by memory; a thread takes ROWS batch rows, whose loads are in flight together, with
-// the taps of its channels in registers (2,048 rows of 1536 bfloat16: one row 25 us).
+// the taps of its channels in registers (2,048 rows of 1536 bfloat16, W4: one row 25 us,
+// four 10.4, 4.8 TB/s).
 template <typename In, int V, int W, int ROWS>
 __global__ __launch_bounds__(THREADS) void conv_step_kernel(Step a) {
   const int rows = blockIdx.x / a.blocks;
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(THREADS) void conv_step_kernel(Step a) {
   for (int m = 0; m < ROWS; ++m) {
     const long b = first + m;
     on[m] = b < a.B && (!a.active || a.active[b]);
-    if (b >= a.B) continue;
+    if (!on[m] && (b >= a.B || a.new_state == a.state)) continue;
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) x[m][j] = load<In, V>(a.state, (b * (W - 1) + j) * a.D + c);
     if (on[m]) x[m][W - 1] = load<In, V>(a.x, b * a.xb + c);

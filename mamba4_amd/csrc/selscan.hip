@@ -6,16 +6,20 @@
 //   flow = sum over n of g b,  rate[n] = g exp(s a) h_before,  g <- g exp(s a),
 //   dx = s flow + skip dy,  ds = x flow + sum over n of rate a,  da = sum of rate s.
 // The decays differ by channel and state, so that no product of matrices takes the
-// place of the recurrence: it is walked, a few instructions a state and token, and
-// the exponential (8.6 cycles a wave against 2.5 of a multiply-add with operands in
-// vector registers) is most of them.
+// place of the recurrence: it is walked, and vector instructions bound it: five a state
+// and token forwards (one of them the exponential, which takes a SIMD 8 cycles for 4 of the
+// others), fourteen in the gradient, which walks forwards first.
 //
 // A wave holds 16 channels: lane 16 q + ch has the states 4 q .. 4 q + 3 of channel ch
 // (and of each further 16 states).  Tokens come in tiles of 16: lane k of row q holds
 // b and c of token k for the row's states, and a multiply-add reads them by the row
 // broadcast of its operand; what belongs to a channel (the step, s x, dy) goes through
-// the wave's own LDS.  Sums over the states join the four rows of a wave once every
-// four tokens.
+// the wave's own LDS, and so do the sums over the states: each row of lanes writes its own,
+// four numbers a token and channel, and the lane that forms the result adds them (joined in
+// registers by exchanges of rows they took 322 us in place of 301: T32768 D2048 N16,
+// outputs).  Measured and left: b and c by token from LDS (335 us for 335), their
+// products with x and h as outer products on the matrix units (427 for 355; of b x alone,
+// no change).
 #include <hip/hip_runtime.h>
 
 #include "selscan.hpp"
@@ -477,6 +481,11 @@ __device__ __forceinline__ void store_token_sums(const Place& p, float (&v)[4], 
 // OUT: a segment's outputs from its start state (and the last one's end state); else
 // what the segment adds to the state, and the sum of its steps.  A tile's steps are
 // formed while the one before is computed, and its outputs written while the next is.
+// T32768 D2048 N16 bfloat16, 64 segments: 303 us and 226, both issuing a vector instruction
+// in every cycle: 478 and 348 a tile and wave, 320 and 256 of them the recurrence's own; the
+// rest are softplus, gate, conversions and joins.  B16 T1024 D1536, walked from end to end:
+// 171 us, 1.5 waves a SIMD, which leave a third of the cycles empty; in two to four
+// segments 140 and the states' 65 to 75 more.
 template <typename In, int NG, bool OUT, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel(Scan a) {
   __shared__ f2 shared_su[WAVES][2][256];              // [16 tokens][16 channels]
@@ -595,6 +604,8 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
 }
 
 // What each segment starts from, in the place of what it adds: h <- exp(a sum s) h + end.
+// Bound by latency: a chain over the segments, 5 us for 21 (T2000 D1536), 12 for 64 (T32768
+// D2048).
 // Backward: from the last to the first, from the state's cotangent.  (What the last one of
 // these adds is not needed, nor formed.)
 template <bool BWD>
@@ -633,8 +644,13 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
 
 // ALL: a segment's gradients from the cotangent of the state after it; else what the
 // segment adds to the cotangent of the state before it, and the sum of its steps.  A
-// tile is walked forwards from the state that the forward call kept, its states and
-// decays staying in registers, then backwards.
+// tile (or half of one) is walked forwards from the state that the forward call kept, its
+// states and decays staying in registers, then backwards.  B16 T1024 D1536 N16 bfloat16, 4
+// segments: 377 us and 87.  Two waves a SIMD issue in 77% of the cycles; three with half
+// tiles came to the same (406 us for 387), and half tiles' twice as many kept states buy
+// registers only for more than 16 states, where whole ones spill 54 to 165 a lane (N64
+// training 2370 us, so 2116).  Of 1,510 vector instructions a tile and wave 900 are the
+// recurrences', 290 the sums over a row's channels (through LDS: 439 us).
 template <typename In, int NG, bool ALL, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backward_kernel(Scan a) {
   // A wave's steps, inflows, cotangents and x [16 tokens][16 channels], two sums over the
@@ -894,6 +910,7 @@ __global__ __launch_bounds__(64 * WAVES, ALL || !WHOLE ? 2 : 4) void scan_backwa
   }
 }
 
+// Bound by latency and memory (B16 T1024 D1536: 11 us for 50 MB of parts).
 // The gradients of b and c: the sums over the channel blocks, in their order; by the
 // first `bc_blocks` blocks.  By the rest those of a, skip and the bias: the sums over the
 // batch rows and segments, in four parts, joined in their order.
@@ -966,7 +983,8 @@ __global__ __launch_bounds__(256) void join_kernel(Join a) {
 
 // Bound by memory: the states are read and written once.  2^span lanes hold a channel,
 // four states each, and take ROWS batch rows, whose loads are in flight together; what
-// belongs to the channel stays in registers.
+// belongs to the channel stays in registers.  2,048 rows of D1536 N16 bfloat16 in place, an
+// eighth of them idle: 101 us for 0.43 GB, 4.3 TB/s (one row a thread 149); 4 rows 3.6 us.
 template <typename In, int ROWS>
 __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   const int rows = blockIdx.x / a.blocks;
@@ -990,7 +1008,8 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   for (int j = 0; j < ROWS; ++j) {
     const long row = first + j;
     on[j] = row < a.B && (!a.active || a.active[row]);
-    if (row < a.B) h[j] = load4(a.state + (row * a.D + d) * a.N + n, have, a.whole_n);
+    if (on[j] || (row < a.B && a.new_state != a.state))
+      h[j] = load4(a.state + (row * a.D + d) * a.N + n, have, a.whole_n);
     if (!on[j]) continue;
     b[j] = load4(static_cast<const In*>(a.b.p) + row * a.b.batch + g * a.bg + n, have, a.whole_bc);
     c[j] = load4(static_cast<const In*>(a.c.p) + row * a.c.batch + g * a.cg + n, have, a.whole_bc);
