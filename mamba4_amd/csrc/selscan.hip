@@ -984,7 +984,8 @@ __global__ __launch_bounds__(256) void join_kernel(Join a) {
 // Bound by memory: the states are read and written once.  2^span lanes hold a channel,
 // four states each, and take ROWS batch rows, whose loads are in flight together; what
 // belongs to the channel stays in registers.  2,048 rows of D1536 N16 bfloat16 in place, an
-// eighth of them idle: 101 us for 0.43 GB, 4.3 TB/s (one row a thread 149); 4 rows 3.6 us.
+// tenth of them idle: 95 us for 0.39 GB, 4.1 TB/s (one row a thread 149, two 105, eight 125;
+// states past the caches, as here where there are several rows: 104 without); 4 rows 3.6 us.
 template <typename In, int ROWS>
 __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   const int rows = blockIdx.x / a.blocks;
@@ -1000,6 +1001,21 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
   Four<float> rate = load4(a.a + (long)d * a.N + n, have, a.whole_n);
   const float bias = a.bias ? a.bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
   const long first = (long)rows * ROWS;
+  constexpr bool ONCE = ROWS > 1;
+  const auto load_state = [](const Step& a, long at, int have) {
+    Four<float> v;
+    v.r = 0;
+    if (!ONCE || !a.whole_n) v = load4(a.state + at, have, a.whole_n);
+    else if (have > 0) v.r = __builtin_nontemporal_load(reinterpret_cast<const f4*>(a.state + at));
+    return v;
+  };
+  const auto store_state = [](const Step& a, long at, const float (&v)[4], int have) {
+    if (!ONCE || !a.whole_n)
+      store4(a.new_state + at, v, have, a.whole_n);
+    else if (have > 0)
+      __builtin_nontemporal_store(f4{v[0], v[1], v[2], v[3]},
+                                  reinterpret_cast<f4*>(a.new_state + at));
+  };
   Four<float> h[ROWS];
   Four<In> b[ROWS], c[ROWS];
   float x[ROWS], delta[ROWS], z[ROWS];
@@ -1009,7 +1025,7 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
     const long row = first + j;
     on[j] = row < a.B && (!a.active || a.active[row]);
     if (on[j] || (row < a.B && a.new_state != a.state))
-      h[j] = load4(a.state + (row * a.D + d) * a.N + n, have, a.whole_n);
+      h[j] = load_state(a, (row * a.D + d) * a.N + n, have);
     if (!on[j]) continue;
     b[j] = load4(static_cast<const In*>(a.b.p) + row * a.b.batch + g * a.bg + n, have, a.whole_bc);
     c[j] = load4(static_cast<const In*>(a.c.p) + row * a.c.batch + g * a.cg + n, have, a.whole_bc);
@@ -1035,7 +1051,7 @@ __global__ __launch_bounds__(STEP_THREADS) void step_kernel(Step a) {
       }
     }
     if (on[j] || a.new_state != a.state)
-      store4(a.new_state + (row * a.D + d) * a.N + n, v, have, a.whole_n);
+      store_state(a, (row * a.D + d) * a.N + n, v, have);
     for (int m = 1; m < 1 << a.span; m *= 2) y += __shfl_xor(y, m);
     if (n) continue;
     if (on[j]) {
