@@ -40,11 +40,15 @@ def rows():
     return _normal(1, T, D, dtype=BF16)
 
 
-def test_scan(gpu_lib, rows):
-    announce("selective scan of 2^31 elements")
+@pytest.mark.parametrize("dense", [False, True])
+def test_scan(gpu_lib, rows, dense):
+    # (Steps of one row for all tokens are read an element at a time, and so all rows.)
+    announce(f"selective scan of 2^31 elements, dense steps {dense}")
     a = -torch.rand(D, 4, device="cuda")
     b, c = _normal(1, T, 4, dtype=BF16), _normal(1, T, 4, dtype=BF16)
     delta = torch.full((1, 1, D), 0.05, device="cuda", dtype=BF16).expand(1, T, D)
+    if dense:
+        delta = delta.contiguous()
     inputs = [rows.detach().requires_grad_(), b.requires_grad_(), c.requires_grad_()]
     d_out = torch.zeros_like(rows)
     d_out[:, -LAST:] = _normal(1, LAST, D, dtype=BF16)
@@ -60,6 +64,35 @@ def test_scan(gpu_lib, rows):
     for g, h in zip(torch.autograd.grad(s.output, some, d_out[:, cut:]), grads):
         _near(g, h[:, cut:], 2.0 ** -8 + 2e-5)
     del r, grads, d_out
+
+
+@pytest.mark.parametrize("stride,segments", [(1 << 22, 10), (1 << 22, 1), (1 << 24, 10)])
+def test_rows_far_apart(gpu_lib, monkeypatch, stride, segments):
+    """Of a segment below 2^31 bytes, of one that has to be cut for that, and of none: the
+    results of rows beside each other."""
+    announce(f"selective scan of rows {stride} elements apart, {segments} segments")
+    monkeypatch.setenv("M4SL_SEGMENTS", str(segments))
+    time, d, n = 160 if stride == 1 << 22 else 80, 64, 16
+    torch.manual_seed(1)
+    wide = torch.zeros(time, stride, device="cuda", dtype=BF16)
+    wide[:, :3 * d + 2 * n] = _normal(time, 3 * d + 2 * n, dtype=BF16)
+    a = -torch.rand(d, n, device="cuda")
+    d_out = _normal(1, time, d, dtype=BF16)
+
+    def run(rows):
+        x, delta, gate, b, c = (
+            t.detach().requires_grad_() for t in rows[None].split([d, d, d, n, n], -1))
+        r = selective_scan(x, delta, a, b, c, gate=gate, softplus=True)
+        return [r.output, r.state,
+                *torch.autograd.grad(r.output, [x, delta, gate, b, c], d_out)]
+
+    near = run(wide[:, :3 * d + 2 * n].contiguous())
+    far = run(wide[:, :3 * d + 2 * n])
+    for x, y in zip(near, far):
+        if segments == 10:
+            assert torch.equal(x, y)
+        else:
+            _near(x, y, 2.0 ** -8 + 2e-5)
 
 
 def test_conv_and_norm(gpu_lib, rows):
