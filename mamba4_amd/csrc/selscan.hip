@@ -414,6 +414,37 @@ __device__ __forceinline__ void load_states(const Scan& a, const Place& p, const
   }
 }
 
+// The state that a segment of the forward starts from: the carry's steps over those before
+// it, in its order, where there are few.
+template <int NG>
+__device__ __forceinline__ void segment_start(const Scan& a, const Place& p,
+                                              const float (&rate)[NG][4], float (&h)[NG][4]) {
+  const float* outer = a.initial;
+  if (a.NS > 1 && !a.folded) outer = a.ends + p.row * a.D * a.N;
+  else if (outer) outer += (long)p.b * a.D * a.N;
+  load_states(a, p, outer ? outer + (long)p.d * a.N : nullptr, h);
+  if (!a.folded) return;
+  constexpr int U = NG == 1 ? 4 : 2;
+  for (int j = 0; j < p.s; j += U) {
+    float end[U][NG][4], sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long row = (long)p.b * a.NS + min(j + u, p.s - 1);
+      load_states(a, p, a.ends + (row * a.D + p.d) * a.N, end[u]);
+      sum[u] = p.on ? a.sums[row * a.D + p.d] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j + u >= p.s) continue;
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          h[i][r] = fmaf(__builtin_amdgcn_exp2f(sum[u] * rate[i][r]), h[i][r], end[u][i][r]);
+    }
+  }
+}
+
 __device__ __forceinline__ void store_some(const Scan& a, const Place& p, int i, float* to,
                                            const float (&h)[4]) {
   const int n = 16 * i + 4 * p.q;
@@ -500,11 +531,8 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
   load_decays(a, p, rate);
   load_bias(a.bias, p, bias);
   load_bias(a.skip, p, skip);
-  const float* begin = nullptr;
-  if (OUT)
-    begin = a.NS > 1 ? a.ends + (p.row * a.D + p.d) * a.N
-           : a.initial ? a.initial + ((long)p.b * a.D + p.d) * a.N : nullptr;
-  load_states(a, p, begin, h);
+  if (OUT) segment_start(a, p, rate, h);
+  else load_states(a, p, nullptr, h);
   const int tiles = (a.T + TILE - 1) / TILE;
   const int last = min(p.end, p.len);
   const Sources<In, NG> from(a, p, last);
@@ -605,7 +633,7 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
 
 // What each segment starts from, in the place of what it adds: h <- exp(a sum s) h + end.
 // Bound by latency: a chain over the segments, 5 us for 21 (T2000 D1536), 12 for 64 (T32768
-// D2048).
+// D2048).  The forward of few segments does without.
 // Backward: from the last to the first, from the state's cotangent.  (What the last one of
 // these adds is not needed, nor formed.)
 template <bool BWD>

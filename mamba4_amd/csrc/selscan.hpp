@@ -32,6 +32,7 @@ struct Scan {
   int blocks;                     // blocks of a group's channels
   int seg, NS;                    // tokens of a segment, segments
   int skipped;                    // first segments that a launch leaves out
+  int folded;                     // whether a segment joins those before it by itself
   const float* initial;           // [B,D,N], or NULL (NS == 1: the start state)
   // Of the segments ([B,NS,D,N] and [B,NS,D]): what each adds to the state (forward)
   // or its cotangent (backward) from zero, then, carried, what each starts from; and
