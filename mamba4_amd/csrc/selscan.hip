@@ -512,10 +512,10 @@ __device__ __forceinline__ void store_token_sums(const Place& p, float (&v)[4], 
 // OUT: a segment's outputs from its start state (and the last one's end state); else
 // what the segment adds to the state, and the sum of its steps.  A tile's steps are
 // formed while the one before is computed, and its outputs written while the next is.
-// T32768 D2048 N16 bfloat16, 64 segments: 303 us and 226, both issuing a vector instruction
+// T32768 D2048 N16 bfloat16, 64 segments: 315 us and 231, both issuing a vector instruction
 // in every cycle: 478 and 348 a tile and wave, 320 and 256 of them the recurrence's own; the
 // rest are softplus, gate, conversions and joins.  B16 T1024 D1536, walked from end to end:
-// 171 us, 1.5 waves a SIMD, which leave a third of the cycles empty; in two to four
+// 176 us, 1.5 waves a SIMD, which leave a third of the cycles empty; in two to four
 // segments 140 and the states' 65 to 75 more.
 template <typename In, int NG, bool OUT, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel(Scan a) {
@@ -632,8 +632,8 @@ __global__ __launch_bounds__(64 * WAVES, OUT || !WHOLE ? 2 : 4) void scan_kernel
 }
 
 // What each segment starts from, in the place of what it adds: h <- exp(a sum s) h + end.
-// Bound by latency: a chain over the segments, 5 us for 21 (T2000 D1536), 12 for 64 (T32768
-// D2048).  The forward of few segments does without.
+// Bound by latency: a chain over the segments, 6 us for 16 (B8 T1000 D768 N16), 12 for 64
+// (T32768 D2048).  The forward of few segments does without.
 // Backward: from the last to the first, from the state's cotangent.  (What the last one of
 // these adds is not needed, nor formed.)
 template <bool BWD>
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256) void carry_kernel(Scan a) {
 // segment adds to the cotangent of the state before it, and the sum of its steps.  A
 // tile (or half of one) is walked forwards from the state that the forward call kept, its
 // states and decays staying in registers, then backwards.  B16 T1024 D1536 N16 bfloat16, 4
-// segments: 377 us and 87.  Two waves a SIMD issue in 77% of the cycles; three with half
+// segments: 379 us and 88.  Two waves a SIMD issue in 77% of the cycles; three with half
 // tiles came to the same (406 us for 387), and half tiles' twice as many kept states buy
 // registers only for more than 16 states, where whole ones spill 54 to 165 a lane (N64
 // training 2370 us, so 2116).  Of 1,510 vector instructions a tile and wave 900 are the
